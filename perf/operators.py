@@ -306,10 +306,11 @@ def _plain_tables(state):
     row = torch.searchsorted(ends, at, right=True)
     inside = row < lengths.shape[0]
     row = row.clamp(max=lengths.shape[0] - 1)
+    inside &= served[row]
     position = torch.where(inside, lengths[row] + at - starts[row], 0)
     block = (position // page).clamp(0, width - 1)
     slot = table[row, block].long() * page + position % page
-    slots = torch.where(inside & served[row], slot, -1)
+    slots = torch.where(inside, slot, -1)
     state_out = torch.stack([(first + granted.sum()) % pool, free - granted.sum() + freed.sum()])
     return {"slots": slots, "positions": position.to(torch.int32), "starts": starts.to(torch.int32),
             "lengths": torch.where(served, after, lengths).to(torch.int32), "state": state_out.to(torch.int32),
