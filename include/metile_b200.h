@@ -249,6 +249,72 @@ int mt_rope_kv_prefill(const void* q, const void* k, const void* v, const float*
                        void* k_cache, void* v_cache, int* positions, int batch, int steps, int first,
                        int q_heads, int kv_heads, int capacity, int head_dim, void* stream);
 
+/* A key-value cache in pages.  A pool has `pages` pages of `page_size` tokens (8, 16, 32, 64, 128 or 256); keys and values
+ * of a page are [kv_heads, page_size, head_dim] at the strides given as three element counts on the HOST (page, head, token;
+ * multiples of 8; the head dimension is dense).  Row r of block_tables (int32 [requests, width], rows `table_stride`
+ * elements apart) names the pages of request r in order: its token t is in slot
+ * block_tables[r][t / page_size] * page_size + t % page_size.  No counterpart in the reference.  What a kernel finds outside
+ * its table it leaves out and records (mt_device_status, -9): a slot (0x302), a page (0x303), a length the table has no room
+ * for (0x304), a parent outside its group (0x305). */
+#define MT_TYPE_BF16 0
+#define MT_TYPE_FP16 1
+#define MT_TYPE_FP32 2
+
+/* Requests grow by counts[r] > 0 tokens or lose the last -counts[r].  Pages are taken from, and go back to, a ring of
+ * free ids: free_pages int32 [pool], free_state int32 [2] = {index of the first free id, how many there are}.
+ * Of the tokens added, request after request: slots int64 [tokens], positions int32 [tokens] (behind the last one: -1 and
+ * 0); starts int32 [requests + 1] the first token of each request.  block_tables gets the new pages' ids;
+ * lengths_out int32 [requests] and free_state_out may be lengths and free_state.
+ * A request is left as it is, its tokens with -1 and 0, if its length or count makes no sense, its row of the table or the map
+ * has no room, or the free pages do not reach for it and all asking before it.  Pages given back by a
+ * call are there for the next one. */
+int mt_paged_resize(int* block_tables, long long table_stride, int width, const int* lengths, const int* counts,
+                    int* free_pages, int pool, const int* free_state, long long* slots, int* positions, int* starts,
+                    int* lengths_out, int* free_state_out, int requests, int page_size, int tokens, void* stream);
+
+/* Rotary embedding (pairs (i, i + D/2), angle = positions[r] * inverse[i], taken in 64 bits) of `rows` query and key rows,
+ * and the append of key and value of row r to slot slots[r]; a row whose slot is negative is not appended.  q [rows,
+ * q_heads, head_dim] with `q_stride` elements from row to row, k and v likewise [rows, kv_heads, head_dim]; q_out dense.
+ * bf16 or fp16; head_dim a multiple of 16; addresses 16-byte aligned, strides multiples of 8.  No two rows name one slot. */
+int mt_rope_kv_append_paged(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                            long long v_stride, const float* inverse, const int* positions, const long long* slots,
+                            void* q_out, void* key_pages, const long long* key_strides, void* value_pages,
+                            const long long* value_strides, int rows, int q_heads, int kv_heads, int head_dim, int pages,
+                            int page_size, int type, void* stream);
+
+/* mt_attention_decode over pages: out[b] = softmax(scale * q[b] . K) V over the first lengths[b] tokens that row b of the
+ * block table names; zeros where that is none.  q, out: dense [batch, q_heads, head_dim], bf16 or fp16; head_dim 64, 128
+ * or 256.  A request's bits depend on its own tokens only. */
+size_t mt_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, int width, int page_size);
+int mt_paged_attention_decode(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
+                              const long long* value_strides, const int* block_tables, long long table_stride, int width,
+                              const int* lengths, void* out, void* workspace, size_t workspace_bytes, int batch, int q_heads,
+                              int kv_heads, int head_dim, int pages, int page_size, int type, float scale, void* stream);
+
+/* A step of beam search.  Of the beams * vocabulary candidates of a group, score + log softmax(logits) in 64 bits, the `keep`
+ * (1 ... 64) largest in descending order, the lower beam and then the lower token first among equals.  logits [groups *
+ * beams, vocabulary] bf16, fp16 or fp32, rows `row_stride` elements apart; scores fp32 [groups, beams].  A beam that has
+ * `finished` (bytes, may be NULL) offers end_token alone, at its score.  As -inf count: every candidate of a score
+ * up to -1e15 or of a row with a NaN, with +inf or with nothing above -inf.  parents: the beam within its group;
+ * finished_out: the parent had finished, or the token is end_token (-1: there is none).  beams up to 32. */
+#define MT_BEAM_MAX_ROWS 0x000FFFFF
+#define MT_BEAM_MAX_VOCABULARY 0x00FFFFFF
+size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep);
+int mt_beam_select(const void* logits, long long row_stride, int type, const float* scores, const unsigned char* finished,
+                   long long end_token, float* scores_out, int* parents_out, long long* tokens_out, unsigned char* finished_out,
+                   void* workspace, size_t workspace_bytes, int groups, int beams, int vocabulary, int keep, void* stream);
+
+/* Block tables of [groups * beams] rows follow their parents (int32, within the group): tables_out (dense, another
+ * array) gets the parent's ids of full pages.  The page in work stays one beam's own: a parent's first child goes on in
+ * it, any other child takes the one of a beam without children, into which the tokens of the parent's are copied, in
+ * `caches` caches (HOST arrays of addresses, two-byte elements, head_dim a multiple of 8).  Later entries stay each
+ * row's own.  All beams of a group hold equally many tokens: lengths[row] of the group's first row counts; the pages in work
+ * are distinct. */
+int mt_beam_reorder(const int* block_tables, long long table_stride, int width, const int* lengths, const int* parents,
+                    int* tables_out, void* const* key_pages, const long long* key_strides, void* const* value_pages,
+                    const long long* value_strides, int caches, int groups, int beams, int kv_heads, int head_dim, int pages,
+                    int page_size, void* stream);
+
 /* Sum of bf16 partial results over the GPUs of one node (one process per GPU), for the
  * tensor-parallel form of the fused MLP: the down projection of a K-sharded MLP leaves a partial
  * [M, H] result on every rank.  NO COUNTERPART IN THE REFERENCE, which is single-device.

@@ -29,6 +29,7 @@ _i = ctypes.c_int
 _u = ctypes.c_uint
 _z = ctypes.c_size_t
 _f = ctypes.c_float
+_l = ctypes.c_longlong
 
 SIGNATURES = {
     "mt_version": (_i, []),
@@ -53,6 +54,13 @@ SIGNATURES = {
     "mt_gather_rows": (_i, [_p, _p, _p, _i, ctypes.c_longlong, _i, _p]),
     "mt_rope_kv_prefill": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p]),
     "mt_rope_kv_append": (_i, [_p, _p, _p, ctypes.c_longlong, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p]),
+    "mt_paged_resize": (_i, [_p, _l, _i, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p]),
+    "mt_rope_kv_append_paged": (_i, [_p, _l, _p, _l, _p, _l] + [_p] * 8 + [_i] * 7 + [_p]),
+    "mt_paged_attention_decode_workspace_bytes": (_z, [_i] * 6),
+    "mt_paged_attention_decode": (_i, [_p] * 6 + [_l, _i, _p, _p, _p, _z] + [_i] * 7 + [_f, _p]),
+    "mt_beam_select_workspace_bytes": (_z, [_i] * 4),
+    "mt_beam_select": (_i, [_p, _l, _i, _p, _p, _l, _p, _p, _p, _p, _p, _z, _i, _i, _i, _i, _p]),
+    "mt_beam_reorder": (_i, [_p, _l, _i] + [_p] * 7 + [_i] * 7 + [_p]),
     "mt_peer_group_create": (_i, [_i, _i, _z, ctypes.POINTER(ctypes.c_void_p), _p]),
     "mt_peer_group_connect": (_i, [_p, _p]),
     "mt_peer_group_set_mode": (_i, [_p, _i]),
@@ -115,8 +123,9 @@ def check(code, what):
 
 
 def device_status(reset=True):
-    """(ok, words) -- words[0] != 0 means a bounded device-side wait gave up, or (0x301) that an embedding met a token
-    outside its table: words[1] is the output row, words[2] the token."""
+    """(ok, words) -- words[0] != 0 means a bounded device-side wait gave up, or (0x301 ... 0x305) that a kernel met an
+    index outside its table: words[1] is the row, words[2] the index (0x301 an embedding's token, 0x302 a slot outside the
+    paged cache, 0x303 a page outside it, 0x304 a length its block table has no room for, 0x305 a beam's parent)."""
     words = (ctypes.c_uint * 4)()
     code = load().mt_device_status(words, 1 if reset else 0)
     return code == 0, tuple(int(v) for v in words)

@@ -10,11 +10,13 @@ from .cuda import (  # noqa: F401
     rope_kv_prefill,
     supports_attention_decode,
 )
+from .cuda_beam import beam_reorder, beam_select  # noqa: F401
 from .cuda_affine import MLXAffineWeight, mlx_affine_matmul  # noqa: F401
 from .cuda_dense import (  # noqa: F401
     mlx_dense_residual_qmv,
     mlx_dense_swiglu,
 )
+from .cuda_paged import paged_attention_decode, paged_resize, rope_kv_append_paged  # noqa: F401
 from .cuda_quantized import (  # noqa: F401
     batch_invariant,
     fixed_order,

@@ -24,6 +24,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "../../include/metile_b200.h"
 
 namespace {
@@ -432,6 +435,262 @@ PyObject* embedding(PyObject* const* args) {
     return code_or(code, std::move(out));
 }
 
+// ---- the paged cache and beam search ------------------------------------------------------------------------
+
+inline bool ints_on(const Tensor* t, c10::Device device, int64_t count) {
+    return t && t->device() == device && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() == count;
+}
+
+// A block table int32 [requests, width] whose rows do not overlap: the stride of its rows, or -1.
+inline int64_t table_stride(const Tensor* t) {
+    if (!t || !t->is_cuda() || t->dim() != 2 || t->scalar_type() != at::kInt || t->size(1) < 1) return -1;
+    if (t->size(1) > 1 && t->stride(1) != 1) return -1;
+    if (t->size(0) <= 1) return t->size(1);
+    return t->stride(0) >= t->size(1) ? t->stride(0) : -1;
+}
+
+inline int half_type(const Tensor& t) {
+    return t.scalar_type() == at::kBFloat16 ? MT_TYPE_BF16 : t.scalar_type() == at::kHalf ? MT_TYPE_FP16 : -1;
+}
+
+inline bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
+    if (!c10::GradMode::is_enabled()) return false;
+    for (const Tensor* t : tensors)
+        if (t->requires_grad()) return true;
+    return false;
+}
+
+// Pages [pages, heads, page size, dim] with a dense last dimension, where every element has a place of its own.
+struct Pages {
+    void* base;
+    long long strides[3];
+};
+inline bool pages_of(const Tensor* t, c10::Device device, at::ScalarType type, Pages& pages) {
+    if (!t || t->dim() != 4 || t->device() != device || t->scalar_type() != type || t->numel() == 0 || t->stride(3) != 1) return false;
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return t->stride(a) < t->stride(b); });
+    int64_t extent = t->size(3);  // of what the smaller strides reach
+    for (int i : order) {
+        pages.strides[i] = t->size(i) > 1 ? t->stride(i) : 0;
+        if (t->size(i) == 1) continue;
+        if (t->stride(i) < extent || t->stride(i) % 8) return false;
+        extent += t->stride(i) * (t->size(i) - 1);
+    }
+    pages.base = address(*t);
+    return reinterpret_cast<uintptr_t>(pages.base) % 16 == 0;
+}
+
+inline PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
+    PyObject* tuple = PyTuple_New((Py_ssize_t)tensors.size());
+    if (!tuple) return nullptr;
+    Py_ssize_t i = 0;
+    for (const Tensor& t : tensors) PyTuple_SET_ITEM(tuple, i++, THPVariable_Wrap(t));
+    return tuple;
+}
+
+inline Tensor new_of(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
+    return at::detail::empty_cuda(sizes, type, device, std::nullopt);
+}
+
+// paged_resize(block_tables, lengths, counts, free_pages, free_state, page_size, tokens, advance)
+PyObject* paged_resize(PyObject* const* args) {
+    const Tensor* t[5];
+    for (int i = 0; i < 5; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const long page_size = PyLong_AsLong(args[5]), tokens = PyLong_AsLong(args[6]);
+    const bool advance = args[7] == Py_True;
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    const Tensor &tables = *t[0], &lengths = *t[1], &ring = *t[3], &state = *t[4];
+    const int64_t stride = table_stride(&tables);
+    if (stride < 0 || tokens < 0 || !fits_int(tokens) || !fits_int(page_size)) Py_RETURN_NONE;
+    const auto device = tables.device();
+    const int64_t requests = tables.size(0);
+    if (!ints_on(t[1], device, requests) || !ints_on(t[2], device, requests) || !ints_on(t[3], device, ring.numel()) ||
+        !ints_on(t[4], device, 2) || ring.numel() < 1 || !fits_int(ring.numel()) || !fits_int(requests) || !fits_int(tables.size(1)))
+        Py_RETURN_NONE;
+    const Launch launch(device);
+    Tensor slots = new_of({tokens}, at::kLong, device), positions = new_of({tokens}, at::kInt, device);
+    Tensor starts = new_of({requests + 1}, at::kInt, device);
+    Tensor lengths_out = advance ? lengths : new_of({requests}, at::kInt, device), state_out = advance ? state : new_of({2}, at::kInt, device);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_paged_resize(static_cast<int*>(address(tables)), stride, (int)tables.size(1), static_cast<const int*>(address(lengths)),
+                               static_cast<const int*>(address(*t[2])), static_cast<int*>(address(ring)), (int)ring.numel(),
+                               static_cast<const int*>(address(state)), static_cast<long long*>(address(slots)),
+                               static_cast<int*>(address(positions)), static_cast<int*>(address(starts)),
+                               static_cast<int*>(address(lengths_out)), static_cast<int*>(address(state_out)), (int)requests,
+                               (int)page_size, (int)tokens, launch.stream());
+    }
+    if (code != 0) return PyLong_FromLong(code);
+    return tuple_of({slots, positions, starts, lengths_out, state_out});
+}
+
+// Rows [rows, heads, dim] of dense heads, whose stride is a multiple of 8 elements: that stride, or -1.
+inline int64_t head_rows(const Tensor& t, int64_t dim) {
+    if (t.dim() != 3 || t.size(2) != dim || t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != dim)) return -1;
+    if (reinterpret_cast<uintptr_t>(address(t)) % 16) return -1;
+    if (t.size(0) <= 1) return t.size(1) * dim;
+    return t.stride(0) >= 0 && t.stride(0) % 8 == 0 ? t.stride(0) : -1;
+}
+
+// rope_kv_append_paged(query, key, value, inverse, positions, slots, key_pages, value_pages)
+PyObject* rope_kv_append_paged(PyObject* const* args) {
+    const Tensor* t[8];
+    for (int i = 0; i < 8; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const Tensor &q = *t[0], &k = *t[1], &v = *t[2], &inverse = *t[3], &slots = *t[5], &keys = *t[6], &values = *t[7];
+    if (!q.is_cuda() || q.dim() != 3 || k.dim() != 3 || v.dim() != 3 || keys.dim() != 4 || q.numel() == 0 || k.numel() == 0)
+        Py_RETURN_NONE;
+    const auto device = q.device();
+    const int64_t rows = q.size(0), heads = q.size(1), dim = q.size(2), kv_heads = k.size(1);
+    const int type = half_type(q);
+    Pages key_pages, value_pages;
+    if (type < 0 || wants_gradient({&q, &k, &v, &keys, &values}) || !pages_of(&keys, device, q.scalar_type(), key_pages) ||
+        !pages_of(&values, device, q.scalar_type(), value_pages) || values.sizes() != keys.sizes() || keys.size(1) != kv_heads || keys.size(3) != dim)
+        Py_RETURN_NONE;
+    if (k.size(0) != rows || k.device() != device || v.device() != device || v.sizes() != k.sizes() || k.scalar_type() != q.scalar_type() ||
+        v.scalar_type() != q.scalar_type())
+        Py_RETURN_NONE;
+    const int64_t q_stride = head_rows(q, dim), k_stride = head_rows(k, dim), v_stride = head_rows(v, dim);
+    if (q_stride < 0 || k_stride < 0 || v_stride < 0 || !fits_int(rows) || !fits_int(heads) || !fits_int(dim) || !fits_int(keys.size(0)) ||
+        !fits_int(keys.size(2)))
+        Py_RETURN_NONE;
+    if (inverse.device() != device || inverse.scalar_type() != at::kFloat || !inverse.is_contiguous() || inverse.numel() * 2 != dim ||
+        !ints_on(t[4], device, rows) || slots.device() != device || slots.scalar_type() != at::kLong || !slots.is_contiguous() ||
+        slots.numel() != rows)
+        Py_RETURN_NONE;
+    const Launch launch(device);
+    Tensor out = new_of({rows, heads, dim}, q.scalar_type(), device);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_rope_kv_append_paged(address(q), q_stride, address(k), k_stride, address(v), v_stride,
+                                       static_cast<const float*>(address(inverse)), static_cast<const int*>(address(*t[4])),
+                                       static_cast<const long long*>(address(slots)), address(out), key_pages.base, key_pages.strides,
+                                       value_pages.base, value_pages.strides, (int)rows, (int)heads, (int)kv_heads, (int)dim,
+                                       (int)keys.size(0), (int)keys.size(2), type, launch.stream());
+    }
+    return code_or(code, std::move(out));
+}
+
+// paged_attention_decode(query, key_pages, value_pages, block_tables, lengths, scale)
+PyObject* paged_attention_decode(PyObject* const* args) {
+    const Tensor* t[5];
+    for (int i = 0; i < 5; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const double scale = PyFloat_AsDouble(args[5]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    const Tensor &q = *t[0], &keys = *t[1], &values = *t[2], &tables = *t[3];
+    if (!q.is_cuda() || q.dim() != 3 || keys.dim() != 4 || q.numel() == 0 || !q.is_contiguous()) Py_RETURN_NONE;
+    const auto device = q.device();
+    const int64_t batch = q.size(0), heads = q.size(1), dim = q.size(2), kv_heads = keys.size(1), stride = table_stride(&tables);
+    const int type = half_type(q);
+    Pages key_pages, value_pages;
+    if (type < 0 || stride < 0 || wants_gradient({&q, &keys, &values}) || tables.device() != device || tables.size(0) != batch ||
+        !pages_of(&keys, device, q.scalar_type(), key_pages) || !pages_of(&values, device, q.scalar_type(), value_pages) ||
+        values.sizes() != keys.sizes() || keys.size(3) != dim || !ints_on(t[4], device, batch))
+        Py_RETURN_NONE;
+    if (!fits_int(batch * heads) || !fits_int(dim) || !fits_int(keys.size(0)) || !fits_int(keys.size(2)) || !fits_int(tables.size(1))) Py_RETURN_NONE;
+    const Launch launch(device);
+    Tensor out = new_of({batch, heads, dim}, q.scalar_type(), device);
+    const size_t needed = mt_paged_attention_decode_workspace_bytes((int)batch, (int)heads, (int)kv_heads, (int)dim, (int)tables.size(1),
+                                                                    (int)keys.size(2));
+    c10::DataPtr scratch;
+    if (needed) scratch = call_scratch(needed);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_paged_attention_decode(address(q), key_pages.base, key_pages.strides, value_pages.base, value_pages.strides,
+                                         static_cast<const int*>(address(tables)), stride, (int)tables.size(1),
+                                         static_cast<const int*>(address(*t[4])), address(out), scratch.get(), needed, (int)batch, (int)heads,
+                                         (int)kv_heads, (int)dim, (int)keys.size(0), (int)keys.size(2), type, (float)scale, launch.stream());
+    }
+    return code_or(code, std::move(out));
+}
+
+// beam_select(logits, scores, keep, finished | None, end_token)
+PyObject* beam_select(PyObject* const* args) {
+    const Tensor *logits = plain(args[0]), *scores = plain(args[1]);
+    const Tensor* finished = args[3] == Py_None ? nullptr : plain(args[3]);
+    const long keep = PyLong_AsLong(args[2]), end_token = PyLong_AsLong(args[4]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (!logits || !scores || (args[3] != Py_None && !finished) || !logits->is_cuda() || logits->dim() != 2 || scores->dim() != 2 ||
+        logits->numel() == 0 || wants_gradient({logits, scores}))
+        Py_RETURN_NONE;
+    const auto device = logits->device();
+    const int64_t groups = scores->size(0), beams = scores->size(1), rows = logits->size(0), vocabulary = logits->size(1);
+    const int type = logits->scalar_type() == at::kFloat ? MT_TYPE_FP32 : half_type(*logits);
+    if (type < 0 || rows != groups * beams || (vocabulary > 1 && logits->stride(1) != 1) || (rows > 1 && logits->stride(0) < 0) ||
+        rows > MT_BEAM_MAX_ROWS || vocabulary > MT_BEAM_MAX_VOCABULARY || keep < 1 || keep > 64)
+        Py_RETURN_NONE;
+    if (scores->device() != device || scores->scalar_type() != at::kFloat || !scores->is_contiguous()) Py_RETURN_NONE;
+    if (finished && (finished->device() != device || finished->scalar_type() != at::kBool || !finished->is_contiguous() ||
+                     finished->sizes() != scores->sizes()))
+        Py_RETURN_NONE;
+    const Launch launch(device);
+    Tensor scores_out = new_of({groups, keep}, at::kFloat, device), parents = new_of({groups, keep}, at::kInt, device);
+    Tensor tokens = new_of({groups, keep}, at::kLong, device), finished_out = new_of({groups, keep}, at::kBool, device);
+    const size_t needed = mt_beam_select_workspace_bytes((int)groups, (int)beams, (int)vocabulary, (int)keep);
+    c10::DataPtr scratch;
+    if (needed) scratch = call_scratch(needed);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_beam_select(address(*logits), rows > 1 ? logits->stride(0) : vocabulary, type, static_cast<const float*>(address(*scores)),
+                              finished ? static_cast<const unsigned char*>(address(*finished)) : nullptr, end_token,
+                              static_cast<float*>(address(scores_out)), static_cast<int*>(address(parents)),
+                              static_cast<long long*>(address(tokens)), static_cast<unsigned char*>(address(finished_out)), scratch.get(),
+                              needed, (int)groups, (int)beams, (int)vocabulary, (int)keep, launch.stream());
+    }
+    if (code != 0) return PyLong_FromLong(code);
+    return tuple_of({scores_out, parents, tokens, finished_out});
+}
+
+// beam_reorder(block_tables, lengths, parents, caches: sequence of (key_pages, value_pages))
+PyObject* beam_reorder(PyObject* const* args) {
+    const Tensor *tables = plain(args[0]), *lengths = plain(args[1]), *parents = plain(args[2]);
+    const int64_t stride = table_stride(tables);
+    if (stride < 0 || !parents || parents->dim() != 2 || parents->numel() == 0 || !PyTuple_Check(args[3])) Py_RETURN_NONE;
+    const auto device = tables->device();
+    const int64_t groups = parents->size(0), beams = parents->size(1), rows = tables->size(0), width = tables->size(1);
+    if (rows != groups * beams || !ints_on(lengths, device, rows) || !ints_on(parents, device, rows) || !fits_int(rows) || !fits_int(width))
+        Py_RETURN_NONE;
+    const Py_ssize_t count = PyTuple_GET_SIZE(args[3]);
+    if (count < 1 || !fits_int(count)) Py_RETURN_NONE;
+    std::vector<void*> addresses[2];
+    Pages first[2];
+    const Tensor* sample = nullptr;
+    for (Py_ssize_t c = 0; c < count; ++c) {
+        PyObject* pair = PyTuple_GET_ITEM(args[3], c);
+        if (!PyTuple_Check(pair) || PyTuple_GET_SIZE(pair) != 2) Py_RETURN_NONE;
+        for (int which = 0; which < 2; ++which) {
+            const Tensor* pages = plain(PyTuple_GET_ITEM(pair, which));
+            if (!pages || half_type(*pages) < 0) Py_RETURN_NONE;
+            if (!sample) sample = pages;
+            Pages here;
+            if (!pages_of(pages, device, sample->scalar_type(), here) || pages->sizes() != sample->sizes() || wants_gradient({pages})) Py_RETURN_NONE;
+            if (c == 0) first[which] = here;
+            for (int i = 0; i < 3; ++i)
+                if (here.strides[i] != first[which].strides[i]) Py_RETURN_NONE;
+            addresses[which].push_back(here.base);
+        }
+    }
+    for (int i = 0; i < 4; ++i)
+        if (!fits_int(sample->size(i))) Py_RETURN_NONE;
+    const Launch launch(device);
+    Tensor out = new_of({rows, width}, at::kInt, device);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_beam_reorder(static_cast<const int*>(address(*tables)), stride, (int)width, static_cast<const int*>(address(*lengths)),
+                               static_cast<const int*>(address(*parents)), static_cast<int*>(address(out)), addresses[0].data(),
+                               first[0].strides, addresses[1].data(), first[1].strides, (int)count, (int)groups, (int)beams,
+                               (int)sample->size(1), (int)sample->size(3), (int)sample->size(0), (int)sample->size(2), launch.stream());
+    }
+    return code_or(code, std::move(out));
+}
+
 template <PyObject* (*kBody)(PyObject* const*), Py_ssize_t kCount>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
     try {
@@ -447,7 +706,9 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(entry<name, count>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MT_METHOD(project, 8), MT_METHOD(swiglu, 8), MT_METHOD(mlp_plan, 9), MT_METHOD(mlp, 4), MT_METHOD(norm, 4),
                          MT_METHOD(dense, 4), MT_METHOD(attention, 5), MT_METHOD(rope_kv_append, 8), MT_METHOD(rope_kv_prefill, 8),
-                         MT_METHOD(greedy_token, 2), MT_METHOD(embedding, 2), {nullptr, nullptr, 0, nullptr}};
+                         MT_METHOD(greedy_token, 2), MT_METHOD(embedding, 2),
+                         MT_METHOD(paged_resize, 8), MT_METHOD(rope_kv_append_paged, 8), MT_METHOD(paged_attention_decode, 6),
+                         MT_METHOD(beam_select, 5), MT_METHOD(beam_reorder, 4), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

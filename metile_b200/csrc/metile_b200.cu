@@ -10,6 +10,9 @@
 #include "affine_umma.cuh"
 #include "affine_mlp_fused.cuh"
 #include "gather_rows.cuh"
+#include "paged_cache.cuh"
+#include "paged_attention.cuh"
+#include "beam_select.cuh"
 #include <string.h>
 
 #include "common.cuh"
@@ -282,7 +285,8 @@ int mt_device_status(unsigned int words[4], int reset) {
         // A single-launch MLP that gave up may have left its slot's counter and flags as no other launch expects them.
         if (words[0] && !clear_meeting_places()) return MT_ERR_LAUNCH;
     }
-    return words[0] == kGatherIndexOutside ? MT_ERR_INDEX : words[0] ? MT_ERR_DEVICE_WAIT : MT_OK;
+    const bool index = words[0] == kGatherIndexOutside || (words[0] >= kSlotOutside && words[0] <= kParentOutside);
+    return index ? MT_ERR_INDEX : words[0] ? MT_ERR_DEVICE_WAIT : MT_OK;
 }
 
 int mt_selftest_bounded_wait(int which, unsigned int limit_us, void* stream) {
@@ -682,6 +686,211 @@ int mt_rope_kv_prefill(const void* q, const void* k, const void* v, const float*
     const cudaError_t rc = vector ? cudaLaunchKernelEx(&config, rope_kv_prefill_kernel<true>, params)
                                   : cudaLaunchKernelEx(&config, rope_kv_prefill_kernel<false>, params);
     return rc == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+}
+
+// log2 of a page size the paged kernels take, or -1.
+static int page_shift_of(int page_size) {
+    for (int shift = 3; shift <= 8; ++shift)
+        if (page_size == 1 << shift) return shift;
+    return -1;
+}
+
+// Strides of a cache in pages: rows of 16-byte vectors that start on 16 bytes.
+static bool page_strides_of(const long long* given, PageStrides& strides) {
+    strides = {given[0], given[1], given[2]};
+    return given[0] >= 0 && given[1] >= 0 && given[2] >= 0 && given[0] % 8 == 0 && given[1] % 8 == 0 && given[2] % 8 == 0;
+}
+
+static cudaLaunchConfig_t dependent_launch(dim3 grid, int threads, size_t smem, void* stream, cudaLaunchAttribute* attribute) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads, 1, 1);
+    config.dynamicSmemBytes = smem;
+    config.stream = static_cast<cudaStream_t>(stream);
+    attribute->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute->val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    return config;
+}
+
+int mt_paged_resize(int* block_tables, long long table_stride, int width, const int* lengths, const int* counts,
+                    int* free_pages, int pool, const int* free_state, long long* slots, int* positions, int* starts,
+                    int* lengths_out, int* free_state_out, int requests, int page_size, int tokens, void* stream) {
+    const int shift = page_shift_of(page_size);
+    if (requests < 0 || tokens < 0 || width < 1 || pool < 1 || shift < 0 || table_stride < width) return MT_ERR_SHAPE;
+    if (!starts || !free_state || !free_state_out) return MT_ERR_NULL;
+    if (requests > 0 && (!block_tables || !lengths || !counts || !free_pages || !lengths_out)) return MT_ERR_NULL;
+    if (tokens > 0 && (!slots || !positions)) return MT_ERR_NULL;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    ResizeParams params{block_tables, lengths, counts, free_pages, free_state, slots, positions, starts, lengths_out,
+                        free_state_out, table_stride, width, pool, requests, shift, tokens};
+    cudaLaunchAttribute attribute;
+    const cudaLaunchConfig_t config = dependent_launch(dim3(1, 1, 1), kResizeThreads, 0, stream, &attribute);
+    return cudaLaunchKernelEx(&config, paged_resize_kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+}
+
+int mt_rope_kv_append_paged(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                            long long v_stride, const float* inverse, const int* positions, const long long* slots,
+                            void* q_out, void* key_pages, const long long* key_strides, void* value_pages,
+                            const long long* value_strides, int rows, int q_heads, int kv_heads, int head_dim, int pages,
+                            int page_size, int type, void* stream) {
+    const int shift = page_shift_of(page_size);
+    RopeAppendPagedParams params;
+    if (rows < 0 || q_heads < 1 || kv_heads < 1 || head_dim < 16 || head_dim % 16 || head_dim > 4096 || pages < 1 || shift < 0)
+        return MT_ERR_SHAPE;
+    if ((type != MT_TYPE_BF16 && type != MT_TYPE_FP16) || (long long)q_heads + 2ll * kv_heads > 0x7FFFFFFF / head_dim) return MT_ERR_SHAPE;
+    if (rows == 0) return MT_OK;
+    if (!q || !k || !v || !inverse || !positions || !slots || !q_out || !key_pages || !value_pages || !key_strides || !value_strides)
+        return MT_ERR_NULL;
+    for (const void* pointer : {q, k, v, (const void*)q_out, (const void*)key_pages, (const void*)value_pages})
+        if (!aligned_to(pointer, 16)) return MT_ERR_ALIGN;
+    if (q_stride % 8 || k_stride % 8 || v_stride % 8 || !page_strides_of(key_strides, params.key_strides) ||
+        !page_strides_of(value_strides, params.value_strides))
+        return MT_ERR_ALIGN;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    params.q = static_cast<const uint16_t*>(q);
+    params.k = static_cast<const uint16_t*>(k);
+    params.v = static_cast<const uint16_t*>(v);
+    params.inverse = inverse;
+    params.positions = positions;
+    params.slots = slots;
+    params.q_out = static_cast<uint16_t*>(q_out);
+    params.key_pages = static_cast<uint16_t*>(key_pages);
+    params.value_pages = static_cast<uint16_t*>(value_pages);
+    params.q_stride = q_stride;
+    params.k_stride = k_stride;
+    params.v_stride = v_stride;
+    params.slot_count = (long long)pages << shift;
+    params.q_heads = q_heads;
+    params.kv_heads = kv_heads;
+    params.head_dim = head_dim;
+    params.page_shift = shift;
+    cudaLaunchAttribute attribute;
+    const cudaLaunchConfig_t config = dependent_launch(dim3(rows, 1, 1), kRopePagedThreads, head_dim * sizeof(float), stream, &attribute);
+    const cudaError_t rc = type == MT_TYPE_FP16 ? cudaLaunchKernelEx(&config, rope_kv_append_paged_kernel<true>, params)
+                                                : cudaLaunchKernelEx(&config, rope_kv_append_paged_kernel<false>, params);
+    return rc == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+}
+
+size_t mt_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, int width, int page_size) {
+    (void)batch, (void)q_heads, (void)kv_heads, (void)head_dim, (void)width, (void)page_size;
+    return 0;
+}
+
+int mt_paged_attention_decode(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
+                              const long long* value_strides, const int* block_tables, long long table_stride, int width,
+                              const int* lengths, void* out, void* workspace, size_t workspace_bytes, int batch, int q_heads,
+                              int kv_heads, int head_dim, int pages, int page_size, int type, float scale, void* stream) {
+    const int shift = page_shift_of(page_size);
+    PagedAttentionParams params;
+    if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || width < 1 || pages < 1 || shift < 0 || table_stride < width)
+        return MT_ERR_SHAPE;
+    if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || (type != MT_TYPE_BF16 && type != MT_TYPE_FP16)) return MT_ERR_SHAPE;
+    if ((long long)batch * q_heads > 0x7FFFFFFF || (long long)width << shift > 0x7FFFFFFF) return MT_ERR_SHAPE;
+    if (batch == 0) return MT_OK;
+    if (!q || !key_pages || !value_pages || !key_strides || !value_strides || !block_tables || !lengths || !out) return MT_ERR_NULL;
+    if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 16) ||
+        !page_strides_of(key_strides, params.key_strides) || !page_strides_of(value_strides, params.value_strides))
+        return MT_ERR_ALIGN;
+    const size_t needed = mt_paged_attention_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim, width, page_size);
+    if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    params.q = static_cast<const uint16_t*>(q);
+    params.key_pages = static_cast<const uint16_t*>(key_pages);
+    params.value_pages = static_cast<const uint16_t*>(value_pages);
+    params.tables = block_tables;
+    params.lengths = lengths;
+    params.out = static_cast<uint16_t*>(out);
+    params.partial = static_cast<float*>(workspace);
+    params.table_stride = table_stride;
+    params.width = width;
+    params.batch = batch;
+    params.q_heads = q_heads;
+    params.kv_heads = kv_heads;
+    params.page_shift = shift;
+    params.page_count = pages;
+    params.scale = scale;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool half = type == MT_TYPE_FP16;
+    if (head_dim == 64) return half ? launch_paged_attention<64, true>(params, s) : launch_paged_attention<64, false>(params, s);
+    if (head_dim == 128) return half ? launch_paged_attention<128, true>(params, s) : launch_paged_attention<128, false>(params, s);
+    return half ? launch_paged_attention<256, true>(params, s) : launch_paged_attention<256, false>(params, s);
+}
+
+size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep) {
+    (void)groups, (void)beams, (void)vocabulary, (void)keep;
+    return 0;
+}
+
+int mt_beam_select(const void* logits, long long row_stride, int type, const float* scores, const unsigned char* finished,
+                   long long end_token, float* scores_out, int* parents_out, long long* tokens_out, unsigned char* finished_out,
+                   void* workspace, size_t workspace_bytes, int groups, int beams, int vocabulary, int keep, void* stream) {
+    if (groups < 0 || beams < 1 || beams > kBeamMaxBeams || vocabulary < 1 || vocabulary > MT_BEAM_MAX_VOCABULARY || keep < 1 ||
+        keep > kBeamMaxKeep || keep > (long long)beams * vocabulary || (long long)groups * beams > MT_BEAM_MAX_ROWS)
+        return MT_ERR_SHAPE;
+    if ((type != MT_TYPE_BF16 && type != MT_TYPE_FP16 && type != MT_TYPE_FP32) || row_stride < 0) return MT_ERR_SHAPE;
+    if (finished ? end_token < 0 || end_token >= vocabulary : end_token < -1 || end_token >= vocabulary) return MT_ERR_SHAPE;
+    if (groups == 0) return MT_OK;
+    if (!logits || !scores || !scores_out || !parents_out || !tokens_out || !finished_out) return MT_ERR_NULL;
+    if (!aligned_to(logits, type == MT_TYPE_FP32 ? 4 : 2)) return MT_ERR_ALIGN;
+    const size_t needed = mt_beam_select_workspace_bytes(groups, beams, vocabulary, keep);
+    if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    BeamSelectParams params{logits, scores, finished, scores_out, parents_out, tokens_out, finished_out, row_stride, end_token,
+                            groups, beams, vocabulary, keep, type};
+    cudaLaunchAttribute attribute;
+    const cudaLaunchConfig_t config = dependent_launch(dim3(groups, 1, 1), 1024, 0, stream, &attribute);
+    return cudaLaunchKernelEx(&config, beam_select_kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+}
+
+int mt_beam_reorder(const int* block_tables, long long table_stride, int width, const int* lengths, const int* parents,
+                    int* tables_out, void* const* key_pages, const long long* key_strides, void* const* value_pages,
+                    const long long* value_strides, int caches, int groups, int beams, int kv_heads, int head_dim, int pages,
+                    int page_size, void* stream) {
+    const int shift = page_shift_of(page_size);
+    ReorderParams params;
+    if (groups < 0 || beams < 1 || beams > kReorderMaxBeams || width < 1 || table_stride < width || caches < 0 || kv_heads < 1 ||
+        head_dim < 8 || head_dim % 8 || pages < 1 || shift < 0)
+        return MT_ERR_SHAPE;
+    if ((long long)groups * beams > 0x7FFFFFFF || (long long)kv_heads * head_dim > 0x7FFFFFFF >> shift) return MT_ERR_SHAPE;
+    if (groups == 0) return MT_OK;
+    if (!block_tables || !lengths || !parents || !tables_out || (caches > 0 && (!key_pages || !value_pages || !key_strides || !value_strides)))
+        return MT_ERR_NULL;
+    if (tables_out == block_tables) return MT_ERR_SHAPE;  // rows are read after others have been written
+    for (int c = 0; c < caches; ++c) {
+        if (!key_pages[c] || !value_pages[c]) return MT_ERR_NULL;
+        if (!aligned_to(key_pages[c], 16) || !aligned_to(value_pages[c], 16)) return MT_ERR_ALIGN;
+    }
+    params.key_strides = params.value_strides = {0, 0, 0};
+    if (caches > 0 && (!page_strides_of(key_strides, params.key_strides) || !page_strides_of(value_strides, params.value_strides)))
+        return MT_ERR_ALIGN;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    params.tables = block_tables;
+    params.lengths = lengths;
+    params.parents = parents;
+    params.tables_out = tables_out;
+    params.table_stride = table_stride;
+    params.width = width;
+    params.beams = beams;
+    params.kv_heads = kv_heads;
+    params.head_dim = head_dim;
+    params.page_shift = shift;
+    params.page_count = pages;
+    // A launch takes the addresses of up to 64 caches; the first one writes the tables too.
+    for (int first = 0; first == 0 || first < caches; first += kReorderMaxCaches) {
+        const int here = caches - first < kReorderMaxCaches ? caches - first : kReorderMaxCaches;
+        for (int c = 0; c < here; ++c) {
+            params.pages[c] = static_cast<uint16_t*>(key_pages[first + c]);
+            params.pages[kReorderMaxCaches + c] = static_cast<uint16_t*>(value_pages[first + c]);
+        }
+        params.caches = here;
+        params.first_cache = first;
+        cudaLaunchAttribute attribute;
+        const cudaLaunchConfig_t config = dependent_launch(dim3(groups * beams, 1 + here, 1), kReorderThreads, 0, stream, &attribute);
+        if (cudaLaunchKernelEx(&config, beam_reorder_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    }
+    return MT_OK;
 }
 
 int mt_dense_rows(const void* x, const void* w, const void* residual, void* out, int M, int K, int N, void* stream) {

@@ -1,0 +1,372 @@
+// A key-value cache in pages: block tables and slot maps on the GPU, the rotary embedding with its append to the
+// pages, and the reordering of beams.
+//
+// A pool holds `pages` pages of `page_size` tokens (a power of two) for every layer; row r of a block table names the
+// pages of request r in order, so that token p of it lies in slot table[r][p / page_size] * page_size + p % page_size.
+// The ids of the pages no request uses stand in a ring: they are taken at its head and given back at its tail, so the
+// entries one call reads and the entries it writes are never the same, and a call with the same state does the same again.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace mt {
+
+constexpr unsigned int kSlotOutside = 0x302;    // rope_kv_append_paged: word 1 = row, 2 and 3 = the slot
+constexpr unsigned int kPageOutside = 0x303;    // a block table names a page outside the pool: word 1 = its row, 2 = the page
+constexpr unsigned int kLengthOutside = 0x304;  // a length the block table has no room for: word 1 = its row, 2 = the length
+constexpr unsigned int kParentOutside = 0x305;  // beam_reorder: word 1 = row, 2 = the parent
+
+__device__ __forceinline__ void record_index(unsigned int code, unsigned int where, unsigned long long value) {
+    if (atomicCAS(&g_device_status[0], 0u, code) == 0u) {
+        g_device_status[1] = where;
+        g_device_status[2] = (unsigned int)value;
+        g_device_status[3] = (unsigned int)(value >> 32);
+    }
+}
+
+struct PageStrides {
+    long long page, head, token;  // elements
+};
+
+// ---------------------------------------------------------------------------------------------
+// Requests grow and shrink: counts[r] > 0 tokens are added to request r, -counts[r] taken from its end.
+struct ResizeParams {
+    int* tables;              // [requests, width], rows `table_stride` apart
+    const int* lengths;       // [requests]
+    const int* counts;        // [requests]
+    int* ring;                // [pool] free page ids
+    const int* state;         // [2]: first free entry of the ring, how many there are
+    long long* slots;         // [tokens]
+    int* positions;           // [tokens]
+    int* starts;              // [requests + 1]
+    int* lengths_out;         // [requests], may be `lengths`
+    int* state_out;           // [2], may be `state`
+    long long table_stride;
+    int width, pool, requests, page_shift, tokens;
+};
+
+constexpr int kResizeThreads = 1024;
+
+// Inclusive sum over the block of three numbers at once; `scratch` holds 3 x 32.
+__device__ __forceinline__ void block_scan3(long long& a, long long& b, long long& c, long long (*scratch)[32]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    auto warp_scan = [&](long long v) {
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const long long other = __shfl_up_sync(0xFFFFFFFFu, v, offset);
+            if (lane >= offset) v += other;
+        }
+        return v;
+    };
+    a = warp_scan(a);
+    b = warp_scan(b);
+    c = warp_scan(c);
+    if (lane == 31) {
+        scratch[0][warp] = a;
+        scratch[1][warp] = b;
+        scratch[2][warp] = c;
+    }
+    __syncthreads();
+    if (warp < 3) {
+        const long long v = lane < warps ? scratch[warp][lane] : 0;
+        scratch[warp][lane] = warp_scan(v) - v;
+    }
+    __syncthreads();
+    a += scratch[0][warp];
+    b += scratch[1][warp];
+    c += scratch[2][warp];
+    __syncthreads();
+}
+
+// The last i in [0, n) with starts[i] <= value, where starts[0] <= value and starts ascends.
+__device__ __forceinline__ int last_not_above(const long long* starts, int n, long long value) {
+    int low = 0, high = n;
+    while (high - low > 1) {
+        const int middle = (low + high) >> 1;
+        if (starts[middle] <= value) low = middle; else high = middle;
+    }
+    return low;
+}
+
+// One CTA takes the requests 1024 at a time, in order.  Three sums run along them: tokens added, pages asked for, pages
+// given back.  Then tokens, granted and returned pages are dealt to the threads, each of which looks its request up.
+__global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const ResizeParams p) {
+    __shared__ long long token_start[kResizeThreads], grant_start[kResizeThreads], free_start[kResizeThreads];
+    __shared__ int held[kResizeThreads], added[kResizeThreads];
+    __shared__ unsigned char is_served[kResizeThreads];
+    __shared__ long long scratch[3][32];
+    __shared__ long long totals[3];
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const int page = 1 << p.page_shift;
+    // The ring's state as a caller may have it: kept within the ring whatever it says.
+    int first = p.state[0], available = p.state[1];
+    if (first < 0 || first >= p.pool) first = 0;
+    available = max(0, min(available, p.pool));
+    const long long room = (long long)p.width << p.page_shift;
+    auto wrapped = [&](long long taken) {  // of fewer entries than the ring has
+        const long long at = first + taken;
+        return at < p.pool ? at : at - p.pool;
+    };
+    long long tokens_before = 0, asked_before = 0, granted_before = 0, freed_before = 0;
+    for (int base = 0; base < p.requests; base += kResizeThreads) {
+        const int r = base + threadIdx.x, here = min(kResizeThreads, p.requests - base);
+        const bool exists = r < p.requests;
+        const int length = exists ? p.lengths[r] : 0, count = exists ? p.counts[r] : 0;
+        const long long after = (long long)length + count;
+        bool valid = length >= 0 && after >= 0 && length <= room && after <= room;
+        const long long old_blocks = ((long long)length + page - 1) >> p.page_shift;
+        const long long new_blocks = (after + page - 1) >> p.page_shift;
+        // First the tokens alone: whether they fit the map decides which requests ask for pages.
+        long long ends = max(count, 0), unused0 = 0, unused1 = 0;
+        block_scan3(ends, unused0, unused1, scratch);
+        ends += tokens_before;
+        valid = valid && (count <= 0 || ends <= p.tokens);
+        const long long need = valid ? max(0ll, new_blocks - old_blocks) : 0, back = valid ? max(0ll, old_blocks - new_blocks) : 0;
+        long long reach = need, unused2 = 0, returned = back;
+        block_scan3(reach, unused2, returned, scratch);
+        reach += asked_before;
+        // In order and without overtaking: once the free pages do not reach, nobody behind is given any.
+        const bool served = valid && (need == 0 || reach <= available);
+        token_start[threadIdx.x] = ends - max(count, 0);
+        grant_start[threadIdx.x] = reach - need;
+        free_start[threadIdx.x] = returned - back + freed_before;
+        held[threadIdx.x] = length;
+        added[threadIdx.x] = count;
+        is_served[threadIdx.x] = served;
+        if (exists) p.starts[r] = (int)min(ends - max(count, 0), 0x7FFFFFFFll);
+        if (threadIdx.x == kResizeThreads - 1) {
+            totals[0] = ends;
+            totals[1] = reach;
+            totals[2] = returned + freed_before;
+        }
+        __syncthreads();
+        const long long tokens_here = min((long long)p.tokens, totals[0]), asked_here = min((long long)available, totals[1]);
+        for (long long t = tokens_before + threadIdx.x; t < tokens_here; t += kResizeThreads) {
+            const int i = last_not_above(token_start, here, t);
+            long long slot = -1, position = 0;
+            if (is_served[i]) {
+                position = held[i] + (t - token_start[i]);
+                const long long block = position >> p.page_shift;
+                const long long fresh = block - (((long long)held[i] + page - 1) >> p.page_shift);
+                const int id = fresh < 0 ? p.tables[(base + i) * p.table_stride + block] : p.ring[wrapped(grant_start[i] + fresh)];
+                slot = id < 0 ? -1 : ((long long)id << p.page_shift) + (position & (page - 1));
+            }
+            p.slots[t] = slot;
+            p.positions[t] = (int)position;
+        }
+        for (long long g = asked_before + threadIdx.x; g < asked_here; g += kResizeThreads) {
+            const int i = last_not_above(grant_start, here, g);
+            if (!is_served[i]) continue;
+            const long long block = (((long long)held[i] + page - 1) >> p.page_shift) + (g - grant_start[i]);
+            p.tables[(base + i) * p.table_stride + block] = p.ring[wrapped(g)];
+        }
+        for (long long f = freed_before + threadIdx.x; f < totals[2]; f += kResizeThreads) {
+            const int i = last_not_above(free_start, here, f);
+            const long long block = (((long long)held[i] + added[i] + page - 1) >> p.page_shift) + (f - free_start[i]);
+            p.ring[((long long)first + available + f) % p.pool] = p.tables[(base + i) * p.table_stride + block];
+        }
+        long long granted = served ? need : 0, unused3 = 0, unused4 = 0;
+        block_scan3(granted, unused3, unused4, scratch);
+        if (exists) p.lengths_out[r] = served ? (int)after : length;
+        tokens_before = totals[0];
+        asked_before = totals[1];
+        freed_before = totals[2];
+        __syncthreads();
+        if (threadIdx.x == kResizeThreads - 1) totals[0] = granted;
+        __syncthreads();
+        granted_before += totals[0];
+        __syncthreads();
+    }
+    for (long long t = tokens_before + threadIdx.x; t < p.tokens; t += kResizeThreads) {
+        p.slots[t] = -1;
+        p.positions[t] = 0;
+    }
+    if (threadIdx.x == 0) {
+        p.starts[p.requests] = (int)min(tokens_before, 0x7FFFFFFFll);
+        p.state_out[0] = (int)((first + granted_before) % p.pool);
+        p.state_out[1] = (int)min((long long)p.pool, available - granted_before + freed_before);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Rotary embedding of the rows of a ragged batch (half-split pairs (i, i + D/2)) and their append to the pages: the
+// keys rotated, the values as they are, each row to its slot.  The angle position * inverse[i] is taken in 64 bits and
+// reduced to a turn there: in 32 bits a position of 100000 leaves it 0.004 off.  Sine and cosine are those of 32 bits.
+struct RopeAppendPagedParams {
+    const uint16_t *q, *k, *v;            // [rows, heads, D], rows `q_stride` ... elements apart
+    const float* inverse;                 // [D / 2]
+    const int* positions;                 // [rows]
+    const long long* slots;               // [rows]; negative: the row has none
+    uint16_t* q_out;                      // [rows, Hq, D]
+    uint16_t *key_pages, *value_pages;
+    PageStrides key_strides, value_strides;
+    long long q_stride, k_stride, v_stride, slot_count;
+    int q_heads, kv_heads, head_dim, page_shift;
+};
+
+template <bool kHalf>
+__device__ __forceinline__ float2 unpack_pair(uint32_t pair) {
+    if constexpr (kHalf) return __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    else return make_float2(bf16_lo(pair), bf16_hi(pair));
+}
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack_pair(float low, float high) {
+    if constexpr (kHalf) {
+        const __half2 pair = __floats2half2_rn(low, high);
+        return *reinterpret_cast<const uint32_t*>(&pair);
+    } else {
+        return pack_bf16x2(low, high);
+    }
+}
+
+constexpr int kRopePagedThreads = 128;
+
+template <bool kHalf>
+__global__ void __launch_bounds__(kRopePagedThreads) rope_kv_append_paged_kernel(const RopeAppendPagedParams p) {
+    extern __shared__ float rope_angles[];  // cosines, then sines
+    const int row = blockIdx.x, dim = p.head_dim, half = dim >> 1;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const double position = (double)p.positions[row];
+    long long slot = p.slots[row];
+    for (int i = threadIdx.x; i < half; i += blockDim.x) {
+        // In half turns: sin(pi x) has the period 2, which is taken off exactly.
+        const double turns = position * (double)p.inverse[i] * 0.31830988618379067154;
+        sincospif((float)(turns - 2.0 * rint(0.5 * turns)), &rope_angles[half + i], &rope_angles[i]);
+    }
+    if (slot >= p.slot_count) {
+        if (threadIdx.x == 0) record_index(kSlotOutside, row, slot);
+        slot = -1;
+    }
+    const long long page = slot >> p.page_shift, token = slot & ((1 << p.page_shift) - 1);
+    __syncthreads();
+    const int units = half / 8;  // threads of a head, eight pairs each
+    for (int at = threadIdx.x; at < (p.q_heads + 2 * p.kv_heads) * units; at += blockDim.x) {
+        int head = at / units;
+        const int i = (at - head * units) * 8;
+        const uint16_t* from;
+        uint16_t* to;
+        bool rotated = true;
+        if (head < p.q_heads) {
+            from = p.q + row * p.q_stride + (long long)head * dim;
+            to = p.q_out + ((long long)row * p.q_heads + head) * dim;
+        } else {
+            if (slot < 0) continue;
+            head -= p.q_heads;
+            rotated = head < p.kv_heads;
+            if (rotated) {
+                from = p.k + row * p.k_stride + (long long)head * dim;
+                to = p.key_pages + page * p.key_strides.page + head * p.key_strides.head + token * p.key_strides.token;
+            } else {
+                head -= p.kv_heads;
+                from = p.v + row * p.v_stride + (long long)head * dim;
+                to = p.value_pages + page * p.value_strides.page + head * p.value_strides.head + token * p.value_strides.token;
+            }
+        }
+        const uint4 a = ptx::ld_global_dependent_u4(from + i), z = ptx::ld_global_dependent_u4(from + i + half);
+        uint4 low = a, high = z;
+        if (rotated) {
+            const uint32_t first[4] = {a.x, a.y, a.z, a.w}, second[4] = {z.x, z.y, z.z, z.w};
+            uint32_t l[4], h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 x = unpack_pair<kHalf>(first[j]), y = unpack_pair<kHalf>(second[j]);
+                const float c0 = rope_angles[i + 2 * j], s0 = rope_angles[half + i + 2 * j];
+                const float c1 = rope_angles[i + 2 * j + 1], s1 = rope_angles[half + i + 2 * j + 1];
+                l[j] = pack_pair<kHalf>(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
+                h[j] = pack_pair<kHalf>(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
+            }
+            low = make_uint4(l[0], l[1], l[2], l[3]);
+            high = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        *reinterpret_cast<uint4*>(to + i) = low;
+        *reinterpret_cast<uint4*>(to + i + half) = high;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Block tables follow the surviving beams.  All beams of a group hold equally many tokens.  A page that is full is never
+// written again, so children share it with their parent: only its id is copied.  The page in work belongs to one beam:
+// the first child of a parent goes on in its page, every further child gets the page of a beam without children and a
+// copy of what is in its parent's.  So as many pages are copied as there are parents missing, and none is allocated.
+constexpr int kReorderMaxBeams = 32, kReorderMaxCaches = 64, kReorderThreads = 256;
+
+struct ReorderParams {
+    const int* tables;        // [groups * beams, width]
+    const int* lengths;       // [groups * beams]
+    const int* parents;       // [groups * beams], within the group
+    int* tables_out;          // [groups * beams, width], dense
+    uint16_t* pages[2 * kReorderMaxCaches];  // keys of every cache, then values
+    PageStrides key_strides, value_strides;
+    long long table_stride;
+    int width, beams, caches, kv_heads, head_dim, page_shift, page_count, first_cache;
+};
+
+// CTA (row, y): y = 0 writes the row's table, y = 1 + c copies cache c's keys and values.
+__global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
+    const int row = blockIdx.x, group = row / p.beams, k = row - group * p.beams, base = group * p.beams;
+    const int lane = threadIdx.x & 31;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    // Every warp has the group's parents, one in a lane.
+    int parent = lane;
+    if (lane < p.beams) {
+        parent = p.parents[base + lane];
+        if (parent < 0 || parent >= p.beams) {  // recorded, and taken as its own
+            if (lane == k && threadIdx.x < 32 && blockIdx.y == 0) record_index(kParentOutside, row, (unsigned int)parent);
+            parent = lane;
+        }
+    }
+    const int length = p.lengths[base];
+    const long long capacity = (long long)p.width << p.page_shift;
+    if ((length < 0 || length > capacity) && threadIdx.x == 0 && blockIdx.y == 0) record_index(kLengthOutside, base, (unsigned int)length);
+    const int held = (int)max(0ll, min((long long)length, capacity));
+    const int block = held >> p.page_shift, part = held & ((1 << p.page_shift) - 1);
+    // Lanes of a parent's first children, and the beams that have none.
+    const unsigned int all = p.beams == 32 ? 0xFFFFFFFFu : (1u << p.beams) - 1u;
+    const unsigned int firsts = __ballot_sync(0xFFFFFFFFu, __ffs(__match_any_sync(0xFFFFFFFFu, parent)) - 1 == lane) & all;
+    unsigned int childless = all & ~__reduce_or_sync(0xFFFFFFFFu, lane < p.beams ? 1u << parent : 0u);
+    const int mine = __shfl_sync(0xFFFFFFFFu, parent, k);
+    const bool first = firsts >> k & 1u;
+    int owner = mine;       // whose page in work this beam gets
+    if (!first) {
+        // As many children are not the first of theirs as there are beams without any.
+        for (int skip = __popc(all & ~firsts & ((1u << k) - 1u)); skip > 0; --skip) childless &= childless - 1u;
+        owner = __ffs(childless) - 1;
+    }
+    const int* from = p.tables + (base + mine) * p.table_stride;
+    const int* own = p.tables + (long long)row * p.table_stride;
+    if (blockIdx.y == 0 && p.first_cache == 0) {
+        int* to = p.tables_out + (long long)row * p.width;
+        for (int j = threadIdx.x; j < p.width; j += blockDim.x) {
+            int id = j < block ? from[j] : own[j];
+            if (j == block && part > 0) id = p.tables[(base + owner) * p.table_stride + j];
+            to[j] = id;
+        }
+    }
+    if (blockIdx.y == 0 || first || part == 0) return;
+    const int source = from[block], target = p.tables[(base + owner) * p.table_stride + block];
+    if (source < 0 || source >= p.page_count || target < 0 || target >= p.page_count) {
+        if (threadIdx.x == 0) record_index(kPageOutside, row, (unsigned int)(source < 0 || source >= p.page_count ? source : target));
+        return;
+    }
+    const int vectors = p.head_dim / 8, count = p.kv_heads * part * vectors;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        uint16_t* pages = p.pages[which * kReorderMaxCaches + blockIdx.y - 1];
+        const PageStrides strides = which ? p.value_strides : p.key_strides;
+        for (int at = threadIdx.x; at < count; at += blockDim.x) {
+            const int head = at / (part * vectors), rest = at - head * part * vectors;
+            const int token = rest / vectors, i = (rest - token * vectors) * 8;
+            const long long offset = head * strides.head + token * strides.token + i;
+            *reinterpret_cast<uint4*>(pages + target * strides.page + offset) =
+                ptx::ld_global_dependent_u4(pages + source * strides.page + offset);
+        }
+    }
+}
+
+}  // namespace mt
