@@ -774,8 +774,9 @@ int mt_rope_kv_append_paged(const void* q, long long q_stride, const void* k, lo
 }
 
 size_t mt_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, int width, int page_size) {
-    (void)batch, (void)q_heads, (void)kv_heads, (void)head_dim, (void)width, (void)page_size;
-    return 0;
+    (void)kv_heads;
+    if (batch <= 0 || q_heads <= 0 || head_dim <= 0 || width <= 0 || page_size <= 0) return 0;
+    return paged_attention_workspace_bytes(batch, q_heads, head_dim, (long long)width * page_size);
 }
 
 int mt_paged_attention_decode(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
@@ -787,7 +788,8 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
     if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || width < 1 || pages < 1 || shift < 0 || table_stride < width)
         return MT_ERR_SHAPE;
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || (type != MT_TYPE_BF16 && type != MT_TYPE_FP16)) return MT_ERR_SHAPE;
-    if ((long long)batch * q_heads > 0x7FFFFFFF || (long long)width << shift > 0x7FFFFFFF) return MT_ERR_SHAPE;
+    // Units of work (a split of a KV head, 16 query heads at once) are counted in 32 bits.
+    if ((long long)batch * q_heads > 0x7FFFFFFF / kPagedMostSplits || (long long)width << shift > 0x7FFFFFFF) return MT_ERR_SHAPE;
     if (batch == 0) return MT_OK;
     if (!q || !key_pages || !value_pages || !key_strides || !value_strides || !block_tables || !lengths || !out) return MT_ERR_NULL;
     if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 16) ||
@@ -802,7 +804,9 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
     params.tables = block_tables;
     params.lengths = lengths;
     params.out = static_cast<uint16_t*>(out);
+    params.most_splits = paged_most_splits((long long)width << shift);
     params.partial = static_cast<float*>(workspace);
+    params.stats = reinterpret_cast<float2*>(params.partial + (size_t)batch * q_heads * params.most_splits * head_dim);
     params.table_stride = table_stride;
     params.width = width;
     params.batch = batch;
@@ -812,10 +816,12 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
     params.page_count = pages;
     params.scale = scale;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int sms = device_sm_count();
+    if (sms < 1) return MT_ERR_LAUNCH;
     const bool half = type == MT_TYPE_FP16;
-    if (head_dim == 64) return half ? launch_paged_attention<64, true>(params, s) : launch_paged_attention<64, false>(params, s);
-    if (head_dim == 128) return half ? launch_paged_attention<128, true>(params, s) : launch_paged_attention<128, false>(params, s);
-    return half ? launch_paged_attention<256, true>(params, s) : launch_paged_attention<256, false>(params, s);
+    if (head_dim == 64) return half ? launch_paged_attention<64, true>(params, sms, s) : launch_paged_attention<64, false>(params, sms, s);
+    if (head_dim == 128) return half ? launch_paged_attention<128, true>(params, sms, s) : launch_paged_attention<128, false>(params, sms, s);
+    return half ? launch_paged_attention<256, true>(params, sms, s) : launch_paged_attention<256, false>(params, sms, s);
 }
 
 size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep) {

@@ -1,9 +1,52 @@
-// Decode attention of one new token per request over a paged key-value cache.
+// Decode attention of one new token per request over a paged key-value cache, split over the cache's length and joined.
+//
+// out[b, h] = softmax(scale q[b, h] K^T) V over the tokens row b of the block table names.  Bound by the bytes of keys
+// and values: 4 Hq / Hkv operations for each, far below what the tensor cores have to offer.
+//
+// Split.  A sequence is cut into splits of 128 tokens, twice as many for every doubling above 16384, so that there are 128
+// at most (a partial result is D + 2 numbers of 32 bits per head: a sixteenth of what 128 tokens of eight heads read).
+// The cut is the sequence's own, so its bits do not depend on the others of the call.  A unit is one split of one KV head
+// (its query heads, up to 16 at once) and belongs to one WARP.  The grid is one CTA per SM; the CTAs count the units of the
+// lengths they find on the device and deal them out, a unit to each SM in turn: a table wide enough for
+// the longest request costs nothing, and ragged lengths even out.
+//
+// A warp keeps a ring of chunks of 16 tokens (keys and values) of its own in flight, 16-byte asynchronous copies from
+// wherever the pages lie, and never meets another warp.  What is masked (the tail behind the sequence, a page outside the
+// cache) is filled with zeros by the copy itself, whatever lies there.
+//
+// Per chunk, on mma.sync m16n8k16 with 32-bit sums:
+//   scores  S[16 tokens x 8 heads] = K[16 x D] Q^T[D x 8]
+//   values  O^T[D x 8 heads] += V^T[D x 16] P^T[16 x 8], V^T by transposing matrix loads; the scores leave the first
+//           product as rows of tokens and enter the second as its columns: movmatrix turns them over.
+// The weights enter as two 16-bit numbers, high and low part: one alone would be off by 2^-9 (bf16).  A running maximum
+// per head is moved, and the sums with it, only when a score passes it by more than 2^8: the weights stay below 256 and
+// keep their relative precision, and a lane adds up its own tokens' weights until the end.
 #pragma once
 
+#include "attention_decode.cuh"
 #include "paged_cache.cuh"
 
 namespace mt {
+
+constexpr int kPagedChunk = 16;          // tokens
+constexpr int kPagedSplitShift = 7;      // the shortest split: 128 tokens
+constexpr int kPagedMostSplits = 128;    // of a sequence
+constexpr int kPagedRowPad = 8;          // elements: rows 16 bytes longer keep matrix loads free of conflicts
+constexpr float kPagedHeadroom = 8.0f;   // log2 of what a weight may reach
+
+__host__ __device__ constexpr int paged_split_shift(int tokens) {
+    int shift = kPagedSplitShift;
+    while ((tokens - 1) >> shift >= kPagedMostSplits) ++shift;
+    return shift;
+}
+__host__ __device__ constexpr int paged_splits(int tokens) {
+    return tokens <= 1 ? 1 : ((tokens - 1) >> paged_split_shift(tokens)) + 1;
+}
+// The most splits any length up to `capacity` has.
+inline int paged_most_splits(long long capacity) {
+    const long long shortest = (capacity + (1 << kPagedSplitShift) - 1) >> kPagedSplitShift;
+    return shortest < kPagedMostSplits ? (int)shortest : kPagedMostSplits;
+}
 
 struct PagedAttentionParams {
     const uint16_t* q;                 // [batch, Hq, D]
@@ -12,89 +55,388 @@ struct PagedAttentionParams {
     const int* tables;                 // [batch, width], rows `table_stride` apart
     const int* lengths;                // [batch]
     uint16_t* out;                     // [batch, Hq, D]
-    float* partial;
+    float* partial;                    // [batch * Hq, most_splits, D]
+    float2* stats;                     // [batch * Hq, most_splits]: maximum (log2) and sum
     long long table_stride;
-    int width, batch, q_heads, kv_heads, page_shift, page_count;
+    int width, batch, q_heads, kv_heads, page_shift, page_count, most_splits;
     float scale;
 };
 
-// One CTA per request and query head; its four warps take the tokens in turn, a lane holds D / 32 of a row.
-template <bool kHalf>
-__device__ __forceinline__ float element_f32(uint16_t bits) {
-    if constexpr (kHalf) return __half2float(*reinterpret_cast<const __half*>(&bits));
-    else return bf16_bits_to_f32(bits);
+template <int kD>
+struct PagedShape {
+    static constexpr int kWarps = kD == 256 ? 4 : 8;
+    static constexpr int kStages = kD == 64 ? 6 : 3;
+    static constexpr int kRow = kD + kPagedRowPad;
+    static constexpr int kStageElements = 2 * kPagedChunk * kRow;
+    static constexpr int kSmem = kWarps * kStages * kStageElements * 2;
+};
+
+// 16 bytes, or zeros where `bytes` is 0 (the address is a valid one all the same).
+__device__ __forceinline__ void cp_async_16_or_zeros(void* smem_dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(smem_dst)), "l"(src), "r"(bytes) : "memory");
 }
 
-template <int kD, bool kHalf>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const PagedAttentionParams p) {
-    constexpr int kPer = kD / 32;
-    __shared__ float top_of[4], sum_of[4], acc_of[4][kD];
-    const int b = blockIdx.x / p.q_heads, qh = blockIdx.x - b * p.q_heads, h = qh / (p.q_heads / p.kv_heads);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+template <bool kHalf>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (kHalf)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        mma_bf16_16816(d, a, b0, b1);
+}
+
+// An 8x8 matrix of 16-bit numbers spread over the warp as an MMA fragment, turned over.
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t pair) {
+    uint32_t out;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(out) : "r"(pair));
+    return out;
+}
+
+// A length as the kernels use it: recorded and cut where the table has no room for it.
+__device__ __forceinline__ int paged_length(const PagedAttentionParams& p, int b, bool report) {
+    const int n = p.lengths[b];
+    const long long capacity = (long long)p.width << p.page_shift;
+    if (n >= 0 && n <= capacity) return n;
+    if (report) record_index(kLengthOutside, b, (unsigned int)n);
+    return n < 0 ? 0 : (int)capacity;
+}
+
+// kTiles: tiles of eight query heads a unit takes at once.
+template <int kD, bool kHalf, int kTiles>
+__global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attention_kernel(const __grid_constant__ PagedAttentionParams p) {
+    using Shape = PagedShape<kD>;
+    constexpr int kRow = Shape::kRow, kStages = Shape::kStages, kThreads = Shape::kWarps * 32, kSlices = kD / 16;
+    constexpr int kCopies = kD / 32;                 // 16-byte copies of a lane for eight rows
+    constexpr int kLanesPerRow = kD / 8;             // 8, 16 or 32
+    constexpr int kRowsPerCopy = 32 / kLanesPerRow;  // rows a warp's copy covers
+    extern __shared__ __align__(16) uint16_t rings[];
+    __shared__ int unit_start[kThreads + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = p.q_heads / p.kv_heads, parts = (group + 8 * kTiles - 1) / (8 * kTiles), per_split = p.kv_heads * parts;
+    uint16_t* ring = rings + warp * (kStages * Shape::kStageElements);
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    const long long capacity = (long long)p.width << p.page_shift;
-    int n = p.lengths[b];
-    if (n < 0 || n > capacity) {
-        if (threadIdx.x == 0) record_index(kLengthOutside, b, (unsigned int)n);
-        n = n < 0 ? 0 : (int)capacity;
-    }
-    float q[kPer], acc[kPer], top = -INFINITY, sum = 0.0f;
-    for (int i = 0; i < kPer; ++i) {
-        q[i] = element_f32<kHalf>(p.q[(long long)blockIdx.x * kD + i * 32 + lane]);
-        acc[i] = 0.0f;
-    }
-    for (int t = warp; t < n; t += 4) {
-        const int page = p.tables[b * p.table_stride + (t >> p.page_shift)];
-        if (page < 0 || page >= p.page_count) {
-            if (lane == 0) record_index(kPageOutside, b, (unsigned int)page);
-            continue;
+
+    // Units in front of every run of requests (a request each up to 256 of them).
+    const int run = (p.batch + kThreads - 1) / kThreads;
+    {
+        __shared__ int warp_units[Shape::kWarps];
+        int mine = 0;
+        for (int b = threadIdx.x * run; b < min((int)(threadIdx.x + 1) * run, p.batch); ++b)
+            mine += paged_splits(paged_length(p, b, blockIdx.x == 0)) * per_split;
+        int sum = mine;
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const int other = __shfl_up_sync(0xFFFFFFFFu, sum, offset);
+            if (lane >= offset) sum += other;
         }
-        const int row = t & ((1 << p.page_shift) - 1);
-        const uint16_t* key = p.key_pages + page * p.key_strides.page + h * p.key_strides.head + row * p.key_strides.token;
-        const uint16_t* value = p.value_pages + page * p.value_strides.page + h * p.value_strides.head + row * p.value_strides.token;
-        float dot = 0.0f;
-        for (int i = 0; i < kPer; ++i) dot = fmaf(q[i], element_f32<kHalf>(key[i * 32 + lane]), dot);
-        const float score = warp_sum_xor(dot) * p.scale, now = fmaxf(top, score);
-        if (now == -INFINITY) continue;
-        const float keep = __expf(top - now), weight = __expf(score - now);
-        sum = sum * keep + weight;
-        for (int i = 0; i < kPer; ++i) acc[i] = fmaf(weight, element_f32<kHalf>(value[i * 32 + lane]), acc[i] * keep);
-        top = now;
+        if (lane == 31) warp_units[warp] = sum;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < warp; ++w) before += warp_units[w];
+        unit_start[threadIdx.x + 1] = before + sum;
+        if (threadIdx.x == 0) unit_start[0] = 0;
+        __syncthreads();
     }
-    if (lane == 0) {
-        top_of[warp] = top;
-        sum_of[warp] = sum;
-    }
-    for (int i = 0; i < kPer; ++i) acc_of[warp][i * 32 + lane] = acc[i];
-    __syncthreads();
-    float best = -INFINITY, total = 0.0f;
-    for (int w = 0; w < 4; ++w) best = fmaxf(best, top_of[w]);
-    float factor[4];
-    for (int w = 0; w < 4; ++w) {
-        factor[w] = top_of[w] == -INFINITY ? 0.0f : __expf(top_of[w] - best);
-        total += sum_of[w] * factor[w];
-    }
-    for (int d = threadIdx.x; d < kD; d += blockDim.x) {
-        float value = 0.0f;
-        for (int w = 0; w < 4; ++w) value = fmaf(acc_of[w][d], factor[w], value);
-        const uint32_t pair = pack_pair<kHalf>(total == 0.0f ? 0.0f : value / total, 0.0f);
-        p.out[(long long)blockIdx.x * kD + d] = (uint16_t)pair;
+    const int units = unit_start[kThreads];
+    const float scale_log2 = p.scale * 1.4426950408889634f;
+
+    for (long long next = blockIdx.x + (long long)gridDim.x * warp; next < units; next += (long long)gridDim.x * Shape::kWarps) {
+        int unit = (int)next;
+        int low = 0, high = kThreads;
+        while (high - low > 1) {
+            const int middle = (low + high) >> 1;
+            if (unit_start[middle] <= unit) low = middle; else high = middle;
+        }
+        int b = low * run, n, splits;
+        unit -= unit_start[low];
+        for (;; ++b) {
+            n = paged_length(p, b, false);
+            splits = paged_splits(n);
+            if (unit < splits * per_split) break;
+            unit -= splits * per_split;
+        }
+        const int split = unit / per_split, rest = unit - split * per_split, h = rest / parts, part = rest - h * parts;
+        const int shift = paged_split_shift(n), first = split << shift, end = min(n, first + (1 << shift));
+        const int head0 = h * group + part * 8 * kTiles, heads = min(8 * kTiles, group - part * 8 * kTiles);
+        const int chunks = (end - first + kPagedChunk - 1) / kPagedChunk;
+
+        // The pages of the unit, 32 at a time, one in a lane; the next 32 are asked for one window ahead.
+        const int* table = p.tables + b * p.table_stride;
+        const int page0 = first >> p.page_shift, pages = ((end - 1) >> p.page_shift) - page0 + 1;
+        auto window = [&](int w) {
+            const int i = 32 * w + lane;
+            return end > first && i < pages ? table[page0 + i] : 0;
+        };
+        int in_window = 0, ids = window(0), ids_next = window(1);
+        unsigned int outside = 0;  // two bits a ring slot: its first, its second eight tokens lie in a page outside the cache
+
+        auto copy_chunk = [&](int c, int slot) {
+            const int token0 = first + c * kPagedChunk, i0 = (token0 >> p.page_shift) - page0;
+            if (i0 >> 5 != in_window) {
+                ids = ids_next;
+                ids_next = window(++in_window + 1);
+            }
+            uint16_t* keys = ring + slot * Shape::kStageElements;
+            uint16_t* values = keys + kPagedChunk * kRow;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int token = token0 + 8 * half;
+                int id = __shfl_sync(0xFFFFFFFFu, ids, ((token >> p.page_shift) - page0) & 31);
+                const bool inside = id >= 0 && id < p.page_count;
+                if (!inside) {
+                    if (lane == 0 && token < end) record_index(kPageOutside, b, (unsigned int)id);
+                    id = 0;
+                }
+                outside = (outside & ~(1u << (2 * slot + half))) | (inside ? 0u : 1u << (2 * slot + half));
+                const int row0 = lane / kLanesPerRow, at = lane % kLanesPerRow * 8;
+                const int in_page = (token & ((1 << p.page_shift) - 1)) + row0;
+                const uint16_t* key = p.key_pages + id * p.key_strides.page + h * p.key_strides.head + in_page * p.key_strides.token + at;
+                const uint16_t* value =
+                    p.value_pages + id * p.value_strides.page + h * p.value_strides.head + in_page * p.value_strides.token + at;
+                const int usable = inside ? end - token - row0 : 0;  // rows from this lane's first one on
+                uint16_t* key_to = keys + (8 * half + row0) * kRow + at;
+                uint16_t* value_to = values + (8 * half + row0) * kRow + at;
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    const int bytes = i * kRowsPerCopy < usable ? 16 : 0;
+                    // A row behind the end has an address inside the page all the same.
+                    cp_async_16_or_zeros(key_to + i * kRowsPerCopy * kRow, key + i * kRowsPerCopy * p.key_strides.token, bytes);
+                    cp_async_16_or_zeros(value_to + i * kRowsPerCopy * kRow, value + i * kRowsPerCopy * p.value_strides.token, bytes);
+                }
+            }
+        };
+#pragma unroll
+        for (int c = 0; c < kStages - 1; ++c) {
+            if (c < chunks) copy_chunk(c, c);
+            ptx::cp_async_commit();
+        }
+
+        // Query fragments: head g of each tile, dims 16 s + 2 t (+1) and + 8.
+        uint32_t qf[kTiles][kSlices][2];
+#pragma unroll
+        for (int tile = 0; tile < kTiles; ++tile) {
+            const bool real = 8 * tile + g < heads;
+            const uint16_t* row = p.q + ((long long)b * p.q_heads + head0 + (real ? 8 * tile + g : 0)) * kD;
+#pragma unroll
+            for (int s = 0; s < kSlices; ++s) {
+                uint32_t lower, upper;
+                asm volatile("ld.global.u32 %0, [%1];" : "=r"(lower) : "l"(row + 16 * s + 2 * t));
+                asm volatile("ld.global.u32 %0, [%1];" : "=r"(upper) : "l"(row + 16 * s + 2 * t + 8));
+                qf[tile][s][0] = real ? lower : 0u;
+                qf[tile][s][1] = real ? upper : 0u;
+            }
+        }
+        float acc[kSlices][kTiles][4], top[kTiles][2], sum[kTiles][2];
+#pragma unroll
+        for (int tile = 0; tile < kTiles; ++tile) {
+            top[tile][0] = top[tile][1] = -INFINITY;
+            sum[tile][0] = sum[tile][1] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSlices; ++s) acc[s][tile][0] = acc[s][tile][1] = acc[s][tile][2] = acc[s][tile][3] = 0.0f;
+        }
+
+        for (int c = 0, slot = 0; c < chunks; ++c) {
+            ptx::cp_async_wait_group<kStages - 2>();
+            __syncwarp();
+            const uint16_t* keys = ring + slot * Shape::kStageElements;
+            const uint16_t* values = keys + kPagedChunk * kRow;
+            // Scores: [0], [1]: token g, heads 2 t and 2 t + 1 of the tile; [2], [3]: token g + 8.
+            float score[kTiles][4];
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) score[tile][0] = score[tile][1] = score[tile][2] = score[tile][3] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSlices; ++s) {
+                uint32_t a[4];
+                ldmatrix_x4(a, keys + (lane & 15) * kRow + 8 * (lane >> 4) + 16 * s);
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile) mma_16816<kHalf>(score[tile], a, qf[tile][s][0], qf[tile][s][1]);
+            }
+            const int token = first + c * kPagedChunk + g;
+            const bool there[2] = {token < end && !(outside >> (2 * slot) & 1u), token + 8 < end && !(outside >> (2 * slot + 1) & 1u)};
+            bool passes = false;
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    score[tile][i] = there[i >> 1] ? score[tile][i] * scale_log2 : -INFINITY;
+                    passes = passes || score[tile][i] > top[tile][i & 1] + kPagedHeadroom;
+                }
+            if (__any_sync(0xFFFFFFFFu, passes)) {
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float now = fmaxf(score[tile][j], score[tile][j + 2]);
+#pragma unroll
+                        for (int offset = 4; offset <= 16; offset <<= 1) now = fmaxf(now, __shfl_xor_sync(0xFFFFFFFFu, now, offset));
+                        now = fmaxf(now, top[tile][j]);
+                        const float factor = now == -INFINITY ? 1.0f : exp2f(top[tile][j] - now);
+                        top[tile][j] = now;
+                        sum[tile][j] *= factor;
+#pragma unroll
+                        for (int s = 0; s < kSlices; ++s) {
+                            acc[s][tile][j] *= factor;
+                            acc[s][tile][j + 2] *= factor;
+                        }
+                    }
+            }
+            // Weights, high and low part, as columns of tokens.
+            uint32_t high[kTiles][2], lower[kTiles][2];
+#pragma unroll
+            for (int tile = 0; tile < kTiles; ++tile) {
+                float weight[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    weight[i] = top[tile][i & 1] == -INFINITY ? 0.0f : exp2f(score[tile][i] - top[tile][i & 1]);
+                    sum[tile][i & 1] += weight[i];
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t pair = pack_pair<kHalf>(weight[2 * half], weight[2 * half + 1]);
+                    const float2 back = unpack_pair<kHalf>(pair);
+                    high[tile][half] = transposed_8x8(pair);
+                    lower[tile][half] = transposed_8x8(pack_pair<kHalf>(weight[2 * half] - back.x, weight[2 * half + 1] - back.y));
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < kSlices; ++s) {
+                uint32_t a[4];
+                ldmatrix_x4_trans(a, values + ((lane & 7) + 8 * (lane >> 4)) * kRow + 16 * s + (lane & 8));
+#pragma unroll
+                for (int tile = 0; tile < kTiles; ++tile) {
+                    mma_16816<kHalf>(acc[s][tile], a, high[tile][0], high[tile][1]);
+                    mma_16816<kHalf>(acc[s][tile], a, lower[tile][0], lower[tile][1]);
+                }
+            }
+            __syncwarp();  // the slot read last time round is free: every lane is past its matrix loads
+            if (c + kStages - 1 < chunks) copy_chunk(c + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
+            ptx::cp_async_commit();
+            slot = slot == kStages - 1 ? 0 : slot + 1;
+        }
+
+        // acc[s][tile]: [0], [1]: dim 16 s + g, heads 2 t and 2 t + 1; [2], [3]: dim + 8.
+#pragma unroll
+        for (int tile = 0; tile < kTiles; ++tile)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float total = sum[tile][j];
+#pragma unroll
+                for (int offset = 4; offset <= 16; offset <<= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, offset);
+                const int head = 8 * tile + 2 * t + j;
+                if (head >= heads) continue;
+                const long long at = (long long)b * p.q_heads + head0 + head;
+                if (splits == 1) {
+                    const float factor = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                    for (int s = 0; s < kSlices; ++s) {
+                        p.out[at * kD + 16 * s + g] = (uint16_t)pack_pair<kHalf>(acc[s][tile][j] * factor, 0.0f);
+                        p.out[at * kD + 16 * s + g + 8] = (uint16_t)pack_pair<kHalf>(acc[s][tile][j + 2] * factor, 0.0f);
+                    }
+                } else {
+                    float* to = p.partial + (at * p.most_splits + split) * kD;
+#pragma unroll
+                    for (int s = 0; s < kSlices; ++s) {
+                        to[16 * s + g] = acc[s][tile][j];
+                        to[16 * s + g + 8] = acc[s][tile][j + 2];
+                    }
+                    if (g == 0) p.stats[at * p.most_splits + split] = make_float2(top[tile][j], total);
+                }
+            }
+        ptx::cp_async_wait_group<0>();
+        __syncwarp();
     }
 }
 
+// Joins the splits of one request and query head, in split order; a request of one split has its result already.
 template <int kD, bool kHalf>
-inline int launch_paged_attention(const PagedAttentionParams& params, cudaStream_t stream) {
+__global__ void __launch_bounds__(kD) paged_attention_join_kernel(const __grid_constant__ PagedAttentionParams p) {
+    constexpr int kAhead = 16, kRounds = kPagedMostSplits / 32;
+    const long long at = blockIdx.x;                // b * Hq + query head
+    const int b = (int)(at / p.q_heads), d = threadIdx.x, lane = threadIdx.x & 31;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const int splits = paged_splits(paged_length(p, b, false));
+    if (splits == 1) return;
+    const float* from = p.partial + at * p.most_splits * kD + d;
+    const float2* stats = p.stats + at * p.most_splits;
+    float2 mine[kRounds];
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        mine[r] = 32 * r + lane < splits ? stats[32 * r + lane] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, mine[r].x);
+    }
+#pragma unroll
+    for (int offset = 16; offset >= 1; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
+    float total = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        if (32 * r >= splits) break;
+        const float factor = mine[r].x == -INFINITY ? 0.0f : exp2f(mine[r].x - top);
+#pragma unroll
+        for (int part = 0; part < 32; part += kAhead) {
+            float numbers[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int s = 32 * r + part + i;
+                numbers[i] = s < splits ? from[(long long)s * kD] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float f = __shfl_sync(0xFFFFFFFFu, factor, part + i), sum = __shfl_sync(0xFFFFFFFFu, mine[r].y, part + i);
+                total = fmaf(sum, f, total);
+                value = fmaf(numbers[i], f, value);
+            }
+        }
+    }
+    p.out[at * kD + d] = (uint16_t)pack_pair<kHalf>(total == 0.0f ? 0.0f : value / total, 0.0f);
+}
+
+inline size_t paged_attention_workspace_bytes(int batch, int q_heads, int head_dim, long long capacity) {
+    const int splits = paged_most_splits(capacity);
+    if (splits <= 1) return 0;
+    return (size_t)batch * q_heads * splits * (head_dim + 2) * sizeof(float);
+}
+
+template <int kD, bool kHalf, int kTiles>
+inline int launch_paged_attention_instance(const PagedAttentionParams& params, int sm_count, cudaStream_t stream) {
+    using Shape = PagedShape<kD>;
+    static bool configured[64] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return MT_ERR_LAUNCH;
+    if (device >= 64 || !configured[device]) {
+        if (cudaFuncSetAttribute(paged_attention_kernel<kD, kHalf, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess)
+            return MT_ERR_LAUNCH;
+        if (device < 64) configured[device] = true;
+    }
+    const int group = params.q_heads / params.kv_heads;
+    const long long most_units = (long long)params.batch * params.kv_heads * ((group + 8 * kTiles - 1) / (8 * kTiles)) * params.most_splits;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(params.batch * params.q_heads, 1, 1);
-    config.blockDim = dim3(128, 1, 1);
+    config.gridDim = dim3(most_units < sm_count ? (unsigned int)most_units : sm_count, 1, 1);
+    config.blockDim = dim3(Shape::kWarps * 32, 1, 1);
+    config.dynamicSmemBytes = Shape::kSmem;
     config.stream = stream;
     cudaLaunchAttribute attrs[1];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attrs;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, paged_attention_kernel<kD, kHalf>, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&config, paged_attention_kernel<kD, kHalf, kTiles>, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    if (params.most_splits > 1) {
+        config.gridDim = dim3(params.batch * params.q_heads, 1, 1);
+        config.blockDim = dim3(kD, 1, 1);
+        config.dynamicSmemBytes = 0;
+        if (cudaLaunchKernelEx(&config, paged_attention_join_kernel<kD, kHalf>, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    }
+    return MT_OK;
+}
+
+template <int kD, bool kHalf>
+inline int launch_paged_attention(const PagedAttentionParams& params, int sm_count, cudaStream_t stream) {
+    return params.q_heads / params.kv_heads <= 8 ? launch_paged_attention_instance<kD, kHalf, 1>(params, sm_count, stream)
+                                                 : launch_paged_attention_instance<kD, kHalf, 2>(params, sm_count, stream);
 }
 
 }  // namespace mt
