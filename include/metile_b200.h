@@ -295,10 +295,12 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
  * (1 ... 64) largest in descending order, the lower beam and then the lower token first among equals.  logits [groups *
  * beams, vocabulary] bf16, fp16 or fp32, rows `row_stride` elements apart; scores fp32 [groups, beams].  A beam that has
  * `finished` (bytes, may be NULL) offers end_token alone, at its score.  As -inf count: every candidate of a score
- * up to -1e15 or of a row with a NaN, with +inf or with nothing above -inf.  parents: the beam within its group;
- * finished_out: the parent had finished, or the token is end_token (-1: there is none).  beams up to 32. */
+ * up to -1e9 or of a row with a NaN, with +inf or with nothing above -inf.  parents: the beam within its group;
+ * finished_out: the parent had finished, or the token is end_token (-1: there is none).  beams up to 32.  The aligned 16
+ * bytes around the first and the last logit of a row must be readable (any allocation's granularity sees to that); what lies
+ * there beside the row is never used. */
 #define MT_BEAM_MAX_ROWS 0x000FFFFF
-#define MT_BEAM_MAX_VOCABULARY 0x00FFFFFF
+#define MT_BEAM_MAX_VOCABULARY 0x00080000
 size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep);
 int mt_beam_select(const void* logits, long long row_stride, int type, const float* scores, const unsigned char* finished,
                    long long end_token, float* scores_out, int* parents_out, long long* tokens_out, unsigned char* finished_out,

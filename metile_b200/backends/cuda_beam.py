@@ -10,7 +10,7 @@ from ._common import native, native_result, require_on_device
 from .cuda_paged import _bare, _refuse_gradient, _require_cuda, _require_ints, _require_pages, _require_table
 
 MAX_BEAMS, MAX_KEEP = 32, 64
-MAX_ROWS, MAX_VOCABULARY = 0x000FFFFF, 0x00FFFFFF
+MAX_ROWS, MAX_VOCABULARY = 0x000FFFFF, 0x00080000
 LOGIT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -20,7 +20,7 @@ def beam_select(logits, scores, *, keep=None, finished=None, end_token=None):
     logits [groups * beams, vocabulary] bfloat16, float16 or float32; scores float32 [groups, beams], the sums of
     log-probabilities so far.  A candidate is worth scores + log_softmax(logits), in 64 bits; the largest come first, among
     equals the lower beam, then the lower token.  A beam that has `finished` (bool [groups, beams]) offers `end_token`
-    alone, at the score it has.  A score up to -1e15 is a mask: that beam's candidates count as -inf, and so do those of
+    alone, at the score it has.  A score up to -1e9 is a mask: that beam's candidates count as -inf, and so do those of
     logits with a NaN, with +inf or with nothing above -inf.
 
     Returns (scores float32, parents int32 -- the beam within its group --, tokens int64, finished bool), all

@@ -825,8 +825,8 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
 }
 
 size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep) {
-    (void)groups, (void)beams, (void)vocabulary, (void)keep;
-    return 0;
+    if (groups <= 0 || beams <= 0 || vocabulary <= 0 || keep <= 0) return 0;
+    return beam_workspace_bytes(groups, beams, vocabulary, keep);
 }
 
 int mt_beam_select(const void* logits, long long row_stride, int type, const float* scores, const unsigned char* finished,
@@ -843,11 +843,13 @@ int mt_beam_select(const void* logits, long long row_stride, int type, const flo
     const size_t needed = mt_beam_select_workspace_bytes(groups, beams, vocabulary, keep);
     if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
     if (!device_is_sm100()) return MT_ERR_DEVICE;
-    BeamSelectParams params{logits, scores, finished, scores_out, parents_out, tokens_out, finished_out, row_stride, end_token,
-                            groups, beams, vocabulary, keep, type};
-    cudaLaunchAttribute attribute;
-    const cudaLaunchConfig_t config = dependent_launch(dim3(groups, 1, 1), 1024, 0, stream, &attribute);
-    return cudaLaunchKernelEx(&config, beam_select_kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    BeamSelectParams params{logits, scores, finished, scores_out, parents_out, tokens_out, finished_out, nullptr, nullptr, row_stride,
+                            end_token, groups, beams, vocabulary, keep, beam_spans(vocabulary)};
+    params.stats = static_cast<BeamSpanStats*>(workspace);
+    params.lists = reinterpret_cast<BeamEntry*>(params.stats + (size_t)groups * beams * params.spans);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return type == MT_TYPE_FP32 ? launch_beam_select<2>(params, s) : type == MT_TYPE_FP16 ? launch_beam_select<1>(params, s)
+                                                                                            : launch_beam_select<0>(params, s);
 }
 
 int mt_beam_reorder(const int* block_tables, long long table_stride, int width, const int* lengths, const int* parents,

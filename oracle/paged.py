@@ -85,7 +85,7 @@ def beam_select(logits, scores, keep, finished=None, end=-1):
         found = np.full((beams, vocab), -np.inf)
         for k in range(beams):
             score, row = scores[g, k], logits[g * beams + k]
-            if not score > -1e15:
+            if not score > -1e9:
                 continue
             if finished is not None and finished[g, k]:
                 found[k, end] = score

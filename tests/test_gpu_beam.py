@@ -72,6 +72,17 @@ def test_equal_candidates_go_by_beam_and_token(cuda_device):
     check_select(row.repeat(4, 1), torch.full((1, 4), -3.25, device=cuda_device), 16)
 
 
+@pytest.mark.parametrize("levels,keep", [(2, 8), (3, 64), (40, 16), (4000, 5)])
+def test_many_equal_logits_at_any_level(cuda_device, levels, keep):
+    generator = torch.Generator().manual_seed(levels)
+    logits = torch.randint(0, levels, (6, 40003), generator=generator).to(torch.float16).to(cuda_device) / 8
+    logits[1] = torch.where(logits[1] > 0, logits[1], -torch.inf)
+    logits[2, 16384:32768] = -torch.inf  # a span with nothing in it
+    scores = torch.tensor([[-1.0, -1.25, -0.5], [-3.0, -3.0, -2.0]], device=cuda_device)
+    check_select(logits, scores, keep)
+    check_select(logits[:1], scores[:1, :1].contiguous(), keep)
+
+
 def test_candidates_of_two_beams_closer_than_32_bits_tell(cuda_device):
     """One beam's score is moved so that its best candidate lies a hair above or below the other beam's: the order is
     the one of 64 bits."""
@@ -98,7 +109,7 @@ def test_masked_tokens_beams_and_rows(cuda_device):
         logits[5, 78] = torch.inf
         logits[6, ::2] = -torch.inf
         scores[1] = torch.tensor([0.0, -torch.inf, -1e30, torch.nan], device=cuda_device)
-        scores[2] = torch.tensor([-torch.inf, LOWEST[torch.float32], -torch.inf, -1e15], device=cuda_device)
+        scores[2] = torch.tensor([-torch.inf, LOWEST[torch.float32], -torch.inf, -1e9], device=cuda_device)
         check_select(logits, scores, 16)
         check_select(logits[:4], scores[:1], 64)
 

@@ -71,7 +71,7 @@ def test_select_and_reorder_refusals_of_the_abi():
     def select(logits=ONE, type=0, finished=ONE, end=3, groups=2, beams=4, vocab=100, keep=8, space=ONE, size=workspace):
         return lib.mt_beam_select(logits, vocab, type, ONE, finished, end, ONE, ONE, ONE, ONE, space, size, groups, beams, vocab, keep, None)
 
-    for bad in (dict(groups=-1), dict(beams=0), dict(beams=33), dict(vocab=0), dict(vocab=2**24), dict(keep=0), dict(keep=65),
+    for bad in (dict(groups=-1), dict(beams=0), dict(beams=33), dict(vocab=0), dict(vocab=2**19 + 1), dict(keep=0), dict(keep=65),
                 dict(vocab=1, end=0, keep=5), dict(type=3), dict(end=100), dict(end=-1), dict(finished=None, end=-2), dict(groups=2**19)):
         assert select(**bad) == -1, bad
     assert select(logits=None) == -6 and select(logits=ctypes.c_void_p(17)) == -2 and select(groups=0) == 0
