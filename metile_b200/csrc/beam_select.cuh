@@ -5,10 +5,11 @@
 // -inf; a score that is a mask) counts as -inf.  Bound by the bytes of the logits, and near to it by the exponentials (an
 // SM takes 16 a cycle: 9 TB/s of 16-bit logits on 148 of them).
 //
-// One pass.  A CTA holds a span of 16384 logits of a row in registers, 64 a thread, and leaves its maximum, the sum of
-// its exponentials and its `keep` best.  Within a beam candidates are ordered as their logits are, so no sum is needed for
-// that.  Of 64 bucket maxima (four threads each) the keep-th largest bounds the keep-th best from below; only the few
-// logits that reach it are collected and ranked.  Spans have one size for all calls: a row's bits do not depend on the others.
+// One pass.  A CTA has some of a row's spans of 8192 logits, 32 a thread and span; each of its warps leaves
+// the maximum and the sum of exponentials of its share of every span, and the CTA the `keep` best of all.  Within a beam candidates
+// are ordered as their logits are, so no sum is needed for that.  Of 64 bucket maxima (four threads each) the keep-th largest
+// bounds the keep-th best from below; the few threads that reach it look at their logits again, and what they find is
+// ranked.  Shares have one size for all calls: a row's bits do not depend on the others.
 //
 // Then a CTA per group joins spans and beams.  The sums are of 32-bit exponentials, each beam's log-sum off by up to
 // kBeamError; where two beams' candidates are closer than twice that, the sums of the two are taken again, in 64 bits, so
@@ -23,21 +24,21 @@
 namespace mt {
 
 constexpr double kDeadScore = -1e9;  // no sum of log-probabilities but the mask of a beam that is out; above it 64 bits keep logits apart
-// |d| 2^-24 for the rounding of the argument d log2 e (the weighted mean of |d| is at most the log of the row's
-// length, 13, and e^d |d| is small beyond it), 2^-22 for ex2.approx, six roundings of 2^-24 in a thread's
-// sum (the rest is added in 64 bits): 1.4e-6.
-constexpr double kBeamError = 0x1p-19;
+// d = logit - top rounded, then d log2 e: |d| 2^-24 each and |d| 1.4e-8 for log2 e itself, 2^-22 for ex2.approx, ten roundings of
+// 2^-24 in a warp's sum (the rest is added in 64 bits).  The mean of |d| by the weights is at most the log of the row's
+// length, 13.2: 2.7e-6.
+constexpr double kBeamError = 0x1p-18;
 
 constexpr int kBeamMaxBeams = 32, kBeamMaxKeep = 64;
-constexpr int kBeamThreads = 256, kBeamPerThread = 64, kBeamSpan = kBeamThreads * kBeamPerThread;
-constexpr int kBeamMaxVocabulary = 32 * kBeamSpan;           // of the join: at most 1024 lists
-constexpr int kBeamBuckets = 64, kBeamCollect = 1024;        // of a span
-constexpr int kBeamJoinCollect = kBeamMaxKeep * kBeamMaxKeep;
+constexpr int kBeamThreads = 256, kBeamPerThread = 32, kBeamSpan = kBeamThreads * kBeamPerThread, kBeamShares = kBeamThreads / 32;
+constexpr int kBeamMaxParts = 32, kBeamMostPerPart = 16;     // CTAs of a row (at most 1024 lists to join), spans of a CTA
+constexpr int kBeamMaxVocabulary = 64 * kBeamSpan;
+constexpr int kBeamBuckets = 64, kBeamCollect = 1024;        // of a CTA
+constexpr int kBeamSlack = 8, kBeamJoinCollect = (kBeamMaxKeep + kBeamSlack) * kBeamMaxKeep, kBeamStage = 4096;
 static_assert(kBeamBuckets >= kBeamMaxKeep && kBeamMaxVocabulary == MT_BEAM_MAX_VOCABULARY, "bounds of the selection");
 
-struct BeamSpanStats {
-    double sum;   // of exp(logit - top); NaN: the span has a NaN or +inf
-    float top;
+struct BeamShareStats {
+    float top, sum;  // of exp(logit - top); NaN: there is a NaN or +inf
 };
 
 struct BeamEntry {
@@ -53,15 +54,16 @@ struct BeamSelectParams {
     int* parents_out;
     long long* tokens_out;
     unsigned char* finished_out;
-    BeamSpanStats* stats;           // [groups * beams, spans]
-    BeamEntry* lists;               // [groups * beams, spans, keep]
+    BeamShareStats* stats;          // [groups * beams, spans * 8]
+    BeamEntry* lists;               // [groups * beams, parts, keep]
     long long row_stride, end_token;  // no end token: -1
     int groups, beams, vocabulary, keep, spans;
+    int parts, per_part;            // CTAs of a row, spans of each
 };
 
 inline int beam_spans(int vocabulary) { return (vocabulary + kBeamSpan - 1) / kBeamSpan; }
 inline size_t beam_workspace_bytes(int groups, int beams, int vocabulary, int keep) {
-    return (size_t)groups * beams * beam_spans(vocabulary) * (sizeof(BeamSpanStats) + (size_t)keep * sizeof(BeamEntry));
+    return (size_t)groups * beams * beam_spans(vocabulary) * (kBeamShares * sizeof(BeamShareStats) + (size_t)keep * sizeof(BeamEntry));
 }
 
 // kType: 0 bf16, 1 fp16, 2 fp32.
@@ -81,166 +83,225 @@ __device__ __forceinline__ float beam_logit_at(const void* row, long long i) {
     else return static_cast<const float*>(row)[i];
 }
 
-// 16 bytes from an address that is `skew` bytes behind a boundary, by aligned loads; of the second only if `more`.
-__device__ __forceinline__ uint4 load_skewed(const char* address, int skew, bool more) {
-    const uint4 a = ptx::ld_global_dependent_u4(address - skew);
-    if (skew == 0) return a;
-    const uint4 b = more ? ptx::ld_global_dependent_u4(address - skew + 16) : make_uint4(0u, 0u, 0u, 0u);
+// Bytes skew ... skew + 15 of two 16-byte vectors that follow one another.
+__device__ __forceinline__ void take_skewed(uint32_t (&out)[4], const uint4& a, const uint4& b, int skew) {
     const uint32_t words[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     const int first = skew >> 2, bits = (skew & 3) * 8;
     uint32_t shifted[5];
 #pragma unroll
     for (int i = 0; i < 5; ++i)
         shifted[i] = first == 0 ? words[i] : first == 1 ? words[i + 1] : first == 2 ? words[i + 2] : words[i + 3];
-    return make_uint4(__funnelshift_r(shifted[0], shifted[1], bits), __funnelshift_r(shifted[1], shifted[2], bits),
-                      __funnelshift_r(shifted[2], shifted[3], bits), __funnelshift_r(shifted[3], shifted[4], bits));
-}
-
-__device__ __forceinline__ float warp_max_f32(float v) {
 #pragma unroll
-    for (int offset = 16; offset >= 1; offset >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, offset));
-    return v;
+    for (int i = 0; i < 4; ++i) out[i] = __funnelshift_r(shifted[i], shifted[i + 1], bits);
 }
 
+// The larger of two words of logits, pair by pair.
 template <int kType>
-__global__ void __launch_bounds__(kBeamThreads) beam_span_kernel(const BeamSelectParams p) {
-    constexpr int kPer = kType == 2 ? 4 : 8, kVectors = kBeamPerThread / kPer, kSize = kType == 2 ? 4 : 2, kWarps = kBeamThreads / 32;
-    __shared__ float warp_top[kWarps], bucket[kBeamBuckets];
-    __shared__ double warp_sum[kWarps];
-    __shared__ float collected[kBeamCollect], bound_shared;
-    __shared__ int collected_token[kBeamCollect], count, above;
-    const int span = blockIdx.x % p.spans, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long row = blockIdx.x / p.spans;
-    const int first = span * kBeamSpan, here = min(kBeamSpan, p.vocabulary - first);
-    ptx::griddep_launch_dependents();
-    ptx::griddep_wait();
-    const char* from = static_cast<const char*>(p.logits) + (row * p.row_stride + first) * kSize;
-    const int skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
-    // Element e of vector v: the span's (v * 256 + thread) * kPer + e; those behind the row are -inf and left out below.
-    uint32_t raw[kVectors][4];
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const int at = (v * kBeamThreads + threadIdx.x) * kPer;
-        uint4 vector = make_uint4(0u, 0u, 0u, 0u);
-        if (at < here) vector = load_skewed(from + (long long)at * kSize, skew, at + (16 - skew) / kSize < here);
-        raw[v][0] = vector.x; raw[v][1] = vector.y; raw[v][2] = vector.z; raw[v][3] = vector.w;
-    }
-    if (here < kBeamSpan) {
-#pragma unroll
-        for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if ((v * kBeamThreads + (int)threadIdx.x) * kPer + e >= here) {
-                    if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
-                    else {
-                        const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
-                        raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
-                    }
-                }
-    }
-    float mine = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) mine = fmaxf(mine, beam_logit<kType>(raw[v], e));
-    float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-    if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = top;
-#pragma unroll
-    for (int offset = 4; offset <= 16; offset <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
-    if (lane == 0) warp_top[warp] = top;
-    if (threadIdx.x == 0) count = above = 0;
-    __syncthreads();
-    top = warp_top[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_top[w]);
-    // The keep-th largest bucket: at least `keep` logits of the span are not below it.
-    if (threadIdx.x < kBeamBuckets) {
-        const float own = bucket[threadIdx.x];
-        int rank = 0;
-#pragma unroll 16
-        for (int j = 0; j < kBeamBuckets; ++j) {
-            const float other = bucket[j];
-            rank += other > own || (other == own && j < (int)threadIdx.x);
-        }
-        if (rank == p.keep - 1) bound_shared = own;
-    }
-    // Exponentials of the differences to the span's maximum; a vector's sums as a tree.
-    double total = 0.0;
-    if (top == -INFINITY) {
-        bool bad = false;
-#pragma unroll
-        for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) bad = bad || beam_logit<kType>(raw[v], e) != beam_logit<kType>(raw[v], e);
-        total = bad ? NAN : 0.0;
-    } else {
-        float sums[kVectors];
+__device__ __forceinline__ uint32_t beam_word_max(uint32_t a, uint32_t b) {
+    if constexpr (kType == 2) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    uint32_t out = 0;
+    if constexpr (kType == 1) asm("max.f16x2 %0, %1, %2;" : "=r"(out) : "r"(a), "r"(b));
+    if constexpr (kType == 0) asm("max.bf16x2 %0, %1, %2;" : "=r"(out) : "r"(a), "r"(b));
+    return out;
+}
+template <int kType>
+__device__ __forceinline__ float beam_word_top(uint32_t word) {
+    const uint32_t words[4] = {word, 0u, 0u, 0u};
+    if constexpr (kType == 2) return __uint_as_float(word);
+    else return fmaxf(beam_logit<kType>(words, 0), beam_logit<kType>(words, 1));
+}
+
+__device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// A thread's logits of a span: element e of vector v is the span's (v * 256 + thread) * kPer + e; those behind the row are -inf.
+template <int kType>
+struct BeamLoader {
+    static constexpr int kPer = kType == 2 ? 4 : 8, kVectors = kBeamPerThread / kPer, kSize = kType == 2 ? 4 : 2;
+    const char* row;
+    int vocabulary;
+
+    __device__ __forceinline__ void load(int first, uint32_t (&raw)[kVectors][4]) const {
+        const int here = min(kBeamSpan, vocabulary - first);
+        const char* from = row + (long long)first * kSize;
+        const int skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
-            float weight[kPer];
+            const int at = (v * kBeamThreads + threadIdx.x) * kPer;
+            uint4 vector = make_uint4(0u, 0u, 0u, 0u);
+            if (at < here) vector = ptx::ld_global_dependent_u4(from - skew + (long long)at * kSize);
+            raw[v][0] = vector.x; raw[v][1] = vector.y; raw[v][2] = vector.z; raw[v][3] = vector.w;
+        }
+        if (skew) {  // a row that starts off a boundary: the aligned vector behind each as well
+            uint4 behind[kVectors];
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const float d = beam_logit<kType>(raw[v], e) - top;  // log2 e in two parts
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e]) : "f"(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661484e-8f)));
+            for (int v = 0; v < kVectors; ++v) {
+                const int at = (v * kBeamThreads + threadIdx.x) * kPer;
+                behind[v] = make_uint4(0u, 0u, 0u, 0u);
+                if (at + (16 - skew) / kSize < here) behind[v] = ptx::ld_global_dependent_u4(from - skew + (long long)at * kSize + 16);
             }
 #pragma unroll
-            for (int width = kPer / 2; width >= 1; width >>= 1)
-#pragma unroll
-                for (int e = 0; e < width; ++e) weight[e] += weight[e + width];
-            sums[v] = weight[0];
+            for (int v = 0; v < kVectors; ++v)
+                take_skewed(raw[v], make_uint4(raw[v][0], raw[v][1], raw[v][2], raw[v][3]), behind[v], skew);
         }
+        if (here < kBeamSpan) {
 #pragma unroll
-        for (int width = kVectors / 2; width >= 1; width >>= 1)
+            for (int v = 0; v < kVectors; ++v)
 #pragma unroll
-            for (int v = 0; v < width; ++v) sums[v] += sums[v + width];
-        total = sums[0];
+                for (int e = 0; e < kPer; ++e)
+                    if ((v * kBeamThreads + (int)threadIdx.x) * kPer + e >= here) {
+                        if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
+                        else {
+                            const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
+                            raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
+                        }
+                    }
+        }
     }
-#pragma unroll
-    for (int offset = 16; offset >= 1; offset >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, offset);
-    if (lane == 0) warp_sum[warp] = total;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        total = warp_sum[0];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) total += warp_sum[w];
-        p.stats[blockIdx.x] = {total, top};
-    }
-    const float bound = bound_shared;
-    // What each element's thread does with it where it qualifies.
-    auto collect = [&](auto qualifies) {
+};
+
+template <int kType>
+constexpr int kBeamAtOnce = kType == 2 ? 3 : 5;  // CTAs of an SM
+
+template <int kType>
+__global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce<kType>) beam_span_kernel(const BeamSelectParams p) {
+    using Loader = BeamLoader<kType>;
+    constexpr int kPer = Loader::kPer, kVectors = Loader::kVectors, kWarps = kBeamShares;
+    __shared__ float span_top[kBeamMostPerPart][kBeamThreads], bucket[kBeamBuckets];
+    __shared__ float collected[kBeamCollect], bound_shared;
+    __shared__ int collected_token[kBeamCollect], count, above;
+    const int part = blockIdx.x % p.parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long row = blockIdx.x / p.parts;
+    const int span0 = part * p.per_part, span1 = min(p.spans, span0 + p.per_part);
+    const Loader loader{static_cast<const char*>(p.logits) + row * p.row_stride * Loader::kSize, p.vocabulary};
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    if (threadIdx.x == 0) count = above = 0;
+    float mine = -INFINITY;
+    uint32_t raw[kVectors][4];
+    for (int span = span0; span < span1; ++span) {
+        loader.load(span * kBeamSpan, raw);
+        uint32_t largest = raw[0][0];
 #pragma unroll
         for (int v = 0; v < kVectors; ++v)
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const float logit = beam_logit<kType>(raw[v], e);
-                const int at = (v * kBeamThreads + threadIdx.x) * kPer + e;
-                if (qualifies(logit, at) && at < here) {
-                    const int place = atomicAdd(&count, 1);
-                    if (place < kBeamCollect) {
-                        collected[place] = logit;
-                        collected_token[place] = first + at;
-                    }
+            for (int i = 0; i < 4; ++i) largest = beam_word_max<kType>(largest, raw[v][i]);
+        float top = beam_word_top<kType>(largest);
+        if (top != top) top = -INFINITY;  // nothing but NaN
+        span_top[span - span0][threadIdx.x] = top;
+        mine = fmaxf(mine, top);
+#pragma unroll
+        for (int offset = 16; offset >= 1; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
+        float total = 0.0f;
+        if (top == -INFINITY) {
+            bool bad = false;
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) bad = bad || beam_logit<kType>(raw[v], e) != beam_logit<kType>(raw[v], e);
+            total = bad ? NAN : 0.0f;
+        } else {
+            // The exponentials of the differences to the share's maximum, added as a tree.
+            float2 sums[kVectors];
+            const float2 shift = make_float2(-top, -top), log2_e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v) {
+                float2 weight[kPer / 2];
+#pragma unroll
+                for (int e = 0; e < kPer / 2; ++e) {
+                    const float2 d = add_f32x2(make_float2(beam_logit<kType>(raw[v], 2 * e), beam_logit<kType>(raw[v], 2 * e + 1)), shift);
+                    const float2 power = mul_f32x2(d, log2_e);
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].x) : "f"(power.x));
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].y) : "f"(power.y));
+                }
+#pragma unroll
+                for (int width = kPer / 4; width >= 1; width >>= 1)
+#pragma unroll
+                    for (int e = 0; e < width; ++e) weight[e] = add_f32x2(weight[e], weight[e + width]);
+                sums[v] = weight[0];
+            }
+#pragma unroll
+            for (int width = kVectors / 2; width >= 1; width >>= 1)
+#pragma unroll
+                for (int v = 0; v < width; ++v) sums[v] = add_f32x2(sums[v], sums[v + width]);
+            total = sums[0].x + sums[0].y;
+        }
+        total = warp_sum_xor(total);
+        if (lane == 0) p.stats[(row * p.spans + span) * kWarps + warp] = {top, total};
+    }
+    {
+        float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = top;
+    }
+    __syncthreads();
+    // The keep-th largest bucket, four threads to a bucket: at least `keep` logits of the CTA are not below it.
+    {
+        const int own = threadIdx.x >> 2;
+        const float value = bucket[own];
+        int rank = 0;
+#pragma unroll
+        for (int i = 0; i < kBeamBuckets / 4; ++i) {
+            const int j = 4 * i + (lane & 3);
+            const float other = bucket[j];
+            rank += other > value || (other == value && j < own);
+        }
+        rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
+        rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
+        if (rank == p.keep - 1 && (lane & 3) == 0) bound_shared = value;
+    }
+    __syncthreads();
+    const float bound = bound_shared;
+    // Of the thread's logits not below the bound, each with its token, to `visit`; again from memory.
+    auto reach = [&](auto visit) {
+        if (!(mine >= bound)) return;
+        for (int span = span0; span < span1; ++span) {
+            if (!(span_top[span - span0][threadIdx.x] >= bound)) continue;
+            loader.load(span * kBeamSpan, raw);
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v) {
+                const uint32_t largest = beam_word_max<kType>(beam_word_max<kType>(raw[v][0], raw[v][1]), beam_word_max<kType>(raw[v][2], raw[v][3]));
+                if (!(beam_word_top<kType>(largest) >= bound)) continue;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const int token = span * kBeamSpan + (v * kBeamThreads + (int)threadIdx.x) * kPer + e;
+                    const float logit = beam_logit<kType>(raw[v], e);
+                    if (logit >= bound && token < p.vocabulary) visit(logit, token);
                 }
             }
+        }
     };
-    if (mine >= bound) collect([&](float logit, int) { return logit >= bound; });
+    auto collect = [&](float logit, int token) {
+        const int place = atomicAdd(&count, 1);
+        if (place < kBeamCollect) {
+            collected[place] = logit;
+            collected_token[place] = token;
+        }
+    };
+    reach(collect);
     __syncthreads();
     BeamEntry* list = p.lists + (long long)blockIdx.x * p.keep;
+    const int first = span0 * kBeamSpan, here = min(p.vocabulary, span1 * kBeamSpan) - first;
     int found = count;
     if (found > kBeamCollect) {
-        // More equal ones than the buffer takes.  Where they are the span's least (masked tokens, a constant row) and
-        // few lie above, the first `keep` of them are among its first keep + above elements.
+        // More equal ones than the buffer takes.  Where they are the least there is (masked tokens, a constant row) and
+        // few lie above, the first `keep` of them are among the first keep + above elements.
         int greater = 0;
-#pragma unroll
-        for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) greater += beam_logit<kType>(raw[v], e) > bound;
-        atomicAdd(&above, greater);
+        reach([&](float logit, int) { greater += logit > bound; });
+        if (greater) atomicAdd(&above, greater);
         __syncthreads();
         greater = above;
         const bool least = found == here && 2 * greater + p.keep <= kBeamCollect;
-        __syncthreads();
         if (threadIdx.x == 0) count = 0;
         __syncthreads();
         if (!least) {
@@ -249,89 +310,122 @@ __global__ void __launch_bounds__(kBeamThreads) beam_span_kernel(const BeamSelec
             int last_token = -1;
             for (int r = 0; r < p.keep; ++r) {
                 float best = -INFINITY;
-                int token = 0x7FFFFFFF;
-#pragma unroll
-                for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e) {
-                        const float logit = beam_logit<kType>(raw[v], e);
-                        const int at = (v * kBeamThreads + threadIdx.x) * kPer + e;
-                        const bool behind = logit < last || (logit == last && first + at > last_token);
-                        if (at < here && behind && (logit > best || (logit == best && first + at < token))) {
-                            best = logit;
-                            token = first + at;
-                        }
+                int best_token = 0x7FFFFFFF;
+                reach([&](float logit, int token) {
+                    const bool behind = logit < last || (logit == last && token > last_token);
+                    if (behind && (logit > best || (logit == best && token < best_token))) {
+                        best = logit;
+                        best_token = token;
                     }
+                });
 #pragma unroll
                 for (int offset = 16; offset >= 1; offset >>= 1) {
                     const float other = __shfl_xor_sync(0xFFFFFFFFu, best, offset);
-                    const int other_token = __shfl_xor_sync(0xFFFFFFFFu, token, offset);
-                    if (other > best || (other == best && other_token < token)) { best = other; token = other_token; }
+                    const int other_token = __shfl_xor_sync(0xFFFFFFFFu, best_token, offset);
+                    if (other > best || (other == best && other_token < best_token)) { best = other; best_token = other_token; }
                 }
                 if (lane == 0) {
                     collected[warp] = best;
-                    collected_token[warp] = token;
+                    collected_token[warp] = best_token;
                 }
                 __syncthreads();
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w)
-                    if (collected[w] > best || (collected[w] == best && collected_token[w] < token)) { best = collected[w]; token = collected_token[w]; }
-                if (threadIdx.x == 0) list[r] = {best, token == 0x7FFFFFFF ? -1 : token};
+                    if (collected[w] > best || (collected[w] == best && collected_token[w] < best_token)) { best = collected[w]; best_token = collected_token[w]; }
+                if (threadIdx.x == 0) list[r] = {best, best_token == 0x7FFFFFFF ? -1 : best_token};
                 last = best;
-                last_token = token;
+                last_token = best_token;
                 __syncthreads();
             }
             return;
         }
-        collect([&](float logit, int at) { return logit > bound || (logit == bound && at < p.keep + greater); });
+        reach([&](float logit, int token) {
+            if (logit > bound || token - first < p.keep + greater) collect(logit, token);
+        });
         __syncthreads();
         found = count;
     }
-    for (int i = threadIdx.x; i < found; i += kBeamThreads) {
-        const float logit = collected[i];
-        const int token = collected_token[i];
+    // Eight threads rank an entry.
+    for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += kBeamThreads / 8) {
+        const float logit = i < found ? collected[i] : 0.0f;
+        const int token = i < found ? collected_token[i] : 0;
         int rank = 0;
-        for (int j = 0; j < found; ++j) rank += collected[j] > logit || (collected[j] == logit && collected_token[j] < token);
-        if (rank < p.keep) list[rank] = {logit, token};
+        for (int j = threadIdx.x & 7; j < found; j += 8) rank += collected[j] > logit || (collected[j] == logit && collected_token[j] < token);
+#pragma unroll
+        for (int offset = 1; offset <= 4; offset <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, offset);
+        if (i < found && (lane & 7) == 0 && rank < p.keep) list[rank] = {logit, token};
     }
     for (int i = found + threadIdx.x; i < p.keep; i += kBeamThreads) list[i] = {-INFINITY, -1};
 }
 
-struct BeamCandidate {
-    double value;
-    long long flat;  // beam * vocabulary + token; -1: there is none
+struct __align__(16) BeamCandidate {
+    long long value;  // the 64-bit number as a whole one of the same order
+    long long place;  // beam 2^32 + token; -1: there is none
 };
 __device__ __forceinline__ bool beam_before(const BeamCandidate& a, const BeamCandidate& b) {
-    return a.value > b.value || (a.value == b.value && a.flat < b.flat);
+    return a.value > b.value || (a.value == b.value && a.place < b.place);
+}
+__device__ __forceinline__ long long beam_order(double value) {
+    const long long bits = __double_as_longlong(value + 0.0);  // one zero
+    return bits ^ (bits >> 63 & 0x7FFFFFFFFFFFFFFFll);
+}
+__device__ __forceinline__ double beam_value(long long order) {
+    return __longlong_as_double(order ^ (order >> 63 & 0x7FFFFFFFFFFFFFFFll));
 }
 
-// One CTA per group; a list of sorted candidates for every span of every beam.
+// How many of n candidates come before `own`, eight neighbouring threads together; those without a place do not count.
+__device__ __forceinline__ int beam_rank(const BeamCandidate* candidates, int n, const BeamCandidate& own) {
+    int rank = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x & 7; j < n; j += 8) {
+        const BeamCandidate other = candidates[j];
+        rank += other.place >= 0 && beam_before(other, own);
+    }
+#pragma unroll
+    for (int offset = 1; offset <= 4; offset <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, offset);
+    return rank;
+}
+
+// One CTA per group; a list of sorted candidates for every part of every beam.  Bound by the latency of its steps: what it
+// reads is asked for at once, the first `staged` entries of every list among it.
 template <int kType>
-__global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams p) {
+__global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams p, int staged) {
     extern __shared__ __align__(16) unsigned char join_smem[];
     BeamCandidate* collected = reinterpret_cast<BeamCandidate*>(join_smem);          // [kBeamJoinCollect]
-    BeamCandidate* sample = collected + kBeamJoinCollect;                            // [lists + keep]
-    int* order = reinterpret_cast<int*>(sample + p.beams * p.spans + kBeamMaxKeep);  // [kBeamJoinCollect]
+    BeamEntry* stage = reinterpret_cast<BeamEntry*>(collected + kBeamJoinCollect);   // [lists, staged]
+    int* order = reinterpret_cast<int*>(stage + kBeamStage);                         // [kBeamJoinCollect]
     __shared__ double top[kBeamMaxBeams], log_sum[kBeamMaxBeams], score[kBeamMaxBeams], scratch[32];
     __shared__ unsigned char kind[kBeamMaxBeams];  // 0: a beam's own lists, 1: it has finished, 2: it has no candidate
-    __shared__ BeamCandidate bound;
     __shared__ int count;
     __shared__ unsigned int close;
     const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int lists = p.beams * p.spans;
+    const int lists = p.beams * p.parts;
     const long long row0 = (long long)group * p.beams;
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
+    const BeamEntry* entries = p.lists + row0 * p.parts * p.keep;
+    for (int i = threadIdx.x; i < lists * staged; i += blockDim.x) {
+        const int list = i / staged;
+        ptx::cp_async_8(stage + i, entries + (long long)list * p.keep + (i - list * staged));
+    }
+    ptx::cp_async_commit();
     for (int beam = warp; beam < p.beams; beam += warps) {
         const float given = p.scores[row0 + beam];
         const bool ended = p.finished && p.finished[row0 + beam];
+        const BeamShareStats* stats = p.stats + (row0 + beam) * p.spans * kBeamShares;
+        const int shares = p.spans * kBeamShares;
         float best = -INFINITY;
+#pragma unroll 4
+        for (int i = lane; i < shares; i += 32) best = fmaxf(best, stats[i].top);
+#pragma unroll
+        for (int offset = 16; offset >= 1; offset >>= 1) best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, offset));
         double sum = 0.0;
-        const BeamSpanStats* stats = p.stats + (row0 + beam) * p.spans;
-        BeamSpanStats own = {0.0, -INFINITY};
-        if (lane < p.spans) own = stats[lane];  // 32 spans at most
-        best = warp_max_f32(own.top);
-        if (lane < p.spans) sum = own.sum == 0.0 ? 0.0 : own.sum * exp((double)own.top - (double)best);
+#pragma unroll 4
+        for (int i = lane; i < shares; i += 32) {
+            const BeamShareStats own = stats[i];
+            const double factor = own.sum == 0.0f ? 0.0 : exp((double)own.top - (double)best);
+            sum += (double)own.sum * factor;
+        }
 #pragma unroll
         for (int offset = 16; offset >= 1; offset >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);
         if (lane == 0) {
@@ -342,59 +436,75 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
         }
     }
     if (threadIdx.x == 0) close = 0;
+    ptx::cp_async_wait_group<0>();
     __syncthreads();
-    // Candidate `depth` of a list.
-    auto candidate = [&](int list, int depth) -> BeamCandidate {
-        const int beam = list / p.spans, span = list - beam * p.spans;
-        const long long base = (long long)beam * p.vocabulary;
+    const long long nothing = beam_order(-INFINITY);
+    // Candidate `depth` of a list of a beam.
+    auto candidate = [&](int list, int beam, int depth) -> BeamCandidate {
+        const long long base = (long long)beam << 32;
         if (kind[beam] == 0) {
-            const BeamEntry entry = p.lists[((row0 + beam) * p.spans + span) * p.keep + depth];
-            if (entry.token < 0) return {-INFINITY, -1};
-            return {score[beam] + (((double)entry.logit - top[beam]) - log_sum[beam]), base + entry.token};
+            const BeamEntry entry = depth < staged ? stage[list * staged + depth] : entries[(long long)list * p.keep + depth];
+            if (entry.token < 0) return {nothing, -1};
+            return {beam_order(score[beam] + (((double)entry.logit - top[beam]) - log_sum[beam])), base + entry.token};
         }
+        const int part = list - beam * p.parts;
         long long token = depth;  // no candidate: the first tokens, at -inf
         if (kind[beam] == 1) {
-            if (depth == 0) return span == 0 ? BeamCandidate{score[beam], base + p.end_token} : BeamCandidate{-INFINITY, -1};
+            if (depth == 0) return part == 0 ? BeamCandidate{beam_order(score[beam]), base + p.end_token} : BeamCandidate{nothing, -1};
             token = depth - 1 < p.end_token ? depth - 1 : depth;
         }
-        if (span > 0 || token >= p.vocabulary) return {-INFINITY, -1};
-        return {-INFINITY, base + token};
+        if (part > 0 || token >= p.vocabulary) return {nothing, -1};
+        return {nothing, base + token};
     };
-    // Samples enough for `keep`, the first ones of every list; the keep-th best of them is not above the keep-th best of all.
-    const int depths = min(p.keep, (p.keep + lists - 1) / lists), samples = lists * depths;
+    // The first entries of every list, one to a thread and `keep` at least: what the keep-th best of them reaches bounds the
+    // keep-th best of all from below.  It is found bit by bit, by value and among equals by place, until few reach it.
+    const int depths = min(p.keep, max((p.keep + lists - 1) / lists, (int)blockDim.x / lists)), samples = lists * depths;
+    constexpr unsigned long long kTopBit = 0x8000000000000000ull;
     for (int phase = 0;; ++phase) {
         const double margin = phase == 0 && p.beams > 1 ? 2.0 * kBeamError : 0.0;
-        if (threadIdx.x == 0) {
-            bound = {-INFINITY, 0x7FFFFFFFFFFFFFFFll};
-            count = 0;
+        if (threadIdx.x == 0) count = 0;
+        BeamCandidate sample = {0, -1};
+        if (threadIdx.x < samples) {
+            const int list = threadIdx.x / depths;
+            sample = candidate(list, list / p.parts, threadIdx.x - list * depths);
         }
-        for (int i = threadIdx.x; i < samples; i += blockDim.x) sample[i] = candidate(i / depths, i % depths);
-        __syncthreads();
-        for (int i = threadIdx.x; i < samples; i += blockDim.x) {
-            const BeamCandidate own = sample[i];
-            if (own.flat < 0) continue;
-            int rank = 0;
-            for (int j = 0; j < samples; ++j) rank += sample[j].flat >= 0 && beam_before(sample[j], own);
-            if (rank == p.keep - 1) bound = own;
-        }
-        __syncthreads();
-        const BeamCandidate limit = bound;
-        for (int list = threadIdx.x; list < lists; list += blockDim.x)
-            for (int depth = 0; depth < p.keep; ++depth) {
-                const BeamCandidate own = candidate(list, depth);
-                if (own.flat < 0) break;
-                if (own.value == -INFINITY ? beam_before(limit, own) : own.value < limit.value - margin || (margin == 0.0 && beam_before(limit, own))) break;
-                const int place = atomicAdd(&count, 1);
-                if (place < kBeamJoinCollect) collected[place] = own;
+        const unsigned long long value = (unsigned long long)sample.value ^ kTopBit, place = ~(unsigned long long)sample.place;
+        unsigned long long value_bound = 0, place_bound = 0;
+        int reaching = 0x7FFFFFFF;
+        for (unsigned long long bit = kTopBit; bit && reaching > p.keep + kBeamSlack; bit >>= 1) {
+            const int now = __syncthreads_count(sample.place >= 0 && value >= (value_bound | bit));
+            if (now >= p.keep) {
+                value_bound |= bit;
+                reaching = now;
             }
+        }
+        for (unsigned long long bit = kTopBit; bit && reaching > p.keep + kBeamSlack && value_bound; bit >>= 1) {
+            const int now = __syncthreads_count(sample.place >= 0 && (value > value_bound || (value == value_bound && place >= (place_bound | bit))));
+            if (now >= p.keep) {
+                place_bound |= bit;
+                reaching = now;
+            }
+        }
+        __syncthreads();
+        const unsigned long long least = (unsigned long long)nothing ^ kTopBit;
+        const bool wider = margin > 0.0 && value_bound > least;
+        const unsigned long long reach = wider ? (unsigned long long)beam_order(beam_value((long long)(value_bound ^ kTopBit)) - margin) ^ kTopBit : value_bound;
+        for (int i = threadIdx.x; i < lists * p.keep; i += blockDim.x) {
+            const int list = i / p.keep;
+            const BeamCandidate own = candidate(list, list / p.parts, i - list * p.keep);
+            const unsigned long long value = (unsigned long long)own.value ^ kTopBit;
+            if (own.place < 0 || value < reach || (!wider && value == reach && ~(unsigned long long)own.place < place_bound)) continue;
+            const int at = atomicAdd(&count, 1);
+            if (at < kBeamJoinCollect) collected[at] = own;
+        }
         __syncthreads();
         const int found = count;
-        const bool overflow = found > kBeamJoinCollect;  // of the margin only: without it there are keep lists of keep
+        // Only the margin can let in more: without it what is collected comes from keep + slack lists at most, `keep` from each.
+        const bool overflow = found > kBeamJoinCollect;
         if (!overflow) {
-            for (int i = threadIdx.x; i < found; i += blockDim.x) {
-                int rank = 0;
-                for (int j = 0; j < found; ++j) rank += beam_before(collected[j], collected[i]);
-                order[rank] = i;
+            for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += blockDim.x >> 3) {
+                const int rank = beam_rank(collected, found, collected[min(i, found - 1)]);
+                if (i < found && (lane & 7) == 0) order[rank] = i;
             }
             __syncthreads();
         }
@@ -402,11 +512,12 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             if (overflow) {
                 if (threadIdx.x == 0) close = 0xFFFFFFFFu;
             } else {
+                const double last = beam_value(collected[order[p.keep - 1]].value);  // nobody further below it than the margin can rise
                 for (int i = threadIdx.x; i + 1 < found; i += blockDim.x) {
                     const BeamCandidate upper = collected[order[i]], lower = collected[order[i + 1]];
-                    const int a = (int)(upper.flat / p.vocabulary), b = (int)(lower.flat / p.vocabulary);
-                    if (a != b && lower.value > -INFINITY && upper.value - lower.value <= margin)
-                        atomicOr(&close, 1u << a | 1u << b);
+                    if (i + 1 >= p.keep && last - beam_value(lower.value) > margin) break;
+                    const int a = (int)(upper.place >> 32), b = (int)(lower.place >> 32);
+                    if (a != b && lower.value > nothing && beam_value(upper.value) - beam_value(lower.value) <= margin) atomicOr(&close, 1u << a | 1u << b);
                 }
             }
             __syncthreads();
@@ -415,6 +526,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
                     if (!(close >> beam & 1u) || kind[beam] != 0) continue;
                     const char* row = static_cast<const char*>(p.logits) + (row0 + beam) * p.row_stride * (kType == 2 ? 4 : 2);
                     double sum = 0.0;
+#pragma unroll 4
                     for (int i = threadIdx.x; i < p.vocabulary; i += blockDim.x) sum += exp((double)beam_logit_at<kType>(row, i) - top[beam]);
 #pragma unroll
                     for (int offset = 16; offset >= 1; offset >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);
@@ -432,33 +544,40 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
         }
         for (int r = threadIdx.x; r < p.keep; r += blockDim.x) {
             const BeamCandidate best = collected[order[r]];
-            const int parent = (int)(best.flat / p.vocabulary);
-            const long long token = best.flat - (long long)parent * p.vocabulary, at = (long long)group * p.keep + r;
-            p.scores_out[at] = (float)best.value;
+            const int parent = (int)(best.place >> 32);
+            const long long token = best.place & 0xFFFFFFFFll, at = (long long)group * p.keep + r;
+            p.scores_out[at] = (float)beam_value(best.value);
             p.parents_out[at] = parent;
             p.tokens_out[at] = token;
-            p.finished_out[at] = kind[parent] == 1 || (p.finished && p.finished[row0 + parent]) || token == p.end_token;
+            p.finished_out[at] = (p.finished && p.finished[row0 + parent]) || token == p.end_token;
         }
         return;
     }
 }
 
 template <int kType>
-inline int launch_beam_select(const BeamSelectParams& params, cudaStream_t stream) {
-    const int lists = params.beams * params.spans;
-    int threads = (lists + 31) / 32 * 32;
-    threads = threads < 128 ? 128 : threads;
-    auto smem_of = [](int lists) { return (kBeamJoinCollect + lists + kBeamMaxKeep) * sizeof(BeamCandidate) + kBeamJoinCollect * sizeof(int); };
+inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_t stream) {
+    // As few spans to a CTA as let all CTAs run at once.
+    const long long rows = (long long)params.groups * params.beams, at_once = (long long)sm_count * kBeamAtOnce<kType>;
+    const int most = params.spans < kBeamMostPerPart ? params.spans : kBeamMostPerPart;
+    params.per_part = (params.spans + kBeamMaxParts - 1) / kBeamMaxParts;
+    auto parts_of = [&](int per) { return (params.spans + per - 1) / per; };
+    while (params.per_part < most && rows * parts_of(params.per_part) > at_once) ++params.per_part;
+    params.parts = parts_of(params.per_part);
+    const int lists = params.beams * params.parts;
+    const int threads = lists > 512 ? 1024 : 512;  // a list or more of each
+    const int staged = params.keep < kBeamStage / lists ? params.keep : kBeamStage / lists;
+    constexpr int kSmem = kBeamJoinCollect * (sizeof(BeamCandidate) + sizeof(int)) + kBeamStage * sizeof(BeamEntry);
     static bool configured[64] = {};
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return MT_ERR_LAUNCH;
     if (device >= 64 || !configured[device]) {
-        if (cudaFuncSetAttribute(beam_join_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(1024)) != cudaSuccess)
+        if (cudaFuncSetAttribute(beam_join_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
             return MT_ERR_LAUNCH;
         if (device < 64) configured[device] = true;
     }
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(params.groups * lists, 1, 1);
+    config.gridDim = dim3(params.groups * params.beams * params.parts, 1, 1);
     config.blockDim = dim3(kBeamThreads, 1, 1);
     config.stream = stream;
     cudaLaunchAttribute attrs[1];
@@ -469,8 +588,8 @@ inline int launch_beam_select(const BeamSelectParams& params, cudaStream_t strea
     if (cudaLaunchKernelEx(&config, beam_span_kernel<kType>, params) != cudaSuccess) return MT_ERR_LAUNCH;
     config.gridDim = dim3(params.groups, 1, 1);
     config.blockDim = dim3(threads, 1, 1);
-    config.dynamicSmemBytes = smem_of(lists);
-    return cudaLaunchKernelEx(&config, beam_join_kernel<kType>, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    config.dynamicSmemBytes = kSmem;
+    return cudaLaunchKernelEx(&config, beam_join_kernel<kType>, params, staged) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
 }
 
 }  // namespace mt

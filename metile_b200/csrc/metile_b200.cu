@@ -844,12 +844,14 @@ int mt_beam_select(const void* logits, long long row_stride, int type, const flo
     if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
     if (!device_is_sm100()) return MT_ERR_DEVICE;
     BeamSelectParams params{logits, scores, finished, scores_out, parents_out, tokens_out, finished_out, nullptr, nullptr, row_stride,
-                            end_token, groups, beams, vocabulary, keep, beam_spans(vocabulary)};
-    params.stats = static_cast<BeamSpanStats*>(workspace);
-    params.lists = reinterpret_cast<BeamEntry*>(params.stats + (size_t)groups * beams * params.spans);
+                            end_token, groups, beams, vocabulary, keep, beam_spans(vocabulary), 0, 0};
+    params.stats = static_cast<BeamShareStats*>(workspace);
+    params.lists = reinterpret_cast<BeamEntry*>(params.stats + (size_t)groups * beams * params.spans * kBeamShares);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return type == MT_TYPE_FP32 ? launch_beam_select<2>(params, s) : type == MT_TYPE_FP16 ? launch_beam_select<1>(params, s)
-                                                                                            : launch_beam_select<0>(params, s);
+    const int sms = device_sm_count();
+    if (sms < 1) return MT_ERR_LAUNCH;
+    return type == MT_TYPE_FP32 ? launch_beam_select<2>(params, sms, s) : type == MT_TYPE_FP16 ? launch_beam_select<1>(params, sms, s)
+                                                                                                 : launch_beam_select<0>(params, sms, s);
 }
 
 int mt_beam_reorder(const int* block_tables, long long table_stride, int width, const int* lengths, const int* parents,
