@@ -301,7 +301,7 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
  * there beside the row is never used. */
 #define MT_BEAM_MAX_ROWS 0x000FFFFF
 #define MT_BEAM_MAX_VOCABULARY 0x00080000
-size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep);
+size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep, int type);
 int mt_beam_select(const void* logits, long long row_stride, int type, const float* scores, const unsigned char* finished,
                    long long end_token, float* scores_out, int* parents_out, long long* tokens_out, unsigned char* finished_out,
                    void* workspace, size_t workspace_bytes, int groups, int beams, int vocabulary, int keep, void* stream);

@@ -58,7 +58,7 @@ SIGNATURES = {
     "mt_rope_kv_append_paged": (_i, [_p, _l, _p, _l, _p, _l] + [_p] * 8 + [_i] * 7 + [_p]),
     "mt_paged_attention_decode_workspace_bytes": (_z, [_i] * 6),
     "mt_paged_attention_decode": (_i, [_p] * 6 + [_l, _i, _p, _p, _p, _z] + [_i] * 7 + [_f, _p]),
-    "mt_beam_select_workspace_bytes": (_z, [_i] * 4),
+    "mt_beam_select_workspace_bytes": (_z, [_i] * 5),
     "mt_beam_select": (_i, [_p, _l, _i, _p, _p, _l, _p, _p, _p, _p, _p, _z, _i, _i, _i, _i, _p]),
     "mt_beam_reorder": (_i, [_p, _l, _i] + [_p] * 7 + [_i] * 7 + [_p]),
     "mt_peer_group_create": (_i, [_i, _i, _z, ctypes.POINTER(ctypes.c_void_p), _p]),

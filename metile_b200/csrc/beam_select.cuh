@@ -5,11 +5,12 @@
 // -inf; a score that is a mask) counts as -inf.  Bound by the bytes of the logits, and near to it by the exponentials (an
 // SM takes 16 a cycle: 9 TB/s of 16-bit logits on 148 of them).
 //
-// One pass.  A CTA has some of a row's spans of 8192 logits, 32 a thread and span; each of its warps leaves
-// the maximum and the sum of exponentials of its share of every span, and the CTA the `keep` best of all.  Within a beam candidates
-// are ordered as their logits are, so no sum is needed for that.  Of 64 bucket maxima (four threads each) the keep-th largest
-// bounds the keep-th best from below; the few threads that reach it look at their logits again, and what they find is
-// ranked.  Shares have one size for all calls: a row's bits do not depend on the others.
+// One pass.  Rows are cut into spans of 16 KB, 64 bytes a thread, and the spans of all rows dealt out in runs, one to a CTA; a
+// CTA's share of a row is a part.  Every warp leaves the maximum and the sum of exponentials of its share of a span, and the CTA
+// the `keep` best of each part.  Within a beam candidates are ordered as their logits are, so no sum is needed for that.  Of
+// 64 bucket maxima (four threads each) the keep-th largest bounds the keep-th best from below; the few threads that reach it
+// look at their logits again, and what they find is ranked.  The shares of a row have one size for all calls: its bits do
+// not depend on the others.
 //
 // Then a CTA per group joins spans and beams.  The sums are of 32-bit exponentials, each beam's log-sum off by up to
 // kBeamError; where two beams' candidates are closer than twice that, the sums of the two are taken again, in 64 bits, so
@@ -30,12 +31,18 @@ constexpr double kDeadScore = -1e9;  // no sum of log-probabilities but the mask
 constexpr double kBeamError = 0x1p-18;
 
 constexpr int kBeamMaxBeams = 32, kBeamMaxKeep = 64;
-constexpr int kBeamThreads = 256, kBeamPerThread = 32, kBeamSpan = kBeamThreads * kBeamPerThread, kBeamShares = kBeamThreads / 32;
-constexpr int kBeamMaxParts = 32, kBeamMostPerPart = 16;     // CTAs of a row (at most 1024 lists to join), spans of a CTA
-constexpr int kBeamMaxVocabulary = 64 * kBeamSpan;
-constexpr int kBeamBuckets = 64, kBeamCollect = 1024;        // of a CTA
+constexpr int kBeamThreads = 256, kBeamVectors = 4, kBeamSpanBytes = kBeamThreads * kBeamVectors * 16, kBeamShares = kBeamThreads / 32;
+constexpr int kBeamMaxParts = 32, kBeamMostPerPart = 16;     // parts of a row (at most 1024 lists to join), spans of a part
+constexpr int kBeamAtOnce = 3, kBeamStages = 3;              // CTAs of an SM, spans each has in flight or in work
+constexpr int kBeamBlock = 512 + 16;                         // a warp's vectors of one step, and the one behind them
+constexpr int kBeamRing = kBeamStages * kBeamShares * kBeamVectors * kBeamBlock;
+constexpr int kBeamBuckets = 64, kBeamCollect = 512;         // of a part
+static_assert(kBeamCollect >= kBeamMaxKeep + kBeamThreads, "equal ones are collected a step of all threads at a time");
 constexpr int kBeamSlack = 8, kBeamJoinCollect = (kBeamMaxKeep + kBeamSlack) * kBeamMaxKeep, kBeamStage = 4096;
-static_assert(kBeamBuckets >= kBeamMaxKeep && kBeamMaxVocabulary == MT_BEAM_MAX_VOCABULARY, "bounds of the selection");
+static_assert(kBeamBuckets >= kBeamMaxKeep, "the bound of a part comes from its buckets");
+
+__host__ __device__ constexpr int beam_size(int type) { return type == 2 ? 4 : 2; }               // bytes of a logit
+__host__ __device__ constexpr int beam_span(int type) { return kBeamSpanBytes / beam_size(type); }  // logits
 
 struct BeamShareStats {
     float top, sum;  // of exp(logit - top); NaN: there is a NaN or +inf
@@ -55,15 +62,34 @@ struct BeamSelectParams {
     long long* tokens_out;
     unsigned char* finished_out;
     BeamShareStats* stats;          // [groups * beams, spans * 8]
-    BeamEntry* lists;               // [groups * beams, parts, keep]
+    BeamEntry* lists;               // [groups * beams, parts, keep], as many as a row has parts
     long long row_stride, end_token;  // no end token: -1
     int groups, beams, vocabulary, keep, spans;
-    int parts, per_part;            // CTAs of a row, spans of each
+    int parts, runs;                // the most parts of a row; CTAs
 };
 
-inline int beam_spans(int vocabulary) { return (vocabulary + kBeamSpan - 1) / kBeamSpan; }
-inline size_t beam_workspace_bytes(int groups, int beams, int vocabulary, int keep) {
-    return (size_t)groups * beams * beam_spans(vocabulary) * (kBeamShares * sizeof(BeamShareStats) + (size_t)keep * sizeof(BeamEntry));
+// Run r of S spans dealt out to R: from its first span to the next one's.  And the run a span is in.
+__host__ __device__ inline long long beam_run_start(long long run, long long spans, long long runs) { return run * spans / runs; }
+__host__ __device__ inline long long beam_run_of(long long span, long long spans, long long runs) { return ((span + 1) * runs - 1) / spans; }
+
+inline int beam_spans(int vocabulary, int type) { return (vocabulary + beam_span(type) - 1) / beam_span(type); }
+
+// What the host and the kernels go by: as many CTAs as run at once, but no run longer than a part may be, and no row in more
+// parts than the join takes.
+inline void beam_plan(int rows, int spans, int sm_count, int& parts, int& runs) {
+    const long long all = (long long)rows * spans;
+    long long count = (long long)sm_count * kBeamAtOnce;
+    if (count < (all + kBeamMostPerPart - 1) / kBeamMostPerPart) count = (all + kBeamMostPerPart - 1) / kBeamMostPerPart;
+    if (count > (long long)rows * (kBeamMaxParts - 2)) count = (long long)rows * (kBeamMaxParts - 2);
+    if (count > all) count = all;
+    runs = (int)count;
+    parts = (int)((spans - 1) * count / all) + 2;
+    if (parts > spans) parts = spans;
+}
+
+inline size_t beam_workspace_bytes(int groups, int beams, int vocabulary, int keep, int type) {
+    const int spans = beam_spans(vocabulary, type);  // parts at most
+    return (size_t)groups * beams * ((size_t)spans * kBeamShares * sizeof(BeamShareStats) + (size_t)(spans < kBeamMaxParts ? spans : kBeamMaxParts) * keep * sizeof(BeamEntry));
 }
 
 // kType: 0 bf16, 1 fp16, 2 fp32.
@@ -126,236 +152,265 @@ __device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
 
 // A thread's logits of a span: element e of vector v is the span's (v * 256 + thread) * kPer + e; those behind the row are -inf.
 template <int kType>
-struct BeamLoader {
-    static constexpr int kPer = kType == 2 ? 4 : 8, kVectors = kBeamPerThread / kPer, kSize = kType == 2 ? 4 : 2;
-    const char* row;
-    int vocabulary;
+struct BeamSpan {
+    static constexpr int kSize = beam_size(kType), kPer = 16 / kSize;
+    const char* from;  // the first logit
+    int here, skew;    // logits of the span; bytes by which it starts behind a boundary
 
-    __device__ __forceinline__ void load(int first, uint32_t (&raw)[kVectors][4]) const {
-        const int here = min(kBeamSpan, vocabulary - first);
-        const char* from = row + (long long)first * kSize;
-        const int skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+    __device__ __forceinline__ BeamSpan(const BeamSelectParams& p, long long row, int span) {
+        from = static_cast<const char*>(p.logits) + (row * p.row_stride + (long long)span * beam_span(kType)) * kSize;
+        here = min(beam_span(kType), p.vocabulary - span * beam_span(kType));
+        skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+    }
+    __device__ __forceinline__ int at(int v) const { return (v * kBeamThreads + (int)threadIdx.x) * kPer; }
+    __device__ __forceinline__ const char* vector(int at) const { return from - skew + (long long)at * kSize; }  // aligned
+
+    // Into a warp's part of the ring: its vectors of a step one after the other, and the one behind them.
+    __device__ __forceinline__ void copy(char* ring) const {
+        const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int v = 0; v < kVectors; ++v) {
-            const int at = (v * kBeamThreads + threadIdx.x) * kPer;
-            uint4 vector = make_uint4(0u, 0u, 0u, 0u);
-            if (at < here) vector = ptx::ld_global_dependent_u4(from - skew + (long long)at * kSize);
-            raw[v][0] = vector.x; raw[v][1] = vector.y; raw[v][2] = vector.z; raw[v][3] = vector.w;
+        for (int v = 0; v < kBeamVectors; ++v) {
+            // (The neighbour may need this one where the thread itself has no logit in it.)
+            if (at(v) - skew / kSize < here) ptx::cp_async_16(ring + v * kBeamBlock + lane * 16, vector(at(v)));
+            if (lane == 31 && skew && at(v) + (16 - skew) / kSize < here) ptx::cp_async_16(ring + v * kBeamBlock + 512, vector(at(v)) + 16);
         }
-        if (skew) {  // a row that starts off a boundary: the aligned vector behind each as well
-            uint4 behind[kVectors];
+    }
+    __device__ __forceinline__ void take(uint32_t (&raw)[kBeamVectors][4], const char* ring) const {
+        const int lane = threadIdx.x & 31;
 #pragma unroll
-            for (int v = 0; v < kVectors; ++v) {
-                const int at = (v * kBeamThreads + threadIdx.x) * kPer;
-                behind[v] = make_uint4(0u, 0u, 0u, 0u);
-                if (at + (16 - skew) / kSize < here) behind[v] = ptx::ld_global_dependent_u4(from - skew + (long long)at * kSize + 16);
+        for (int v = 0; v < kBeamVectors; ++v) {
+            const uint4 own = *reinterpret_cast<const uint4*>(ring + v * kBeamBlock + lane * 16);
+            if (skew) {
+                take_skewed(raw[v], own, *reinterpret_cast<const uint4*>(ring + v * kBeamBlock + lane * 16 + 16), skew);
+            } else {
+                raw[v][0] = own.x; raw[v][1] = own.y; raw[v][2] = own.z; raw[v][3] = own.w;
             }
-#pragma unroll
-            for (int v = 0; v < kVectors; ++v)
-                take_skewed(raw[v], make_uint4(raw[v][0], raw[v][1], raw[v][2], raw[v][3]), behind[v], skew);
         }
-        if (here < kBeamSpan) {
+        mask(raw);
+    }
+
+private:
+    __device__ __forceinline__ void mask(uint32_t (&raw)[kBeamVectors][4]) const {
+        if (here == beam_span(kType)) return;
 #pragma unroll
-            for (int v = 0; v < kVectors; ++v)
+        for (int v = 0; v < kBeamVectors; ++v)
 #pragma unroll
-                for (int e = 0; e < kPer; ++e)
-                    if ((v * kBeamThreads + (int)threadIdx.x) * kPer + e >= here) {
-                        if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
-                        else {
-                            const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
-                            raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
-                        }
+            for (int e = 0; e < kPer; ++e)
+                if (at(v) + e >= here) {
+                    if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
+                    else {
+                        const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
+                        raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
                     }
-        }
+                }
     }
 };
 
 template <int kType>
-constexpr int kBeamAtOnce = kType == 2 ? 3 : 5;  // CTAs of an SM
-
-template <int kType>
-__global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce<kType>) beam_span_kernel(const BeamSelectParams p) {
-    using Loader = BeamLoader<kType>;
-    constexpr int kPer = Loader::kPer, kVectors = Loader::kVectors, kWarps = kBeamShares;
+__global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(const BeamSelectParams p) {
+    using Span = BeamSpan<kType>;
+    constexpr int kPer = Span::kPer, kVectors = kBeamVectors, kWarps = kBeamShares;
+    extern __shared__ __align__(16) char beam_ring[];  // [warps][stages][vectors][block]
     __shared__ float span_top[kBeamMostPerPart][kBeamThreads], bucket[kBeamBuckets];
     __shared__ float collected[kBeamCollect], bound_shared;
     __shared__ int collected_token[kBeamCollect], count, above;
-    const int part = blockIdx.x % p.parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long row = blockIdx.x / p.parts;
-    const int span0 = part * p.per_part, span1 = min(p.spans, span0 + p.per_part);
-    const Loader loader{static_cast<const char*>(p.logits) + row * p.row_stride * Loader::kSize, p.vocabulary};
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long spans = (long long)p.groups * p.beams * p.spans;
+    const long long run0 = beam_run_start(blockIdx.x, spans, p.runs), run1 = beam_run_start(blockIdx.x + 1, spans, p.runs);
+    char* ring = beam_ring + warp * (kBeamStages * kVectors * kBeamBlock);
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    if (threadIdx.x == 0) count = above = 0;
-    float mine = -INFINITY;
-    uint32_t raw[kVectors][4];
-    for (int span = span0; span < span1; ++span) {
-        loader.load(span * kBeamSpan, raw);
-        uint32_t largest = raw[0][0];
+    long long copy_row = run0 / p.spans;
+    int copy_span = (int)(run0 - copy_row * p.spans), to_copy = (int)(run1 - run0);
+    auto copy_next = [&](int slot) {
+        if (to_copy > 0) {
+            Span(p, copy_row, copy_span).copy(ring + slot * (kVectors * kBeamBlock));
+            --to_copy;
+            if (++copy_span == p.spans) {
+                copy_span = 0;
+                ++copy_row;
+            }
+        }
+        ptx::cp_async_commit();
+    };
 #pragma unroll
-        for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) largest = beam_word_max<kType>(largest, raw[v][i]);
-        float top = beam_word_top<kType>(largest);
-        if (top != top) top = -INFINITY;  // nothing but NaN
-        span_top[span - span0][threadIdx.x] = top;
-        mine = fmaxf(mine, top);
-#pragma unroll
-        for (int offset = 16; offset >= 1; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
-        float total = 0.0f;
-        if (top == -INFINITY) {
-            bool bad = false;
+    for (int i = 0; i < kBeamStages - 1; ++i) copy_next(i);
+    int slot = 0;
+    for (long long start = run0; start < run1;) {  // a part: what the run has of one row
+        const long long row = start / p.spans;
+        const int span0 = (int)(start - row * p.spans), span1 = (int)min((long long)p.spans, span0 + (run1 - start));
+        start += span1 - span0;
+        if (threadIdx.x == 0) count = above = 0;
+        float mine = -INFINITY;
+        uint32_t raw[kVectors][4];
+        for (int span = span0; span < span1; ++span) {
+            ptx::cp_async_wait_group<kBeamStages - 2>();
+            __syncwarp();
+            Span(p, row, span).take(raw, ring + slot * (kVectors * kBeamBlock));
+            __syncwarp();
+            copy_next(slot == 0 ? kBeamStages - 1 : slot - 1);
+            slot = slot == kBeamStages - 1 ? 0 : slot + 1;
+            uint32_t largest = raw[0][0];
 #pragma unroll
             for (int v = 0; v < kVectors; ++v)
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) bad = bad || beam_logit<kType>(raw[v], e) != beam_logit<kType>(raw[v], e);
-            total = bad ? NAN : 0.0f;
-        } else {
-            // The exponentials of the differences to the share's maximum, added as a tree.
-            float2 sums[kVectors];
-            const float2 shift = make_float2(-top, -top), log2_e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+                for (int i = 0; i < 4; ++i) largest = beam_word_max<kType>(largest, raw[v][i]);
+            float top = beam_word_top<kType>(largest);
+            if (top != top) top = -INFINITY;  // nothing but NaN
+            span_top[span - span0][threadIdx.x] = top;
+            mine = fmaxf(mine, top);
 #pragma unroll
-            for (int v = 0; v < kVectors; ++v) {
-                float2 weight[kPer / 2];
+            for (int offset = 16; offset >= 1; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
+            float total = 0.0f;
+            if (top == -INFINITY) {
+                bool bad = false;
 #pragma unroll
-                for (int e = 0; e < kPer / 2; ++e) {
-                    const float2 d = add_f32x2(make_float2(beam_logit<kType>(raw[v], 2 * e), beam_logit<kType>(raw[v], 2 * e + 1)), shift);
-                    const float2 power = mul_f32x2(d, log2_e);
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].x) : "f"(power.x));
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].y) : "f"(power.y));
-                }
+                for (int v = 0; v < kVectors; ++v)
 #pragma unroll
-                for (int width = kPer / 4; width >= 1; width >>= 1)
+                    for (int e = 0; e < kPer; ++e) bad = bad || beam_logit<kType>(raw[v], e) != beam_logit<kType>(raw[v], e);
+                total = bad ? NAN : 0.0f;
+            } else {
+                // The exponentials of the differences to the share's maximum, added as a tree.
+                float2 sums[kVectors];
+                const float2 shift = make_float2(-top, -top), log2_e = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-                    for (int e = 0; e < width; ++e) weight[e] = add_f32x2(weight[e], weight[e + width]);
-                sums[v] = weight[0];
-            }
+                for (int v = 0; v < kVectors; ++v) {
+                    float2 weight[kPer / 2];
 #pragma unroll
-            for (int width = kVectors / 2; width >= 1; width >>= 1)
-#pragma unroll
-                for (int v = 0; v < width; ++v) sums[v] = add_f32x2(sums[v], sums[v + width]);
-            total = sums[0].x + sums[0].y;
-        }
-        total = warp_sum_xor(total);
-        if (lane == 0) p.stats[(row * p.spans + span) * kWarps + warp] = {top, total};
-    }
-    {
-        float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = top;
-    }
-    __syncthreads();
-    // The keep-th largest bucket, four threads to a bucket: at least `keep` logits of the CTA are not below it.
-    {
-        const int own = threadIdx.x >> 2;
-        const float value = bucket[own];
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < kBeamBuckets / 4; ++i) {
-            const int j = 4 * i + (lane & 3);
-            const float other = bucket[j];
-            rank += other > value || (other == value && j < own);
-        }
-        rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
-        rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
-        if (rank == p.keep - 1 && (lane & 3) == 0) bound_shared = value;
-    }
-    __syncthreads();
-    const float bound = bound_shared;
-    // Of the thread's logits not below the bound, each with its token, to `visit`; again from memory.
-    auto reach = [&](auto visit) {
-        if (!(mine >= bound)) return;
-        for (int span = span0; span < span1; ++span) {
-            if (!(span_top[span - span0][threadIdx.x] >= bound)) continue;
-            loader.load(span * kBeamSpan, raw);
-#pragma unroll
-            for (int v = 0; v < kVectors; ++v) {
-                const uint32_t largest = beam_word_max<kType>(beam_word_max<kType>(raw[v][0], raw[v][1]), beam_word_max<kType>(raw[v][2], raw[v][3]));
-                if (!(beam_word_top<kType>(largest) >= bound)) continue;
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const int token = span * kBeamSpan + (v * kBeamThreads + (int)threadIdx.x) * kPer + e;
-                    const float logit = beam_logit<kType>(raw[v], e);
-                    if (logit >= bound && token < p.vocabulary) visit(logit, token);
-                }
-            }
-        }
-    };
-    auto collect = [&](float logit, int token) {
-        const int place = atomicAdd(&count, 1);
-        if (place < kBeamCollect) {
-            collected[place] = logit;
-            collected_token[place] = token;
-        }
-    };
-    reach(collect);
-    __syncthreads();
-    BeamEntry* list = p.lists + (long long)blockIdx.x * p.keep;
-    const int first = span0 * kBeamSpan, here = min(p.vocabulary, span1 * kBeamSpan) - first;
-    int found = count;
-    if (found > kBeamCollect) {
-        // More equal ones than the buffer takes.  Where they are the least there is (masked tokens, a constant row) and
-        // few lie above, the first `keep` of them are among the first keep + above elements.
-        int greater = 0;
-        reach([&](float logit, int) { greater += logit > bound; });
-        if (greater) atomicAdd(&above, greater);
-        __syncthreads();
-        greater = above;
-        const bool least = found == here && 2 * greater + p.keep <= kBeamCollect;
-        if (threadIdx.x == 0) count = 0;
-        __syncthreads();
-        if (!least) {
-            // `keep` rounds: the best behind the last one.
-            float last = INFINITY;
-            int last_token = -1;
-            for (int r = 0; r < p.keep; ++r) {
-                float best = -INFINITY;
-                int best_token = 0x7FFFFFFF;
-                reach([&](float logit, int token) {
-                    const bool behind = logit < last || (logit == last && token > last_token);
-                    if (behind && (logit > best || (logit == best && token < best_token))) {
-                        best = logit;
-                        best_token = token;
+                    for (int e = 0; e < kPer / 2; ++e) {
+                        const float2 d = add_f32x2(make_float2(beam_logit<kType>(raw[v], 2 * e), beam_logit<kType>(raw[v], 2 * e + 1)), shift);
+                        const float2 power = mul_f32x2(d, log2_e);
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].x) : "f"(power.x));
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].y) : "f"(power.y));
                     }
-                });
 #pragma unroll
-                for (int offset = 16; offset >= 1; offset >>= 1) {
-                    const float other = __shfl_xor_sync(0xFFFFFFFFu, best, offset);
-                    const int other_token = __shfl_xor_sync(0xFFFFFFFFu, best_token, offset);
-                    if (other > best || (other == best && other_token < best_token)) { best = other; best_token = other_token; }
+                    for (int width = kPer / 4; width >= 1; width >>= 1)
+#pragma unroll
+                        for (int e = 0; e < width; ++e) weight[e] = add_f32x2(weight[e], weight[e + width]);
+                    sums[v] = weight[0];
                 }
-                if (lane == 0) {
-                    collected[warp] = best;
-                    collected_token[warp] = best_token;
+#pragma unroll
+                for (int width = kVectors / 2; width >= 1; width >>= 1)
+#pragma unroll
+                    for (int v = 0; v < width; ++v) sums[v] = add_f32x2(sums[v], sums[v + width]);
+                total = sums[0].x + sums[0].y;
+            }
+            total = warp_sum_xor(total);
+            if (lane == 0) p.stats[(row * p.spans + span) * kWarps + warp] = {top, total};
+        }
+        {
+            float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = top;
+        }
+        __syncthreads();
+        // The keep-th largest bucket, four threads to a bucket: at least `keep` logits of the CTA are not below it.
+        {
+            const int own = threadIdx.x >> 2;
+            const float value = bucket[own];
+            int rank = 0;
+#pragma unroll
+            for (int i = 0; i < kBeamBuckets / 4; ++i) {
+                const int j = 4 * i + (lane & 3);
+                const float other = bucket[j];
+                rank += other > value || (other == value && j < own);
+            }
+            rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
+            rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
+            if (rank == p.keep - 1 && (lane & 3) == 0) bound_shared = value;
+        }
+        __syncthreads();
+        const float bound = bound_shared;
+        // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens.
+        const char* from = static_cast<const char*>(p.logits) + row * p.row_stride * beam_size(kType);
+        auto reach = [&](auto qualifies, auto visit) {
+            for (int span = span0; span < span1 && count <= kBeamCollect; ++span) {
+                unsigned int threads = __ballot_sync(0xFFFFFFFFu, qualifies(span_top[span - span0][threadIdx.x]));
+                for (; threads; threads &= threads - 1u) {
+                    const int thread = warp * 32 + __ffs(threads) - 1;
+                    const int token = span * beam_span(kType) + ((lane / kPer) * kBeamThreads + thread) * kPer + lane % kPer;
+                    if (lane < kVectors * kPer && token < p.vocabulary) visit(beam_logit_at<kType>(from, token), token);
                 }
+            }
+        };
+        auto collect = [&](float logit, int token) {
+            const int place = atomicAdd(&count, 1);
+            if (place < kBeamCollect) {
+                collected[place] = logit;
+                collected_token[place] = token;
+            }
+        };
+        reach([&](float top) { return top >= bound; }, [&](float logit, int token) { if (logit >= bound) collect(logit, token); });
+        __syncthreads();
+        const int part = (int)(blockIdx.x - beam_run_of(row * p.spans, spans, p.runs));
+        BeamEntry* list = p.lists + (row * p.parts + part) * p.keep;
+        int found = count;
+        if (found > kBeamCollect) {
+            // Very many equal ones (masked tokens, a constant row).  What lies above them, then the first of themselves.
+            const int first = span0 * beam_span(kType), last = min(p.vocabulary, span1 * beam_span(kType));
+            __syncthreads();
+            if (threadIdx.x == 0) count = 0;
+            __syncthreads();
+            reach([&](float top) { return top > bound; }, [&](float logit, int token) { if (logit > bound) collect(logit, token); });
+            __syncthreads();
+            found = count;
+            if (found > kBeamCollect) {
+                // The large ones lie in few buckets: `keep` rounds over everything, each for the best behind the last.
+                float before = INFINITY;
+                int before_token = -1;
+                for (int r = 0; r < p.keep; ++r) {
+                    float best = -INFINITY;
+                    int best_token = 0x7FFFFFFF;
+                    for (int token = first + threadIdx.x; token < last; token += kBeamThreads) {
+                        const float logit = beam_logit_at<kType>(from, token);
+                        const bool behind = logit < before || (logit == before && token > before_token);
+                        if (behind && (logit > best || (logit == best && token < best_token))) {
+                            best = logit;
+                            best_token = token;
+                        }
+                    }
+#pragma unroll
+                    for (int offset = 16; offset >= 1; offset >>= 1) {
+                        const float other = __shfl_xor_sync(0xFFFFFFFFu, best, offset);
+                        const int other_token = __shfl_xor_sync(0xFFFFFFFFu, best_token, offset);
+                        if (other > best || (other == best && other_token < best_token)) { best = other; best_token = other_token; }
+                    }
+                    if (lane == 0) {
+                        collected[warp] = best;
+                        collected_token[warp] = best_token;
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w)
+                        if (collected[w] > best || (collected[w] == best && collected_token[w] < best_token)) { best = collected[w]; best_token = collected_token[w]; }
+                    if (threadIdx.x == 0) list[r] = {best, best_token == 0x7FFFFFFF ? -1 : best_token};
+                    before = best;
+                    before_token = best_token;
+                    __syncthreads();
+                }
+                continue;
+            }
+            for (int at = first; at < last && found < p.keep; at += kBeamThreads) {  // room for all of a step: keep + 256
+                const int token = at + threadIdx.x;
+                if (token < last && beam_logit_at<kType>(from, token) == bound) collect(bound, token);
                 __syncthreads();
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w)
-                    if (collected[w] > best || (collected[w] == best && collected_token[w] < best_token)) { best = collected[w]; best_token = collected_token[w]; }
-                if (threadIdx.x == 0) list[r] = {best, best_token == 0x7FFFFFFF ? -1 : best_token};
-                last = best;
-                last_token = best_token;
+                found = count;
                 __syncthreads();
             }
-            return;
         }
-        reach([&](float logit, int token) {
-            if (logit > bound || token - first < p.keep + greater) collect(logit, token);
-        });
-        __syncthreads();
-        found = count;
-    }
-    // Eight threads rank an entry.
-    for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += kBeamThreads / 8) {
-        const float logit = i < found ? collected[i] : 0.0f;
-        const int token = i < found ? collected_token[i] : 0;
-        int rank = 0;
-        for (int j = threadIdx.x & 7; j < found; j += 8) rank += collected[j] > logit || (collected[j] == logit && collected_token[j] < token);
+        // Eight threads rank an entry.
+        for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += kBeamThreads / 8) {
+            const float logit = i < found ? collected[i] : 0.0f;
+            const int token = i < found ? collected_token[i] : 0;
+            int rank = 0;
+            for (int j = threadIdx.x & 7; j < found; j += 8) rank += collected[j] > logit || (collected[j] == logit && collected_token[j] < token);
 #pragma unroll
-        for (int offset = 1; offset <= 4; offset <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, offset);
-        if (i < found && (lane & 7) == 0 && rank < p.keep) list[rank] = {logit, token};
+            for (int offset = 1; offset <= 4; offset <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, offset);
+            if (i < found && (lane & 7) == 0 && rank < p.keep) list[rank] = {logit, token};
+        }
+        for (int i = found + threadIdx.x; i < p.keep; i += kBeamThreads) list[i] = {-INFINITY, -1};
+        __syncthreads();
     }
-    for (int i = found + threadIdx.x; i < p.keep; i += kBeamThreads) list[i] = {-INFINITY, -1};
 }
 
 struct __align__(16) BeamCandidate {
@@ -396,7 +451,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
     int* order = reinterpret_cast<int*>(stage + kBeamStage);                         // [kBeamJoinCollect]
     __shared__ double top[kBeamMaxBeams], log_sum[kBeamMaxBeams], score[kBeamMaxBeams], scratch[32];
     __shared__ unsigned char kind[kBeamMaxBeams];  // 0: a beam's own lists, 1: it has finished, 2: it has no candidate
-    __shared__ int count;
+    __shared__ int count, own_parts[kBeamMaxBeams];
     __shared__ unsigned int close;
     const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int lists = p.beams * p.parts;
@@ -432,6 +487,8 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             top[beam] = best;
             log_sum[beam] = log(sum);
             score[beam] = given;
+            const long long all = (long long)p.groups * p.beams * p.spans, first = (row0 + beam) * p.spans;
+            own_parts[beam] = (int)(beam_run_of(first + p.spans - 1, all, p.runs) - beam_run_of(first, all, p.runs)) + 1;
             kind[beam] = !(given > kDeadScore) ? 2 : ended ? 1 : !(sum > 0.0 && sum < INFINITY && best < INFINITY) ? 2 : 0;
         }
     }
@@ -443,6 +500,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
     auto candidate = [&](int list, int beam, int depth) -> BeamCandidate {
         const long long base = (long long)beam << 32;
         if (kind[beam] == 0) {
+            if (list - beam * p.parts >= own_parts[beam]) return {nothing, -1};
             const BeamEntry entry = depth < staged ? stage[list * staged + depth] : entries[(long long)list * p.keep + depth];
             if (entry.token < 0) return {nothing, -1};
             return {beam_order(score[beam] + (((double)entry.logit - top[beam]) - log_sum[beam])), base + entry.token};
@@ -557,13 +615,8 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
 
 template <int kType>
 inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_t stream) {
-    // As few spans to a CTA as let all CTAs run at once.
-    const long long rows = (long long)params.groups * params.beams, at_once = (long long)sm_count * kBeamAtOnce<kType>;
-    const int most = params.spans < kBeamMostPerPart ? params.spans : kBeamMostPerPart;
-    params.per_part = (params.spans + kBeamMaxParts - 1) / kBeamMaxParts;
-    auto parts_of = [&](int per) { return (params.spans + per - 1) / per; };
-    while (params.per_part < most && rows * parts_of(params.per_part) > at_once) ++params.per_part;
-    params.parts = parts_of(params.per_part);
+    params.spans = beam_spans(params.vocabulary, kType);
+    beam_plan(params.groups * params.beams, params.spans, sm_count, params.parts, params.runs);
     const int lists = params.beams * params.parts;
     const int threads = lists > 512 ? 1024 : 512;  // a list or more of each
     const int staged = params.keep < kBeamStage / lists ? params.keep : kBeamStage / lists;
@@ -574,11 +627,13 @@ inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_
     if (device >= 64 || !configured[device]) {
         if (cudaFuncSetAttribute(beam_join_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
             return MT_ERR_LAUNCH;
+        if (cudaFuncSetAttribute(beam_span_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamRing) != cudaSuccess) return MT_ERR_LAUNCH;
         if (device < 64) configured[device] = true;
     }
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(params.groups * params.beams * params.parts, 1, 1);
+    config.gridDim = dim3(params.runs, 1, 1);
     config.blockDim = dim3(kBeamThreads, 1, 1);
+    config.dynamicSmemBytes = kBeamRing;
     config.stream = stream;
     cudaLaunchAttribute attrs[1];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

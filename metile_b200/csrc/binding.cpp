@@ -631,7 +631,7 @@ PyObject* beam_select(PyObject* const* args) {
     const Launch launch(device);
     Tensor scores_out = new_of({groups, keep}, at::kFloat, device), parents = new_of({groups, keep}, at::kInt, device);
     Tensor tokens = new_of({groups, keep}, at::kLong, device), finished_out = new_of({groups, keep}, at::kBool, device);
-    const size_t needed = mt_beam_select_workspace_bytes((int)groups, (int)beams, (int)vocabulary, (int)keep);
+    const size_t needed = mt_beam_select_workspace_bytes((int)groups, (int)beams, (int)vocabulary, (int)keep, type);
     c10::DataPtr scratch;
     if (needed) scratch = call_scratch(needed);
     int code;

@@ -824,9 +824,9 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
     return half ? launch_paged_attention<256, true>(params, sms, s) : launch_paged_attention<256, false>(params, sms, s);
 }
 
-size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep) {
+size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep, int type) {
     if (groups <= 0 || beams <= 0 || vocabulary <= 0 || keep <= 0) return 0;
-    return beam_workspace_bytes(groups, beams, vocabulary, keep);
+    return beam_workspace_bytes(groups, beams, vocabulary, keep, type);
 }
 
 int mt_beam_select(const void* logits, long long row_stride, int type, const float* scores, const unsigned char* finished,
@@ -840,11 +840,11 @@ int mt_beam_select(const void* logits, long long row_stride, int type, const flo
     if (groups == 0) return MT_OK;
     if (!logits || !scores || !scores_out || !parents_out || !tokens_out || !finished_out) return MT_ERR_NULL;
     if (!aligned_to(logits, type == MT_TYPE_FP32 ? 4 : 2)) return MT_ERR_ALIGN;
-    const size_t needed = mt_beam_select_workspace_bytes(groups, beams, vocabulary, keep);
+    const size_t needed = mt_beam_select_workspace_bytes(groups, beams, vocabulary, keep, type);
     if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
     if (!device_is_sm100()) return MT_ERR_DEVICE;
     BeamSelectParams params{logits, scores, finished, scores_out, parents_out, tokens_out, finished_out, nullptr, nullptr, row_stride,
-                            end_token, groups, beams, vocabulary, keep, beam_spans(vocabulary), 0, 0};
+                            end_token, groups, beams, vocabulary, keep, beam_spans(vocabulary, type), 0, 0};
     params.stats = static_cast<BeamShareStats*>(workspace);
     params.lists = reinterpret_cast<BeamEntry*>(params.stats + (size_t)groups * beams * params.spans * kBeamShares);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -83,6 +83,18 @@ def test_many_equal_logits_at_any_level(cuda_device, levels, keep):
     check_select(logits[:1], scores[:1, :1].contiguous(), keep)
 
 
+def test_the_largest_logits_side_by_side(cuda_device):
+    """All of the large ones in the vectors of few threads, more of them than a buffer takes, and in order."""
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.zeros((2, 100000), device=cuda_device)
+        at = torch.arange(100000, device=cuda_device)
+        near = at // (32 if dtype == torch.float32 else 64) % 32 == 5
+        logits[0, near] = 1.0 + at[near].float() / 100000
+        logits[1] = at.float() / 100000
+        for keep in (2, 64):
+            check_select(logits.to(dtype), torch.zeros((1, 2), device=cuda_device), keep)
+
+
 def test_candidates_of_two_beams_closer_than_32_bits_tell(cuda_device):
     """One beam's score is moved so that its best candidate lies a hair above or below the other beam's: the order is
     the one of 64 bits."""

@@ -66,7 +66,7 @@ def test_attention_refusals_of_the_abi():
 
 def test_select_and_reorder_refusals_of_the_abi():
     lib = _lib.load()
-    workspace = lib.mt_beam_select_workspace_bytes(2, 4, 100, 8)
+    workspace = lib.mt_beam_select_workspace_bytes(2, 4, 100, 8, 0)
 
     def select(logits=ONE, type=0, finished=ONE, end=3, groups=2, beams=4, vocab=100, keep=8, space=ONE, size=workspace):
         return lib.mt_beam_select(logits, vocab, type, ONE, finished, end, ONE, ONE, ONE, ONE, space, size, groups, beams, vocab, keep, None)
