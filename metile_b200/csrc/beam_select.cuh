@@ -25,17 +25,17 @@
 namespace mt {
 
 constexpr double kDeadScore = -1e9;  // no sum of log-probabilities but the mask of a beam that is out; above it 64 bits keep logits apart
-// d = logit - top rounded, then d log2 e: |d| 2^-24 each and |d| 1.4e-8 for log2 e itself, 2^-22 for ex2.approx, ten roundings of
-// 2^-24 in a warp's sum (the rest is added in 64 bits).  The mean of |d| by the weights is at most the log of the row's
-// length, 13.2: 2.7e-6.
+// d = logit - top rounded, then d log2 e: |d| 2^-24 each and |d| 1.4e-8 for log2 e itself, 2^-22 for ex2.approx, within a share
+// and once more for the share in the row, where the two |d| add up to the one to the row's maximum; ten roundings of 2^-24 in
+// a warp's sum (the rest is added in 64 bits).  The mean of |d| by the weights is at most the log of the row's length, 13.2: 2.9e-6.
 constexpr double kBeamError = 0x1p-18;
 
 constexpr int kBeamMaxBeams = 32, kBeamMaxKeep = 64;
 constexpr int kBeamThreads = 256, kBeamVectors = 4, kBeamSpanBytes = kBeamThreads * kBeamVectors * 16, kBeamShares = kBeamThreads / 32;
 constexpr int kBeamMaxParts = 32, kBeamMostPerPart = 16;     // parts of a row (at most 1024 lists to join), spans of a part
-constexpr int kBeamAtOnce = 3, kBeamStages = 3;              // CTAs of an SM, spans each has in flight or in work
-constexpr int kBeamBlock = 512 + 16;                         // a warp's vectors of one step, and the one behind them
-constexpr int kBeamRing = kBeamStages * kBeamShares * kBeamVectors * kBeamBlock;
+constexpr int kBeamAtOnce = 4, kBeamStages = 2;              // CTAs of an SM, spans each has in flight or in work
+constexpr int kBeamShareBytes = kBeamVectors * 512, kBeamBlock = kBeamShareBytes + 16;  // a warp's share of a span, in the ring with the vector behind it
+constexpr int kBeamRing = kBeamStages * kBeamShares * kBeamBlock;
 constexpr int kBeamBuckets = 64, kBeamCollect = 512;         // of a part
 static_assert(kBeamCollect >= kBeamMaxKeep + kBeamThreads, "equal ones are collected a step of all threads at a time");
 constexpr int kBeamSlack = 8, kBeamJoinCollect = (kBeamMaxKeep + kBeamSlack) * kBeamMaxKeep, kBeamStage = 4096;
@@ -150,103 +150,111 @@ __device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
     return d;
 }
 
-// A thread's logits of a span: element e of vector v is the span's (v * 256 + thread) * kPer + e; those behind the row are -inf.
+// A warp's shares of the spans of a run, copied ahead into its part of the ring.  A share is 2 KB in one piece: element e of a
+// lane's vector v is its (32 v + lane) * kPer + e.
 template <int kType>
-struct BeamSpan {
-    static constexpr int kSize = beam_size(kType), kPer = 16 / kSize;
-    const char* from;  // the first logit
-    int here, skew;    // logits of the span; bytes by which it starts behind a boundary
+struct BeamCopies {
+    static constexpr int kPer = 16 / beam_size(kType), kShare = kBeamShareBytes / beam_size(kType);
+    const BeamSelectParams& p;
+    const char* vector;  // this lane's first one of the next share, aligned
+    long long row;
+    int span, left, skew;  // logits of the row from the share on, counted from the boundary in front; bytes behind that
 
-    __device__ __forceinline__ BeamSpan(const BeamSelectParams& p, long long row, int span) {
-        from = static_cast<const char*>(p.logits) + (row * p.row_stride + (long long)span * beam_span(kType)) * kSize;
-        here = min(beam_span(kType), p.vocabulary - span * beam_span(kType));
+    __device__ __forceinline__ BeamCopies(const BeamSelectParams& params, long long first_row, int first_span)
+        : p(params), row(first_row), span(first_span) { enter(); }
+    __device__ __forceinline__ void enter() {
+        const int share = span * beam_span(kType) + (int)(threadIdx.x >> 5) * kShare;
+        const char* from = static_cast<const char*>(p.logits) + (row * p.row_stride + share) * beam_size(kType);
         skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+        vector = from - skew + (threadIdx.x & 31) * 16;
+        left = p.vocabulary - share + skew / beam_size(kType);
     }
-    __device__ __forceinline__ int at(int v) const { return (v * kBeamThreads + (int)threadIdx.x) * kPer; }
-    __device__ __forceinline__ const char* vector(int at) const { return from - skew + (long long)at * kSize; }  // aligned
-
-    // Into a warp's part of the ring: its vectors of a step one after the other, and the one behind them.
-    __device__ __forceinline__ void copy(char* ring) const {
+    __device__ __forceinline__ void next(char* ring) {
         const int lane = threadIdx.x & 31;
+        char* to = ring + lane * 16;
+        if (left >= kShare + kPer) {
 #pragma unroll
-        for (int v = 0; v < kBeamVectors; ++v) {
-            // (The neighbour may need this one where the thread itself has no logit in it.)
-            if (at(v) - skew / kSize < here) ptx::cp_async_16(ring + v * kBeamBlock + lane * 16, vector(at(v)));
-            if (lane == 31 && skew && at(v) + (16 - skew) / kSize < here) ptx::cp_async_16(ring + v * kBeamBlock + 512, vector(at(v)) + 16);
+            for (int v = 0; v < kBeamVectors; ++v) ptx::cp_async_16(to + v * 512, vector + v * 512);
+            if (skew && lane == 0) ptx::cp_async_16(to + kBeamShareBytes, vector + kBeamShareBytes);
+        } else {
+#pragma unroll
+            for (int v = 0; v < kBeamVectors; ++v)
+                if ((32 * v + lane) * kPer < left) ptx::cp_async_16(to + v * 512, vector + v * 512);
+            if (skew && lane == 0 && kShare < left) ptx::cp_async_16(to + kBeamShareBytes, vector + kBeamShareBytes);
         }
-    }
-    __device__ __forceinline__ void take(uint32_t (&raw)[kBeamVectors][4], const char* ring) const {
-        const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int v = 0; v < kBeamVectors; ++v) {
-            const uint4 own = *reinterpret_cast<const uint4*>(ring + v * kBeamBlock + lane * 16);
-            if (skew) {
-                take_skewed(raw[v], own, *reinterpret_cast<const uint4*>(ring + v * kBeamBlock + lane * 16 + 16), skew);
-            } else {
-                raw[v][0] = own.x; raw[v][1] = own.y; raw[v][2] = own.z; raw[v][3] = own.w;
-            }
+        vector += kBeamSpanBytes;
+        left -= beam_span(kType);
+        if (++span == p.spans) {
+            span = 0;
+            ++row;
+            enter();
         }
-        mask(raw);
-    }
-
-private:
-    __device__ __forceinline__ void mask(uint32_t (&raw)[kBeamVectors][4]) const {
-        if (here == beam_span(kType)) return;
-#pragma unroll
-        for (int v = 0; v < kBeamVectors; ++v)
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (at(v) + e >= here) {
-                    if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
-                    else {
-                        const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
-                        raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
-                    }
-                }
     }
 };
 
 template <int kType>
 __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(const BeamSelectParams p) {
-    using Span = BeamSpan<kType>;
-    constexpr int kPer = Span::kPer, kVectors = kBeamVectors, kWarps = kBeamShares;
-    extern __shared__ __align__(16) char beam_ring[];  // [warps][stages][vectors][block]
+    using Copies = BeamCopies<kType>;
+    constexpr int kPer = Copies::kPer, kShare = Copies::kShare, kVectors = kBeamVectors, kWarps = kBeamShares;
+    extern __shared__ __align__(16) char beam_ring[];  // [warps][stages][block]
     __shared__ float span_top[kBeamMostPerPart][kBeamThreads], bucket[kBeamBuckets];
     __shared__ float collected[kBeamCollect], bound_shared;
-    __shared__ int collected_token[kBeamCollect], count, above;
+    __shared__ int collected_token[kBeamCollect], count;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long spans = (long long)p.groups * p.beams * p.spans;
     const long long run0 = beam_run_start(blockIdx.x, spans, p.runs), run1 = beam_run_start(blockIdx.x + 1, spans, p.runs);
-    char* ring = beam_ring + warp * (kBeamStages * kVectors * kBeamBlock);
+    char* ring = beam_ring + warp * (kBeamStages * kBeamBlock);
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    long long copy_row = run0 / p.spans;
-    int copy_span = (int)(run0 - copy_row * p.spans), to_copy = (int)(run1 - run0);
+    long long row = run0 / p.spans;
+    int span0 = (int)(run0 - row * p.spans), part = (int)(blockIdx.x - beam_run_of(row * p.spans, spans, p.runs));
+    Copies copies(p, row, span0);
+    int to_copy = (int)(run1 - run0);
     auto copy_next = [&](int slot) {
-        if (to_copy > 0) {
-            Span(p, copy_row, copy_span).copy(ring + slot * (kVectors * kBeamBlock));
-            --to_copy;
-            if (++copy_span == p.spans) {
-                copy_span = 0;
-                ++copy_row;
-            }
-        }
+        if (to_copy-- > 0) copies.next(ring + slot * kBeamBlock);
         ptx::cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < kBeamStages - 1; ++i) copy_next(i);
     int slot = 0;
-    for (long long start = run0; start < run1;) {  // a part: what the run has of one row
-        const long long row = start / p.spans;
-        const int span0 = (int)(start - row * p.spans), span1 = (int)min((long long)p.spans, span0 + (run1 - start));
-        start += span1 - span0;
-        if (threadIdx.x == 0) count = above = 0;
+    // A part: what the run has of one row.  The rows behind its first one start in it.
+    for (int to_do = (int)(run1 - run0); to_do > 0; ++row, span0 = part = 0) {
+        const int span1 = min(p.spans, span0 + to_do);
+        to_do -= span1 - span0;
+        if (threadIdx.x == 0) count = 0;
         float mine = -INFINITY;
         uint32_t raw[kVectors][4];
+        const char* from = static_cast<const char*>(p.logits) + row * p.row_stride * beam_size(kType);
+        const int skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
+        BeamShareStats* stats = p.stats + (row * p.spans + span0) * kWarps + warp;
+        float last_top = 0.0f, last_total = 0.0f;
         for (int span = span0; span < span1; ++span) {
             ptx::cp_async_wait_group<kBeamStages - 2>();
             __syncwarp();
-            Span(p, row, span).take(raw, ring + slot * (kVectors * kBeamBlock));
+            const char* share = ring + slot * kBeamBlock + lane * 16;
+#pragma unroll
+            for (int v = 0; v < kVectors; ++v) {
+                const uint4 own = *reinterpret_cast<const uint4*>(share + v * 512);
+                if (skew) {
+                    take_skewed(raw[v], own, *reinterpret_cast<const uint4*>(share + v * 512 + 16), skew);
+                } else {
+                    raw[v][0] = own.x; raw[v][1] = own.y; raw[v][2] = own.z; raw[v][3] = own.w;
+                }
+            }
+            const int left = p.vocabulary - span * beam_span(kType) - warp * kShare;  // behind the row: -inf, and left out below
+            if (left < kShare) {
+#pragma unroll
+                for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e)
+                        if ((32 * v + lane) * kPer + e >= left) {
+                            if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
+                            else {
+                                const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
+                                raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
+                            }
+                        }
+            }
             __syncwarp();
             copy_next(slot == 0 ? kBeamStages - 1 : slot - 1);
             slot = slot == kBeamStages - 1 ? 0 : slot + 1;
@@ -259,45 +267,40 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
             if (top != top) top = -INFINITY;  // nothing but NaN
             span_top[span - span0][threadIdx.x] = top;
             mine = fmaxf(mine, top);
+            asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
+            // The exponentials of the differences to the share's maximum, added as a tree.  (With nothing above -inf the sum is
+            // zero, or NaN where there is one.)  What the warp's lanes have is added one span later, beside the next exponentials.
+            float2 sums[kVectors];
+            const float away = top == -INFINITY ? 0.0f : -top;
+            const float2 shift = make_float2(away, away), log2_e = make_float2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-            for (int offset = 16; offset >= 1; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
-            float total = 0.0f;
-            if (top == -INFINITY) {
-                bool bad = false;
+            for (int v = 0; v < kVectors; ++v) {
+                float2 weight[kPer / 2];
 #pragma unroll
-                for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e) bad = bad || beam_logit<kType>(raw[v], e) != beam_logit<kType>(raw[v], e);
-                total = bad ? NAN : 0.0f;
-            } else {
-                // The exponentials of the differences to the share's maximum, added as a tree.
-                float2 sums[kVectors];
-                const float2 shift = make_float2(-top, -top), log2_e = make_float2(1.4426950408889634f, 1.4426950408889634f);
-#pragma unroll
-                for (int v = 0; v < kVectors; ++v) {
-                    float2 weight[kPer / 2];
-#pragma unroll
-                    for (int e = 0; e < kPer / 2; ++e) {
-                        const float2 d = add_f32x2(make_float2(beam_logit<kType>(raw[v], 2 * e), beam_logit<kType>(raw[v], 2 * e + 1)), shift);
-                        const float2 power = mul_f32x2(d, log2_e);
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].x) : "f"(power.x));
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].y) : "f"(power.y));
-                    }
-#pragma unroll
-                    for (int width = kPer / 4; width >= 1; width >>= 1)
-#pragma unroll
-                        for (int e = 0; e < width; ++e) weight[e] = add_f32x2(weight[e], weight[e + width]);
-                    sums[v] = weight[0];
+                for (int e = 0; e < kPer / 2; ++e) {
+                    const float2 d = add_f32x2(make_float2(beam_logit<kType>(raw[v], 2 * e), beam_logit<kType>(raw[v], 2 * e + 1)), shift);
+                    const float2 power = mul_f32x2(d, log2_e);
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].x) : "f"(power.x));
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].y) : "f"(power.y));
                 }
 #pragma unroll
-                for (int width = kVectors / 2; width >= 1; width >>= 1)
+                for (int width = kPer / 4; width >= 1; width >>= 1)
 #pragma unroll
-                    for (int v = 0; v < width; ++v) sums[v] = add_f32x2(sums[v], sums[v + width]);
-                total = sums[0].x + sums[0].y;
+                    for (int e = 0; e < width; ++e) weight[e] = add_f32x2(weight[e], weight[e + width]);
+                sums[v] = weight[0];
             }
-            total = warp_sum_xor(total);
-            if (lane == 0) p.stats[(row * p.spans + span) * kWarps + warp] = {top, total};
+#pragma unroll
+            for (int width = kVectors / 2; width >= 1; width >>= 1)
+#pragma unroll
+                for (int v = 0; v < width; ++v) sums[v] = add_f32x2(sums[v], sums[v + width]);
+            const float total = warp_sum_xor(last_total);
+            if (lane == 0 && span > span0) *(stats - kWarps) = {last_top, total};
+            stats += kWarps;
+            last_top = top;
+            last_total = sums[0].x + sums[0].y;
         }
+        last_total = warp_sum_xor(last_total);
+        if (lane == 0) *(stats - kWarps) = {last_top, last_total};
         {
             float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -322,13 +325,11 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
         __syncthreads();
         const float bound = bound_shared;
         // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens.
-        const char* from = static_cast<const char*>(p.logits) + row * p.row_stride * beam_size(kType);
         auto reach = [&](auto qualifies, auto visit) {
             for (int span = span0; span < span1 && count <= kBeamCollect; ++span) {
                 unsigned int threads = __ballot_sync(0xFFFFFFFFu, qualifies(span_top[span - span0][threadIdx.x]));
                 for (; threads; threads &= threads - 1u) {
-                    const int thread = warp * 32 + __ffs(threads) - 1;
-                    const int token = span * beam_span(kType) + ((lane / kPer) * kBeamThreads + thread) * kPer + lane % kPer;
+                    const int token = span * beam_span(kType) + warp * kShare + (lane / kPer * 32 + __ffs(threads) - 1) * kPer + lane % kPer;
                     if (lane < kVectors * kPer && token < p.vocabulary) visit(beam_logit_at<kType>(from, token), token);
                 }
             }
@@ -342,7 +343,6 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
         };
         reach([&](float top) { return top >= bound; }, [&](float logit, int token) { if (logit >= bound) collect(logit, token); });
         __syncthreads();
-        const int part = (int)(blockIdx.x - beam_run_of(row * p.spans, spans, p.runs));
         BeamEntry* list = p.lists + (row * p.parts + part) * p.keep;
         int found = count;
         if (found > kBeamCollect) {
@@ -478,8 +478,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
 #pragma unroll 4
         for (int i = lane; i < shares; i += 32) {
             const BeamShareStats own = stats[i];
-            const double factor = own.sum == 0.0f ? 0.0 : exp((double)own.top - (double)best);
-            sum += (double)own.sum * factor;
+            sum += (double)own.sum * (own.sum == 0.0f ? 0.0 : (double)__expf(own.top - best));  // of the same error as within a share
         }
 #pragma unroll
         for (int offset = 16; offset >= 1; offset >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);
