@@ -488,6 +488,26 @@ inline PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
     return tuple;
 }
 
+// Several results in one allocation: a tensor costs a third of the host time of one with its own.
+class Carved {
+public:
+    Carved(size_t bytes, c10::Device device) : whole_(at::detail::empty_cuda({(int64_t)bytes}, at::kByte, device, std::nullopt)) {}
+    static size_t room(int64_t count, size_t size) { return ((size_t)count * size + 15) / 16 * 16; }
+    Tensor next(at::IntArrayRef sizes, at::ScalarType type) {
+        const auto meta = c10::scalarTypeToTypeMeta(type);
+        Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole_.storage()), whole_.key_set(), meta);
+        c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+        impl->set_sizes_contiguous(sizes);
+        impl->set_storage_offset((int64_t)(used_ / meta.itemsize()));
+        used_ += room(t.numel(), meta.itemsize());
+        return t;
+    }
+
+private:
+    Tensor whole_;
+    size_t used_ = 0;
+};
+
 inline Tensor new_of(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
     return at::detail::empty_cuda(sizes, type, device, std::nullopt);
 }
@@ -509,9 +529,9 @@ PyObject* paged_resize(PyObject* const* args) {
         !ints_on(t[4], device, 2) || ring.numel() < 1 || !fits_int(ring.numel()) || !fits_int(requests) || !fits_int(tables.size(1)))
         Py_RETURN_NONE;
     const Launch launch(device);
-    Tensor slots = new_of({tokens}, at::kLong, device), positions = new_of({tokens}, at::kInt, device);
-    Tensor starts = new_of({requests + 1}, at::kInt, device);
-    Tensor lengths_out = advance ? lengths : new_of({requests}, at::kInt, device), state_out = advance ? state : new_of({2}, at::kInt, device);
+    Carved carved(Carved::room(tokens, 8) + Carved::room(tokens, 4) + Carved::room(requests + 1, 4) + Carved::room(requests, 4) + 16, device);
+    Tensor slots = carved.next({tokens}, at::kLong), positions = carved.next({tokens}, at::kInt), starts = carved.next({requests + 1}, at::kInt);
+    Tensor lengths_out = advance ? lengths : carved.next({requests}, at::kInt), state_out = advance ? state : carved.next({2}, at::kInt);
     int code;
     {
         const Unlocked unlocked;
@@ -629,8 +649,10 @@ PyObject* beam_select(PyObject* const* args) {
                      finished->sizes() != scores->sizes()))
         Py_RETURN_NONE;
     const Launch launch(device);
-    Tensor scores_out = new_of({groups, keep}, at::kFloat, device), parents = new_of({groups, keep}, at::kInt, device);
-    Tensor tokens = new_of({groups, keep}, at::kLong, device), finished_out = new_of({groups, keep}, at::kBool, device);
+    const int64_t kept = groups * keep;
+    Carved carved(2 * Carved::room(kept, 4) + Carved::room(kept, 8) + Carved::room(kept, 1), device);
+    Tensor scores_out = carved.next({groups, keep}, at::kFloat), parents = carved.next({groups, keep}, at::kInt);
+    Tensor tokens = carved.next({groups, keep}, at::kLong), finished_out = carved.next({groups, keep}, at::kBool);
     const size_t needed = mt_beam_select_workspace_bytes((int)groups, (int)beams, (int)vocabulary, (int)keep, type);
     c10::DataPtr scratch;
     if (needed) scratch = call_scratch(needed);

@@ -725,9 +725,7 @@ int mt_paged_resize(int* block_tables, long long table_stride, int width, const 
     if (!device_is_sm100()) return MT_ERR_DEVICE;
     ResizeParams params{block_tables, lengths, counts, free_pages, free_state, slots, positions, starts, lengths_out,
                         free_state_out, table_stride, width, pool, requests, shift, tokens};
-    cudaLaunchAttribute attribute;
-    const cudaLaunchConfig_t config = dependent_launch(dim3(1, 1, 1), kResizeThreads, 0, stream, &attribute);
-    return cudaLaunchKernelEx(&config, paged_resize_kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    return launch_paged_resize(params, static_cast<cudaStream_t>(stream));
 }
 
 int mt_rope_kv_append_paged(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,

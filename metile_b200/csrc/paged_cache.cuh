@@ -48,10 +48,12 @@ struct ResizeParams {
     int width, pool, requests, page_shift, tokens;
 };
 
-constexpr int kResizeThreads = 1024;
+constexpr int kResizeThreads = 1024;  // the most; and the requests taken at once
+constexpr int kResizeCluster = 8;
 
-// Inclusive sum over the block of three numbers at once; `scratch` holds 3 x 32.
-__device__ __forceinline__ void block_scan3(long long& a, long long& b, long long& c, long long (*scratch)[32]) {
+// Inclusive sums over the block of kCount numbers at once.
+template <int kCount>
+__device__ __forceinline__ void block_scan(long long (&values)[kCount], long long (*scratch)[32]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     auto warp_scan = [&](long long v) {
 #pragma unroll
@@ -61,23 +63,20 @@ __device__ __forceinline__ void block_scan3(long long& a, long long& b, long lon
         }
         return v;
     };
-    a = warp_scan(a);
-    b = warp_scan(b);
-    c = warp_scan(c);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) values[i] = warp_scan(values[i]);
     if (lane == 31) {
-        scratch[0][warp] = a;
-        scratch[1][warp] = b;
-        scratch[2][warp] = c;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) scratch[i][warp] = values[i];
     }
     __syncthreads();
-    if (warp < 3) {
-        const long long v = lane < warps ? scratch[warp][lane] : 0;
-        scratch[warp][lane] = warp_scan(v) - v;
+    // Every warp adds up the warps in front of it.
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+        const long long v = lane < warps ? scratch[i][lane] : 0;
+        const long long before = warp_scan(v) - v;
+        values[i] += __shfl_sync(0xFFFFFFFFu, before, warp);
     }
-    __syncthreads();
-    a += scratch[0][warp];
-    b += scratch[1][warp];
-    c += scratch[2][warp];
     __syncthreads();
 }
 
@@ -91,17 +90,31 @@ __device__ __forceinline__ int last_not_above(const long long* starts, int n, lo
     return low;
 }
 
-// One CTA takes the requests 1024 at a time, in order.  Three sums run along them: tokens added, pages asked for, pages
-// given back.  Then tokens, granted and returned pages are dealt to the threads, each of which looks its request up.
-__global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const ResizeParams p) {
+// The requests are taken as many as threads at a time, in order.  Three sums run along them: tokens added, pages asked for, pages
+// given back.  Then tokens, granted and returned pages are dealt to the threads, each of which looks its request up; a thread
+// has four tokens in a row.  Bound by latency, and for long prompts by the threads: several CTAs then, which all take the
+// sums and share what follows.  Where lengths and state are written in place the CTAs are one cluster, and the first of them
+// writes behind a barrier.
+__global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const ResizeParams p, bool in_place) {
     __shared__ long long token_start[kResizeThreads], grant_start[kResizeThreads], free_start[kResizeThreads];
     __shared__ int held[kResizeThreads], added[kResizeThreads];
     __shared__ unsigned char is_served[kResizeThreads];
-    __shared__ long long scratch[3][32];
+    __shared__ long long scratch[2][32];
     __shared__ long long totals[3];
+    __shared__ int granted_shared;
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
+    const int threads = blockDim.x;
+    const bool leads = blockIdx.x == 0;
+    const long long worker = (long long)blockIdx.x * threads + threadIdx.x, workers = (long long)gridDim.x * threads;
     const int page = 1 << p.page_shift;
+    auto blocks_of = [&](long long tokens) { return (tokens + page - 1) >> p.page_shift; };
+    auto all_have_read = [&] {
+        if (in_place) {
+            ptx::cluster_arrive();
+            ptx::cluster_wait();
+        }
+    };
     // The ring's state as a caller may have it: kept within the ring whatever it says.
     int first = p.state[0], available = p.state[1];
     if (first < 0 || first >= p.pool) first = 0;
@@ -111,85 +124,118 @@ __global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const Resi
         const long long at = first + taken;
         return at < p.pool ? at : at - p.pool;
     };
-    long long tokens_before = 0, asked_before = 0, granted_before = 0, freed_before = 0;
-    for (int base = 0; base < p.requests; base += kResizeThreads) {
-        const int r = base + threadIdx.x, here = min(kResizeThreads, p.requests - base);
+    if (threadIdx.x == 0) granted_shared = 0;
+    long long tokens_before = 0, asked_before = 0, freed_before = 0;
+    for (int base = 0; base < p.requests; base += threads) {
+        const int r = base + threadIdx.x, here = min(threads, p.requests - base);
         const bool exists = r < p.requests;
         const int length = exists ? p.lengths[r] : 0, count = exists ? p.counts[r] : 0;
         const long long after = (long long)length + count;
         bool valid = length >= 0 && after >= 0 && length <= room && after <= room;
-        const long long old_blocks = ((long long)length + page - 1) >> p.page_shift;
-        const long long new_blocks = (after + page - 1) >> p.page_shift;
         // First the tokens alone: whether they fit the map decides which requests ask for pages.
-        long long ends = max(count, 0), unused0 = 0, unused1 = 0;
-        block_scan3(ends, unused0, unused1, scratch);
-        ends += tokens_before;
-        valid = valid && (count <= 0 || ends <= p.tokens);
-        const long long need = valid ? max(0ll, new_blocks - old_blocks) : 0, back = valid ? max(0ll, old_blocks - new_blocks) : 0;
-        long long reach = need, unused2 = 0, returned = back;
-        block_scan3(reach, unused2, returned, scratch);
-        reach += asked_before;
+        long long ends[1] = {max(count, 0)};
+        block_scan(ends, scratch);
+        ends[0] += tokens_before;
+        valid = valid && (count <= 0 || ends[0] <= p.tokens);
+        const long long change = valid ? blocks_of(after) - blocks_of(length) : 0, need = max(0ll, change), back = max(0ll, -change);
+        long long pages[2] = {need, back};
+        block_scan(pages, scratch);
+        const long long reach = pages[0] + asked_before, returned = pages[1] + freed_before;
         // In order and without overtaking: once the free pages do not reach, nobody behind is given any.
         const bool served = valid && (need == 0 || reach <= available);
-        token_start[threadIdx.x] = ends - max(count, 0);
+        token_start[threadIdx.x] = ends[0] - max(count, 0);
         grant_start[threadIdx.x] = reach - need;
-        free_start[threadIdx.x] = returned - back + freed_before;
+        free_start[threadIdx.x] = returned - back;
         held[threadIdx.x] = length;
         added[threadIdx.x] = count;
         is_served[threadIdx.x] = served;
-        if (exists) p.starts[r] = (int)min(ends - max(count, 0), 0x7FFFFFFFll);
-        if (threadIdx.x == kResizeThreads - 1) {
-            totals[0] = ends;
+        if (served && need > 0) atomicMax(&granted_shared, (int)reach);  // at most `available`
+        if (threadIdx.x == threads - 1) {
+            totals[0] = ends[0];
             totals[1] = reach;
-            totals[2] = returned + freed_before;
+            totals[2] = returned;
         }
         __syncthreads();
+        all_have_read();
+        if (exists && leads) {
+            p.starts[r] = (int)min(ends[0] - max(count, 0), 0x7FFFFFFFll);
+            p.lengths_out[r] = served ? (int)after : length;
+        }
         const long long tokens_here = min((long long)p.tokens, totals[0]), asked_here = min((long long)available, totals[1]);
-        for (long long t = tokens_before + threadIdx.x; t < tokens_here; t += kResizeThreads) {
-            const int i = last_not_above(token_start, here, t);
-            long long slot = -1, position = 0;
-            if (is_served[i]) {
-                position = held[i] + (t - token_start[i]);
-                const long long block = position >> p.page_shift;
-                const long long fresh = block - (((long long)held[i] + page - 1) >> p.page_shift);
-                const int id = fresh < 0 ? p.tables[(base + i) * p.table_stride + block] : p.ring[wrapped(grant_start[i] + fresh)];
-                slot = id < 0 ? -1 : ((long long)id << p.page_shift) + (position & (page - 1));
+        for (long long t0 = tokens_before + 4 * worker; t0 < tokens_here; t0 += 4 * workers) {
+            int i = last_not_above(token_start, here, t0);
+            int position[4], id[4];
+            const int* named[4];  // where the id of the token's page stands
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                while (i + 1 < here && token_start[i + 1] <= t0 + k) ++i;
+                position[k] = 0;
+                named[k] = nullptr;
+                if (t0 + k < tokens_here && is_served[i]) {
+                    position[k] = held[i] + (int)(t0 + k - token_start[i]);
+                    const int block = position[k] >> p.page_shift, fresh = block - (int)blocks_of(held[i]);
+                    named[k] = fresh < 0 ? p.tables + (base + i) * p.table_stride + block : p.ring + wrapped(grant_start[i] + fresh);
+                }
             }
-            p.slots[t] = slot;
-            p.positions[t] = (int)position;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) id[k] = named[k] ? *named[k] : -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (t0 + k >= tokens_here) break;
+                p.slots[t0 + k] = id[k] < 0 ? -1 : ((long long)id[k] << p.page_shift) + (position[k] & (page - 1));
+                p.positions[t0 + k] = position[k];
+            }
         }
-        for (long long g = asked_before + threadIdx.x; g < asked_here; g += kResizeThreads) {
+        for (long long g = asked_before + worker; g < asked_here; g += workers) {
             const int i = last_not_above(grant_start, here, g);
-            if (!is_served[i]) continue;
-            const long long block = (((long long)held[i] + page - 1) >> p.page_shift) + (g - grant_start[i]);
-            p.tables[(base + i) * p.table_stride + block] = p.ring[wrapped(g)];
+            if (is_served[i]) p.tables[(base + i) * p.table_stride + blocks_of(held[i]) + (g - grant_start[i])] = p.ring[wrapped(g)];
         }
-        for (long long f = freed_before + threadIdx.x; f < totals[2]; f += kResizeThreads) {
+        for (long long f = freed_before + worker; f < totals[2]; f += workers) {
             const int i = last_not_above(free_start, here, f);
-            const long long block = (((long long)held[i] + added[i] + page - 1) >> p.page_shift) + (f - free_start[i]);
+            const long long block = blocks_of((long long)held[i] + added[i]) + (f - free_start[i]);
             p.ring[((long long)first + available + f) % p.pool] = p.tables[(base + i) * p.table_stride + block];
         }
-        long long granted = served ? need : 0, unused3 = 0, unused4 = 0;
-        block_scan3(granted, unused3, unused4, scratch);
-        if (exists) p.lengths_out[r] = served ? (int)after : length;
         tokens_before = totals[0];
         asked_before = totals[1];
         freed_before = totals[2];
         __syncthreads();
-        if (threadIdx.x == kResizeThreads - 1) totals[0] = granted;
-        __syncthreads();
-        granted_before += totals[0];
-        __syncthreads();
     }
-    for (long long t = tokens_before + threadIdx.x; t < p.tokens; t += kResizeThreads) {
+    for (long long t = tokens_before + worker; t < p.tokens; t += workers) {
         p.slots[t] = -1;
         p.positions[t] = 0;
     }
-    if (threadIdx.x == 0) {
-        p.starts[p.requests] = (int)min(tokens_before, 0x7FFFFFFFll);
-        p.state_out[0] = (int)((first + granted_before) % p.pool);
-        p.state_out[1] = (int)min((long long)p.pool, available - granted_before + freed_before);
+    if (p.requests == 0) {
+        __syncthreads();
+        all_have_read();
     }
+    if (threadIdx.x == 0 && leads) {
+        p.starts[p.requests] = (int)min(tokens_before, 0x7FFFFFFFll);
+        p.state_out[0] = (int)wrapped(granted_shared) % p.pool;
+        p.state_out[1] = (int)min((long long)p.pool, (long long)available - granted_shared + freed_before);
+    }
+}
+
+inline int launch_paged_resize(const ResizeParams& params, cudaStream_t stream) {
+    const bool in_place = params.lengths_out == params.lengths || params.state_out == params.state;
+    // A CTA for every four tokens of its threads; up to 64, or a cluster of eight.
+    const int most = in_place ? kResizeCluster : 64;
+    const long long wanted = ((long long)params.tokens + 4 * kResizeThreads - 1) / (4 * kResizeThreads);
+    const int ctas = wanted <= 1 ? 1 : in_place || wanted >= most ? most : (int)wanted;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ctas, 1, 1);
+    // 256 threads where that gives every request and four tokens one.
+    config.blockDim = dim3(params.requests <= 256 && params.tokens <= 1024 ? 256 : kResizeThreads, 1, 1);
+    config.stream = stream;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = ctas;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    config.attrs = attrs;
+    config.numAttrs = in_place && ctas > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, paged_resize_kernel, params, in_place && ctas > 1) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -62,6 +62,10 @@ def resize_case(seed, requests, page, width, most, free, start, device):
 
 def check_resize(arrays, page, tokens, device, **kwargs):
     expected = O.resize(*arrays, page, tokens)
+    in_place = [torch.tensor(a, device=device) for a in arrays]
+    got = B.paged_resize(*in_place, page_size=page, tokens=tokens, advance=True)
+    for name, a, b in zip(("slots", "positions", "starts", "lengths", "state", "table", "ring"), (*got, in_place[0], in_place[3]), expected):
+        assert np.array_equal(a.cpu().numpy(), b), name
     tensors = [torch.tensor(a, device=device) for a in arrays]
     for _ in range(2):  # a call with the same lengths and state does the same again
         got = B.paged_resize(*tensors, page_size=page, tokens=tokens, **kwargs)
@@ -73,7 +77,7 @@ def check_resize(arrays, page, tokens, device, **kwargs):
 
 @pytest.mark.parametrize("requests,page,width,most,free,start", [
     (1, 16, 4, 1, 1, 0), (3, 8, 5, 9, 40, 17), (64, 16, 40, 1, 64, 5), (65, 32, 9, 70, 300, 1000), (1, 256, 3, 700, 3, 2),
-    (1024, 16, 8, 40, 4000, 3), (1025, 64, 4, 30, 1500, 9999), (2500, 8, 6, 20, 3000, 77),
+    (1024, 16, 8, 40, 4000, 3), (300, 16, 900, 4000, 80000, 5), (2, 32, 3000, 60000, 4000, 1), (1025, 64, 4, 30, 1500, 9999), (2500, 8, 6, 20, 3000, 77),
 ])
 def test_requests_grow_and_shrink(cuda_device, requests, page, width, most, free, start):
     arrays = resize_case(requests, requests, page, width, most, free, start, cuda_device)
