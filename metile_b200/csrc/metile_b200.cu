@@ -783,6 +783,7 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
                               int kv_heads, int head_dim, int pages, int page_size, int type, float scale, void* stream) {
     const int shift = page_shift_of(page_size);
     PagedAttentionParams params;
+    PageStrides keys, values;
     if (batch < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || width < 1 || pages < 1 || shift < 0 || table_stride < width)
         return MT_ERR_SHAPE;
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || (type != MT_TYPE_BF16 && type != MT_TYPE_FP16)) return MT_ERR_SHAPE;
@@ -791,14 +792,18 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
     if (batch == 0) return MT_OK;
     if (!q || !key_pages || !value_pages || !key_strides || !value_strides || !block_tables || !lengths || !out) return MT_ERR_NULL;
     if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 16) ||
-        !page_strides_of(key_strides, params.key_strides) || !page_strides_of(value_strides, params.value_strides))
+        !page_strides_of(key_strides, keys) || !page_strides_of(value_strides, values))
         return MT_ERR_ALIGN;
+    for (const PageStrides* strides : {&keys, &values})  // a page and its heads lie within 2 GB
+        if (strides->page > 0x3FFFFFFF || strides->head > 0x3FFFFFFF || strides->token > 0x3FFFFFFF / page_size) return MT_ERR_SHAPE;
+    params.key_strides = {(int)keys.page * 2, (int)keys.head * 2, (int)keys.token * 2};
+    params.value_strides = {(int)values.page * 2, (int)values.head * 2, (int)values.token * 2};
     const size_t needed = mt_paged_attention_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim, width, page_size);
     if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
     if (!device_is_sm100()) return MT_ERR_DEVICE;
     params.q = static_cast<const uint16_t*>(q);
-    params.key_pages = static_cast<const uint16_t*>(key_pages);
-    params.value_pages = static_cast<const uint16_t*>(value_pages);
+    params.key_pages = static_cast<const char*>(key_pages);
+    params.value_pages = static_cast<const char*>(value_pages);
     params.tables = block_tables;
     params.lengths = lengths;
     params.out = static_cast<uint16_t*>(out);

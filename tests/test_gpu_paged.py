@@ -253,6 +253,10 @@ def check_attention(case, scale, device, out=None):
     ([4097, 12, 2048], 10, 2, 128, 16, torch.bfloat16, "head"),
     ([33000], 2, 2, 64, 32, torch.float16, "head"),
     ([0, 0], 3, 1, 128, 16, torch.bfloat16, "head"),
+    ([700, 0, 130, 1], 20, 2, 128, 16, torch.bfloat16, "token"),
+    ([900], 33, 1, 64, 8, torch.float16, "head"),
+    ([400, 512], 12, 3, 256, 32, torch.bfloat16, "pool"),
+    ([129] * 80, 8, 4, 128, 16, torch.bfloat16, "head"),
 ])
 def test_paged_attention_against_the_oracle(cuda_device, lengths, heads, kv_heads, dim, page, dtype, layout):
     check_attention(attention_case(31, lengths, heads, kv_heads, dim, page, dtype, layout, cuda_device), dim ** -0.5, cuda_device)
@@ -291,6 +295,10 @@ def test_a_request_alone_and_in_a_batch_and_in_other_pages_has_the_same_bits(cud
     for b in range(len(lengths)):
         alone = B.paged_attention_decode(q[b:b + 1], keys, values, table[b:b + 1], torch.tensor(n[b:b + 1], device=cuda_device), scale=0.09)
         assert torch.equal(alone, out[b:b + 1]), b
+    # Short requests by a narrow table (one launch) and by a wide one (two).
+    short = B.paged_attention_decode(q[1:], keys, values, table[1:, :48].contiguous(), torch.tensor([17, 129, 700, 1], dtype=torch.int32, device=cuda_device), scale=0.09)
+    again = B.paged_attention_decode(q[1:], keys, values, table[1:], torch.tensor([17, 129, 700, 1], dtype=torch.int32, device=cuda_device), scale=0.09)
+    assert torch.equal(short, again)
     # The same tokens in pages of 64, in the other layout, with a wider table.
     larger = torch.full((sum(-(-x // 64) for x in lengths), 64, 2, 128), float("nan"), dtype=torch.bfloat16, device=cuda_device)
     larger = [larger.clone().transpose(1, 2) for _ in range(2)]
@@ -317,6 +325,12 @@ def test_pages_and_lengths_outside_are_recorded_and_left_out(cuda_device):
         assert not ok and words[:3] == (0x303, 1, page & 0xFFFFFFFF)
         rest = np.array([[tables[1, 0], tables[1, 2]]])  # its other tokens: 16 of one page, one of the last
         check_attention((q[1:], keys, values, rest, np.array([17])), 0.1, cuda_device, out[1:])
+    wide_table = torch.full((2, 200), -1, dtype=torch.int32, device=cuda_device)  # as many launches as a long request takes
+    wide_table[:, :3] = torch.tensor(tables, device=cuda_device)
+    for length in (-4, 3201):
+        B.paged_attention_decode(q, keys, values, wide_table, ints([40, length], cuda_device), scale=0.1)
+        ok, words = _lib.device_status()
+        assert not ok and words[0] in ((0x304,) if length < 0 else (0x303, 0x304)) and words[1] == 1
     for length in (-4, 49, 2**31 - 1):  # the table has room for 48
         out = B.paged_attention_decode(q, keys, values, torch.tensor(tables, device=cuda_device), ints([length, 33], cuda_device), scale=0.1)
         ok, words = _lib.device_status()
