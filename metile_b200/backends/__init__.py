@@ -16,7 +16,7 @@ from .cuda_dense import (  # noqa: F401
     mlx_dense_residual_qmv,
     mlx_dense_swiglu,
 )
-from .cuda_paged import paged_attention_decode, paged_resize, rope_kv_append_paged  # noqa: F401
+from .cuda_paged import PAGE_SIZES, paged_attention_decode, paged_resize, rope_kv_append_paged  # noqa: F401
 from .cuda_quantized import (  # noqa: F401
     batch_invariant,
     fixed_order,

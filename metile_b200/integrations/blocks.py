@@ -189,6 +189,119 @@ class KVCache:
         self.positions.fill_(self.length)
 
 
+class PagedTables:
+    """Block tables, lengths and free pages of a paged cache, for the `requests` rows of a batch and all layers of a model.
+
+    The device has the truth: a step that a CUDA graph replays takes its pages there.  The host keeps the same counts
+    beside it (`held` tokens of every request, `free` pages) to refuse what would not fit before anything is queued.
+
+    Before a forward pass the caller lets the requests `grow`; the layers of that pass then write and read the new
+    tokens.  A pass is either one token of every request (grow()) or the prompts of some, one after the other in
+    a batch of one (grow(counts))."""
+
+    def __init__(self, requests, pages, page_size, width, device):
+        if requests < 1 or pages < 1 or width < 1 or page_size not in backends.PAGE_SIZES:
+            raise ValueError(f"a paged cache needs requests, pages, blocks and a page size of {backends.PAGE_SIZES}")
+        self.requests, self.pages, self.page_size, self.width = int(requests), int(pages), int(page_size), int(width)
+        self.block_tables = torch.zeros((self.requests, self.width), dtype=torch.int32, device=device)
+        self.lengths = torch.zeros((self.requests,), dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(self.pages, dtype=torch.int32, device=device)
+        self.free_state = torch.tensor([0, self.pages], dtype=torch.int32, device=device)
+        self._ones = torch.ones((self.requests,), dtype=torch.int32, device=device)
+        self.held, self.free = [0] * self.requests, self.pages
+        self.slots = self.positions = None   # of the tokens of the pass
+        self.prompts = None                  # [(request, first row, rows)], or None: one token of every request
+
+    @property
+    def capacity(self):
+        return self.width * self.page_size
+
+    def reset(self):
+        """Forget every request; all pages are free."""
+        self.block_tables.zero_()
+        self.lengths.zero_()
+        torch.arange(self.pages, dtype=torch.int32, device=self.free_pages.device, out=self.free_pages)
+        self.free_state.copy_(torch.tensor([0, self.pages], dtype=torch.int32))
+        self.held, self.free = [0] * self.requests, self.pages
+
+    def account(self, counts):
+        """The host's side of a change by counts[r] tokens; refuses what does not fit."""
+        def blocks(tokens):
+            return -(-tokens // self.page_size)
+
+        after = [held + count for held, count in zip(self.held, counts)]
+        if len(counts) != self.requests or min(after) < 0 or max(after) > self.capacity:
+            raise ValueError("paged cache: a request has no room, or fewer tokens than are taken back")
+        changes = [blocks(new) - blocks(old) for new, old in zip(after, self.held)]
+        if sum(max(0, change) for change in changes) > self.free:
+            raise ValueError("paged cache: out of pages")
+        self.held, self.free = after, self.free - sum(changes)
+
+    def grow(self, counts=None):
+        """One new token for every request, or counts[r] for request r; negative counts give back the last tokens.
+
+        Pages that requests share (after `fork`, or beams) are given back by `reset` alone: a page must not go back twice."""
+        ones = counts is None
+        counts = [1] * self.requests if ones else [int(count) for count in counts]
+        self.account(counts)
+        self.prompts, first = None, 0
+        if not ones:
+            self.prompts = []
+            for request, count in enumerate(counts):
+                if count > 0:
+                    self.prompts.append((request, first, count))
+                    first += count
+        on_device = self._ones if ones else torch.tensor(counts, dtype=torch.int32).to(self.lengths.device)
+        self.slots, self.positions, _, _, _ = backends.paged_resize(
+            self.block_tables, self.lengths, on_device, self.free_pages, self.free_state, page_size=self.page_size,
+            tokens=self.requests if ones else first, advance=True)
+
+    def fork(self, beams, caches):
+        """Every first request of `beams` in a row is continued by all of them: full pages are shared, what is begun is copied
+        in the PagedKVCache of every layer."""
+        groups = self.requests // beams
+        if groups * beams != self.requests or any(self.held[r] and r % beams for r in range(self.requests)):
+            raise ValueError("only the first request of each group may have tokens")
+        held = [self.held[r - r % beams] for r in range(self.requests)]
+        # The others hold the full pages in name, which cost none, and a page of their own for the rest.
+        whole = [n // self.page_size * self.page_size for n in held]
+        part = [0 if r % beams == 0 else held[r] - whole[r] for r in range(self.requests)]
+        self.held = [held[r] if r % beams == 0 else whole[r] for r in range(self.requests)]
+        self.lengths.copy_(torch.tensor(self.held, dtype=torch.int32))
+        self.grow(part)
+        self.reorder(torch.zeros((groups, beams), dtype=torch.int32, device=self.lengths.device), caches)
+
+    def reorder(self, parents, caches):
+        """The requests of every group of beams continue those that `parents` [groups, beams] (int32) names."""
+        self.block_tables.copy_(backends.beam_reorder(self.block_tables, self.lengths, parents,
+                                                      [(cache.keys, cache.values) for cache in caches]))
+
+
+class PagedKVCache:
+    """One layer's keys and values [pages, kv_heads, page_size, head_dim] behind the tables of the whole model."""
+
+    def __init__(self, tables, kv_heads, head_dim, dtype=torch.bfloat16):
+        self.tables = tables
+        shape = (tables.pages, kv_heads, tables.page_size, head_dim)
+        self.keys = torch.zeros(shape, dtype=dtype, device=tables.lengths.device)
+        self.values = torch.zeros_like(self.keys)
+
+    def append(self, queries, keys, values, frequencies):
+        """Rotate the pass's rows and write keys and values to their slots; rows [tokens, heads, head_dim].  Returns the
+        rotated queries."""
+        tables = self.tables
+        if tables.slots is None or queries.shape[0] != tables.slots.shape[0]:
+            raise ValueError("paged cache: the pass does not have the tokens that its tables grew by")
+        return backends.rope_kv_append_paged(queries, keys, values, frequencies, tables.positions, tables.slots, self.keys,
+                                             self.values)
+
+    def fetch(self, first, count):
+        """Keys and values [count, kv_heads, head_dim] of the pass's rows `first` on, as they are stored."""
+        slots = self.tables.slots[first:first + count]
+        page, row = slots // self.tables.page_size, slots % self.tables.page_size
+        return self.keys[page, :, row], self.values[page, :, row]
+
+
 _UPDATE, _ADVANCE = KVCache.update_and_fetch, KVCache.advance
 
 
@@ -237,6 +350,8 @@ class Attention(nn.Module):
 
     def attend(self, q, k, v, cache=None):
         """Rotary embedding, cache and attention of projected rows [B, T, heads D]; returns [B, T, Hq D]."""
+        if isinstance(cache, PagedKVCache):
+            return self._attend_paged(q, k, v, cache)
         batch, steps, _ = q.shape
         q = q.view(batch, steps, self.heads, self.head_dim)
         k = k.view(batch, steps, self.kv_heads, self.head_dim)
@@ -258,6 +373,29 @@ class Attention(nn.Module):
                 k, v = cache.update_and_fetch(k, v)
         out = scaled_dot_product_attention(q, k, v, cache, self.scale, "causal" if steps > 1 else None)
         return out.transpose(1, 2).reshape(batch, steps, self.heads * self.head_dim)
+
+
+    def _attend_paged(self, q, k, v, cache):
+        batch, steps, _ = q.shape
+        rows, tables = batch * steps, cache.tables
+        q = q.reshape(rows, self.heads, self.head_dim)
+        k = k.reshape(rows, self.kv_heads, self.head_dim)
+        v = v.reshape(rows, self.kv_heads, self.head_dim)
+        rotated = cache.append(q, k, v, self._frequencies_on(q.device))
+        if tables.prompts is None:
+            out = backends.paged_attention_decode(rotated, cache.keys, cache.values, tables.block_tables, tables.lengths,
+                                                  scale=self.scale)
+            return out.view(batch, steps, self.heads * self.head_dim)
+        out = torch.empty_like(rotated)
+        for request, first, count in tables.prompts:
+            if tables.held[request] != count:
+                raise ValueError("multi-token continuation is not supported by this harness")
+            keys, values = cache.fetch(first, count)
+            attended = scaled_dot_product_attention(
+                rotated[None, first:first + count].transpose(1, 2), keys[None].transpose(1, 2), values[None].transpose(1, 2),
+                cache, self.scale, "causal" if count > 1 else None)
+            out[first:first + count] = attended[0].transpose(0, 1)
+        return out.view(batch, steps, self.heads * self.head_dim)
 
 
 class DecoderBlock(nn.Module):
@@ -312,6 +450,13 @@ class TinyCausalLM(nn.Module):
             caches.append(KVCache(batch, attention.kv_heads, capacity, attention.head_dim,
                                   attention.q_proj.weight.device))
         return caches
+
+    def make_paged_cache(self, requests, pages, page_size=16, capacity=4096):
+        """A PagedKVCache for every layer, over the same tables: `pages` pages for `requests` requests of up to `capacity`
+        tokens each."""
+        first = self.layers[0].self_attn
+        tables = PagedTables(requests, pages, page_size, -(-capacity // page_size), first.q_proj.weight.device)
+        return [PagedKVCache(tables, layer.self_attn.kv_heads, layer.self_attn.head_dim) for layer in self.layers]
 
     def forward(self, tokens, cache=None, logits_to_keep=0):
         """Logits [batch, tokens, vocabulary]; with `logits_to_keep`, of that many last positions only."""

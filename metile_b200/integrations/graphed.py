@@ -121,3 +121,116 @@ class GraphedDecoder:
             self.step()
             generated.append(self.token.clone())
         return torch.cat(generated, dim=1)
+
+
+class GraphedBeamDecoder:
+    """Beam search for a batch of requests over a paged cache, a step at a time as a replayed CUDA graph.
+
+    The beams of a request share the pages of its prompt and of every page that was full when they parted, so a step
+    copies at most the page in work of the beams that were dropped, whatever the length.  A step takes its pages, runs the
+    model, selects and reorders on the device.  With one beam it is greedy decoding of requests of different lengths.
+
+        decoder = GraphedBeamDecoder(model, batch=2, beams=4, capacity=4096)
+        tokens, scores = decoder.search([first_prompt, second_prompt], steps=64)
+
+    The model must offer `make_paged_cache` (blocks.TinyCausalLM does)."""
+
+    def __init__(self, model, batch=1, beams=4, capacity=4096, page_size=16, pages=None, end_token=None):
+        self.model, self.batch, self.beams, self.end_token = model, int(batch), int(beams), end_token
+        rows, width = self.batch * self.beams, -(-capacity // page_size)
+        self.cache = model.make_paged_cache(rows, rows * width if pages is None else pages, page_size, capacity)
+        self.tables = self.cache[0].tables
+        device = self.device = self.tables.lengths.device
+        self.token = torch.zeros((rows, 1), dtype=torch.long, device=device)      # input of the next step
+        self.scores = torch.zeros((self.batch, self.beams), dtype=torch.float32, device=device)
+        self.finished = torch.zeros((self.batch, self.beams), dtype=torch.bool, device=device)
+        self.parents = torch.zeros((self.batch, self.beams), dtype=torch.int32, device=device)
+        self.graph = None
+        self.stream = torch.cuda.Stream(device)
+        self._keeps_logits = _takes(model.forward, "logits_to_keep")
+
+    def _select(self, logits, scores, finished):
+        selected = backends.beam_select(logits, scores, keep=self.beams,
+                                        finished=None if self.end_token is None else finished, end_token=self.end_token)
+        for kept, new in zip((self.scores, self.parents, self.token, self.finished), selected):
+            kept.copy_(new.view(kept.shape))
+
+    def _step(self):
+        self.tables.grow()
+        logits = _logits_of(self.model(self.token, cache=self.cache))
+        self._select(logits[:, -1, :], self.scores, self.finished)
+        self.tables.reorder(self.parents, self.cache)
+
+    def prefill(self, prompts):
+        """Read one prompt (a row of token ids) for every request and select the first beams."""
+        if len(prompts) != self.batch:
+            raise ValueError("one prompt for every request of the batch")
+        if not all(prompt.numel() for prompt in prompts):
+            raise ValueError("a prompt has no token")
+        self.tables.reset()
+        # Only the last position's logits are asked for: a head over the whole prompt is most of a small model.
+        last_only = {"logits_to_keep": 1} if self._keeps_logits else {}
+        logits = []
+        with torch.no_grad():
+            for index, prompt in enumerate(prompts):
+                self.tables.grow([prompt.numel() if row == index * self.beams else 0 for row in range(self.tables.requests)])
+                tokens = prompt.reshape(1, -1).to(self.device)
+                logits.append(_logits_of(self.model(tokens, cache=self.cache, **last_only))[:, -1])
+            self.tables.fork(self.beams, self.cache)
+            # The beams are still one: the first of them offers the candidates.
+            start = torch.full((self.batch, self.beams), -torch.inf, device=self.device)
+            start[:, 0] = 0.0
+            self.finished.zero_()
+            self._select(torch.cat(logits).repeat_interleave(self.beams, dim=0), start, self.finished)
+
+    def _capture(self):
+        """Warm what is built lazily on a scratch cache, then capture one step on the real one."""
+        kept = [t.clone() for t in (self.token, self.scores, self.parents, self.finished)]
+        self.stream.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.no_grad(), torch.cuda.stream(self.stream):
+            real, tables = self.cache, self.tables
+            self.cache = self.model.make_paged_cache(tables.requests, tables.requests, tables.page_size, tables.page_size)
+            self.tables = self.cache[0].tables
+            self._step()
+            self.cache, self.tables = real, tables
+            for own, value in zip((self.token, self.scores, self.parents, self.finished), kept):
+                own.copy_(value)
+            held, free = list(tables.held), tables.free
+            self.stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=self.stream):
+                self._step()
+            tables.held, tables.free = held, free     # capture ran the host's bookkeeping once
+        torch.cuda.current_stream(self.device).wait_stream(self.stream)
+        self.graph = graph
+
+    def step(self):
+        """One token for every beam; the decoder's token, scores, parents and finished are those of the new beams."""
+        if self.graph is None:
+            self._capture()
+        self.tables.account([1] * self.tables.requests)   # what the graph does on the device
+        caller = torch.cuda.current_stream(self.device)
+        self.stream.wait_stream(caller)
+        with torch.cuda.stream(self.stream):
+            self.graph.replay()
+        caller.wait_stream(self.stream)
+
+    def search(self, prompts, steps):
+        """The `beams` best continuations by `steps` tokens found for every prompt: tokens [batch, beams, steps] and the sums
+        of their log-probabilities [batch, beams], the best first.  A beam that has met the end token repeats it."""
+        if steps < 1:
+            raise ValueError("a search takes one step or more")
+        self.prefill(prompts)
+        tokens, parents = [self.token.clone()], []
+        for _ in range(steps - 1):
+            self.step()
+            tokens.append(self.token.clone())
+            parents.append(self.parents.clone())
+        # Back along the parents, from the last selection to the first.
+        at = torch.arange(self.beams, device=self.device).expand(self.batch, -1)
+        out = []
+        for index in range(steps - 1, -1, -1):
+            out.append(torch.gather(tokens[index].view(self.batch, self.beams), 1, at))
+            if index:
+                at = torch.gather(parents[index - 1].long(), 1, at)
+        return torch.stack(out[::-1], dim=2), self.scores.clone()

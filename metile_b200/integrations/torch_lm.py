@@ -30,7 +30,7 @@ from torch.nn.modules import module as torch_module
 
 from .. import backends
 from . import blocks
-from .blocks import KVCache
+from .blocks import KVCache, PagedKVCache
 
 FEATURES = ("attention", "rms_norm", "graph_fusion", "quantized_mlp")
 _GATED_MLP_ATTRIBUTES = ("gate_proj", "up_proj", "down_proj")
@@ -213,13 +213,18 @@ _qkv_cache = weakref.WeakKeyDictionary()
 
 def attention_decode_refusal(module, values, cache):
     """None when the five-kernel decode step can serve this call of an attention module, else why not:
-    one new token per sequence, an in-place cache with room left, four affine 4-bit projections
-    without additive bias, bfloat16 activations on CUDA, and a head layout the kernels take."""
+    one new token per sequence, an in-place cache with room left (or a paged one whose tables have grown by that
+    token), four affine 4-bit projections without additive bias, bfloat16 activations on CUDA, and a head
+    layout the kernels take."""
     if values.ndim != 3 or values.shape[1] != 1:
         return "not a single-token decode step"
-    if cache is None or not all(hasattr(cache, name) for name in ("keys", "values", "length", "positions", "advance")):
+    paged = isinstance(cache, PagedKVCache)
+    if paged:
+        if cache.tables.prompts is not None or cache.tables.slots is None or cache.keys.dtype != values.dtype:
+            return "the paged cache does not stand before a step of this type"
+    elif cache is None or not all(hasattr(cache, name) for name in ("keys", "values", "length", "positions", "advance")):
         return "no in-place KV cache"
-    if cache.length < 1 or cache.length >= cache.keys.shape[2]:
+    elif cache.length < 1 or cache.length >= cache.keys.shape[2]:
         return "the cache is empty or full"
     for name in _ATTENTION_ATTRIBUTES:
         linear = getattr(module, name, None)
@@ -228,13 +233,14 @@ def attention_decode_refusal(module, values, cache):
         if getattr(linear, "bias", None) is not None:
             return f"{name} has an additive bias"
     heads, kv_heads, dim = (getattr(module, name, None) for name in ("heads", "kv_heads", "head_dim"))
-    if not heads or not kv_heads or dim not in (64, 128) or heads % kv_heads or heads // kv_heads > 8:
+    if not heads or not kv_heads or heads % kv_heads or (
+            dim not in (64, 128, 256) if paged else dim not in (64, 128) or heads // kv_heads > 8):
         return "head layout outside what the decode kernel serves"
     if getattr(module, "rope_theta", None) is None:
         return "no rotary base"
     if values.dtype != torch.bfloat16 or not values.is_cuda:
         return "activations are not bfloat16 on a CUDA device"
-    if values.shape[0] != cache.keys.shape[0]:
+    if values.shape[0] != (cache.tables.requests if paged else cache.keys.shape[0]):
         return "batch does not match the cache"
     return None
 
@@ -272,6 +278,13 @@ def _attention_decode(module, values, cache, residual):
     q = qkv[:, :heads * dim].view(batch, heads, dim)
     k = qkv[:, heads * dim:(heads + kv_heads) * dim].view(batch, kv_heads, dim)
     v = qkv[:, (heads + kv_heads) * dim:].view(batch, kv_heads, dim)
+    scale = getattr(module, "scale", dim ** -0.5)
+    if isinstance(cache, PagedKVCache):
+        rotated = cache.append(q, k, v, module._frequencies_on(q.device) if hasattr(module, "_frequencies_on")
+                               else blocks._rope_frequencies(module.rope_theta, dim, q.device))
+        attended = backends.paged_attention_decode(rotated, cache.keys, cache.values, cache.tables.block_tables,
+                                                   cache.tables.lengths, scale=scale)
+        return _output_projection(module.o_proj, attended.view(batch, heads * dim), values, residual)
     own_cache = blocks.appends_in_place(cache)  # then advancing is counting, on the host and on the device
     rotated = backends.rope_kv_append(q, k, v, cache.positions, cache.keys, cache.values, theta=module.rope_theta,
                                       advance=own_cache)
@@ -279,19 +292,20 @@ def _attention_decode(module, values, cache, residual):
         cache.length += 1
     else:
         cache.advance(1)
-    scale = getattr(module, "scale", dim ** -0.5)
     # The whole cache with the per-sequence lengths on the device (not a slice cut at the host's count):
     # the same 128-token splits are merged either way, and nothing of the step depends on a host number,
     # so a captured CUDA graph of it stays valid as the sequences grow.
     attended = backends.mlx_attention_decode(rotated.view(batch, heads, 1, dim), cache.keys, cache.values,
                                              scale=scale, lengths=cache.positions)
-    attended = attended.view(batch, heads * dim)
-    o = module.o_proj
+    return _output_projection(module.o_proj, attended.view(batch, heads * dim), values, residual)
+
+
+def _output_projection(o, attended, values, residual):
     if residual is None:
         out = backends.mlx_affine_qmv(attended, o.weight, o.scales, o.biases)
     else:
         out = backends.mlx_affine_residual_qmv(attended, o.weight, o.scales, o.biases,
-                                               residual.reshape(batch, residual.shape[-1]))
+                                               residual.reshape(attended.shape[0], residual.shape[-1]))
     return out.view(values.shape)
 
 
