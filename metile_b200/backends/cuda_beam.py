@@ -74,8 +74,6 @@ def beam_reorder(block_tables, lengths, parents, caches):
     it stays one beam's own: a parent's first child goes on in it, any other child takes that of a beam without children,
     and what the parent's holds is copied there, in place, in every cache.  Entries behind it stay each row's own.  The pages in
     work of a group must be distinct before the call, and are after it."""
-    if isinstance(caches, list):
-        caches = tuple(tuple(pair) if isinstance(pair, list) else pair for pair in caches)
     out = native().beam_reorder(block_tables, lengths, parents, caches)
     if out is None:
         _require_table(block_tables)

@@ -26,8 +26,8 @@ namespace mt {
 
 constexpr double kDeadScore = -1e9;  // no sum of log-probabilities but the mask of a beam that is out; above it 64 bits keep logits apart
 // d = logit - top rounded, then d log2 e: |d| 2^-24 each and |d| 1.4e-8 for log2 e itself, 2^-22 for ex2.approx, within a share
-// and once more for the share in the row, where the two |d| add up to the one to the row's maximum; ten roundings of 2^-24 in
-// a warp's sum (the rest is added in 64 bits).  The mean of |d| by the weights is at most the log of the row's length, 13.2: 2.9e-6.
+// and once more for the share in the row, where the two |d| add up to the one to the row's maximum; twelve roundings of 2^-24
+// in sums (the rest is added in 64 bits).  The mean of |d| by the weights is at most the log of the row's length, 13.2: 3.0e-6.
 constexpr double kBeamError = 0x1p-18;
 
 constexpr int kBeamMaxBeams = 32, kBeamMaxKeep = 64;
@@ -38,7 +38,7 @@ constexpr int kBeamShareBytes = kBeamVectors * 512, kBeamBlock = kBeamShareBytes
 constexpr int kBeamRing = kBeamStages * kBeamShares * kBeamBlock;
 constexpr int kBeamBuckets = 64, kBeamCollect = 512;         // of a part
 static_assert(kBeamCollect >= kBeamMaxKeep + kBeamThreads, "equal ones are collected a step of all threads at a time");
-constexpr int kBeamSlack = 8, kBeamJoinCollect = (kBeamMaxKeep + kBeamSlack) * kBeamMaxKeep, kBeamStage = 4096;
+constexpr int kBeamSlack = 8, kBeamKeys = 256, kBeamStage = 4096;              // entries of the lists that the join has in shared memory
 static_assert(kBeamBuckets >= kBeamMaxKeep, "the bound of a part comes from its buckets");
 
 __host__ __device__ constexpr int beam_size(int type) { return type == 2 ? 4 : 2; }               // bytes of a logit
@@ -66,13 +66,23 @@ struct BeamSelectParams {
     long long row_stride, end_token;  // no end token: -1
     int groups, beams, vocabulary, keep, spans;
     int parts, runs;                // the most parts of a row; CTAs
+    // Of the join: entries of a list in shared memory and among the samples; 2^32 / n rounded up, for whole quotients of
+    // numbers up to 65536 (0 where n is 1).
+    int staged, depths;
+    unsigned int per_keep, per_staged, per_depths, per_parts;
 };
+
+__host__ __device__ inline unsigned int beam_reciprocal(unsigned int n) { return n == 1 ? 0u : (unsigned int)((0x100000000ull + n - 1) / n); }
+__device__ __forceinline__ int beam_divided(int i, unsigned int reciprocal) { return reciprocal ? (int)__umulhi((unsigned int)i, reciprocal) : i; }
 
 // Run r of S spans dealt out to R: from its first span to the next one's.  And the run a span is in.
 __host__ __device__ inline long long beam_run_start(long long run, long long spans, long long runs) { return run * spans / runs; }
 __host__ __device__ inline long long beam_run_of(long long span, long long spans, long long runs) { return ((span + 1) * runs - 1) / spans; }
 
 inline int beam_spans(int vocabulary, int type) { return (vocabulary + beam_span(type) - 1) / beam_span(type); }
+
+// The most candidates the join collects without a margin: from keep + slack lists, `keep` of each.
+__host__ __device__ inline int beam_join_most(int keep) { return (keep + kBeamSlack) * keep; }
 
 // What the host and the kernels go by: as many CTAs as run at once, but no run longer than a part may be, and no row in more
 // parts than the join takes.
@@ -82,6 +92,8 @@ inline void beam_plan(int rows, int spans, int sm_count, int& parts, int& runs) 
     if (count < (all + kBeamMostPerPart - 1) / kBeamMostPerPart) count = (all + kBeamMostPerPart - 1) / kBeamMostPerPart;
     if (count > (long long)rows * (kBeamMaxParts - 2)) count = (long long)rows * (kBeamMaxParts - 2);
     if (count > all) count = all;
+    if (count < rows && spans <= kBeamMostPerPart) count = rows;
+    if (count >= rows) count = count / rows * rows;  // a run ends with a row: it has no second part to finish
     runs = (int)count;
     parts = (int)((spans - 1) * count / all) + 2;
     if (parts > spans) parts = spans;
@@ -197,9 +209,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     using Copies = BeamCopies<kType>;
     constexpr int kPer = Copies::kPer, kShare = Copies::kShare, kVectors = kBeamVectors, kWarps = kBeamShares;
     extern __shared__ __align__(16) char beam_ring[];  // [warps][stages][block]
-    __shared__ float span_top[kBeamMostPerPart][kBeamThreads], bucket[kBeamBuckets];
+    __shared__ float span_top[kBeamMostPerPart][kBeamThreads];
+    __shared__ __align__(16) float bucket[kBeamBuckets];
     __shared__ float collected[kBeamCollect], bound_shared;
-    __shared__ int collected_token[kBeamCollect], count;
+    __shared__ int collected_token[kBeamCollect], hits[kBeamShares][32], count;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long spans = (long long)p.groups * p.beams * p.spans;
     const long long run0 = beam_run_start(blockIdx.x, spans, p.runs), run1 = beam_run_start(blockIdx.x + 1, spans, p.runs);
@@ -313,10 +326,11 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
             const float value = bucket[own];
             int rank = 0;
 #pragma unroll
-            for (int i = 0; i < kBeamBuckets / 4; ++i) {
-                const int j = 4 * i + (lane & 3);
-                const float other = bucket[j];
-                rank += other > value || (other == value && j < own);
+            for (int i = 0; i < kBeamBuckets / 16; ++i) {
+                const int j = 16 * i + 4 * (lane & 3);
+                const float4 others = *reinterpret_cast<const float4*>(&bucket[j]);
+                rank += (others.x > value || (others.x == value && j < own)) + (others.y > value || (others.y == value && j + 1 < own)) +
+                        (others.z > value || (others.z == value && j + 2 < own)) + (others.w > value || (others.w == value && j + 3 < own));
             }
             rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
             rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
@@ -324,15 +338,42 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
         }
         __syncthreads();
         const float bound = bound_shared;
-        // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens.
+        // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens.  A logit is
+        // read again from memory, so up to 32 such threads are noted down and read four at a time.
         auto reach = [&](auto qualifies, auto visit) {
+            int noted = 0;
+            auto look = [&] {
+                __syncwarp();
+                for (int k = 0; k < noted; k += 4) {
+                    float logit[4];
+                    int token[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int hit = hits[warp][min(k + i, noted - 1)];
+                        token[i] = (hit >> 5) * beam_span(kType) + warp * kShare + (lane / kPer * 32 + (hit & 31)) * kPer + lane % kPer;
+                        if (k + i >= noted || lane >= kVectors * kPer || token[i] >= p.vocabulary) token[i] = -1;
+                        logit[i] = token[i] >= 0 ? beam_logit_at<kType>(from, token[i]) : 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (token[i] >= 0) visit(logit[i], token[i]);
+                }
+                noted = 0;
+                __syncwarp();
+            };
             for (int span = span0; span < span1 && count <= kBeamCollect; ++span) {
                 unsigned int threads = __ballot_sync(0xFFFFFFFFu, qualifies(span_top[span - span0][threadIdx.x]));
-                for (; threads; threads &= threads - 1u) {
-                    const int token = span * beam_span(kType) + warp * kShare + (lane / kPer * 32 + __ffs(threads) - 1) * kPer + lane % kPer;
-                    if (lane < kVectors * kPer && token < p.vocabulary) visit(beam_logit_at<kType>(from, token), token);
+                while (threads) {
+                    const int at = noted + __popc(threads & ((1u << lane) - 1u));
+                    const bool fits = (threads >> lane & 1u) && at < 32;
+                    if (fits) hits[warp][at] = span << 5 | lane;
+                    const unsigned int taken = __ballot_sync(0xFFFFFFFFu, fits);
+                    noted += __popc(taken);
+                    threads &= ~taken;
+                    if (noted == 32) look();
                 }
             }
+            look();
         };
         auto collect = [&](float logit, int token) {
             const int place = atomicAdd(&count, 1);
@@ -428,6 +469,17 @@ __device__ __forceinline__ double beam_value(long long order) {
     return __longlong_as_double(order ^ (order >> 63 & 0x7FFFFFFFFFFFFFFFll));
 }
 
+// The order's 64-bit value rounded down to a 32-bit number, as a whole one of the same order (never 0); and the least
+// value with that key, with its top bit turned over.
+__device__ __forceinline__ unsigned int beam_key(long long order) {
+    const unsigned int bits = __float_as_uint(__double2float_rd(beam_value(order)));
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long beam_key_floor(unsigned int key) {
+    const float value = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+    return (unsigned long long)beam_order((double)value) ^ 0x8000000000000000ull;
+}
+
 // How many of n candidates come before `own`, eight neighbouring threads together; those without a place do not count.
 __device__ __forceinline__ int beam_rank(const BeamCandidate* candidates, int n, const BeamCandidate& own) {
     int rank = 0;
@@ -444,23 +496,24 @@ __device__ __forceinline__ int beam_rank(const BeamCandidate* candidates, int n,
 // One CTA per group; a list of sorted candidates for every part of every beam.  Bound by the latency of its steps: what it
 // reads is asked for at once, the first `staged` entries of every list among it.
 template <int kType>
-__global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams p, int staged) {
+__global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams p) {
     extern __shared__ __align__(16) unsigned char join_smem[];
-    BeamCandidate* collected = reinterpret_cast<BeamCandidate*>(join_smem);          // [kBeamJoinCollect]
-    BeamEntry* stage = reinterpret_cast<BeamEntry*>(collected + kBeamJoinCollect);   // [lists, staged]
-    int* order = reinterpret_cast<int*>(stage + kBeamStage);                         // [kBeamJoinCollect]
+    const int lists = p.beams * p.parts, staged = p.staged, most = beam_join_most(p.keep);
+    unsigned int* keys = reinterpret_cast<unsigned int*>(join_smem);                    // [kBeamKeys]
+    BeamCandidate* collected = reinterpret_cast<BeamCandidate*>(keys + kBeamKeys);      // [most]
+    BeamEntry* stage = reinterpret_cast<BeamEntry*>(collected + most);                  // [lists, staged]
+    int* order = reinterpret_cast<int*>(stage + lists * staged);                        // [most]
     __shared__ double top[kBeamMaxBeams], log_sum[kBeamMaxBeams], score[kBeamMaxBeams], scratch[32];
     __shared__ unsigned char kind[kBeamMaxBeams];  // 0: a beam's own lists, 1: it has finished, 2: it has no candidate
-    __shared__ int count, own_parts[kBeamMaxBeams];
-    __shared__ unsigned int close;
+    __shared__ int count, own_parts[kBeamMaxBeams], reaching;
+    __shared__ unsigned int close, key_bound;
     const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int lists = p.beams * p.parts;
     const long long row0 = (long long)group * p.beams;
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
     const BeamEntry* entries = p.lists + row0 * p.parts * p.keep;
     for (int i = threadIdx.x; i < lists * staged; i += blockDim.x) {
-        const int list = i / staged;
+        const int list = beam_divided(i, p.per_staged);
         ptx::cp_async_8(stage + i, entries + (long long)list * p.keep + (i - list * staged));
     }
     ptx::cp_async_commit();
@@ -469,16 +522,24 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
         const bool ended = p.finished && p.finished[row0 + beam];
         const BeamShareStats* stats = p.stats + (row0 + beam) * p.spans * kBeamShares;
         const int shares = p.spans * kBeamShares;
+        // 128 shares at a time: a lane's four of them are asked for together.
         float best = -INFINITY;
-#pragma unroll 4
-        for (int i = lane; i < shares; i += 32) best = fmaxf(best, stats[i].top);
-#pragma unroll
-        for (int offset = 16; offset >= 1; offset >>= 1) best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, offset));
         double sum = 0.0;
-#pragma unroll 4
-        for (int i = lane; i < shares; i += 32) {
-            const BeamShareStats own = stats[i];
-            sum += (double)own.sum * (own.sum == 0.0f ? 0.0 : (double)__expf(own.top - best));  // of the same error as within a share
+        for (int first = 0; first < shares; first += 128) {
+            BeamShareStats own[4];
+            float now = best;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = first + 32 * k + lane;
+                own[k] = i < shares ? stats[i] : BeamShareStats{-INFINITY, 0.0f};
+                now = fmaxf(now, own[k].top);
+            }
+            asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(now) : "f"(now));
+            float part = 0.0f;  // of the same error as within a share
+#pragma unroll
+            for (int k = 0; k < 4; ++k) part += own[k].sum == 0.0f ? 0.0f : own[k].sum * __expf(own[k].top - now);
+            sum = (sum == 0.0 ? 0.0 : sum * (double)__expf(best - now)) + (double)part;
+            best = now;
         }
 #pragma unroll
         for (int offset = 16; offset >= 1; offset >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);
@@ -514,50 +575,96 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
         return {nothing, base + token};
     };
     // The first entries of every list, one to a thread and `keep` at least: what the keep-th best of them reaches bounds the
-    // keep-th best of all from below.  It is found bit by bit, by value and among equals by place, until few reach it.
-    const int depths = min(p.keep, max((p.keep + lists - 1) / lists, (int)blockDim.x / lists)), samples = lists * depths;
+    // keep-th best of all from below.  It is found among the values rounded to 32 bits, which keeps their order; where too many
+    // are equal there, bit by bit, by value and among equals by place.
+    const int samples = lists * p.depths;
     constexpr unsigned long long kTopBit = 0x8000000000000000ull;
     for (int phase = 0;; ++phase) {
         const double margin = phase == 0 && p.beams > 1 ? 2.0 * kBeamError : 0.0;
-        if (threadIdx.x == 0) count = 0;
+        if (threadIdx.x == 0) {
+            count = 0;
+            key_bound = 0;
+            reaching = 0;
+        }
         BeamCandidate sample = {0, -1};
         if (threadIdx.x < samples) {
-            const int list = threadIdx.x / depths;
-            sample = candidate(list, list / p.parts, threadIdx.x - list * depths);
+            const int list = beam_divided(threadIdx.x, p.per_depths);
+            sample = candidate(list, beam_divided(list, p.per_parts), threadIdx.x - list * p.depths);
         }
-        const unsigned long long value = (unsigned long long)sample.value ^ kTopBit, place = ~(unsigned long long)sample.place;
-        unsigned long long value_bound = 0, place_bound = 0;
-        int reaching = 0x7FFFFFFF;
-        for (unsigned long long bit = kTopBit; bit && reaching > p.keep + kBeamSlack; bit >>= 1) {
-            const int now = __syncthreads_count(sample.place >= 0 && value >= (value_bound | bit));
-            if (now >= p.keep) {
-                value_bound |= bit;
-                reaching = now;
+        const unsigned int key = sample.place < 0 ? 0u : beam_key(sample.value);
+        if (threadIdx.x < kBeamKeys) keys[threadIdx.x] = key;
+        __syncthreads();
+        if (warp == 0 && samples <= kBeamKeys) {  // from the first bit in which they differ
+            unsigned int own[kBeamKeys / 32], highest = 0, lowest = 0xFFFFFFFFu;
+            int now = 0;
+#pragma unroll
+            for (int k = 0; k < kBeamKeys / 32; ++k) {
+                own[k] = keys[32 * k + lane];
+                highest = max(highest, own[k]);
+                lowest = min(lowest, own[k] - 1u);  // none is the largest so
+                now += own[k] != 0;
             }
-        }
-        for (unsigned long long bit = kTopBit; bit && reaching > p.keep + kBeamSlack && value_bound; bit >>= 1) {
-            const int now = __syncthreads_count(sample.place >= 0 && (value > value_bound || (value == value_bound && place >= (place_bound | bit))));
+            highest = __reduce_max_sync(0xFFFFFFFFu, highest);
+            lowest = __reduce_min_sync(0xFFFFFFFFu, lowest) + 1u;
+            now = __reduce_add_sync(0xFFFFFFFFu, now);
             if (now >= p.keep) {
-                place_bound |= bit;
-                reaching = now;
+                unsigned int found_key = lowest, bit = highest ^ lowest;
+                for (bit = bit ? 0x80000000u >> __clz(bit) : 0u; bit && now > p.keep + kBeamSlack; bit >>= 1) {
+                    const unsigned int tried = (found_key & ~(bit - 1u)) | bit;
+                    int reach_it = 0;
+#pragma unroll
+                    for (int k = 0; k < kBeamKeys / 32; ++k) reach_it += own[k] >= tried;
+                    reach_it = __reduce_add_sync(0xFFFFFFFFu, reach_it);
+                    if (reach_it >= p.keep) {
+                        found_key = tried;
+                        now = reach_it;
+                    } else {
+                        found_key &= ~bit;
+                    }
+                }
+                if (lane == 0) {
+                    key_bound = max(found_key, lowest);
+                    reaching = now;
+                }
             }
         }
         __syncthreads();
+        unsigned long long value_bound = 0, place_bound = 0;
+        if (reaching > p.keep + kBeamSlack || samples > kBeamKeys) {
+            const unsigned long long value = (unsigned long long)sample.value ^ kTopBit, place = ~(unsigned long long)sample.place;
+            int now_reaching = 0x7FFFFFFF;
+            for (unsigned long long bit = kTopBit; bit && now_reaching > p.keep + kBeamSlack; bit >>= 1) {
+                const int now = __syncthreads_count(sample.place >= 0 && value >= (value_bound | bit));
+                if (now >= p.keep) {
+                    value_bound |= bit;
+                    now_reaching = now;
+                }
+            }
+            for (unsigned long long bit = kTopBit; bit && now_reaching > p.keep + kBeamSlack; bit >>= 1) {
+                const int now = __syncthreads_count(sample.place >= 0 && (value > value_bound || (value == value_bound && place >= (place_bound | bit))));
+                if (now >= p.keep) {
+                    place_bound |= bit;
+                    now_reaching = now;
+                }
+            }
+        } else if (key_bound) {
+            value_bound = beam_key_floor(key_bound);
+        }
         const unsigned long long least = (unsigned long long)nothing ^ kTopBit;
         const bool wider = margin > 0.0 && value_bound > least;
         const unsigned long long reach = wider ? (unsigned long long)beam_order(beam_value((long long)(value_bound ^ kTopBit)) - margin) ^ kTopBit : value_bound;
         for (int i = threadIdx.x; i < lists * p.keep; i += blockDim.x) {
-            const int list = i / p.keep;
-            const BeamCandidate own = candidate(list, list / p.parts, i - list * p.keep);
+            const int list = beam_divided(i, p.per_keep);
+            const BeamCandidate own = candidate(list, beam_divided(list, p.per_parts), i - list * p.keep);
             const unsigned long long value = (unsigned long long)own.value ^ kTopBit;
             if (own.place < 0 || value < reach || (!wider && value == reach && ~(unsigned long long)own.place < place_bound)) continue;
             const int at = atomicAdd(&count, 1);
-            if (at < kBeamJoinCollect) collected[at] = own;
+            if (at < most) collected[at] = own;
         }
         __syncthreads();
         const int found = count;
         // Only the margin can let in more: without it what is collected comes from keep + slack lists at most, `keep` from each.
-        const bool overflow = found > kBeamJoinCollect;
+        const bool overflow = found > most;
         if (!overflow) {
             for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += blockDim.x >> 3) {
                 const int rank = beam_rank(collected, found, collected[min(i, found - 1)]);
@@ -617,14 +724,23 @@ inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_
     params.spans = beam_spans(params.vocabulary, kType);
     beam_plan(params.groups * params.beams, params.spans, sm_count, params.parts, params.runs);
     const int lists = params.beams * params.parts;
-    const int threads = lists > 512 ? 1024 : 512;  // a list or more of each
-    const int staged = params.keep < kBeamStage / lists ? params.keep : kBeamStage / lists;
-    constexpr int kSmem = kBeamJoinCollect * (sizeof(BeamCandidate) + sizeof(int)) + kBeamStage * sizeof(BeamEntry);
+    const int threads = lists > 512 ? 1024 : lists > 256 ? 512 : 256;  // a list or more of each
+    params.staged = params.keep < kBeamStage / lists ? params.keep : kBeamStage / lists;
+    const int covering = (params.keep + lists - 1) / lists, filling = threads / lists;
+    params.depths = covering > filling ? covering : filling;
+    params.depths = params.depths < params.keep ? params.depths : params.keep;
+    params.per_keep = beam_reciprocal(params.keep);
+    params.per_staged = beam_reciprocal(params.staged);
+    params.per_depths = beam_reciprocal(params.depths);
+    params.per_parts = beam_reciprocal(params.parts);
+    auto smem_of = [](int keep, int entries) {
+        return beam_join_most(keep) * (sizeof(BeamCandidate) + sizeof(int)) + entries * sizeof(BeamEntry) + kBeamKeys * sizeof(int);
+    };
     static bool configured[64] = {};
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return MT_ERR_LAUNCH;
     if (device >= 64 || !configured[device]) {
-        if (cudaFuncSetAttribute(beam_join_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+        if (cudaFuncSetAttribute(beam_join_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(kBeamMaxKeep, kBeamStage)) != cudaSuccess)
             return MT_ERR_LAUNCH;
         if (cudaFuncSetAttribute(beam_span_kernel<kType>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamRing) != cudaSuccess) return MT_ERR_LAUNCH;
         if (device < 64) configured[device] = true;
@@ -642,8 +758,8 @@ inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_
     if (cudaLaunchKernelEx(&config, beam_span_kernel<kType>, params) != cudaSuccess) return MT_ERR_LAUNCH;
     config.gridDim = dim3(params.groups, 1, 1);
     config.blockDim = dim3(threads, 1, 1);
-    config.dynamicSmemBytes = kSmem;
-    return cudaLaunchKernelEx(&config, beam_join_kernel<kType>, params, staged) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    config.dynamicSmemBytes = smem_of(params.keep, lists * params.staged);
+    return cudaLaunchKernelEx(&config, beam_join_kernel<kType>, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
 }
 
 }  // namespace mt

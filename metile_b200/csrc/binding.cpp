@@ -673,21 +673,22 @@ PyObject* beam_select(PyObject* const* args) {
 PyObject* beam_reorder(PyObject* const* args) {
     const Tensor *tables = plain(args[0]), *lengths = plain(args[1]), *parents = plain(args[2]);
     const int64_t stride = table_stride(tables);
-    if (stride < 0 || !parents || parents->dim() != 2 || parents->numel() == 0 || !PyTuple_Check(args[3])) Py_RETURN_NONE;
+    auto sequence = [](PyObject* object) { return PyTuple_CheckExact(object) || PyList_CheckExact(object); };
+    if (stride < 0 || !parents || parents->dim() != 2 || parents->numel() == 0 || !sequence(args[3])) Py_RETURN_NONE;
     const auto device = tables->device();
     const int64_t groups = parents->size(0), beams = parents->size(1), rows = tables->size(0), width = tables->size(1);
     if (rows != groups * beams || !ints_on(lengths, device, rows) || !ints_on(parents, device, rows) || !fits_int(rows) || !fits_int(width))
         Py_RETURN_NONE;
-    const Py_ssize_t count = PyTuple_GET_SIZE(args[3]);
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(args[3]);
     if (count < 1 || !fits_int(count)) Py_RETURN_NONE;
     std::vector<void*> addresses[2];
     Pages first[2];
     const Tensor* sample = nullptr;
     for (Py_ssize_t c = 0; c < count; ++c) {
-        PyObject* pair = PyTuple_GET_ITEM(args[3], c);
-        if (!PyTuple_Check(pair) || PyTuple_GET_SIZE(pair) != 2) Py_RETURN_NONE;
+        PyObject* pair = PySequence_Fast_GET_ITEM(args[3], c);
+        if (!sequence(pair) || PySequence_Fast_GET_SIZE(pair) != 2) Py_RETURN_NONE;
         for (int which = 0; which < 2; ++which) {
-            const Tensor* pages = plain(PyTuple_GET_ITEM(pair, which));
+            const Tensor* pages = plain(PySequence_Fast_GET_ITEM(pair, which));
             if (!pages || half_type(*pages) < 0) Py_RETURN_NONE;
             if (!sample) sample = pages;
             Pages here;

@@ -400,17 +400,30 @@ __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const __g
         if (threadIdx.x == 0) record_index(kPageOutside, row, (unsigned int)(source < 0 || source >= p.page_count ? source : target));
         return;
     }
-    const int vectors = p.head_dim / 8, count = p.kv_heads * part * vectors;
+    // A thread has one 16-byte vector of a row and takes every `stride`-th row, four at a time.
+    const int vectors = p.head_dim / 8, rows = p.kv_heads * part;
+    const int stride = max(1, (int)blockDim.x / vectors), first_row = threadIdx.x / vectors;
+    if (first_row >= stride) return;
+    for (int i = (threadIdx.x - first_row * vectors) * 8; i < p.head_dim; i += blockDim.x * 8) {  // one round, but for very wide heads
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+            uint16_t* pages = p.pages[which * kReorderMaxCaches + blockIdx.y - 1];
+            const PageStrides strides = which ? p.value_strides : p.key_strides;
+            const uint16_t* source_page = pages + source * strides.page + i;
+            uint16_t* target_page = pages + target * strides.page + i;
+            for (int at = first_row; at < rows; at += 4 * stride) {
+                uint4 moved[4];
+                long long offset[4];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        uint16_t* pages = p.pages[which * kReorderMaxCaches + blockIdx.y - 1];
-        const PageStrides strides = which ? p.value_strides : p.key_strides;
-        for (int at = threadIdx.x; at < count; at += blockDim.x) {
-            const int head = at / (part * vectors), rest = at - head * part * vectors;
-            const int token = rest / vectors, i = (rest - token * vectors) * 8;
-            const long long offset = head * strides.head + token * strides.token + i;
-            *reinterpret_cast<uint4*>(pages + target * strides.page + offset) =
-                ptx::ld_global_dependent_u4(pages + source * strides.page + offset);
+                for (int k = 0; k < 4; ++k) {
+                    const int one = at + k * stride, head = one / part;
+                    offset[k] = head * strides.head + (one - head * part) * strides.token;
+                    if (one < rows) moved[k] = ptx::ld_global_dependent_u4(source_page + offset[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (at + k * stride < rows) *reinterpret_cast<uint4*>(target_page + offset[k]) = moved[k];
+            }
         }
     }
 }
