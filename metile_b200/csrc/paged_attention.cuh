@@ -32,6 +32,7 @@ constexpr int kPagedChunk = 16;          // tokens
 constexpr int kPagedSplitShift = 7;      // the shortest split: 128 tokens
 constexpr int kPagedMostSplits = 128;    // of a sequence
 constexpr int kPagedRowPad = 8;          // elements: rows 16 bytes longer keep matrix loads free of conflicts
+constexpr int kPagedTogether = 4;        // splits that one CTA joins: a warp to each of the SM's four schedulers
 constexpr float kPagedHeadroom = 8.0f;   // log2 of what a weight may reach
 
 __host__ __device__ constexpr int paged_split_shift(int tokens) {
@@ -74,7 +75,7 @@ struct PagedShape {
     static constexpr int kRow = kD + kPagedRowPad;
     static constexpr int kStageElements = 2 * kPagedChunk * kRow;
     static constexpr int kSmem = kWarps * kStages * kStageElements * 2;
-    static_assert(kSmem >= kWarps * 16 * (kD + 2) * 4, "the rings hold the results of 16 heads from every warp");
+    static_assert(kSmem >= kWarps * 16 * (kD + 6) * 4 && kWarps >= kPagedTogether, "the rings hold the results of 16 heads from every warp");
 };
 
 // 16 bytes, or zeros where `bytes` is 0 (the address is a valid one all the same).
@@ -361,8 +362,9 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
         ptx::cp_async_wait_group<0>();
         if (p.together) __syncthreads();  // the rings give way to the warps' results
         // acc[s][tile]: [0], [1]: dim 16 s + g, heads 2 t and 2 t + 1; [2], [3]: dim + 8.
-        float* shared_partial = reinterpret_cast<float*>(rings);  // [warps][8 kTiles][D], then the maxima and sums
-        float2* shared_stats = reinterpret_cast<float2*>(shared_partial + Shape::kWarps * 8 * kTiles * kD);
+        float* shared_partial = reinterpret_cast<float*>(rings);  // [warps][8 kTiles][D + 4], then the maxima and sums
+        constexpr int kPartialRow = kD + 4;                       // the four heads of a store then lie in different banks
+        float2* shared_stats = reinterpret_cast<float2*>(shared_partial + Shape::kWarps * 8 * kTiles * kPartialRow);
 #pragma unroll
         for (int tile = 0; tile < kTiles; ++tile)
 #pragma unroll
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
                         p.out[at * kD + 16 * s + g + 8] = (uint16_t)pack_pair<kHalf>(acc[s][tile][j + 2] * factor, 0.0f);
                     }
                 } else {
-                    float* to = p.together ? shared_partial + (warp * 8 * kTiles + head) * kD : p.partial + (at * p.most_splits + split) * kD;
+                    float* to = p.together ? shared_partial + (warp * 8 * kTiles + head) * kPartialRow : p.partial + (at * p.most_splits + split) * kD;
 #pragma unroll
                     for (int s = 0; s < kSlices; ++s) {
                         to[16 * s + g] = acc[s][tile][j];
@@ -393,17 +395,29 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
         if (p.together) {
             __syncthreads();
             if (splits > 1)
-                for (int i = threadIdx.x; i < heads * kD; i += kThreads) {  // as the join kernel does it
-                    const int head = i / kD, d = i - head * kD;
-                    float largest = -INFINITY, total = 0.0f, value = 0.0f;
-                    for (int w = 0; w < splits; ++w) largest = fmaxf(largest, shared_stats[w * 8 * kTiles + head].x);
-                    for (int w = 0; w < splits; ++w) {
-                        const float2 own = shared_stats[w * 8 * kTiles + head];
-                        const float factor = own.x == -INFINITY ? 0.0f : power_of_two(own.x - largest);
-                        total = fmaf(own.y, factor, total);
-                        value = fmaf(shared_partial[(w * 8 * kTiles + head) * kD + d], factor, value);
+                for (int i = threadIdx.x; i < heads * (kD / 4); i += kThreads) {  // as the join kernel does it, four dims a thread
+                    const int head = i / (kD / 4), d = (i - head * (kD / 4)) * 4;
+                    float2 own[kPagedTogether];
+                    float4 number[kPagedTogether];
+                    float largest = -INFINITY, total = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kPagedTogether; ++w) {
+                        own[w] = w < splits ? shared_stats[w * 8 * kTiles + head] : make_float2(-INFINITY, 0.0f);
+                        number[w] = w < splits ? *reinterpret_cast<const float4*>(shared_partial + (w * 8 * kTiles + head) * kPartialRow + d)
+                                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        largest = fmaxf(largest, own[w].x);
                     }
-                    p.out[((long long)b * p.q_heads + head0 + head) * kD + d] = (uint16_t)pack_pair<kHalf>(total == 0.0f ? 0.0f : value / total, 0.0f);
+                    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < kPagedTogether; ++w) {
+                        const float factor = own[w].x == -INFINITY ? 0.0f : power_of_two(own[w].x - largest);
+                        total = fmaf(own[w].y, factor, total);
+                        value = make_float4(fmaf(number[w].x, factor, value.x), fmaf(number[w].y, factor, value.y), fmaf(number[w].z, factor, value.z),
+                                            fmaf(number[w].w, factor, value.w));
+                    }
+                    uint2 packed = make_uint2(0u, 0u);
+                    if (total != 0.0f) packed = make_uint2(pack_pair<kHalf>(value.x / total, value.y / total), pack_pair<kHalf>(value.z / total, value.w / total));
+                    *reinterpret_cast<uint2*>(p.out + ((long long)b * p.q_heads + head0 + head) * kD + d) = packed;
                 }
             return;
         }
@@ -423,6 +437,10 @@ __global__ void __launch_bounds__(kD) paged_attention_join_kernel(const __grid_c
     if (splits == 1) return;
     const float* from = p.partial + at * p.most_splits * kD + d;
     const float2* stats = p.stats + at * p.most_splits;
+    // The first results are asked for before the maxima are known, the others sixteen ahead.
+    float ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = i < splits ? from[(long long)i * kD] : 0.0f;
     float2 mine[kRounds];
     float top = -INFINITY;
 #pragma unroll
@@ -439,11 +457,13 @@ __global__ void __launch_bounds__(kD) paged_attention_join_kernel(const __grid_c
         const float factor = mine[r].x == -INFINITY ? 0.0f : power_of_two(mine[r].x - top);
 #pragma unroll
         for (int part = 0; part < 32; part += kAhead) {
+            if (32 * r + part >= splits) break;
             float numbers[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int s = 32 * r + part + i;
-                numbers[i] = s < splits ? from[(long long)s * kD] : 0.0f;
+                const int s = 32 * r + part + kAhead + i;
+                numbers[i] = ahead[i];
+                ahead[i] = s < splits ? from[(long long)s * kD] : 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
@@ -475,9 +495,9 @@ inline int launch_paged_attention_instance(PagedAttentionParams params, int sm_c
     }
     const int group = params.q_heads / params.kv_heads;
     const long long per_split = (long long)params.kv_heads * ((group + 8 * kTiles - 1) / (8 * kTiles));
-    // Short tables and few requests: one launch, a CTA for the splits of a KV head, where every CTA has an SM of its own (one request
-    // of 301 tokens, 8 heads of 128: 6.1 us against 8.8).  The same sums in the same order.
-    params.together = params.most_splits > 1 && params.most_splits <= Shape::kWarps && params.batch * per_split <= sm_count;
+    // Short tables and few requests: one launch, a CTA for the splits of a KV head, where every CTA has an SM of its own.  The same
+    // sums in the same order.  One request, 8 heads of 128, one launch and two: three splits 7.6 and 9.0 us, six 10.2 and 9.0.
+    params.together = params.most_splits > 1 && params.most_splits <= kPagedTogether && params.batch * per_split <= sm_count;
     const long long most_units = params.together ? params.batch * per_split : params.batch * per_split * params.most_splits;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(most_units < sm_count ? (unsigned int)most_units : sm_count, 1, 1);
