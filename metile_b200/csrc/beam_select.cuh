@@ -5,12 +5,11 @@
 // -inf; a score that is a mask) counts as -inf.  Bound by the bytes of the logits, and near to it by the exponentials (an
 // SM takes 16 a cycle: 9 TB/s of 16-bit logits on 148 of them).
 //
-// One pass.  Rows are cut into spans of 16 KB, 64 bytes a thread, and the spans of all rows dealt out in runs, one to a CTA; a
-// CTA's share of a row is a part.  Every warp leaves the maximum and the sum of exponentials of its share of a span, and the CTA
-// the `keep` best of each part.  Within a beam candidates are ordered as their logits are, so no sum is needed for that.  Of
-// 64 bucket maxima (four threads each) the keep-th largest bounds the keep-th best from below; the few threads that reach it
-// look at their logits again, and what they find is ranked.  The shares of a row have one size for all calls: its bits do
-// not depend on the others.
+// One pass.  Rows are cut into spans of 16 KB, 64 bytes a thread, and a row's spans dealt out to CTAs; a CTA's share of a row is a
+// part.  Every warp leaves the maximum and the sum of exponentials of its share of a span, and the CTA the `keep` best of its
+// part.  Within a beam candidates are ordered as their logits are, so no sum is needed for that.  Of 64 bucket maxima (four
+// threads each) the keep-th largest bounds the keep-th best from below; the few threads that reach it look at their logits
+// again, and what they find is ranked.  The shares of a row have one size for all calls: its bits do not depend on the others.
 //
 // Then a CTA per group joins spans and beams.  The sums are of 32-bit exponentials, each beam's log-sum off by up to
 // kBeamError; where two beams' candidates are closer than twice that, the sums of the two are taken again, in 64 bits, so
@@ -62,10 +61,10 @@ struct BeamSelectParams {
     long long* tokens_out;
     unsigned char* finished_out;
     BeamShareStats* stats;          // [groups * beams, spans * 8]
-    BeamEntry* lists;               // [groups * beams, parts, keep], as many as a row has parts
+    BeamEntry* lists;               // [groups * beams, parts, keep]
     long long row_stride, end_token;  // no end token: -1
     int groups, beams, vocabulary, keep, spans;
-    int parts, runs;                // the most parts of a row; CTAs
+    int parts;                      // of a row
     // Of the join: entries of a list in shared memory and among the samples; 2^32 / n rounded up, for whole quotients of
     // numbers up to 65536 (0 where n is 1).
     int staged, depths;
@@ -75,28 +74,20 @@ struct BeamSelectParams {
 __host__ __device__ inline unsigned int beam_reciprocal(unsigned int n) { return n == 1 ? 0u : (unsigned int)((0x100000000ull + n - 1) / n); }
 __device__ __forceinline__ int beam_divided(int i, unsigned int reciprocal) { return reciprocal ? (int)__umulhi((unsigned int)i, reciprocal) : i; }
 
-// Run r of S spans dealt out to R: from its first span to the next one's.  And the run a span is in.
-__host__ __device__ inline long long beam_run_start(long long run, long long spans, long long runs) { return run * spans / runs; }
-__host__ __device__ inline long long beam_run_of(long long span, long long spans, long long runs) { return ((span + 1) * runs - 1) / spans; }
+// Part `part` of a row: from its first span to the next one's.
+__host__ __device__ inline int beam_part_start(int part, int spans, int parts) { return (int)((long long)part * spans / parts); }
 
 inline int beam_spans(int vocabulary, int type) { return (vocabulary + beam_span(type) - 1) / beam_span(type); }
 
 // The most candidates the join collects without a margin: from keep + slack lists, `keep` of each.
 __host__ __device__ inline int beam_join_most(int keep) { return (keep + kBeamSlack) * keep; }
 
-// What the host and the kernels go by: as many CTAs as run at once, but no run longer than a part may be, and no row in more
-// parts than the join takes.
-inline void beam_plan(int rows, int spans, int sm_count, int& parts, int& runs) {
-    const long long all = (long long)rows * spans;
-    long long count = (long long)sm_count * kBeamAtOnce;
-    if (count < (all + kBeamMostPerPart - 1) / kBeamMostPerPart) count = (all + kBeamMostPerPart - 1) / kBeamMostPerPart;
-    if (count > (long long)rows * (kBeamMaxParts - 2)) count = (long long)rows * (kBeamMaxParts - 2);
-    if (count > all) count = all;
-    if (count < rows && spans <= kBeamMostPerPart) count = rows;
-    if (count >= rows) count = count / rows * rows;  // a run ends with a row: it has no second part to finish
-    runs = (int)count;
-    parts = (int)((spans - 1) * count / all) + 2;
-    if (parts > spans) parts = spans;
+// Parts of a row: as many as let all CTAs run at once, but none longer than a part may be, and no more than the join takes.
+inline int beam_parts(int rows, int spans, int sm_count) {
+    const int shortest = (spans + kBeamMostPerPart - 1) / kBeamMostPerPart, at_once = sm_count * kBeamAtOnce / rows;
+    int parts = at_once < shortest ? shortest : at_once;
+    if (parts > kBeamMaxParts) parts = kBeamMaxParts;
+    return parts < spans ? parts : spans;
 }
 
 inline size_t beam_workspace_bytes(int groups, int beams, int vocabulary, int keep, int type) {
@@ -162,24 +153,20 @@ __device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
     return d;
 }
 
-// A warp's shares of the spans of a run, copied ahead into its part of the ring.  A share is 2 KB in one piece: element e of a
+// A warp's shares of the spans of a part, copied ahead into its part of the ring.  A share is 2 KB in one piece: element e of a
 // lane's vector v is its (32 v + lane) * kPer + e.
 template <int kType>
 struct BeamCopies {
     static constexpr int kPer = 16 / beam_size(kType), kShare = kBeamShareBytes / beam_size(kType);
-    const BeamSelectParams& p;
     const char* vector;  // this lane's first one of the next share, aligned
-    long long row;
-    int span, left, skew;  // logits of the row from the share on, counted from the boundary in front; bytes behind that
+    int left, skew;      // logits of the row from the share on, counted from the boundary in front; bytes behind that
 
-    __device__ __forceinline__ BeamCopies(const BeamSelectParams& params, long long first_row, int first_span)
-        : p(params), row(first_row), span(first_span) { enter(); }
-    __device__ __forceinline__ void enter() {
+    __device__ __forceinline__ BeamCopies(const char* row, int vocabulary, int span) {
         const int share = span * beam_span(kType) + (int)(threadIdx.x >> 5) * kShare;
-        const char* from = static_cast<const char*>(p.logits) + (row * p.row_stride + share) * beam_size(kType);
+        const char* from = row + (long long)share * beam_size(kType);
         skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
         vector = from - skew + (threadIdx.x & 31) * 16;
-        left = p.vocabulary - share + skew / beam_size(kType);
+        left = vocabulary - share + skew / beam_size(kType);
     }
     __device__ __forceinline__ void next(char* ring) {
         const int lane = threadIdx.x & 31;
@@ -196,11 +183,6 @@ struct BeamCopies {
         }
         vector += kBeamSpanBytes;
         left -= beam_span(kType);
-        if (++span == p.spans) {
-            span = 0;
-            ++row;
-            enter();
-        }
     }
 };
 
@@ -214,15 +196,15 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     __shared__ float collected[kBeamCollect], bound_shared;
     __shared__ int collected_token[kBeamCollect], hits[kBeamShares][32], count;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long spans = (long long)p.groups * p.beams * p.spans;
-    const long long run0 = beam_run_start(blockIdx.x, spans, p.runs), run1 = beam_run_start(blockIdx.x + 1, spans, p.runs);
+    const long long row = blockIdx.x / p.parts;
+    const int part = (int)(blockIdx.x - row * p.parts);
+    const int span0 = beam_part_start(part, p.spans, p.parts), span1 = beam_part_start(part + 1, p.spans, p.parts);
     char* ring = beam_ring + warp * (kBeamStages * kBeamBlock);
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    long long row = run0 / p.spans;
-    int span0 = (int)(run0 - row * p.spans), part = (int)(blockIdx.x - beam_run_of(row * p.spans, spans, p.runs));
-    Copies copies(p, row, span0);
-    int to_copy = (int)(run1 - run0);
+    const char* from = static_cast<const char*>(p.logits) + row * p.row_stride * beam_size(kType);
+    Copies copies(from, p.vocabulary, span0);
+    int to_copy = span1 - span0;
     auto copy_next = [&](int slot) {
         if (to_copy-- > 0) copies.next(ring + slot * kBeamBlock);
         ptx::cp_async_commit();
@@ -230,228 +212,221 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
 #pragma unroll
     for (int i = 0; i < kBeamStages - 1; ++i) copy_next(i);
     int slot = 0;
-    // A part: what the run has of one row.  The rows behind its first one start in it.
-    for (int to_do = (int)(run1 - run0); to_do > 0; ++row, span0 = part = 0) {
-        const int span1 = min(p.spans, span0 + to_do);
-        to_do -= span1 - span0;
-        if (threadIdx.x == 0) count = 0;
-        float mine = -INFINITY;
-        uint32_t raw[kVectors][4];
-        const char* from = static_cast<const char*>(p.logits) + row * p.row_stride * beam_size(kType);
-        const int skew = (int)(reinterpret_cast<uintptr_t>(from) & 15);
-        BeamShareStats* stats = p.stats + (row * p.spans + span0) * kWarps + warp;
-        float last_top = 0.0f, last_total = 0.0f;
-        for (int span = span0; span < span1; ++span) {
-            ptx::cp_async_wait_group<kBeamStages - 2>();
-            __syncwarp();
-            const char* share = ring + slot * kBeamBlock + lane * 16;
+    if (threadIdx.x == 0) count = 0;
+    float mine = -INFINITY;
+    uint32_t raw[kVectors][4];
+    const int skew = copies.skew;
+    BeamShareStats* stats = p.stats + (row * p.spans + span0) * kWarps + warp;
+    float last_top = 0.0f, last_total = 0.0f;
+    for (int span = span0; span < span1; ++span) {
+        ptx::cp_async_wait_group<kBeamStages - 2>();
+        __syncwarp();
+        const char* share = ring + slot * kBeamBlock + lane * 16;
 #pragma unroll
-            for (int v = 0; v < kVectors; ++v) {
-                const uint4 own = *reinterpret_cast<const uint4*>(share + v * 512);
-                if (skew) {
-                    take_skewed(raw[v], own, *reinterpret_cast<const uint4*>(share + v * 512 + 16), skew);
-                } else {
-                    raw[v][0] = own.x; raw[v][1] = own.y; raw[v][2] = own.z; raw[v][3] = own.w;
-                }
+        for (int v = 0; v < kVectors; ++v) {
+            const uint4 own = *reinterpret_cast<const uint4*>(share + v * 512);
+            if (skew) {
+                take_skewed(raw[v], own, *reinterpret_cast<const uint4*>(share + v * 512 + 16), skew);
+            } else {
+                raw[v][0] = own.x; raw[v][1] = own.y; raw[v][2] = own.z; raw[v][3] = own.w;
             }
-            const int left = p.vocabulary - span * beam_span(kType) - warp * kShare;  // behind the row: -inf, and left out below
-            if (left < kShare) {
-#pragma unroll
-                for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e)
-                        if ((32 * v + lane) * kPer + e >= left) {
-                            if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
-                            else {
-                                const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
-                                raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
-                            }
-                        }
-            }
-            __syncwarp();
-            copy_next(slot == 0 ? kBeamStages - 1 : slot - 1);
-            slot = slot == kBeamStages - 1 ? 0 : slot + 1;
-            uint32_t largest = raw[0][0];
+        }
+        const int left = p.vocabulary - span * beam_span(kType) - warp * kShare;  // behind the row: -inf, and left out below
+        if (left < kShare) {
 #pragma unroll
             for (int v = 0; v < kVectors; ++v)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) largest = beam_word_max<kType>(largest, raw[v][i]);
-            float top = beam_word_top<kType>(largest);
-            if (top != top) top = -INFINITY;  // nothing but NaN
-            span_top[span - span0][threadIdx.x] = top;
-            mine = fmaxf(mine, top);
-            asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
-            // The exponentials of the differences to the share's maximum, added as a tree.  (With nothing above -inf the sum is
-            // zero, or NaN where there is one.)  What the warp's lanes have is added one span later, beside the next exponentials.
-            float2 sums[kVectors];
-            const float away = top == -INFINITY ? 0.0f : -top;
-            const float2 shift = make_float2(away, away), log2_e = make_float2(1.4426950408889634f, 1.4426950408889634f);
-#pragma unroll
-            for (int v = 0; v < kVectors; ++v) {
-                float2 weight[kPer / 2];
-#pragma unroll
-                for (int e = 0; e < kPer / 2; ++e) {
-                    const float2 d = add_f32x2(make_float2(beam_logit<kType>(raw[v], 2 * e), beam_logit<kType>(raw[v], 2 * e + 1)), shift);
-                    const float2 power = mul_f32x2(d, log2_e);
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].x) : "f"(power.x));
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].y) : "f"(power.y));
-                }
-#pragma unroll
-                for (int width = kPer / 4; width >= 1; width >>= 1)
-#pragma unroll
-                    for (int e = 0; e < width; ++e) weight[e] = add_f32x2(weight[e], weight[e + width]);
-                sums[v] = weight[0];
-            }
-#pragma unroll
-            for (int width = kVectors / 2; width >= 1; width >>= 1)
-#pragma unroll
-                for (int v = 0; v < width; ++v) sums[v] = add_f32x2(sums[v], sums[v + width]);
-            const float total = warp_sum_xor(last_total);
-            if (lane == 0 && span > span0) *(stats - kWarps) = {last_top, total};
-            stats += kWarps;
-            last_top = top;
-            last_total = sums[0].x + sums[0].y;
-        }
-        last_total = warp_sum_xor(last_total);
-        if (lane == 0) *(stats - kWarps) = {last_top, last_total};
-        {
-            float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = top;
-        }
-        __syncthreads();
-        // The keep-th largest bucket, four threads to a bucket: at least `keep` logits of the CTA are not below it.
-        {
-            const int own = threadIdx.x >> 2;
-            const float value = bucket[own];
-            int rank = 0;
-#pragma unroll
-            for (int i = 0; i < kBeamBuckets / 16; ++i) {
-                const int j = 16 * i + 4 * (lane & 3);
-                const float4 others = *reinterpret_cast<const float4*>(&bucket[j]);
-                rank += (others.x > value || (others.x == value && j < own)) + (others.y > value || (others.y == value && j + 1 < own)) +
-                        (others.z > value || (others.z == value && j + 2 < own)) + (others.w > value || (others.w == value && j + 3 < own));
-            }
-            rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
-            rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
-            if (rank == p.keep - 1 && (lane & 3) == 0) bound_shared = value;
-        }
-        __syncthreads();
-        const float bound = bound_shared;
-        // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens.  A logit is
-        // read again from memory, so up to 32 such threads are noted down and read four at a time.
-        auto reach = [&](auto qualifies, auto visit) {
-            int noted = 0;
-            auto look = [&] {
-                __syncwarp();
-                for (int k = 0; k < noted; k += 4) {
-                    float logit[4];
-                    int token[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int hit = hits[warp][min(k + i, noted - 1)];
-                        token[i] = (hit >> 5) * beam_span(kType) + warp * kShare + (lane / kPer * 32 + (hit & 31)) * kPer + lane % kPer;
-                        if (k + i >= noted || lane >= kVectors * kPer || token[i] >= p.vocabulary) token[i] = -1;
-                        logit[i] = token[i] >= 0 ? beam_logit_at<kType>(from, token[i]) : 0.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (token[i] >= 0) visit(logit[i], token[i]);
-                }
-                noted = 0;
-                __syncwarp();
-            };
-            for (int span = span0; span < span1 && count <= kBeamCollect; ++span) {
-                unsigned int threads = __ballot_sync(0xFFFFFFFFu, qualifies(span_top[span - span0][threadIdx.x]));
-                while (threads) {
-                    const int at = noted + __popc(threads & ((1u << lane) - 1u));
-                    const bool fits = (threads >> lane & 1u) && at < 32;
-                    if (fits) hits[warp][at] = span << 5 | lane;
-                    const unsigned int taken = __ballot_sync(0xFFFFFFFFu, fits);
-                    noted += __popc(taken);
-                    threads &= ~taken;
-                    if (noted == 32) look();
-                }
-            }
-            look();
-        };
-        auto collect = [&](float logit, int token) {
-            const int place = atomicAdd(&count, 1);
-            if (place < kBeamCollect) {
-                collected[place] = logit;
-                collected_token[place] = token;
-            }
-        };
-        reach([&](float top) { return top >= bound; }, [&](float logit, int token) { if (logit >= bound) collect(logit, token); });
-        __syncthreads();
-        BeamEntry* list = p.lists + (row * p.parts + part) * p.keep;
-        int found = count;
-        if (found > kBeamCollect) {
-            // Very many equal ones (masked tokens, a constant row).  What lies above them, then the first of themselves.
-            const int first = span0 * beam_span(kType), last = min(p.vocabulary, span1 * beam_span(kType));
-            __syncthreads();
-            if (threadIdx.x == 0) count = 0;
-            __syncthreads();
-            reach([&](float top) { return top > bound; }, [&](float logit, int token) { if (logit > bound) collect(logit, token); });
-            __syncthreads();
-            found = count;
-            if (found > kBeamCollect) {
-                // The large ones lie in few buckets: `keep` rounds over everything, each for the best behind the last.
-                float before = INFINITY;
-                int before_token = -1;
-                for (int r = 0; r < p.keep; ++r) {
-                    float best = -INFINITY;
-                    int best_token = 0x7FFFFFFF;
-                    for (int token = first + threadIdx.x; token < last; token += kBeamThreads) {
-                        const float logit = beam_logit_at<kType>(from, token);
-                        const bool behind = logit < before || (logit == before && token > before_token);
-                        if (behind && (logit > best || (logit == best && token < best_token))) {
-                            best = logit;
-                            best_token = token;
+                for (int e = 0; e < kPer; ++e)
+                    if ((32 * v + lane) * kPer + e >= left) {
+                        if constexpr (kType == 2) raw[v][e] = 0xFF800000u;
+                        else {
+                            const uint32_t least = kType == 1 ? 0xFC00u : 0xFF80u;
+                            raw[v][e >> 1] = e & 1 ? (raw[v][e >> 1] & 0xFFFFu) | least << 16 : (raw[v][e >> 1] & 0xFFFF0000u) | least;
                         }
                     }
-#pragma unroll
-                    for (int offset = 16; offset >= 1; offset >>= 1) {
-                        const float other = __shfl_xor_sync(0xFFFFFFFFu, best, offset);
-                        const int other_token = __shfl_xor_sync(0xFFFFFFFFu, best_token, offset);
-                        if (other > best || (other == best && other_token < best_token)) { best = other; best_token = other_token; }
-                    }
-                    if (lane == 0) {
-                        collected[warp] = best;
-                        collected_token[warp] = best_token;
-                    }
-                    __syncthreads();
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w)
-                        if (collected[w] > best || (collected[w] == best && collected_token[w] < best_token)) { best = collected[w]; best_token = collected_token[w]; }
-                    if (threadIdx.x == 0) list[r] = {best, best_token == 0x7FFFFFFF ? -1 : best_token};
-                    before = best;
-                    before_token = best_token;
-                    __syncthreads();
-                }
-                continue;
-            }
-            for (int at = first; at < last && found < p.keep; at += kBeamThreads) {  // room for all of a step: keep + 256
-                const int token = at + threadIdx.x;
-                if (token < last && beam_logit_at<kType>(from, token) == bound) collect(bound, token);
-                __syncthreads();
-                found = count;
-                __syncthreads();
-            }
         }
-        // Eight threads rank an entry.
-        for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += kBeamThreads / 8) {
-            const float logit = i < found ? collected[i] : 0.0f;
-            const int token = i < found ? collected_token[i] : 0;
-            int rank = 0;
-            for (int j = threadIdx.x & 7; j < found; j += 8) rank += collected[j] > logit || (collected[j] == logit && collected_token[j] < token);
+        __syncwarp();
+        copy_next(slot == 0 ? kBeamStages - 1 : slot - 1);
+        slot = slot == kBeamStages - 1 ? 0 : slot + 1;
+        uint32_t largest = raw[0][0];
 #pragma unroll
-            for (int offset = 1; offset <= 4; offset <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, offset);
-            if (i < found && (lane & 7) == 0 && rank < p.keep) list[rank] = {logit, token};
+        for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) largest = beam_word_max<kType>(largest, raw[v][i]);
+        float top = beam_word_top<kType>(largest);
+        if (top != top) top = -INFINITY;  // nothing but NaN
+        span_top[span - span0][threadIdx.x] = top;
+        mine = fmaxf(mine, top);
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
+        // The exponentials of the differences to the share's maximum, added as a tree.  (With nothing above -inf the sum is
+        // zero, or NaN where there is one.)  What the warp's lanes have is added one span later, beside the next exponentials.
+        float2 sums[kVectors];
+        const float away = top == -INFINITY ? 0.0f : -top;
+        const float2 shift = make_float2(away, away), log2_e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            float2 weight[kPer / 2];
+#pragma unroll
+            for (int e = 0; e < kPer / 2; ++e) {
+                const float2 d = add_f32x2(make_float2(beam_logit<kType>(raw[v], 2 * e), beam_logit<kType>(raw[v], 2 * e + 1)), shift);
+                const float2 power = mul_f32x2(d, log2_e);
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].x) : "f"(power.x));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(weight[e].y) : "f"(power.y));
+            }
+#pragma unroll
+            for (int width = kPer / 4; width >= 1; width >>= 1)
+#pragma unroll
+                for (int e = 0; e < width; ++e) weight[e] = add_f32x2(weight[e], weight[e + width]);
+            sums[v] = weight[0];
         }
-        for (int i = found + threadIdx.x; i < p.keep; i += kBeamThreads) list[i] = {-INFINITY, -1};
-        __syncthreads();
+#pragma unroll
+        for (int width = kVectors / 2; width >= 1; width >>= 1)
+#pragma unroll
+            for (int v = 0; v < width; ++v) sums[v] = add_f32x2(sums[v], sums[v + width]);
+        const float total = warp_sum_xor(last_total);
+        if (lane == 0 && span > span0) *(stats - kWarps) = {last_top, total};
+        stats += kWarps;
+        last_top = top;
+        last_total = sums[0].x + sums[0].y;
     }
+    last_total = warp_sum_xor(last_total);
+    if (lane == 0) *(stats - kWarps) = {last_top, last_total};
+    {
+        float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = top;
+    }
+    __syncthreads();
+    // The keep-th largest bucket, four threads to a bucket: at least `keep` logits of the CTA are not below it.
+    {
+        const int own = threadIdx.x >> 2;
+        const float value = bucket[own];
+        int rank = 0;
+#pragma unroll
+        for (int i = 0; i < kBeamBuckets / 16; ++i) {
+            const int j = 16 * i + 4 * (lane & 3);
+            const float4 others = *reinterpret_cast<const float4*>(&bucket[j]);
+            rank += (others.x > value || (others.x == value && j < own)) + (others.y > value || (others.y == value && j + 1 < own)) +
+                    (others.z > value || (others.z == value && j + 2 < own)) + (others.w > value || (others.w == value && j + 3 < own));
+        }
+        rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
+        rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
+        if (rank == p.keep - 1 && (lane & 3) == 0) bound_shared = value;
+    }
+    __syncthreads();
+    const float bound = bound_shared;
+    // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens.  A logit is
+    // read again from memory, so up to 32 such threads are noted down and read four at a time.
+    auto reach = [&](auto qualifies, auto visit) {
+        int noted = 0;
+        auto look = [&] {
+            __syncwarp();
+            for (int k = 0; k < noted; k += 4) {
+                float logit[4];
+                int token[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int hit = hits[warp][min(k + i, noted - 1)];
+                    token[i] = (hit >> 5) * beam_span(kType) + warp * kShare + (lane / kPer * 32 + (hit & 31)) * kPer + lane % kPer;
+                    if (k + i >= noted || lane >= kVectors * kPer || token[i] >= p.vocabulary) token[i] = -1;
+                    logit[i] = token[i] >= 0 ? beam_logit_at<kType>(from, token[i]) : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (token[i] >= 0) visit(logit[i], token[i]);
+            }
+            noted = 0;
+            __syncwarp();
+        };
+        for (int span = span0; span < span1 && count <= kBeamCollect; ++span) {
+            unsigned int threads = __ballot_sync(0xFFFFFFFFu, qualifies(span_top[span - span0][threadIdx.x]));
+            while (threads) {
+                const int at = noted + __popc(threads & ((1u << lane) - 1u));
+                const bool fits = (threads >> lane & 1u) && at < 32;
+                if (fits) hits[warp][at] = span << 5 | lane;
+                const unsigned int taken = __ballot_sync(0xFFFFFFFFu, fits);
+                noted += __popc(taken);
+                threads &= ~taken;
+                if (noted == 32) look();
+            }
+        }
+        look();
+    };
+    auto collect = [&](float logit, int token) {
+        const int place = atomicAdd(&count, 1);
+        if (place < kBeamCollect) {
+            collected[place] = logit;
+            collected_token[place] = token;
+        }
+    };
+    reach([&](float top) { return top >= bound; }, [&](float logit, int token) { if (logit >= bound) collect(logit, token); });
+    __syncthreads();
+    BeamEntry* list = p.lists + (row * p.parts + part) * p.keep;
+    int found = count;
+    if (found > kBeamCollect) {
+        // Very many equal ones (masked tokens, a constant row).  What lies above them, then the first of themselves.
+        const int first = span0 * beam_span(kType), last = min(p.vocabulary, span1 * beam_span(kType));
+        __syncthreads();
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        reach([&](float top) { return top > bound; }, [&](float logit, int token) { if (logit > bound) collect(logit, token); });
+        __syncthreads();
+        found = count;
+        if (found > kBeamCollect) {
+            // The large ones lie in few buckets: `keep` rounds over everything, each for the best behind the last.
+            float before = INFINITY;
+            int before_token = -1;
+            for (int r = 0; r < p.keep; ++r) {
+                float best = -INFINITY;
+                int best_token = 0x7FFFFFFF;
+                for (int token = first + threadIdx.x; token < last; token += kBeamThreads) {
+                    const float logit = beam_logit_at<kType>(from, token);
+                    const bool behind = logit < before || (logit == before && token > before_token);
+                    if (behind && (logit > best || (logit == best && token < best_token))) {
+                        best = logit;
+                        best_token = token;
+                    }
+                }
+#pragma unroll
+                for (int offset = 16; offset >= 1; offset >>= 1) {
+                    const float other = __shfl_xor_sync(0xFFFFFFFFu, best, offset);
+                    const int other_token = __shfl_xor_sync(0xFFFFFFFFu, best_token, offset);
+                    if (other > best || (other == best && other_token < best_token)) { best = other; best_token = other_token; }
+                }
+                if (lane == 0) {
+                    collected[warp] = best;
+                    collected_token[warp] = best_token;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w)
+                    if (collected[w] > best || (collected[w] == best && collected_token[w] < best_token)) { best = collected[w]; best_token = collected_token[w]; }
+                if (threadIdx.x == 0) list[r] = {best, best_token == 0x7FFFFFFF ? -1 : best_token};
+                before = best;
+                before_token = best_token;
+                __syncthreads();
+            }
+            return;
+        }
+        for (int at = first; at < last && found < p.keep; at += kBeamThreads) {  // room for all of a step: keep + 256
+            const int token = at + threadIdx.x;
+            if (token < last && beam_logit_at<kType>(from, token) == bound) collect(bound, token);
+            __syncthreads();
+            found = count;
+            __syncthreads();
+        }
+    }
+    // Eight threads rank an entry.
+    for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += kBeamThreads / 8) {
+        const float logit = i < found ? collected[i] : 0.0f;
+        const int token = i < found ? collected_token[i] : 0;
+        int rank = 0;
+        for (int j = threadIdx.x & 7; j < found; j += 8) rank += collected[j] > logit || (collected[j] == logit && collected_token[j] < token);
+#pragma unroll
+        for (int offset = 1; offset <= 4; offset <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, offset);
+        if (i < found && (lane & 7) == 0 && rank < p.keep) list[rank] = {logit, token};
+    }
+    for (int i = found + threadIdx.x; i < p.keep; i += kBeamThreads) list[i] = {-INFINITY, -1};
 }
 
 struct __align__(16) BeamCandidate {
@@ -505,7 +480,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
     int* order = reinterpret_cast<int*>(stage + lists * staged);                        // [most]
     __shared__ double top[kBeamMaxBeams], log_sum[kBeamMaxBeams], score[kBeamMaxBeams], scratch[32];
     __shared__ unsigned char kind[kBeamMaxBeams];  // 0: a beam's own lists, 1: it has finished, 2: it has no candidate
-    __shared__ int count, own_parts[kBeamMaxBeams], reaching;
+    __shared__ int count, reaching;
     __shared__ unsigned int close, key_bound;
     const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const long long row0 = (long long)group * p.beams;
@@ -547,8 +522,6 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             top[beam] = best;
             log_sum[beam] = log(sum);
             score[beam] = given;
-            const long long all = (long long)p.groups * p.beams * p.spans, first = (row0 + beam) * p.spans;
-            own_parts[beam] = (int)(beam_run_of(first + p.spans - 1, all, p.runs) - beam_run_of(first, all, p.runs)) + 1;
             kind[beam] = !(given > kDeadScore) ? 2 : ended ? 1 : !(sum > 0.0 && sum < INFINITY && best < INFINITY) ? 2 : 0;
         }
     }
@@ -560,7 +533,6 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
     auto candidate = [&](int list, int beam, int depth) -> BeamCandidate {
         const long long base = (long long)beam << 32;
         if (kind[beam] == 0) {
-            if (list - beam * p.parts >= own_parts[beam]) return {nothing, -1};
             const BeamEntry entry = depth < staged ? stage[list * staged + depth] : entries[(long long)list * p.keep + depth];
             if (entry.token < 0) return {nothing, -1};
             return {beam_order(score[beam] + (((double)entry.logit - top[beam]) - log_sum[beam])), base + entry.token};
@@ -722,7 +694,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
 template <int kType>
 inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_t stream) {
     params.spans = beam_spans(params.vocabulary, kType);
-    beam_plan(params.groups * params.beams, params.spans, sm_count, params.parts, params.runs);
+    params.parts = beam_parts(params.groups * params.beams, params.spans, sm_count);
     const int lists = params.beams * params.parts;
     const int threads = lists > 512 ? 1024 : lists > 256 ? 512 : 256;  // a list or more of each
     params.staged = params.keep < kBeamStage / lists ? params.keep : kBeamStage / lists;
@@ -746,7 +718,7 @@ inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_
         if (device < 64) configured[device] = true;
     }
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(params.runs, 1, 1);
+    config.gridDim = dim3(params.groups * params.beams * params.parts, 1, 1);
     config.blockDim = dim3(kBeamThreads, 1, 1);
     config.dynamicSmemBytes = kBeamRing;
     config.stream = stream;

@@ -847,7 +847,7 @@ int mt_beam_select(const void* logits, long long row_stride, int type, const flo
     if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
     if (!device_is_sm100()) return MT_ERR_DEVICE;
     BeamSelectParams params{logits, scores, finished, scores_out, parents_out, tokens_out, finished_out, nullptr, nullptr, row_stride,
-                            end_token, groups, beams, vocabulary, keep, beam_spans(vocabulary, type), 0, 0};
+                            end_token, groups, beams, vocabulary, keep, beam_spans(vocabulary, type), 0};
     params.stats = static_cast<BeamShareStats*>(workspace);
     params.lists = reinterpret_cast<BeamEntry*>(params.stats + (size_t)groups * beams * params.spans * kBeamShares);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

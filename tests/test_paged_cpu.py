@@ -136,3 +136,66 @@ def test_the_oracle_of_reordering():
     out, (moved,) = O.reorder(tables, np.array([6, 6, 6]), np.array([[1, 1, 0]]), [pages], 4)
     assert out.tolist() == [[0, 2, 6], [0, 3, 7], [0, 1, 5]]            # beam 2 has no child: its page takes the copy
     assert moved[3, 0, :, 0].tolist() == [8, 9, 14, 15] and np.array_equal(np.delete(moved, 3, 0), np.delete(pages, 3, 0))
+
+
+def test_spans_are_dealt_out_whole(tmp_path):
+    """The rule by which the selection deals a row's spans to CTAs, from the header: every span in one part, no part empty or
+    longer, and no row in more parts, than the kernels take."""
+    from tests.helpers import host_program
+
+    source = r"""
+#include "../../include/metile_b200.h"
+#include "beam_select.cuh"
+#include <cstdio>
+int main() {
+    const int all_rows[] = {1, 2, 3, 5, 8, 31, 64, 200, 256, 333, 592, 593, 800, 4096, 100000};
+    const int all_spans[] = {1, 2, 3, 4, 7, 15, 16, 17, 31, 32, 33, 64, 100, 128};
+    for (int rows : all_rows)
+        for (int spans : all_spans) {
+            const int parts = mt::beam_parts(rows, spans, 148);
+            int longest = 0, wrong = parts < 1 || mt::beam_part_start(0, spans, parts) != 0 || mt::beam_part_start(parts, spans, parts) != spans;
+            for (int part = 0; part < parts; ++part) {
+                const int length = mt::beam_part_start(part + 1, spans, parts) - mt::beam_part_start(part, spans, parts);
+                wrong += length < 1;
+                if (length > longest) longest = length;
+            }
+            std::printf("%d %d %d %d %d\n", rows, spans, parts, longest, wrong);
+        }
+    for (unsigned int n = 1; n <= 64; ++n) {
+        const unsigned int r = mt::beam_reciprocal(n);
+        int wrong = 0;
+        for (unsigned int i = 0; i <= 65536; ++i) wrong += (r ? (unsigned int)((unsigned long long)i * r >> 32) : i) != i / n;
+        std::printf("%u %d\n", n, wrong);
+    }
+    std::printf("%d %d\n", mt::kBeamMaxParts, mt::kBeamMostPerPart);
+}
+"""
+    rows = host_program(str(tmp_path), source)
+    (most_parts, most_per_part), plans = rows[-1], [row for row in rows if len(row) == 5]
+    assert len(plans) == 15 * 14 and all(row[1] == 0 for row in rows[:-1] if len(row) == 2)
+    for lines, spans, parts, longest, wrong in plans:
+        assert wrong == 0 and longest <= most_per_part and parts <= min(spans, most_parts), (lines, spans, parts, longest)
+
+
+def test_splits_of_a_sequence(tmp_path):
+    """The cut of a sequence, from the header: by its own length alone, never more splits than the scratch has rows for."""
+    from tests.helpers import host_program
+
+    source = r"""
+#include "../../include/metile_b200.h"
+#include "paged_attention.cuh"
+#include <cstdio>
+int main() {
+    for (long long capacity : {1ll, 8ll, 127ll, 128ll, 129ll, 1000ll, 16384ll, 16385ll, 100000ll, 0x7FFFFFFFll}) {
+        int most = 0, wrong = 0;
+        for (long long n = 0; n <= capacity; n += n < 70000 ? 1 : 65521) {
+            const int shift = mt::paged_split_shift((int)n), splits = mt::paged_splits((int)n);
+            if (splits > most) most = splits;
+            wrong += ((long long)splits << shift) < n || (splits > 1 && ((long long)(splits - 1) << shift) >= n) || shift < 7;
+        }
+        std::printf("%lld %d %d %d\n", capacity, most, mt::paged_most_splits(capacity), wrong);
+    }
+}
+"""
+    for capacity, most, declared, wrong in host_program(str(tmp_path), source):
+        assert wrong == 0 and most <= declared <= 128, capacity
