@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const Resi
     int first = p.state[0], available = p.state[1];
     if (first < 0 || first >= p.pool) first = 0;
     available = max(0, min(available, p.pool));
-    const long long room = (long long)p.width << p.page_shift;
+    const long long room = min((long long)p.width << p.page_shift, 0x7FFFFFFFll);  // lengths are of 32 bits
     auto wrapped = [&](long long taken) {  // of fewer entries than the ring has
         const long long at = first + taken;
         return at < p.pool ? at : at - p.pool;

@@ -259,13 +259,15 @@ class PagedTables:
     def fork(self, beams, caches):
         """Every first request of `beams` in a row is continued by all of them: full pages are shared, what is begun is copied
         in the PagedKVCache of every layer."""
-        groups = self.requests // beams
+        groups = self.requests // max(1, beams)
         if groups * beams != self.requests or any(self.held[r] and r % beams for r in range(self.requests)):
             raise ValueError("only the first request of each group may have tokens")
         held = [self.held[r - r % beams] for r in range(self.requests)]
         # The others hold the full pages in name, which cost none, and a page of their own for the rest.
         whole = [n // self.page_size * self.page_size for n in held]
         part = [0 if r % beams == 0 else held[r] - whole[r] for r in range(self.requests)]
+        if sum(1 for count in part if count) > self.free:
+            raise ValueError("paged cache: out of pages")
         self.held = [held[r] if r % beams == 0 else whole[r] for r in range(self.requests)]
         self.lengths.copy_(torch.tensor(self.held, dtype=torch.int32))
         self.grow(part)

@@ -392,3 +392,26 @@ def test_refusals_on_the_device(cuda_device):
     assert B.paged_attention_decode(q[:0], keys, values, table[:0], lengths[:0], scale=0.1).shape == (0, 4, 64)
     strided = torch.cat([q, q], -1)[:, :, :64]
     assert torch.equal(B.paged_attention_decode(strided, *good[1:], scale=0.1), B.paged_attention_decode(*good, scale=0.1))
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """Pages that lie more than 2^31 elements behind the first: append, attention, and the copy of a page in work."""
+    pages, heads, page, dim = 140000, 2, 64, 128
+    keys, values = (torch.empty((pages, heads, page, dim), dtype=torch.bfloat16, device=cuda_device) for _ in range(2))
+    last = [pages - 1, pages - 3, pages - 2, pages - 7]
+    q, k, v = (normal(101 + i, 70, h, dim, device=cuda_device) for i, h in enumerate((4, heads, heads)))
+    slots = torch.tensor([last[t // page] * page + t % page for t in range(70)], device=cuda_device)
+    B.rope_kv_append_paged(q, k, v, torch.zeros(dim // 2, device=cuda_device), torch.arange(70, dtype=torch.int32, device=cuda_device), slots,
+                           keys, values)
+    assert torch.equal(keys[last[0]].transpose(0, 1), k[:64]) and torch.equal(values[last[1], :, :6].transpose(0, 1), v[64:])
+    tables = np.array([[last[0], last[1]], [last[0], last[2]]], np.int32)
+    table, lengths = torch.tensor(tables, device=cuda_device), ints([70, 70], cuda_device)
+    moved = B.beam_reorder(table, lengths, ints([[0, 0]], cuda_device), [(keys, values)])
+    assert moved.tolist() == [[last[0], last[1]], [last[0], last[2]]]
+    assert torch.equal(keys[last[2], :, :6], keys[last[1], :, :6]) and torch.equal(values[last[2], :, :6], values[last[1], :, :6])
+    out = B.paged_attention_decode(q[:2], keys, values, moved, lengths, scale=0.1)
+    small = np.array([[0, 1], [0, 1]], np.int32)
+    near = [torch.stack([t[last[0]], t[last[1]]]) for t in (keys, values)]
+    for tensor in near:
+        tensor[1, :, 6:] = 0
+    check_attention((q[:2], *near, small, np.array([70, 70], np.int32)), 0.1, cuda_device, out)
