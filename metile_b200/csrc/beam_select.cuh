@@ -95,6 +95,21 @@ inline size_t beam_workspace_bytes(int groups, int beams, int vocabulary, int ke
     return (size_t)groups * beams * ((size_t)spans * kBeamShares * sizeof(BeamShareStats) + (size_t)(spans < kBeamMaxParts ? spans : kBeamMaxParts) * keep * sizeof(BeamEntry));
 }
 
+// A logit as a whole number of the same order (one zero, never 0 itself), and back.
+__device__ __forceinline__ unsigned int beam_logit_order(float logit) {
+    const unsigned int bits = __float_as_uint(logit + 0.0f);
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float beam_ordered_logit(unsigned int order) { return __uint_as_float(order & 0x80000000u ? order & 0x7FFFFFFFu : ~order); }
+// An entry as one number: the larger logit, among equals the lower token first.
+__device__ __forceinline__ unsigned long long beam_entry_key(float logit, int token) {
+    return (unsigned long long)beam_logit_order(logit) << 32 | (0xFFFFFFFFu - (unsigned int)token);
+}
+__device__ __forceinline__ BeamEntry beam_entry(unsigned long long key) {
+    if (key == 0) return {-INFINITY, -1};
+    return {beam_ordered_logit((unsigned int)(key >> 32)), (int)(0xFFFFFFFFu - (unsigned int)key)};
+}
+
 // kType: 0 bf16, 1 fp16, 2 fp32.
 template <int kType>
 __device__ __forceinline__ float beam_logit(const uint32_t (&words)[4], int e) {
@@ -192,9 +207,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     constexpr int kPer = Copies::kPer, kShare = Copies::kShare, kVectors = kBeamVectors, kWarps = kBeamShares;
     extern __shared__ __align__(16) char beam_ring[];  // [warps][stages][block]
     __shared__ float span_top[kBeamMostPerPart][kBeamThreads];
-    __shared__ __align__(16) float bucket[kBeamBuckets];
-    __shared__ float collected[kBeamCollect], bound_shared;
-    __shared__ int collected_token[kBeamCollect], hits[kBeamShares][32], count;
+    __shared__ __align__(16) unsigned int bucket[kBeamBuckets];
+    __shared__ unsigned long long collected[kBeamCollect];
+    __shared__ unsigned int bound_order;
+    __shared__ int count;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = blockIdx.x / p.parts;
     const int part = (int)(blockIdx.x - row * p.parts);
@@ -212,7 +228,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
 #pragma unroll
     for (int i = 0; i < kBeamStages - 1; ++i) copy_next(i);
     int slot = 0;
-    if (threadIdx.x == 0) count = 0;
+    if (threadIdx.x == 0) {
+        count = 0;
+        bound_order = 0xFFFFFFFFu;
+    }
     float mine = -INFINITY;
     uint32_t raw[kVectors][4];
     const int skew = copies.skew;
@@ -291,73 +310,53 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     }
     last_total = warp_sum_xor(last_total);
     if (lane == 0) *(stats - kWarps) = {last_top, last_total};
-    {
-        float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = top;
-    }
+    // Four threads to a bucket: of the `keep` largest of 64 the least bounds `keep` logits of the CTA from below.  They are
+    // ranked as whole numbers that differ in their last bits (which rounds those of 32-bit logits, for the ranks alone).
+    float top = fmaxf(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    const unsigned int top_order = beam_logit_order(top), own_bucket = (top_order & ~(kBeamBuckets - 1u)) | threadIdx.x >> 2;
+    if ((lane & 3) == 0) bucket[threadIdx.x >> 2] = own_bucket;
     __syncthreads();
-    // The keep-th largest bucket, four threads to a bucket: at least `keep` logits of the CTA are not below it.
     {
-        const int own = threadIdx.x >> 2;
-        const float value = bucket[own];
         int rank = 0;
 #pragma unroll
         for (int i = 0; i < kBeamBuckets / 16; ++i) {
-            const int j = 16 * i + 4 * (lane & 3);
-            const float4 others = *reinterpret_cast<const float4*>(&bucket[j]);
-            rank += (others.x > value || (others.x == value && j < own)) + (others.y > value || (others.y == value && j + 1 < own)) +
-                    (others.z > value || (others.z == value && j + 2 < own)) + (others.w > value || (others.w == value && j + 3 < own));
+            const uint4 others = *reinterpret_cast<const uint4*>(&bucket[16 * i + 4 * (lane & 3)]);
+            rank += (others.x > own_bucket) + (others.y > own_bucket) + (others.z > own_bucket) + (others.w > own_bucket);
         }
         rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
         rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
-        if (rank == p.keep - 1 && (lane & 3) == 0) bound_shared = value;
+        const unsigned int least = __reduce_min_sync(0xFFFFFFFFu, rank < p.keep ? top_order : 0xFFFFFFFFu);
+        if (lane == 0) atomicMin(&bound_order, least);
     }
     __syncthreads();
-    const float bound = bound_shared;
-    // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens.  A logit is
-    // read again from memory, so up to 32 such threads are noted down and read four at a time.
+    const float bound = beam_ordered_logit(bound_order);
+    // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens; read again
+    // from memory, those of four threads together.
     auto reach = [&](auto qualifies, auto visit) {
-        int noted = 0;
-        auto look = [&] {
-            __syncwarp();
-            for (int k = 0; k < noted; k += 4) {
-                float logit[4];
-                int token[4];
+        unsigned int spans_left = 0;  // of this thread's that qualify
+        for (int span = span0; span < span1; ++span) spans_left |= (qualifies(span_top[span - span0][threadIdx.x]) ? 1u : 0u) << (span - span0);
+        unsigned int lanes = __ballot_sync(0xFFFFFFFFu, spans_left != 0);
+        while (lanes && !__any_sync(0xFFFFFFFFu, count > kBeamCollect)) {
+            float logit[4];
+            int token[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int hit = hits[warp][min(k + i, noted - 1)];
-                    token[i] = (hit >> 5) * beam_span(kType) + warp * kShare + (lane / kPer * 32 + (hit & 31)) * kPer + lane % kPer;
-                    if (k + i >= noted || lane >= kVectors * kPer || token[i] >= p.vocabulary) token[i] = -1;
-                    logit[i] = token[i] >= 0 ? beam_logit_at<kType>(from, token[i]) : 0.0f;
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int of = __ffs(lanes) - 1, span = span0 + __ffs(__shfl_sync(0xFFFFFFFFu, spans_left, max(of, 0))) - 1;
+                token[i] = span * beam_span(kType) + warp * kShare + (lane / kPer * 32 + of) * kPer + lane % kPer;
+                if (!lanes || lane >= kVectors * kPer || token[i] >= p.vocabulary) token[i] = -1;
+                logit[i] = token[i] >= 0 ? beam_logit_at<kType>(from, token[i]) : 0.0f;
+                if (lane == of) spans_left &= spans_left - 1u;
+                lanes = __ballot_sync(0xFFFFFFFFu, spans_left != 0);
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (token[i] >= 0) visit(logit[i], token[i]);
-            }
-            noted = 0;
-            __syncwarp();
-        };
-        for (int span = span0; span < span1 && count <= kBeamCollect; ++span) {
-            unsigned int threads = __ballot_sync(0xFFFFFFFFu, qualifies(span_top[span - span0][threadIdx.x]));
-            while (threads) {
-                const int at = noted + __popc(threads & ((1u << lane) - 1u));
-                const bool fits = (threads >> lane & 1u) && at < 32;
-                if (fits) hits[warp][at] = span << 5 | lane;
-                const unsigned int taken = __ballot_sync(0xFFFFFFFFu, fits);
-                noted += __popc(taken);
-                threads &= ~taken;
-                if (noted == 32) look();
-            }
+            for (int i = 0; i < 4; ++i)
+                if (token[i] >= 0) visit(logit[i], token[i]);
         }
-        look();
     };
     auto collect = [&](float logit, int token) {
         const int place = atomicAdd(&count, 1);
-        if (place < kBeamCollect) {
-            collected[place] = logit;
-            collected_token[place] = token;
-        }
+        if (place < kBeamCollect) collected[place] = beam_entry_key(logit, token);
     };
     reach([&](float top) { return top >= bound; }, [&](float logit, int token) { if (logit >= bound) collect(logit, token); });
     __syncthreads();
@@ -374,36 +373,22 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
         found = count;
         if (found > kBeamCollect) {
             // The large ones lie in few buckets: `keep` rounds over everything, each for the best behind the last.
-            float before = INFINITY;
-            int before_token = -1;
+            unsigned long long before = ~0ull;
             for (int r = 0; r < p.keep; ++r) {
-                float best = -INFINITY;
-                int best_token = 0x7FFFFFFF;
+                unsigned long long best = 0;  // none
                 for (int token = first + threadIdx.x; token < last; token += kBeamThreads) {
                     const float logit = beam_logit_at<kType>(from, token);
-                    const bool behind = logit < before || (logit == before && token > before_token);
-                    if (behind && (logit > best || (logit == best && token < best_token))) {
-                        best = logit;
-                        best_token = token;
-                    }
+                    const unsigned long long key = logit == logit ? beam_entry_key(logit, token) : 0ull;
+                    if (key < before && key > best) best = key;
                 }
 #pragma unroll
-                for (int offset = 16; offset >= 1; offset >>= 1) {
-                    const float other = __shfl_xor_sync(0xFFFFFFFFu, best, offset);
-                    const int other_token = __shfl_xor_sync(0xFFFFFFFFu, best_token, offset);
-                    if (other > best || (other == best && other_token < best_token)) { best = other; best_token = other_token; }
-                }
-                if (lane == 0) {
-                    collected[warp] = best;
-                    collected_token[warp] = best_token;
-                }
+                for (int offset = 16; offset >= 1; offset >>= 1) best = max(best, __shfl_xor_sync(0xFFFFFFFFu, best, offset));
+                if (lane == 0) collected[warp] = best;
                 __syncthreads();
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w)
-                    if (collected[w] > best || (collected[w] == best && collected_token[w] < best_token)) { best = collected[w]; best_token = collected_token[w]; }
-                if (threadIdx.x == 0) list[r] = {best, best_token == 0x7FFFFFFF ? -1 : best_token};
+                for (int w = 0; w < kWarps; ++w) best = max(best, collected[w]);
+                if (threadIdx.x == 0) list[r] = beam_entry(best);
                 before = best;
-                before_token = best_token;
                 __syncthreads();
             }
             return;
@@ -418,13 +403,12 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     }
     // Eight threads rank an entry.
     for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += kBeamThreads / 8) {
-        const float logit = i < found ? collected[i] : 0.0f;
-        const int token = i < found ? collected_token[i] : 0;
+        const unsigned long long own = collected[min(i, found - 1)];
         int rank = 0;
-        for (int j = threadIdx.x & 7; j < found; j += 8) rank += collected[j] > logit || (collected[j] == logit && collected_token[j] < token);
+        for (int j = threadIdx.x & 7; j < found; j += 8) rank += collected[j] > own;
 #pragma unroll
         for (int offset = 1; offset <= 4; offset <<= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, offset);
-        if (i < found && (lane & 7) == 0 && rank < p.keep) list[rank] = {logit, token};
+        if (i < found && (lane & 7) == 0 && rank < p.keep) list[rank] = beam_entry(own);
     }
     for (int i = found + threadIdx.x; i < p.keep; i += kBeamThreads) list[i] = {-INFINITY, -1};
 }
@@ -446,13 +430,9 @@ __device__ __forceinline__ double beam_value(long long order) {
 
 // The order's 64-bit value rounded down to a 32-bit number, as a whole one of the same order (never 0); and the least
 // value with that key, with its top bit turned over.
-__device__ __forceinline__ unsigned int beam_key(long long order) {
-    const unsigned int bits = __float_as_uint(__double2float_rd(beam_value(order)));
-    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-}
+__device__ __forceinline__ unsigned int beam_key(long long order) { return beam_logit_order(__double2float_rd(beam_value(order))); }
 __device__ __forceinline__ unsigned long long beam_key_floor(unsigned int key) {
-    const float value = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-    return (unsigned long long)beam_order((double)value) ^ 0x8000000000000000ull;
+    return (unsigned long long)beam_order((double)beam_ordered_logit(key)) ^ 0x8000000000000000ull;
 }
 
 // How many of n candidates come before `own`, eight neighbouring threads together; those without a place do not count.
