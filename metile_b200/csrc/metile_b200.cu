@@ -900,7 +900,7 @@ int mt_beam_reorder(const int* block_tables, long long table_stride, int width, 
         params.caches = here;
         params.first_cache = first;
         cudaLaunchAttribute attribute;
-        const cudaLaunchConfig_t config = dependent_launch(dim3(groups * beams, 1 + here, 1), kReorderThreads, 0, stream, &attribute);
+        const cudaLaunchConfig_t config = dependent_launch(dim3(groups, 1 + 2 * here, 1), kReorderThreads, 0, stream, &attribute);
         if (cudaLaunchKernelEx(&config, beam_reorder_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
     }
     return MT_OK;

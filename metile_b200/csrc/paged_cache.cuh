@@ -352,10 +352,10 @@ struct ReorderParams {
     int width, beams, caches, kv_heads, head_dim, page_shift, page_count, first_cache;
 };
 
-// CTA (row, y): y = 0 writes the row's table, y = 1 + c copies cache c's keys and values.
+// CTA (group, y): y = 0 writes the group's tables, y = 1 + 2 c and 2 + 2 c copy the keys and the values of cache c.
 __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
-    const int row = blockIdx.x, group = row / p.beams, k = row - group * p.beams, base = group * p.beams;
-    const int lane = threadIdx.x & 31;
+    const int group = blockIdx.x, base = group * p.beams, lane = threadIdx.x & 31;
+    const bool reports = threadIdx.x < 32 && blockIdx.y == 0;
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
     // Every warp has the group's parents, one in a lane.
@@ -363,68 +363,73 @@ __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const __g
     if (lane < p.beams) {
         parent = p.parents[base + lane];
         if (parent < 0 || parent >= p.beams) {  // recorded, and taken as its own
-            if (lane == k && threadIdx.x < 32 && blockIdx.y == 0) record_index(kParentOutside, row, (unsigned int)parent);
+            if (reports) record_index(kParentOutside, base + lane, (unsigned int)parent);
             parent = lane;
         }
     }
     const int length = p.lengths[base];
     const long long capacity = (long long)p.width << p.page_shift;
-    if ((length < 0 || length > capacity) && threadIdx.x == 0 && blockIdx.y == 0) record_index(kLengthOutside, base, (unsigned int)length);
+    if ((length < 0 || length > capacity) && reports && lane == 0) record_index(kLengthOutside, base, (unsigned int)length);
     const int held = (int)max(0ll, min((long long)length, capacity));
     const int block = held >> p.page_shift, part = held & ((1 << p.page_shift) - 1);
-    // Lanes of a parent's first children, and the beams that have none.
+    // First children go on in their parent's page in work; as many are not the first of theirs as there are beams without any,
+    // and the n-th of the former gets the page of the n-th of the latter.
     const unsigned int all = p.beams == 32 ? 0xFFFFFFFFu : (1u << p.beams) - 1u;
     const unsigned int firsts = __ballot_sync(0xFFFFFFFFu, __ffs(__match_any_sync(0xFFFFFFFFu, parent)) - 1 == lane) & all;
     unsigned int childless = all & ~__reduce_or_sync(0xFFFFFFFFu, lane < p.beams ? 1u << parent : 0u);
-    const int mine = __shfl_sync(0xFFFFFFFFu, parent, k);
-    const bool first = firsts >> k & 1u;
-    int owner = mine;       // whose page in work this beam gets
-    if (!first) {
-        // As many children are not the first of theirs as there are beams without any.
-        for (int skip = __popc(all & ~firsts & ((1u << k) - 1u)); skip > 0; --skip) childless &= childless - 1u;
+    int owner = parent;
+    if (!(firsts >> lane & 1u) && lane < p.beams) {
+        for (int skip = __popc(all & ~firsts & ((1u << lane) - 1u)); skip > 0; --skip) childless &= childless - 1u;
         owner = __ffs(childless) - 1;
     }
-    const int* from = p.tables + (base + mine) * p.table_stride;
-    const int* own = p.tables + (long long)row * p.table_stride;
-    if (blockIdx.y == 0 && p.first_cache == 0) {
-        int* to = p.tables_out + (long long)row * p.width;
-        for (int j = threadIdx.x; j < p.width; j += blockDim.x) {
-            int id = j < block ? from[j] : own[j];
-            if (j == block && part > 0) id = p.tables[(base + owner) * p.table_stride + j];
-            to[j] = id;
+    if (blockIdx.y == 0) {
+        if (p.first_cache > 0) return;
+        for (int k = 0; k < p.beams; ++k) {
+            const int from = __shfl_sync(0xFFFFFFFFu, parent, k), of = __shfl_sync(0xFFFFFFFFu, owner, k);
+            for (int j = threadIdx.x; j < p.width; j += blockDim.x) {
+                const int row = j < block ? from : j == block && part > 0 ? of : k;
+                p.tables_out[(long long)(base + k) * p.width + j] = p.tables[(base + row) * p.table_stride + j];
+            }
         }
-    }
-    if (blockIdx.y == 0 || first || part == 0) return;
-    const int source = from[block], target = p.tables[(base + owner) * p.table_stride + block];
-    if (source < 0 || source >= p.page_count || target < 0 || target >= p.page_count) {
-        if (threadIdx.x == 0) record_index(kPageOutside, row, (unsigned int)(source < 0 || source >= p.page_count ? source : target));
         return;
     }
+    if (part == 0 || firsts == all) return;
+    // The pages to copy, in the lanes of the children that are not the first of theirs.
+    int source = -1, target = -1;
+    if (lane < p.beams && !(firsts >> lane & 1u)) {
+        source = p.tables[(base + parent) * p.table_stride + block];
+        target = p.tables[(base + owner) * p.table_stride + block];
+        if (source < 0 || source >= p.page_count || target < 0 || target >= p.page_count) {
+            if (threadIdx.x < 32 && blockIdx.y == 1)
+                record_index(kPageOutside, base + lane, (unsigned int)(source < 0 || source >= p.page_count ? source : target));
+            source = -1;
+        }
+    }
+    unsigned int copies = __ballot_sync(0xFFFFFFFFu, source >= 0);
     // A thread has one 16-byte vector of a row and takes every `stride`-th row, four at a time.
-    const int vectors = p.head_dim / 8, rows = p.kv_heads * part;
+    const int which = (blockIdx.y - 1) & 1, vectors = p.head_dim / 8, rows = p.kv_heads * part;
     const int stride = max(1, (int)blockDim.x / vectors), first_row = threadIdx.x / vectors;
-    if (first_row >= stride) return;
-    for (int i = (threadIdx.x - first_row * vectors) * 8; i < p.head_dim; i += blockDim.x * 8) {  // one round, but for very wide heads
-#pragma unroll 1
-        for (int which = 0; which < 2; ++which) {
-            uint16_t* pages = p.pages[which * kReorderMaxCaches + blockIdx.y - 1];
-            const PageStrides strides = which ? p.value_strides : p.key_strides;
-            const uint16_t* source_page = pages + source * strides.page + i;
-            uint16_t* target_page = pages + target * strides.page + i;
+    uint16_t* pages = p.pages[which * kReorderMaxCaches + (blockIdx.y - 1) / 2];
+    const PageStrides strides = which ? p.value_strides : p.key_strides;
+    for (; copies; copies &= copies - 1u) {
+        const int child = __ffs(copies) - 1;
+        const uint16_t* source_page = pages + __shfl_sync(0xFFFFFFFFu, source, child) * strides.page;
+        uint16_t* target_page = pages + __shfl_sync(0xFFFFFFFFu, target, child) * strides.page;
+        if (first_row >= stride) continue;
+        for (int i = (threadIdx.x - first_row * vectors) * 8; i < p.head_dim; i += blockDim.x * 8)  // one round, but for very wide heads
             for (int at = first_row; at < rows; at += 4 * stride) {
                 uint4 moved[4];
                 long long offset[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int one = at + k * stride, head = one / part;
-                    offset[k] = head * strides.head + (one - head * part) * strides.token;
+                    offset[k] = head * strides.head + (one - head * part) * strides.token + i;
                     if (one < rows) moved[k] = ptx::ld_global_dependent_u4(source_page + offset[k]);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     if (at + k * stride < rows) *reinterpret_cast<uint4*>(target_page + offset[k]) = moved[k];
             }
-        }
     }
 }
 
