@@ -683,22 +683,26 @@ PyObject* beam_reorder(PyObject* const* args) {
     if (count < 1 || !fits_int(count)) Py_RETURN_NONE;
     std::vector<void*> addresses[2];
     Pages first[2];
-    const Tensor* sample = nullptr;
+    const Tensor* like[2] = {};  // the first cache's, which are looked at closely
+    for (auto& list : addresses) list.reserve(count);
     for (Py_ssize_t c = 0; c < count; ++c) {
         PyObject* pair = PySequence_Fast_GET_ITEM(args[3], c);
         if (!sequence(pair) || PySequence_Fast_GET_SIZE(pair) != 2) Py_RETURN_NONE;
         for (int which = 0; which < 2; ++which) {
             const Tensor* pages = plain(PySequence_Fast_GET_ITEM(pair, which));
-            if (!pages || half_type(*pages) < 0) Py_RETURN_NONE;
-            if (!sample) sample = pages;
-            Pages here;
-            if (!pages_of(pages, device, sample->scalar_type(), here) || pages->sizes() != sample->sizes() || wants_gradient({pages})) Py_RETURN_NONE;
-            if (c == 0) first[which] = here;
-            for (int i = 0; i < 3; ++i)
-                if (here.strides[i] != first[which].strides[i]) Py_RETURN_NONE;
-            addresses[which].push_back(here.base);
+            if (!pages || wants_gradient({pages})) Py_RETURN_NONE;
+            if (c == 0) {
+                like[which] = pages;
+                if (half_type(*pages) < 0 || !pages_of(pages, device, like[0]->scalar_type(), first[which]) || pages->sizes() != like[0]->sizes())
+                    Py_RETURN_NONE;
+            } else if (pages->scalar_type() != like[which]->scalar_type() || pages->device() != device ||
+                       pages->sizes() != like[which]->sizes() || pages->strides() != like[which]->strides()) {
+                Py_RETURN_NONE;
+            }
+            addresses[which].push_back(address(*pages));  // the library looks at its alignment
         }
     }
+    const Tensor* sample = like[0];
     for (int i = 0; i < 4; ++i)
         if (!fits_int(sample->size(i))) Py_RETURN_NONE;
     const Launch launch(device);

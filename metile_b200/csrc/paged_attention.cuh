@@ -21,6 +21,10 @@
 // The weights enter as two 16-bit numbers, high and low part: one alone would be off by 2^-9 (bf16).  A running maximum
 // per head is moved, and the sums with it, only when a score passes it by more than 2^8: the weights stay below 256 and
 // keep their relative precision, and a lane adds up its own tokens' weights until the end.
+//
+// Measured (8 KV heads of 4 x 128): 100 requests of up to 8191 tokens 337 us, 5.5 TB/s (reading alone 294); two of 100003 143 us,
+// 5.7 TB/s; one of 301 7.3 us.  16 x 2048 tokens, 2 x 6 heads: 12.3 us.  Six warps with four ring slots hold what eight
+// with three or four with six do (143 us against 154 and 157 for the long ones); without the arithmetic the large cases take the same.
 #pragma once
 
 #include "attention_decode.cuh"
