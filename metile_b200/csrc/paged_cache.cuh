@@ -94,12 +94,13 @@ __device__ __forceinline__ int last_not_above(const long long* starts, int n, lo
 // given back.  Then tokens, granted and returned pages are dealt to the threads, each of which looks its request up; a thread
 // has four tokens in a row.  Bound by latency, and for long prompts by the threads: several CTAs then, which all take the
 // sums and share what follows.  Where lengths and state are written in place the CTAs are one cluster, and the first of them
-// writes behind a barrier.  64 requests of a token each 5.0 us in a graph; 501 with 116 thousand tokens 11.0 us (one CTA 132).
+// writes behind a barrier.  What a decode step needs, a token and at most a page for each, the requests' own threads do at once.  64
+// requests of a token each 3.2 us in a graph (5.0 with the search); 501 with 116 thousand tokens 11.0 us (one CTA 132).
 __global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const ResizeParams p, bool in_place) {
     __shared__ long long token_start[kResizeThreads], grant_start[kResizeThreads], free_start[kResizeThreads];
     __shared__ int held[kResizeThreads], added[kResizeThreads];
     __shared__ unsigned char is_served[kResizeThreads];
-    __shared__ long long scratch[2][32];
+    __shared__ long long scratch[3][32];
     __shared__ long long totals[3];
     __shared__ int granted_shared;
     ptx::griddep_launch_dependents();
@@ -130,20 +131,26 @@ __global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const Resi
         const int r = base + threadIdx.x, here = min(threads, p.requests - base);
         const bool exists = r < p.requests;
         const int length = exists ? p.lengths[r] : 0, count = exists ? p.counts[r] : 0;
-        const long long after = (long long)length + count;
+        const long long after = (long long)length + count, added_here = max(count, 0);
         bool valid = length >= 0 && after >= 0 && length <= room && after <= room;
-        // First the tokens alone: whether they fit the map decides which requests ask for pages.
-        long long ends[1] = {max(count, 0)};
-        block_scan(ends, scratch);
-        ends[0] += tokens_before;
-        valid = valid && (count <= 0 || ends[0] <= p.tokens);
-        const long long change = valid ? blocks_of(after) - blocks_of(length) : 0, need = max(0ll, change), back = max(0ll, -change);
-        long long pages[2] = {need, back};
-        block_scan(pages, scratch);
-        const long long reach = pages[0] + asked_before, returned = pages[1] + freed_before;
+        long long change = valid ? blocks_of(after) - blocks_of(length) : 0;
+        long long sums[3] = {added_here, max(0ll, change), max(0ll, -change)};
+        block_scan(sums, scratch);
+        if (threadIdx.x == threads - 1) totals[0] = sums[0] + tokens_before;
+        __syncthreads();
+        if (totals[0] > p.tokens) {  // whether a request's tokens fit the map decides if it asks for pages
+            valid = valid && (count <= 0 || sums[0] + tokens_before <= p.tokens);
+            change = valid ? change : 0;
+            long long pages[2] = {max(0ll, change), max(0ll, -change)};
+            block_scan(pages, scratch);
+            sums[1] = pages[0];
+            sums[2] = pages[1];
+        }
+        const long long need = max(0ll, change), back = max(0ll, -change), ends = sums[0] + tokens_before, begin = ends - added_here;
+        const long long reach = sums[1] + asked_before, returned = sums[2] + freed_before;
         // In order and without overtaking: once the free pages do not reach, nobody behind is given any.
         const bool served = valid && (need == 0 || reach <= available);
-        token_start[threadIdx.x] = ends[0] - max(count, 0);
+        token_start[threadIdx.x] = begin;
         grant_start[threadIdx.x] = reach - need;
         free_start[threadIdx.x] = returned - back;
         held[threadIdx.x] = length;
@@ -151,27 +158,37 @@ __global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const Resi
         is_served[threadIdx.x] = served;
         if (served && need > 0) atomicMax(&granted_shared, (int)reach);  // at most `available`
         if (threadIdx.x == threads - 1) {
-            totals[0] = ends[0];
             totals[1] = reach;
             totals[2] = returned;
         }
-        __syncthreads();
+        const bool more = __syncthreads_or(count > 1 || need > 1 || back > 0);
         all_have_read();
         if (exists && leads) {
-            p.starts[r] = (int)min(ends[0] - max(count, 0), 0x7FFFFFFFll);
+            // A request's own thread does its first token and page: all there is in a decode step.
+            if (count > 0 && begin < p.tokens) {
+                const bool fresh = (length & (page - 1)) == 0;
+                int id = -1;
+                if (served) id = fresh ? p.ring[wrapped(reach - need)] : p.tables[r * p.table_stride + (length >> p.page_shift)];
+                if (served && need > 0) p.tables[r * p.table_stride + blocks_of(length)] = fresh ? id : p.ring[wrapped(reach - need)];
+                p.slots[begin] = id < 0 ? -1 : ((long long)id << p.page_shift) + (length & (page - 1));
+                p.positions[begin] = served ? length : 0;
+            }
+            p.starts[r] = (int)min(begin, 0x7FFFFFFFll);
             p.lengths_out[r] = served ? (int)after : length;
         }
-        const long long tokens_here = min((long long)p.tokens, totals[0]), asked_here = min((long long)available, totals[1]);
+        const long long tokens_here = more ? min((long long)p.tokens, totals[0]) : 0, asked_here = more ? min((long long)available, totals[1]) : 0;
         for (long long t0 = tokens_before + 4 * worker; t0 < tokens_here; t0 += 4 * workers) {
             int i = last_not_above(token_start, here, t0);
             int position[4], id[4];
+            bool first_one[4];
             const int* named[4];  // where the id of the token's page stands
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 while (i + 1 < here && token_start[i + 1] <= t0 + k) ++i;
                 position[k] = 0;
                 named[k] = nullptr;
-                if (t0 + k < tokens_here && is_served[i]) {
+                first_one[k] = t0 + k >= tokens_here || token_start[i] == t0 + k;
+                if (!first_one[k] && is_served[i]) {
                     position[k] = held[i] + (int)(t0 + k - token_start[i]);
                     const int block = position[k] >> p.page_shift, fresh = block - (int)blocks_of(held[i]);
                     named[k] = fresh < 0 ? p.tables + (base + i) * p.table_stride + block : p.ring + wrapped(grant_start[i] + fresh);
@@ -181,14 +198,15 @@ __global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const Resi
             for (int k = 0; k < 4; ++k) id[k] = named[k] ? *named[k] : -1;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if (t0 + k >= tokens_here) break;
+                if (first_one[k]) continue;
                 p.slots[t0 + k] = id[k] < 0 ? -1 : ((long long)id[k] << p.page_shift) + (position[k] & (page - 1));
                 p.positions[t0 + k] = position[k];
             }
         }
         for (long long g = asked_before + worker; g < asked_here; g += workers) {
             const int i = last_not_above(grant_start, here, g);
-            if (is_served[i]) p.tables[(base + i) * p.table_stride + blocks_of(held[i]) + (g - grant_start[i])] = p.ring[wrapped(g)];
+            if (is_served[i] && g != grant_start[i])
+                p.tables[(base + i) * p.table_stride + blocks_of(held[i]) + (g - grant_start[i])] = p.ring[wrapped(g)];
         }
         for (long long f = freed_before + worker; f < totals[2]; f += workers) {
             const int i = last_not_above(free_start, here, f);

@@ -191,6 +191,28 @@ def test_beam_search_against_one_that_shares_nothing(cuda_device, model, lengths
                 assert set(row[row.index(end):]) == {end}
 
 
+def test_two_searches_side_by_side(cuda_device, model):
+    """Two decoders whose captured steps run on streams of their own, at the same time."""
+    decoders = [GraphedBeamDecoder(model, batch=2, beams=4, capacity=96, page_size=8) for _ in range(2)]
+    prompts = [prompts_of([11, 24], cuda_device, seed=11 + i) for i in range(2)]
+    with B.batch_invariant():
+        apart = [decoder.search(p, 30) for decoder, p in zip(decoders, prompts)]
+        streams = [torch.cuda.Stream(cuda_device) for _ in decoders]
+        for stream in streams:
+            stream.wait_stream(torch.cuda.current_stream())
+        for decoder, p, stream in zip(decoders, prompts, streams):
+            with torch.cuda.stream(stream):
+                decoder.prefill(p)
+        for _ in range(29):
+            for decoder, stream in zip(decoders, streams):
+                with torch.cuda.stream(stream):
+                    decoder.step()
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+    for decoder, (found, scores) in zip(decoders, apart):
+        assert torch.equal(decoder.scores, scores) and torch.equal(decoder.token.view(2, 4), found[:, :, -1])
+
+
 def test_one_beam_is_greedy_decoding(cuda_device, model):
     prompts = prompts_of([12, 12], cuda_device, seed=8)
     decoder = GraphedBeamDecoder(model, batch=2, beams=1, capacity=64)
