@@ -110,6 +110,22 @@ def test_candidates_of_two_beams_closer_than_32_bits_tell(cuda_device):
             check_select(logits, torch.tensor([[s[0], moved]], dtype=torch.float32, device=cuda_device), 6)
 
 
+def test_equal_and_nearly_equal_beams_wherever_their_rows_begin(cuda_device):
+    """Beams with the same row and score tie at every token, and the lower beam comes first; rows of 16 bytes and an odd
+    rest begin at other places of a vector.  One step of a score turns the order."""
+    for dtype in LOWEST:
+        for vocab, beams, keep in ((5, 2, 4), (2051, 3, 9), (32001, 8, 16), (128256, 2, 8)):
+            row, _, _ = select_case(vocab, 1, 1, vocab, dtype, cuda_device)
+            row[0, ::7] = -torch.inf
+            logits = row.repeat(2 * beams, 1)
+            scores = torch.full((2, beams), -3.25, device=cuda_device)
+            scores[1, -1] = float(np.nextafter(np.float32(-3.25), np.float32(0)))
+            out = check_select(logits, scores, keep)
+            tied = out[0][0][1:] == out[0][0][:-1]
+            assert bool((out[1][0][1:] > out[1][0][:-1])[tied & (out[2][0][1:] == out[2][0][:-1])].all())
+            assert out[1][1, 0] == beams - 1
+
+
 def test_masked_tokens_beams_and_rows(cuda_device):
     for dtype in LOWEST:
         logits, scores, _ = select_case(7, 3, 4, 12345, dtype, cuda_device)
