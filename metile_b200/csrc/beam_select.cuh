@@ -9,7 +9,8 @@
 // part.  Every warp leaves the maximum and the sum of exponentials of its share of a span, and the CTA the `keep` best of its
 // part.  Within a beam candidates are ordered as their logits are, so no sum is needed for that.  Of 64 bucket maxima (four
 // threads each) the keep-th largest bounds the keep-th best from below; the few threads that reach it look at their logits
-// again, and what they find is ranked.  The shares of a row have one size for all calls: its bits do not depend on the others.
+// again, and what they find is ranked.  (Short rows and more than 32 kept take 256 maxima: with 64 kept of 128256 in 128 rows 37 us, by
+// the buckets alone 458; 14 rows of 524 with 28 kept 14 us, 34.)  The shares of a row have one size for all calls: its bits do not depend on the others.
 //
 // Then a CTA per group joins parts and beams.  The sums are of 32-bit exponentials, each beam's log-sum off by up to
 // kBeamError; where two beams' candidates are closer than twice that, the sums of the two are taken again, in 64 bits, so
@@ -43,7 +44,7 @@ constexpr int kBeamShareBytes = kBeamVectors * 512, kBeamBlock = kBeamShareBytes
 constexpr int kBeamRing = kBeamStages * kBeamShares * kBeamBlock;
 constexpr int kBeamBuckets = 64, kBeamCollect = 512;         // of a part
 static_assert(kBeamCollect >= kBeamMaxKeep + kBeamThreads, "equal ones are collected a step of all threads at a time");
-constexpr int kBeamSlack = 8, kBeamKeys = 256, kBeamStage = 4096;              // entries of the lists that the join has in shared memory
+constexpr int kBeamSlack = 8, kBeamKeys = 256, kBeamMany = 256, kBeamStage = 4096;              // entries of the lists that the join has in shared memory
 static_assert(kBeamBuckets >= kBeamMaxKeep, "the bound of a part comes from its buckets");
 
 __host__ __device__ constexpr int beam_size(int type) { return type == 2 ? 4 : 2; }               // bytes of a logit
@@ -214,8 +215,8 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     extern __shared__ __align__(16) char beam_ring[];  // [warps][stages][block]
     __shared__ float span_top[kBeamMostPerPart][kBeamThreads];
     __shared__ __align__(16) unsigned int bucket[kBeamBuckets];
-    __shared__ unsigned long long collected[kBeamCollect];
-    __shared__ unsigned int bound_order;
+    __shared__ __align__(16) unsigned long long collected[kBeamCollect];
+    __shared__ unsigned int bound_order, finer_order;
     __shared__ int count;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = blockIdx.x / p.parts;
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     int slot = 0;
     if (threadIdx.x == 0) {
         count = 0;
-        bound_order = 0xFFFFFFFFu;
+        bound_order = finer_order = 0xFFFFFFFFu;
     }
     float mine = -INFINITY;
     uint32_t raw[kVectors][4];
@@ -336,9 +337,33 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
         if (lane == 0) atomicMin(&bound_order, least);
     }
     __syncthreads();
-    const float bound = beam_ordered_logit(bound_order);
+    float bound = beam_ordered_logit(bound_order);
+    const bool single = span1 - span0 == 1;  // span: it is in the ring yet
+    if (p.keep > kBeamBuckets / 2 || (single && bound == -INFINITY)) {
+        // The least of nearly all buckets bounds badly, and a short row or end of one has fewer of them than `keep`: 256 maxima
+        // then, one to a thread; of every 256th logit where they are in the ring, so that as many threads as can have some.
+        float sample = single ? -INFINITY : mine;
+        const int n = single ? min(p.vocabulary - span0 * beam_span(kType), beam_span(kType)) : 0;
+        for (int i = threadIdx.x; i < n; i += kBeamThreads) sample = fmaxf(sample, beam_logit_at<kType>(beam_ring + i / kShare * (kBeamStages * kBeamBlock) + skew, i % kShare));
+        const unsigned int order = beam_logit_order(sample), own = (order & ~(kBeamThreads - 1u)) | threadIdx.x;
+        unsigned int* samples = reinterpret_cast<unsigned int*>(collected);  // which is empty yet
+        samples[threadIdx.x] = own;
+        __syncthreads();
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < kBeamThreads; i += 4) {
+            const uint4 others = *reinterpret_cast<const uint4*>(&samples[i]);
+            rank += (others.x > own) + (others.y > own) + (others.z > own) + (others.w > own);
+        }
+        const unsigned int least = __reduce_min_sync(0xFFFFFFFFu, rank < p.keep ? order : 0xFFFFFFFFu);
+        if (lane == 0) atomicMin(&finer_order, least);
+        __syncthreads();
+        bound = beam_ordered_logit(finer_order);
+    }
     // The logits of the threads whose maximum of a span qualifies, by their warp: a lane each, with their tokens; read again
-    // from memory, those of four threads together.
+    // from the ring or from memory, those of four threads together.
+    const char* source = single ? ring + skew : from;
+    const int source0 = single ? span0 * beam_span(kType) + warp * kShare : 0;
     auto reach = [&](auto qualifies, auto visit) {
         unsigned int spans_left = 0;  // of this thread's that qualify
         for (int span = span0; span < span1; ++span) spans_left |= (qualifies(span_top[span - span0][threadIdx.x]) ? 1u : 0u) << (span - span0);
@@ -351,7 +376,7 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
                 const int of = __ffs(lanes) - 1, span = span0 + __ffs(__shfl_sync(0xFFFFFFFFu, spans_left, max(of, 0))) - 1;
                 token[i] = span * beam_span(kType) + warp * kShare + (lane / kPer * 32 + of) * kPer + lane % kPer;
                 if (!lanes || lane >= kVectors * kPer || token[i] >= p.vocabulary) token[i] = -1;
-                logit[i] = token[i] >= 0 ? beam_logit_at<kType>(from, token[i]) : 0.0f;
+                logit[i] = token[i] >= 0 ? beam_logit_at<kType>(source, token[i] - source0) : 0.0f;
                 if (lane == of) spans_left &= spans_left - 1u;
                 lanes = __ballot_sync(0xFFFFFFFFu, spans_left != 0);
             }
@@ -504,7 +529,9 @@ __device__ __forceinline__ double beam_exact_share(const char* row, int vocabula
 }
 
 // One CTA per group; a list of sorted candidates for every part of every beam.  Bound by the latency of its steps: what it
-// reads is asked for at once, the first `staged` entries of every list among it.
+// reads is asked for at once, the first `staged` entries of every list among it.  Where a beam or two have most of the best
+// candidates, a second search among those collected keeps the ranks short (32 beams over 32001, 64 kept, with the kernel
+// before: 23 us; 480 more without it).
 template <int kType>
 __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams p) {
     extern __shared__ __align__(16) unsigned char join_smem[];
@@ -515,7 +542,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
     int* order = reinterpret_cast<int*>(stage + lists * staged);                        // [most]
     __shared__ double top[kBeamMaxBeams], log_sum[kBeamMaxBeams], score[kBeamMaxBeams], scratch[32], powers[64];
     __shared__ unsigned char kind[kBeamMaxBeams];  // 0: a beam's own lists, 1: it has finished, 2: it has no candidate
-    __shared__ int count, reaching;
+    __shared__ int count, reaching, tally[32];
     __shared__ unsigned int close, key_bound;
     const int group = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const long long row0 = (long long)group * p.beams;
@@ -658,19 +685,56 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             value_bound = beam_key_floor(key_bound);
         }
         const unsigned long long least = (unsigned long long)nothing ^ kTopBit;
-        const bool wider = margin > 0.0 && value_bound > least;
-        const unsigned long long reach = wider ? (unsigned long long)beam_order(beam_value((long long)(value_bound ^ kTopBit)) - margin) ^ kTopBit : value_bound;
-        for (int i = threadIdx.x; i < lists * p.keep; i += blockDim.x) {
-            const int list = beam_divided(i, p.per_keep);
-            const BeamCandidate own = candidate(list, beam_divided(list, p.per_parts), i - list * p.keep);
-            const unsigned long long value = (unsigned long long)own.value ^ kTopBit;
-            if (own.place < 0 || value < reach || (!wider && value == reach && ~(unsigned long long)own.place < place_bound)) continue;
-            const int at = atomicAdd(&count, 1);
-            if (at < most) collected[at] = own;
+        bool wider = margin > 0.0 && value_bound > least, again = true;
+        int found;
+        for (;;) {
+            const unsigned long long reach = wider ? (unsigned long long)beam_order(beam_value((long long)(value_bound ^ kTopBit)) - margin) ^ kTopBit : value_bound;
+            for (int i = threadIdx.x; i < lists * p.keep; i += blockDim.x) {
+                const int list = beam_divided(i, p.per_keep);
+                const BeamCandidate own = candidate(list, beam_divided(list, p.per_parts), i - list * p.keep);
+                const unsigned long long value = (unsigned long long)own.value ^ kTopBit;
+                if (own.place < 0 || value < reach || (!wider && value == reach && ~(unsigned long long)own.place < place_bound)) continue;
+                const int at = atomicAdd(&count, 1);
+                if (at < most) collected[at] = own;
+            }
+            if (threadIdx.x < 32) tally[threadIdx.x] = 0;
+            __syncthreads();
+            // Only the margin can let in more than `most`: without it what is collected comes from keep + slack lists at most,
+            // `keep` from each.
+            found = count;
+            if (!again || found <= kBeamMany || (found > most && !wider)) break;
+            __syncthreads();
+            if (threadIdx.x == 0) count = 0;
+            if (found > most) {
+                wider = false;
+                __syncthreads();
+                continue;
+            }
+            // Few lists hold most of the best, and the first entries of all bounded them badly: the keep-th best of what was
+            // collected, by the values rounded to 32 bits.
+            again = false;
+            unsigned int* rounded = reinterpret_cast<unsigned int*>(order);
+            for (int i = threadIdx.x; i < found; i += blockDim.x) rounded[i] = beam_key(collected[i].value);
+            unsigned int bound_key = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned int tried = bound_key | 1u << bit;
+                int reach_it = 0;
+                for (int i = threadIdx.x; i < found; i += blockDim.x) reach_it += rounded[i] >= tried;
+                reach_it = __reduce_add_sync(0xFFFFFFFFu, reach_it);
+                if (lane == 0) atomicAdd(&tally[bit], reach_it);
+                __syncthreads();
+                reach_it = tally[bit];
+                if (reach_it >= p.keep) bound_key = tried;
+                if (reach_it >= p.keep && reach_it <= p.keep + kBeamSlack) break;
+            }
+            const unsigned long long raised = bound_key ? beam_key_floor(bound_key) : 0ull;
+            if (raised > value_bound) {
+                value_bound = raised;
+                place_bound = 0;
+            }
+            wider = margin > 0.0 && value_bound > least;
+            __syncthreads();
         }
-        __syncthreads();
-        const int found = count;
-        // Only the margin can let in more: without it what is collected comes from keep + slack lists at most, `keep` from each.
         const bool overflow = found > most;
         if (!overflow) {
             for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += blockDim.x >> 3) {
@@ -731,7 +795,7 @@ inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_
     params.spans = beam_spans(params.vocabulary, kType);
     params.parts = beam_parts(params.groups * params.beams, params.spans, sm_count);
     const int lists = params.beams * params.parts;
-    const int threads = lists > 512 ? 1024 : lists > 256 ? 512 : 256;  // a list or more of each
+    const int threads = lists > 512 || params.beams > 16 ? 1024 : lists > 256 || params.beams > 8 ? 512 : 256;  // a list or more of each, and half a beam of a warp (2 us of 16 for 16 beams)
     params.staged = params.keep < kBeamStage / lists ? params.keep : kBeamStage / lists;
     const int covering = (params.keep + lists - 1) / lists, filling = threads / lists;
     params.depths = covering > filling ? covering : filling;

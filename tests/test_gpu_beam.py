@@ -110,6 +110,40 @@ def test_candidates_of_two_beams_closer_than_32_bits_tell(cuda_device):
             check_select(logits, torch.tensor([[s[0], moved]], dtype=torch.float32, device=cuda_device), 6)
 
 
+@pytest.mark.parametrize("vocab", [63, 64, 65, 255, 256, 257, 511, 513, 1023, 1025, 2111, 4097, 8191, 8193, 9000, 20001])
+def test_short_rows_and_ends_of_rows(cuda_device, vocab):
+    """Fewer logits than a span takes, at any place of a vector, with more kept than the span has buckets."""
+    for dtype, beams, keep in ((torch.bfloat16, 3, 64), (torch.float16, 2, 33), (torch.float32, 4, 17)):
+        logits, scores, _ = select_case(vocab, 2, beams, vocab + 3, dtype, cuda_device)
+        for skip in (0, 1, 3):
+            view = logits[:, skip:skip + vocab]
+            check_select(view, scores, keep)
+        masked = logits[:, :vocab].clone()
+        masked[:, vocab // 3:vocab // 3 + vocab // 2] = -torch.inf
+        masked[1] = -torch.inf
+        masked[1, vocab - 40:] = 1.0
+        check_select(masked, scores, keep)
+
+
+@pytest.mark.parametrize("beams,vocab,keep,dtype", [
+    (32, 32001, 64, torch.bfloat16), (32, 32001, 64, torch.float32), (16, 70001, 40, torch.float16), (2, 262144, 64, torch.bfloat16),
+    (12, 12626, 33, torch.float32),
+])
+def test_one_beam_has_nearly_all_of_the_best(cuda_device, beams, vocab, keep, dtype):
+    """The first entries of the other beams' lists say nothing about the keep-th best."""
+    logits, scores, _ = select_case(vocab, 3, beams, vocab, dtype, cuda_device)
+    scores[0, 1:] -= 100.0
+    scores[1] = torch.linspace(0.0, -30.0, beams, device=cuda_device)
+    scores[2] = -1.0
+    check_select(logits, scores, keep)
+    logits[beams:2 * beams] = (logits[beams:2 * beams] * 2).round() / 2  # many equal ones
+    logits[2 * beams:] = logits[2 * beams]                               # the same beam everywhere
+    check_select(logits, scores, keep)
+    finished = torch.zeros((3, beams), dtype=torch.bool, device=cuda_device)
+    finished[:, 0] = True
+    check_select(logits, scores, keep, finished, 5)
+
+
 def test_equal_and_nearly_equal_beams_wherever_their_rows_begin(cuda_device):
     """Beams with the same row and score tie at every token, and the lower beam comes first; rows of 16 bytes and an odd
     rest begin at other places of a vector.  One step of a score turns the order."""
