@@ -9,8 +9,9 @@
 // part.  Every warp leaves the maximum and the sum of exponentials of its share of a span, and the CTA the `keep` best of its
 // part.  Within a beam candidates are ordered as their logits are, so no sum is needed for that.  Of 64 bucket maxima (four
 // threads each) the keep-th largest bounds the keep-th best from below; the few threads that reach it look at their logits
-// again, and what they find is ranked.  (Short rows and more than 32 kept take 256 maxima: with 64 kept of 128256 in 128 rows 37 us, by
-// the buckets alone 458; 14 rows of 524 with 28 kept 14 us, 34.)  The shares of a row have one size for all calls: its bits do not depend on the others.
+// again, and what they find is ranked.  (Short rows and ends of rows, and the most kept, take 256 maxima: with 64 kept of
+// 128256 in 128 rows 37 us, by the buckets alone 458; 14 rows of 524 with 28 kept 14 us, 34.)  The shares of a row have one
+// size for all calls: its bits do not depend on the others.
 //
 // Then a CTA per group joins parts and beams.  The sums are of 32-bit exponentials, each beam's log-sum off by up to
 // kBeamError; where two beams' candidates are closer than twice that, the sums of the two are taken again, in 64 bits, so
@@ -339,12 +340,14 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
     __syncthreads();
     float bound = beam_ordered_logit(bound_order);
     const bool single = span1 - span0 == 1;  // span: it is in the ring yet
-    if (p.keep > kBeamBuckets / 2 || (single && bound == -INFINITY)) {
-        // The least of nearly all buckets bounds badly, and a short row or end of one has fewer of them than `keep`: 256 maxima
-        // then, one to a thread; of every 256th logit where they are in the ring, so that as many threads as can have some.
+    const int n = single ? min(p.vocabulary - span0 * beam_span(kType), beam_span(kType)) : beam_span(kType);
+    if (n / (beam_span(kType) / kBeamBuckets) < p.keep + p.keep / 16) {
+        // The least of all buckets of many, or of one with few logits in a short row or end of one, bounds badly: 256 maxima
+        // then, one to a thread (1.4 us); of every 256th logit where they are in the ring, so that as many threads as can have
+        // some.  Where the buckets can bound the search they do, with some 17 logits found for eight and 110 for 32 of them.
         float sample = single ? -INFINITY : mine;
-        const int n = single ? min(p.vocabulary - span0 * beam_span(kType), beam_span(kType)) : 0;
-        for (int i = threadIdx.x; i < n; i += kBeamThreads) sample = fmaxf(sample, beam_logit_at<kType>(beam_ring + i / kShare * (kBeamStages * kBeamBlock) + skew, i % kShare));
+        if (single)
+            for (int i = threadIdx.x; i < n; i += kBeamThreads) sample = fmaxf(sample, beam_logit_at<kType>(beam_ring + i / kShare * (kBeamStages * kBeamBlock) + skew, i % kShare));
         const unsigned int order = beam_logit_order(sample), own = (order & ~(kBeamThreads - 1u)) | threadIdx.x;
         unsigned int* samples = reinterpret_cast<unsigned int*>(collected);  // which is empty yet
         samples[threadIdx.x] = own;
@@ -795,7 +798,8 @@ inline int launch_beam_select(BeamSelectParams params, int sm_count, cudaStream_
     params.spans = beam_spans(params.vocabulary, kType);
     params.parts = beam_parts(params.groups * params.beams, params.spans, sm_count);
     const int lists = params.beams * params.parts;
-    const int threads = lists > 512 || params.beams > 16 ? 1024 : lists > 256 || params.beams > 8 ? 512 : 256;  // a list or more of each, and half a beam of a warp (2 us of 16 for 16 beams)
+    // A list or more of each, and a beam of each warp (16 beams over 12626: 14 us, with two to a warp 16).
+    const int threads = lists > 512 || params.beams > 16 ? 1024 : lists > 256 || params.beams > 8 ? 512 : 256;
     params.staged = params.keep < kBeamStage / lists ? params.keep : kBeamStage / lists;
     const int covering = (params.keep + lists - 1) / lists, filling = threads / lists;
     params.depths = covering > filling ? covering : filling;

@@ -110,7 +110,7 @@ def test_candidates_of_two_beams_closer_than_32_bits_tell(cuda_device):
             check_select(logits, torch.tensor([[s[0], moved]], dtype=torch.float32, device=cuda_device), 6)
 
 
-@pytest.mark.parametrize("vocab", [63, 64, 65, 255, 256, 257, 511, 513, 1023, 1025, 2111, 4097, 8191, 8193, 9000, 20001])
+@pytest.mark.parametrize("vocab", [63, 64, 65, 255, 256, 257, 511, 513, 1023, 1025, 2082, 2111, 4097, 8191, 8193, 8194, 9000, 20001])
 def test_short_rows_and_ends_of_rows(cuda_device, vocab):
     """Fewer logits than a span takes, at any place of a vector, with more kept than the span has buckets."""
     for dtype, beams, keep in ((torch.bfloat16, 3, 64), (torch.float16, 2, 33), (torch.float32, 4, 17)):
