@@ -772,9 +772,8 @@ int mt_rope_kv_append_paged(const void* q, long long q_stride, const void* k, lo
 }
 
 size_t mt_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, int width, int page_size) {
-    (void)kv_heads;
     if (batch <= 0 || q_heads <= 0 || head_dim <= 0 || width <= 0 || page_size <= 0) return 0;
-    return paged_attention_workspace_bytes(batch, q_heads, head_dim, (long long)width * page_size);
+    return paged_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, (long long)width * page_size);
 }
 
 int mt_paged_attention_decode(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
@@ -788,7 +787,7 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
         return MT_ERR_SHAPE;
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || (type != MT_TYPE_BF16 && type != MT_TYPE_FP16)) return MT_ERR_SHAPE;
     // Units of work (a split of a KV head, 16 query heads at once) are counted in 32 bits.
-    if ((long long)batch * q_heads > 0x7FFFFFFF / kPagedMostSplits || (long long)width << shift > 0x7FFFFFFF) return MT_ERR_SHAPE;
+    if ((long long)batch * q_heads > 0x7FFFFFFF / paged_split_limit(kv_heads) || (long long)width << shift > 0x7FFFFFFF) return MT_ERR_SHAPE;
     if (batch == 0) return MT_OK;
     if (!q || !key_pages || !value_pages || !key_strides || !value_strides || !block_tables || !lengths || !out) return MT_ERR_NULL;
     if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 16) ||
@@ -807,7 +806,9 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
     params.tables = block_tables;
     params.lengths = lengths;
     params.out = static_cast<uint16_t*>(out);
-    params.most_splits = paged_most_splits((long long)width << shift);
+    params.split_limit = paged_split_limit(kv_heads);
+    params.split_floor = paged_split_floor(q_heads / kv_heads);
+    params.most_splits = paged_most_splits((long long)width << shift, params.split_limit);
     params.partial = static_cast<float*>(workspace);
     params.stats = reinterpret_cast<float2*>(params.partial + (size_t)batch * q_heads * params.most_splits * head_dim);
     params.table_stride = table_stride;

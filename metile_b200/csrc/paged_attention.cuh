@@ -4,7 +4,8 @@
 // and values: 4 Hq / Hkv operations for each, far below what the tensor cores have to offer.
 //
 // Split.  A sequence is cut into splits of 128 tokens, twice as many for every doubling above 16384, so that there are 128
-// at most (a partial result is D + 2 numbers of 32 bits per head: a sixteenth of what 128 tokens of eight heads read).
+// at most, or 512 where there are fewer than four KV heads (a partial result is D + 2 numbers of 32 bits per query head: with
+// eight of them a sixteenth of what 128 tokens of their KV head are).
 // The cut is the sequence's own, so its bits do not depend on the others of the call.  A unit is one split of one KV head
 // (its query heads, up to 16 at once) and belongs to one WARP.  The grid is one CTA per SM; the CTAs count the units of the
 // lengths they find on the device and deal them out, a unit to each SM in turn: a table wide enough for
@@ -34,23 +35,35 @@ namespace mt {
 
 constexpr int kPagedChunk = 16;          // tokens
 constexpr int kPagedSplitShift = 7;      // the shortest split: 128 tokens
-constexpr int kPagedMostSplits = 128;    // of a sequence
+constexpr int kPagedMostSplits = 128;    // of a sequence with four KV heads or more
+constexpr int kPagedSlices = 4;          // threads of the join to one number, 128 splits each
 constexpr int kPagedRowPad = 8;          // elements: rows 16 bytes longer keep matrix loads free of conflicts
 constexpr int kPagedTogether = 4;        // splits that one CTA joins: a warp to each of the SM's four schedulers
 constexpr float kPagedHeadroom = 8.0f;   // log2 of what a weight may reach
 
-__host__ __device__ constexpr int paged_split_shift(int tokens) {
+// Most splits of a sequence: with few KV heads more of them, so that one long sequence has 512 units in any case; those beyond
+// 128 are 16 tokens a query head of the group long at least (2^floor), so that partial results stay an eighth of what is read.
+// One request with 1 KV head: 131072 tokens for 8 heads of 128 26 us (40 with 128 splits), 100000 for one of 64 15 (33); a
+// batch of 16 with 2 x 4 heads and 32768 tokens 108 us (101).
+__host__ __device__ constexpr int paged_split_limit(int kv_heads) { return kv_heads >= 4 ? kPagedMostSplits : kv_heads >= 2 ? 2 * kPagedMostSplits : 4 * kPagedMostSplits; }
+static_assert(paged_split_limit(1) <= kPagedSlices * kPagedMostSplits, "the join takes 128 splits a slice");
+__host__ __device__ constexpr int paged_split_floor(int group) {
     int shift = kPagedSplitShift;
-    while ((tokens - 1) >> shift >= kPagedMostSplits) ++shift;
+    while (shift < 20 && 1 << shift < 16 * group) ++shift;
     return shift;
 }
-__host__ __device__ constexpr int paged_splits(int tokens) {
-    return tokens <= 1 ? 1 : ((tokens - 1) >> paged_split_shift(tokens)) + 1;
+__host__ __device__ constexpr int paged_split_shift(int tokens, int limit = kPagedMostSplits, int floor = kPagedSplitShift) {
+    int shift = kPagedSplitShift;
+    while ((tokens - 1) >> shift >= (shift < floor ? kPagedMostSplits : limit)) ++shift;
+    return shift;
+}
+__host__ __device__ constexpr int paged_splits(int tokens, int limit = kPagedMostSplits, int floor = kPagedSplitShift) {
+    return tokens <= 1 ? 1 : ((tokens - 1) >> paged_split_shift(tokens, limit, floor)) + 1;
 }
 // The most splits any length up to `capacity` has.
-inline int paged_most_splits(long long capacity) {
+inline int paged_most_splits(long long capacity, int limit = kPagedMostSplits) {
     const long long shortest = (capacity + (1 << kPagedSplitShift) - 1) >> kPagedSplitShift;
-    return shortest < kPagedMostSplits ? (int)shortest : kPagedMostSplits;
+    return shortest < limit ? (int)shortest : limit;
 }
 
 struct PageByteStrides {
@@ -67,7 +80,7 @@ struct PagedAttentionParams {
     float* partial;                    // [batch * Hq, most_splits, D]
     float2* stats;                     // [batch * Hq, most_splits]: maximum (log2) and sum
     long long table_stride;
-    int width, batch, q_heads, kv_heads, page_shift, page_count, most_splits;
+    int width, batch, q_heads, kv_heads, page_shift, page_count, most_splits, split_limit, split_floor;
     bool together;                     // a CTA has all splits of its KV heads, one to a warp, and joins them
     float scale;
 };
@@ -141,7 +154,7 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
         __shared__ int warp_units[Shape::kWarps];
         int mine = 0;
         for (int b = threadIdx.x * run; b < min((int)(threadIdx.x + 1) * run, p.batch); ++b)
-            mine += paged_splits(paged_length(p, b, blockIdx.x == 0)) * per_split;
+            mine += paged_splits(paged_length(p, b, blockIdx.x == 0), p.split_limit, p.split_floor) * per_split;
         int sum = mine;
 #pragma unroll
         for (int offset = 1; offset < 32; offset <<= 1) {
@@ -166,7 +179,7 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
             b = blockIdx.x / per_split;
             rest = blockIdx.x - b * per_split;
             n = paged_length(p, b, rest == 0 && threadIdx.x == 0);
-            splits = paged_splits(n);
+            splits = paged_splits(n, p.split_limit, p.split_floor);
             split = warp;
         } else {
             int unit = (int)next;
@@ -178,7 +191,7 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
             unit -= unit_start[low];
             for (b = low * run;; ++b) {
                 n = paged_length(p, b, false);
-                splits = paged_splits(n);
+                splits = paged_splits(n, p.split_limit, p.split_floor);
                 if (unit < splits * per_split) break;
                 unit -= splits * per_split;
             }
@@ -186,7 +199,7 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
             rest = unit - split * per_split;
         }
         const int h = rest / parts, part = rest - h * parts;
-        const int shift = paged_split_shift(n), first = split << shift, end = max(first, min(n, first + (1 << shift)));
+        const int shift = paged_split_shift(n, p.split_limit, p.split_floor), first = split << shift, end = max(first, min(n, first + (1 << shift)));
         const int head0 = h * group + part * 8 * kTiles, heads = min(8 * kTiles, group - part * 8 * kTiles);
         const int chunks = (end - first + kPagedChunk - 1) / kPagedChunk;
 
@@ -429,18 +442,21 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
     }
 }
 
-// Joins the splits of one request and query head, in split order; a request of one split has its result already.
-template <int kD, bool kHalf>
-__global__ void __launch_bounds__(kD) paged_attention_join_kernel(const __grid_constant__ PagedAttentionParams p) {
+// Joins the splits of one request and query head, in split order; a request of one split has its result already.  A slice of
+// kD threads takes 128 splits, the first one what the slices have, in their order.
+template <int kD, bool kHalf, int kSlices>
+__global__ void __launch_bounds__(kD * kSlices) paged_attention_join_kernel(const __grid_constant__ PagedAttentionParams p) {
     constexpr int kAhead = 16, kRounds = kPagedMostSplits / 32;
     const long long at = blockIdx.x;                // b * Hq + query head
-    const int b = (int)(at / p.q_heads), d = threadIdx.x, lane = threadIdx.x & 31;
+    const int b = (int)(at / p.q_heads), d = threadIdx.x % kD, slice = threadIdx.x / kD, lane = threadIdx.x & 31;
+    __shared__ float slice_value[kSlices][kD], slice_total[kSlices];
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    const int splits = paged_splits(paged_length(p, b, false));
-    if (splits == 1) return;
-    const float* from = p.partial + at * p.most_splits * kD + d;
-    const float2* stats = p.stats + at * p.most_splits;
+    const int all = paged_splits(paged_length(p, b, false), p.split_limit, p.split_floor), first = slice * kPagedMostSplits;
+    if (all == 1) return;
+    const int splits = min(all - first, kPagedMostSplits);  // of this slice
+    const float* from = p.partial + (at * p.most_splits + first) * kD + d;
+    const float2* stats = p.stats + at * p.most_splits + first;
     // The first results are asked for before the maxima are known, the others sixteen ahead.
     float ahead[kAhead];
 #pragma unroll
@@ -452,6 +468,8 @@ __global__ void __launch_bounds__(kD) paged_attention_join_kernel(const __grid_c
         mine[r] = 32 * r + lane < splits ? stats[32 * r + lane] : make_float2(-INFINITY, 0.0f);
         top = fmaxf(top, mine[r].x);
     }
+    if (kSlices > 1 && all > kPagedMostSplits)  // the maximum is that of all
+        for (int i = lane; i < all; i += 32) top = fmaxf(top, p.stats[at * p.most_splits + i].x);
 #pragma unroll
     for (int offset = 16; offset >= 1; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
     float total = 0.0f, value = 0.0f;
@@ -477,11 +495,21 @@ __global__ void __launch_bounds__(kD) paged_attention_join_kernel(const __grid_c
             }
         }
     }
+    if (kSlices > 1 && all > kPagedMostSplits) {
+        slice_value[slice][d] = value;
+        if (d == 0) slice_total[slice] = total;
+        __syncthreads();
+        for (int other = 1; other < kSlices && other * kPagedMostSplits < all; ++other) {
+            total += slice_total[other];
+            value += slice_value[other][d];
+        }
+    }
+    if (slice > 0) return;
     p.out[at * kD + d] = (uint16_t)pack_pair<kHalf>(total == 0.0f ? 0.0f : value / total, 0.0f);
 }
 
-inline size_t paged_attention_workspace_bytes(int batch, int q_heads, int head_dim, long long capacity) {
-    const int splits = paged_most_splits(capacity);
+inline size_t paged_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, long long capacity) {
+    const int splits = paged_most_splits(capacity, paged_split_limit(kv_heads));
     if (splits <= 1) return 0;
     return (size_t)batch * q_heads * splits * (head_dim + 2) * sizeof(float);
 }
@@ -516,9 +544,11 @@ inline int launch_paged_attention_instance(PagedAttentionParams params, int sm_c
     if (cudaLaunchKernelEx(&config, paged_attention_kernel<kD, kHalf, kTiles>, params) != cudaSuccess) return MT_ERR_LAUNCH;
     if (params.most_splits > 1 && !params.together) {
         config.gridDim = dim3(params.batch * params.q_heads, 1, 1);
-        config.blockDim = dim3(kD, 1, 1);
+        const bool sliced = params.most_splits > kPagedMostSplits;
+        config.blockDim = dim3(sliced ? kPagedSlices * kD : kD, 1, 1);
         config.dynamicSmemBytes = 0;
-        if (cudaLaunchKernelEx(&config, paged_attention_join_kernel<kD, kHalf>, params) != cudaSuccess) return MT_ERR_LAUNCH;
+        if (cudaLaunchKernelEx(&config, sliced ? paged_attention_join_kernel<kD, kHalf, kPagedSlices> : paged_attention_join_kernel<kD, kHalf, 1>, params) != cudaSuccess)
+            return MT_ERR_LAUNCH;
     }
     return MT_OK;
 }

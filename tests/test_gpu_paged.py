@@ -262,6 +262,21 @@ def test_paged_attention_against_the_oracle(cuda_device, lengths, heads, kv_head
     check_attention(attention_case(31, lengths, heads, kv_heads, dim, page, dtype, layout, cuda_device), dim ** -0.5, cuda_device)
 
 
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page,dtype", [
+    ([16384, 16385, 70000, 0, 1], 8, 1, 64, 32, torch.bfloat16), ([65537], 10, 1, 128, 64, torch.float16),
+    ([32769, 16500, 300], 4, 2, 64, 16, torch.bfloat16), ([20000], 16, 1, 256, 128, torch.bfloat16), ([16640], 6, 3, 64, 32, torch.float16),
+])
+def test_long_sequences_of_few_heads(cuda_device, lengths, heads, kv_heads, dim, page, dtype):
+    """Up to 512 splits of a sequence; the bits are its own whatever the table's width and the others."""
+    q, keys, values, tables, n = attention_case(37, lengths, heads, kv_heads, dim, page, dtype, "head", cuda_device)
+    out = check_attention((q, keys, values, tables, n), dim ** -0.5, cuda_device)
+    table = torch.tensor(tables, device=cuda_device)
+    for b, count in enumerate(n):
+        narrow = table[b:b + 1, :max(1, -(-int(count) // page))].contiguous()
+        alone = B.paged_attention_decode(q[b:b + 1], keys, values, narrow, torch.tensor(n[b:b + 1], device=cuda_device), scale=dim ** -0.5)
+        assert torch.equal(alone, out[b:b + 1]), b
+
+
 def test_a_peaked_softmax_and_large_scores(cuda_device):
     check_attention(attention_case(41, [900, 60], 8, 2, 128, 16, torch.bfloat16, "head", cuda_device, spread=40.0), 128 ** -0.5, cuda_device)
     check_attention(attention_case(42, [400], 4, 4, 64, 16, torch.float16, "head", cuda_device), -0.7, cuda_device)

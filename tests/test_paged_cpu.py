@@ -199,3 +199,34 @@ int main() {
 """
     for capacity, most, declared, wrong in host_program(str(tmp_path), source):
         assert wrong == 0 and most <= declared <= 128, capacity
+
+
+def test_splits_of_sequences_with_few_heads(tmp_path):
+    """With one, two or three KV heads a sequence has more splits, as many as the scratch and the join have room for."""
+    from tests.helpers import host_program
+
+    source = r"""
+#include "../../include/metile_b200.h"
+#include "paged_attention.cuh"
+#include <cstdio>
+int main() {
+    for (int heads : {1, 2, 3, 4, 8, 64}) for (int group : {1, 9, 40}) {
+        const int limit = mt::paged_split_limit(heads), floor = mt::paged_split_floor(group);
+        for (long long capacity : {128ll, 129ll, 16384ll, 16385ll, 40000ll, 100000ll, 0x7FFFFFFFll}) {
+            int most = 0, wrong = 0;
+            for (long long n = 0; n <= capacity; n += n < 140000 ? 1 : 65521) {
+                const int shift = mt::paged_split_shift((int)n, limit, floor), splits = mt::paged_splits((int)n, limit, floor);
+                if (splits > most) most = splits;
+                wrong += ((long long)splits << shift) < n || (splits > 1 && ((long long)(splits - 1) << shift) >= n) || shift < 7 || (splits > 128 && 1 << shift < 16 * group);
+            }
+            const size_t bytes = mt::paged_attention_workspace_bytes(3, heads * group, heads, 64, capacity);
+            wrong += bytes != (most > 1 ? (size_t)3 * heads * group * mt::paged_most_splits(capacity, limit) * 66 * 4 : 0);
+            std::printf("%d %d %d %d\n", limit * heads >= 512, most <= mt::paged_most_splits(capacity, limit), limit <= mt::kPagedSlices * mt::kPagedMostSplits, wrong);
+        }
+    }
+}
+"""
+    rows = host_program(str(tmp_path), source)
+    assert len(rows) == 126
+    for units, fits, joined, wrong in rows:
+        assert units and fits and joined and wrong == 0
