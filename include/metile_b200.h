@@ -292,8 +292,8 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
                               int kv_heads, int head_dim, int pages, int page_size, int type, float scale, void* stream);
 
 /* A step of beam search.  Of the beams * vocabulary candidates of a group, score + log softmax(logits) in 64 bits, the `keep`
- * (1 ... 64) largest in descending order, the lower beam and then the lower token first among equals.  logits [groups *
- * beams, vocabulary] bf16, fp16 or fp32, rows `row_stride` elements apart; scores fp32 [groups, beams].  A beam that has
+ * (1 ... 64) largest in descending order; among equals the lower beam first, then the larger logit, then the lower token.
+ * logits [groups * beams, vocabulary] bf16, fp16 or fp32, rows `row_stride` elements apart; scores fp32 [groups, beams].  A beam that has
  * `finished` (bytes, may be NULL) offers end_token alone, at its score.  As -inf count: every candidate of a score
  * up to -1e9 or of a row with a NaN, with +inf or with nothing above -inf.  parents: the beam within its group;
  * finished_out: the parent had finished, or the token is end_token (-1: there is none).  beams up to 32.  The aligned 16

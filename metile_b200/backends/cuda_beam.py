@@ -19,7 +19,7 @@ def beam_select(logits, scores, *, keep=None, finished=None, end_token=None):
 
     logits [groups * beams, vocabulary] bfloat16, float16 or float32; scores float32 [groups, beams], the sums of
     log-probabilities so far.  A candidate is worth scores + log_softmax(logits), in 64 bits; the largest come first, among
-    equals the lower beam, then the lower token.  A beam that has `finished` (bool [groups, beams]) offers `end_token`
+    equals the lower beam, then the larger logit, then the lower token.  A beam that has `finished` (bool [groups, beams]) offers `end_token`
     alone, at the score it has.  A score up to -1e9 is a mask: that beam's candidates count as -inf, and so do those of
     logits with a NaN, with +inf or with nothing above -inf.
 

@@ -1,9 +1,10 @@
 // Beam search's selection: the best continuations over a group's beams and the vocabulary.
 //
 // A candidate is (beam, token) with the value score[beam] + ((logit - max) - log sum exp(logit - max)), in 64 bits; equal
-// ones go by the lower beam, then the lower token.  What has no value (a row with a NaN, with +inf or with nothing above
-// -inf; a score that is a mask) counts as -inf.  Bound by the bytes of the logits, and near to it by the exponentials (an
-// SM takes 16 a cycle: 9 TB/s of 16-bit logits on 148 of them).
+// ones go by the lower beam, then the larger logit (64 bits may round the values of two to one), then the lower token.  So
+// a beam's candidates are always in the order of their logits, which its sorted lists rest on.  What has no value (a row
+// with a NaN, with +inf or with nothing above -inf; a score that is a mask) counts as -inf.  Bound by the bytes of the logits,
+// and near to it by the exponentials (an SM takes 16 a cycle: 9 TB/s of 16-bit logits on 148 of them).
 //
 // One pass.  Rows are cut into spans of 16 KB, 64 bytes a thread, and a row's spans dealt out to CTAs; a CTA's share of a row is a
 // part.  Every warp leaves the maximum and the sum of exponentials of its share of a span, and the CTA the `keep` best of its
@@ -87,7 +88,8 @@ __host__ __device__ inline int beam_part_start(int part, int spans, int parts) {
 
 inline int beam_spans(int vocabulary, int type) { return (vocabulary + beam_span(type) - 1) / beam_span(type); }
 
-// The most candidates the join collects without a margin: from keep + slack lists, `keep` of each.
+// The most candidates the join collects without a margin: from keep + slack lists, `keep` of each.  (No more first entries
+// reach the bound, and what reaches it in a list stands behind a first entry that does: lists are sorted by value and place.)
 __host__ __device__ inline int beam_join_most(int keep) { return (keep + kBeamSlack) * keep; }
 
 // Parts of a row: as many as let all CTAs run at once, but none longer than a part may be, and no more than the join takes.
@@ -449,8 +451,10 @@ __global__ void __launch_bounds__(kBeamThreads, kBeamAtOnce) beam_span_kernel(co
 
 struct __align__(16) BeamCandidate {
     long long value;  // the 64-bit number as a whole one of the same order
-    long long place;  // beam 2^32 + token; -1: there is none
+    long long place;  // beam, logit (the larger first) and token from the top bit down; -1: there is none
 };
+constexpr int kBeamTokenBits = 19, kBeamPlaceShift = kBeamTokenBits + 32;
+static_assert(MT_BEAM_MAX_VOCABULARY <= 1 << kBeamTokenBits && (long long)kBeamMaxBeams << kBeamPlaceShift > 0, "a place is a positive number");
 __device__ __forceinline__ bool beam_before(const BeamCandidate& a, const BeamCandidate& b) {
     return a.value > b.value || (a.value == b.value && a.place < b.place);
 }
@@ -596,11 +600,12 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
     const long long nothing = beam_order(-INFINITY);
     // Candidate `depth` of a list of a beam.
     auto candidate = [&](int list, int beam, int depth) -> BeamCandidate {
-        const long long base = (long long)beam << 32;
+        const long long base = (long long)beam << kBeamPlaceShift;
         if (kind[beam] == 0) {
             const BeamEntry entry = depth < staged ? stage[list * staged + depth] : entries[(long long)list * p.keep + depth];
             if (entry.token < 0) return {nothing, -1};
-            return {beam_order(score[beam] + (((double)entry.logit - top[beam]) - log_sum[beam])), base + entry.token};
+            return {beam_order(score[beam] + (((double)entry.logit - top[beam]) - log_sum[beam])),
+                    base + ((long long)(0xFFFFFFFFu - beam_logit_order(entry.logit)) << kBeamTokenBits) + entry.token};
         }
         const int part = list - beam * p.parts;
         long long token = depth;  // no candidate: the first tokens, at -inf
@@ -754,7 +759,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
                 for (int i = threadIdx.x; i + 1 < found; i += blockDim.x) {
                     const BeamCandidate upper = collected[order[i]], lower = collected[order[i + 1]];
                     if (i + 1 >= p.keep && last - beam_value(lower.value) > margin) break;
-                    const int a = (int)(upper.place >> 32), b = (int)(lower.place >> 32);
+                    const int a = (int)(upper.place >> kBeamPlaceShift), b = (int)(lower.place >> kBeamPlaceShift);
                     if (a != b && lower.value > nothing && beam_value(upper.value) - beam_value(lower.value) <= margin) atomicOr(&close, 1u << a | 1u << b);
                 }
             }
@@ -782,8 +787,8 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
         }
         for (int r = threadIdx.x; r < p.keep; r += blockDim.x) {
             const BeamCandidate best = collected[order[r]];
-            const int parent = (int)(best.place >> 32);
-            const long long token = best.place & 0xFFFFFFFFll, at = (long long)group * p.keep + r;
+            const int parent = (int)(best.place >> kBeamPlaceShift);
+            const long long token = best.place & ((1ll << kBeamTokenBits) - 1), at = (long long)group * p.keep + r;
             p.scores_out[at] = (float)beam_value(best.value);
             p.parents_out[at] = parent;
             p.tokens_out[at] = token;

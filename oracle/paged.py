@@ -77,12 +77,13 @@ def attention(query, keys, values, tables, lengths, scale):
 
 
 def beam_select(logits, scores, keep, finished=None, end=-1):
-    """logits [G * K, V] and scores [G, K] float64; returns (scores, parents, tokens, finished)."""
+    """logits [G * K, V] and scores [G, K] float64; returns (scores, parents, tokens, finished).  Equal candidates: the lower
+    beam, then the larger logit, then the lower token."""
     groups, beams = scores.shape
     vocab = logits.shape[1]
     best, parents, tokens, done = [], [], [], []
     for g in range(groups):
-        found = np.full((beams, vocab), -np.inf)
+        found, own = np.full((beams, vocab), -np.inf), np.zeros((beams, vocab))
         for k in range(beams):
             score, row = scores[g, k], logits[g * beams + k]
             if not score > -1e9:
@@ -93,9 +94,9 @@ def beam_select(logits, scores, keep, finished=None, end=-1):
             top = row.max()
             if not np.isfinite(top):  # NaN, +inf, or nothing above -inf
                 continue
-            found[k] = score + ((row - top) - np.log(np.exp(row - top).sum()))
+            found[k], own[k] = score + ((row - top) - np.log(np.exp(row - top).sum())), row
         flat = found.reshape(-1)
-        order = np.lexsort((np.arange(flat.size), -flat))[:keep]
+        order = np.lexsort((np.arange(flat.size), -own.reshape(-1), np.arange(flat.size) // vocab, -flat))[:keep]
         best.append(flat[order])
         parents.append(order // vocab)
         tokens.append(order % vocab)

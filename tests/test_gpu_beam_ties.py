@@ -1,0 +1,81 @@
+"""Beam selection where very many candidates are equal or nearly so: the order is the one of the exact sums, and a
+group's bits are its own whatever else is in the call."""
+
+import numpy as np
+import pytest
+import torch
+
+from metile_b200 import _lib, backends as B
+from oracle import paged as O
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def nothing_was_recorded(cuda_device):
+    yield
+    ok, words = _lib.device_status()
+    assert ok, [hex(w) for w in words]
+
+
+def wide(tensor):
+    return tensor.detach().cpu().double().numpy()
+
+
+def quantised_rows(seed, rows, vocab, device, levels=40):
+    """Logits of few levels (capped or quantised heads): the largest one stands in every part of a row many times over."""
+    generator = torch.Generator().manual_seed(seed)
+    return (torch.randint(0, levels, (rows, vocab), generator=generator) / 8).to(torch.bfloat16).to(device)
+
+
+def log_sums(logits):
+    rows = wide(logits)
+    top = rows.max(1)
+    return top, np.log(np.exp(rows - top[:, None]).sum(1))
+
+
+def check(logits, scores, keep):
+    out = B.beam_select(logits, scores, keep=keep)
+    expected = O.beam_select(wide(logits), wide(scores), keep)
+    assert np.array_equal(out[1].cpu().numpy(), expected[1]) and np.array_equal(out[2].cpu().numpy(), expected[2])
+    # Half a step of 32 bits, and the bound of a log-sum of 32-bit exponentials.
+    assert (np.abs(wide(out[0]) - expected[0]) <= 2.0 ** -24 * np.abs(expected[0]) + 2.0 ** -18).all()
+    return out
+
+
+def own_order(row, keep):
+    """The tokens of one beam in the order of their logits, the lower token first among equals."""
+    row = wide(row)
+    return np.lexsort((np.arange(row.size), -row))[:keep]
+
+
+@pytest.mark.parametrize("beams,vocab,keep,dtype", [
+    (23, 524288, 4, torch.float32), (1, 524288, 4, torch.float32), (8, 128256, 16, torch.bfloat16), (2, 300, 64, torch.bfloat16),
+    (32, 50001, 1, torch.float32), (5, 77777, 33, torch.float32),
+])
+def test_logits_that_64_bits_cannot_tell_apart(cuda_device, beams, vocab, keep, dtype):
+    """Logits far below the log of their sum, or far below the largest one: all are worth the same in 64 bits and go by
+    themselves.  In every part of a row but one the largest stand in front; in that one the very largest comes last."""
+    generator = torch.Generator().manual_seed(vocab)
+    tiny = (torch.rand((beams, vocab), generator=generator) * 2.0 ** -80).to(dtype)
+    if vocab == 524288:  # 25 parts for 23 rows: the middle of the row lies inside the thirteenth
+        step = torch.arange(vocab) % 20972
+        tiny[0] = (torch.where(step < 4, 2.0 - step / 8, 1.0) * 2.0 ** -80).to(dtype)
+        tiny[0, 262144 - 3:262144] = 2.5 * 2.0 ** -80
+        tiny[0, 262144 + 9] = 3.0 * 2.0 ** -80
+    logits = tiny.to(cuda_device)
+    scores = torch.full((1, beams), -50.0, device=cuda_device)
+    scores[0, 0] = -1.0
+    for alone in (False, True):
+        if alone:  # all but one token 1e30 below it; by itself, since any other beam would come before them
+            logits[0, 7] = 1e30
+        got, parents, tokens, _ = B.beam_select(logits[:1] if alone else logits, scores[:, :1].contiguous() if alone else scores, keep=keep)
+        assert not parents.any()
+        assert np.array_equal(tokens[0].cpu().numpy(), own_order(logits[0], keep))
+        worth = -1.0 - (0.0 if alone else np.log(vocab))
+        assert abs(float(got[0, 0]) - worth) <= 2.0 ** -24 * abs(worth) + 2.0 ** -18
+    # Beams that are one row throughout tie with each other too: the lower one first.
+    got, parents, tokens, _ = B.beam_select(logits[:1].expand(beams, -1), torch.zeros((1, beams), device=cuda_device), keep=keep)
+    first = min(beams, keep)  # every beam's token 7 is worth 0, all others 1e30 less
+    assert parents[0, :first].tolist() == list(range(first)) and tokens[0, :first].tolist() == [7] * first and not got[0, :first].any()
+    assert not parents[0, first:].any() and np.array_equal(tokens[0, first:].cpu().numpy(), own_order(logits[0], keep)[1:keep - first + 1])
