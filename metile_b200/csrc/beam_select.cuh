@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             value_bound = beam_key_floor(key_bound);
         }
         const unsigned long long least = (unsigned long long)nothing ^ kTopBit;
-        bool wider = margin > 0.0 && value_bound > least, again = true;
+        bool wider = margin > 0.0 && value_bound > least, again = true, dropped = false;
         int found;
         for (;;) {
             const unsigned long long reach = wider ? (unsigned long long)beam_order(beam_value((long long)(value_bound ^ kTopBit)) - margin) ^ kTopBit : value_bound;
@@ -713,8 +713,9 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             if (!again || found <= kBeamMany || (found > most && !wider)) break;
             __syncthreads();
             if (threadIdx.x == 0) count = 0;
-            if (found > most) {
+            if (found > most) {  // without the margin, for the bound below; what lies within it has to be looked at all the same
                 wider = false;
+                dropped = true;
                 __syncthreads();
                 continue;
             }
@@ -741,9 +742,10 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
                 place_bound = 0;
             }
             wider = margin > 0.0 && value_bound > least;
+            dropped = dropped && !wider;
             __syncthreads();
         }
-        const bool overflow = found > most;
+        const bool overflow = found > most || dropped;
         if (!overflow) {
             for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += blockDim.x >> 3) {
                 const int rank = beam_rank(collected, found, collected[min(i, found - 1)]);

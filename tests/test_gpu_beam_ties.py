@@ -79,3 +79,18 @@ def test_logits_that_64_bits_cannot_tell_apart(cuda_device, beams, vocab, keep, 
     first = min(beams, keep)  # every beam's token 7 is worth 0, all others 1e30 less
     assert parents[0, :first].tolist() == list(range(first)) and tokens[0, :first].tolist() == [7] * first and not got[0, :first].any()
     assert not parents[0, first:].any() and np.array_equal(tokens[0, first:].cpu().numpy(), own_order(logits[0], keep)[1:keep - first + 1])
+
+
+@pytest.mark.parametrize("beams,keep", [(2, 16), (8, 4), (3, 40)])
+def test_hundreds_of_equal_candidates_in_two_beams_a_hair_apart(cuda_device, beams, keep):
+    """More candidates within the margin of the sums than are collected: the beam whose exact value is larger comes first,
+    by however little (64 bits leave 1e-14 here)."""
+    for seed in range(4):
+        logits = quantised_rows(10 * beams + seed, beams, 128256, cuda_device)
+        _, sums = log_sums(logits)  # the rows have the same largest logit
+        for apart in (1e-8, 3e-8, 1e-7, 3e-7, 1e-6):
+            for sign in (-1.0, 1.0):
+                given = sums - sums[0] - 0.1  # all beams' best are worth the same
+                given[0] = 0.0
+                given[1] = sums[1] - sums[0] + sign * apart
+                check(logits, torch.tensor(given[None], dtype=torch.float32, device=cuda_device), keep)
