@@ -94,3 +94,28 @@ def test_hundreds_of_equal_candidates_in_two_beams_a_hair_apart(cuda_device, bea
                 given[0] = 0.0
                 given[1] = sums[1] - sums[0] + sign * apart
                 check(logits, torch.tensor(given[None], dtype=torch.float32, device=cuda_device), keep)
+
+
+@pytest.mark.parametrize("beams,keep,dtype", [(3, 16, torch.bfloat16), (8, 4, torch.bfloat16), (8, 16, torch.float32), (2, 64, torch.float16)])
+def test_a_group_has_the_same_bits_however_its_rows_are_cut(cuda_device, beams, keep, dtype):
+    """Alone a row is cut into sixteen parts or more, in a batch of 32 into a few.  The values lie near zero, where a score
+    shows how its log-sum was taken: beams 0 and 1 have hundreds of equal candidates a hair apart, the others a few above."""
+    generator = torch.Generator().manual_seed(beams)
+    logits = (torch.randn((32 * beams, 128256), generator=generator) * 2.5).to(dtype).to(cuda_device)
+    scores = torch.zeros((32, beams), device=cuda_device)
+    for g in range(32):
+        if g % 4 < 3:
+            logits[g * beams:g * beams + 2] = quantised_rows(g, 2, 128256, cuda_device).to(dtype)
+        _, sums = log_sums(logits[g * beams:(g + 1) * beams])
+        given = sums + 0.01 * np.arange(beams)
+        if g % 4 < 3:
+            given[:2] = sums[:2] - (0.2 if g % 4 < 2 else 0.0)
+            given[1] += (2e-8, -1e-7, 1e-5, 0.0)[g % 4]
+        scores[g] = torch.tensor(given, dtype=torch.float32, device=cuda_device)
+    together = B.beam_select(logits, scores, keep=keep)
+    for g in range(0, 32, 3):
+        rows = slice(g * beams, (g + 1) * beams)
+        alone = check(logits[rows].clone(), scores[g:g + 1], keep)
+        assert all(torch.equal(a, b[g:g + 1]) for a, b in zip(alone, together)), g
+        few = B.beam_select(logits[:(g + 1) * beams], scores[:g + 1], keep=keep)
+        assert all(torch.equal(a[g:], b[g:g + 1]) for a, b in zip(few, together)), g
