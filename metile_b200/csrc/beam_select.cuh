@@ -34,8 +34,8 @@ namespace mt {
 
 constexpr double kDeadScore = -1e9;  // no sum of log-probabilities but the mask of a beam that is out; above it 64 bits keep logits apart
 // d = logit - top rounded, then d log2 e: |d| 2^-24 each and |d| 1.4e-8 for log2 e itself, 2^-22 for ex2.approx, within a share
-// and once more for the share in the row, where the two |d| add up to the one to the row's maximum; twelve roundings of 2^-24
-// in sums (the rest is added in 64 bits).  The mean of |d| by the weights is at most the log of the row's length, 13.2: 3.0e-6.
+// and once more for the share in the row, where the two |d| add up to the one to the row's maximum; fourteen roundings of 2^-24
+// in sums (the rest is added in 64 bits).  The mean of |d| by the weights is at most the log of the row's length, 13.2: 3.1e-6.
 constexpr double kBeamError = 0x1p-18;
 
 constexpr int kBeamMaxBeams = 32, kBeamMaxKeep = 64;
@@ -566,24 +566,30 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
         const bool ended = p.finished && p.finished[row0 + beam];
         const BeamShareStats* stats = p.stats + (row0 + beam) * p.spans * kBeamShares;
         const int shares = p.spans * kBeamShares;
-        // 128 shares at a time: a lane's four of them are asked for together.
+        // 128 shares at a time: a lane's four of them are asked for together.  The row's maximum first, so that every share is
+        // weighted once; what does not fit the first 128 is read twice.
+        BeamShareStats own[4];
         float best = -INFINITY;
-        double sum = 0.0;
-        for (int first = 0; first < shares; first += 128) {
-            BeamShareStats own[4];
-            float now = best;
+        auto take = [&](int first) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int i = first + 32 * k + lane;
                 own[k] = i < shares ? stats[i] : BeamShareStats{-INFINITY, 0.0f};
-                now = fmaxf(now, own[k].top);
             }
-            asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(now) : "f"(now));
+        };
+        for (int first = (shares - 1) / 128 * 128; first >= 0; first -= 128) {
+            take(first);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) best = fmaxf(best, own[k].top);
+        }
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(best) : "f"(best));
+        double sum = 0.0;
+        for (int first = 0; first < shares; first += 128) {
+            if (first > 0) take(first);
             float part = 0.0f;  // of the same error as within a share
 #pragma unroll
-            for (int k = 0; k < 4; ++k) part += own[k].sum == 0.0f ? 0.0f : own[k].sum * __expf(own[k].top - now);
-            sum = (sum == 0.0 ? 0.0 : sum * (double)__expf(best - now)) + (double)part;
-            best = now;
+            for (int k = 0; k < 4; ++k) part += own[k].sum == 0.0f ? 0.0f : own[k].sum * __expf(own[k].top - best);
+            sum += (double)part;
         }
 #pragma unroll
         for (int offset = 16; offset >= 1; offset >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);

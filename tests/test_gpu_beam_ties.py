@@ -119,3 +119,19 @@ def test_a_group_has_the_same_bits_however_its_rows_are_cut(cuda_device, beams, 
         assert all(torch.equal(a, b[g:g + 1]) for a, b in zip(alone, together)), g
         few = B.beam_select(logits[:(g + 1) * beams], scores[:g + 1], keep=keep)
         assert all(torch.equal(a[g:], b[g:g + 1]) for a, b in zip(few, together)), g
+
+
+def test_a_log_sum_does_not_follow_the_order_of_the_maxima(cuda_device):
+    """Eight stretches of a long row whose maxima rise, fall or go up and down: every logit is weighted against the row's
+    maximum through two exponentials, wherever it stands, and the rest is added in 64 bits."""
+    stretches = torch.linspace(0.0, 1.0, 524288, dtype=torch.float64).float().view(8, 65536)
+    scores = torch.full((4, 1), 12.7, device=cuda_device)  # the value is near zero, where 32 bits show 64
+    rows = torch.stack([stretches[order].reshape(-1) for order in (
+        [0, 1, 2, 3, 4, 5, 6, 7], [7, 6, 5, 4, 3, 2, 1, 0], [3, 6, 0, 7, 1, 5, 2, 4], [0, 2, 4, 6, 1, 3, 5, 7])]).to(cuda_device)
+    top, sums = log_sums(rows[:1])
+    scores[:] = float(np.float32(sums[0]))
+    got = wide(B.beam_select(rows, scores, keep=1)[0])[:, 0]
+    exact = float(scores[0]) - sums[0]
+    # The two exponentials and the sums of 32 bits: 2 * 2^-22, 14 * 2^-24, and |d| * 1.33e-7 with |d| up to 1.
+    assert (np.abs(got - exact) <= 2 * 2.0 ** -22 + 14 * 2.0 ** -24 + 1.33e-7).all()
+    assert np.abs(got - got[0]).max() <= 1e-13  # sums of 64 bits near 13
