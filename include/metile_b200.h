@@ -283,8 +283,8 @@ int mt_rope_kv_append_paged(const void* q, long long q_stride, const void* k, lo
                             int page_size, int type, void* stream);
 
 /* mt_attention_decode over pages: out[b] = softmax(scale * q[b] . K) V over the first lengths[b] tokens that row b of the
- * block table names; zeros where that is none.  q, out: dense [batch, q_heads, head_dim], bf16 or fp16; head_dim 64, 128
- * or 256.  A request's bits depend on its own tokens only. */
+ * block table names; zeros where that is none, NaN from a NaN in what is used.  q, out: dense [batch, q_heads, head_dim],
+ * bf16 or fp16; head_dim 64, 128 or 256.  A request's bits depend on its own tokens only. */
 size_t mt_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim, int width, int page_size);
 int mt_paged_attention_decode(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
                               const long long* value_strides, const int* block_tables, long long table_stride, int width,

@@ -148,7 +148,8 @@ def paged_attention_decode(query, key_pages, value_pages, block_tables, lengths,
     """softmax(scale * q k^T) v for one query row per request and head over a cache in pages.
 
     query [requests, Hq, D], D 64, 128 or 256, Hq a multiple of the pages' heads; lengths int32 [requests]: how many tokens of
-    its row of block_tables a request has, the new one among them.  No tokens: a row of zeros.  Returns [requests, Hq, D].
+    its row of block_tables a request has, the new one among them.  No tokens: a row of zeros.  A NaN in what is used comes
+    out as NaN.  Returns [requests, Hq, D].
     A request's bits depend on its own tokens only, not on the others of the call."""
     arguments = (query, key_pages, value_pages, block_tables, lengths)
     out = native().paged_attention_decode(*arguments, scale)

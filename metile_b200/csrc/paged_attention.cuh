@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
                 float weight[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    weight[i] = top[tile][i & 1] == -INFINITY ? 0.0f : power_of_two(score[tile][i] - top[tile][i & 1]);
+                    // Nothing for what is masked.  A NaN moves no maximum and is NaN here, also where that is -inf yet.
+                    weight[i] = score[tile][i] == -INFINITY ? 0.0f : power_of_two(score[tile][i] - top[tile][i & 1]);
                     sum[tile][i & 1] += weight[i];
                 }
 #pragma unroll
