@@ -20,8 +20,8 @@
 //   values  O^T[D x 8 heads] += V^T[D x 16] P^T[16 x 8], V^T by transposing matrix loads; the scores leave the first
 //           product as rows of tokens and enter the second as its columns: movmatrix turns them over.
 // The weights enter as two 16-bit numbers, high and low part: one alone would be off by 2^-9 (bf16).  A running maximum
-// per head is moved, and the sums with it, only when a score passes it by more than 2^8: the weights stay below 256 and
-// keep their relative precision, and a lane adds up its own tokens' weights until the end.
+// per head is moved, and the sums with it, only when a score passes it by more than 2^8: the weights stay below 256 (2^15 in
+// fp16, see kPagedLift) and keep their relative precision, and a lane adds up its own tokens' weights until the end.
 //
 // Measured (8 KV heads of 4 x 128): 100 requests of up to 8191 tokens 337 us, 5.5 TB/s (reading alone 294); two of 100003 143 us,
 // 5.7 TB/s; one of 301 7.3 us.  16 x 2048 tokens, 2 x 6 heads: 12.3 us.  Six warps with four ring slots hold what eight
@@ -39,7 +39,11 @@ constexpr int kPagedMostSplits = 128;    // of a sequence with four KV heads or 
 constexpr int kPagedSlices = 4;          // threads of the join to one number, 128 splits each
 constexpr int kPagedRowPad = 8;          // elements: rows 16 bytes longer keep matrix loads free of conflicts
 constexpr int kPagedTogether = 4;        // splits that one CTA joins: a warp to each of the SM's four schedulers
-constexpr float kPagedHeadroom = 8.0f;   // log2 of what a weight may reach
+constexpr float kPagedHeadroom = 8.0f;   // log2 of how far a score may pass the running maximum
+// log2 of the maximum's own weight.  fp16 has nothing below 2^-24: with 1 for the maximum what is 2^-26 of it would be lost, an
+// eighth of a sum over 2^23 tokens in splits of 65536.  With 2^7, 2^15 at most, the least is 2^-31 of it.
+template <bool kHalf>
+constexpr float kPagedLift = kHalf ? 7.0f : 0.0f;
 
 // Most splits of a sequence: with few KV heads more of them, so that one long sequence has 512 units in any case; those beyond
 // 128 are 16 tokens a query head of the group long at least (2^floor), so that partial results stay an eighth of what is read.
@@ -321,7 +325,7 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     score[tile][i] = there[i >> 1] ? (score[tile][i] + odd[tile][i]) * scale_log2 : -INFINITY;
-                    passes = passes || score[tile][i] > top[tile][i & 1] + kPagedHeadroom;
+                    passes = passes || score[tile][i] > top[tile][i & 1] + (kPagedHeadroom + kPagedLift<kHalf>);
                 }
             if (__any_sync(0xFFFFFFFFu, passes)) {
 #pragma unroll
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(PagedShape<kD>::kWarps * 32, 1) paged_attentio
                         float now = fmaxf(score[tile][j], score[tile][j + 2]);
 #pragma unroll
                         for (int offset = 4; offset <= 16; offset <<= 1) now = fmaxf(now, __shfl_xor_sync(0xFFFFFFFFu, now, offset));
-                        now = fmaxf(now, top[tile][j]);
+                        now = fmaxf(now - kPagedLift<kHalf>, top[tile][j]);
                         const float factor = now == -INFINITY ? 1.0f : power_of_two(top[tile][j] - now);
                         top[tile][j] = now;
                         sum[tile][j] *= factor;

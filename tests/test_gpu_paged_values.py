@@ -1,5 +1,8 @@
-"""Decode attention over pages: values that are not finite."""
+"""Decode attention over pages: values that are not finite, and weights that 16 bits do not reach."""
 
+import math
+
+import numpy as np
 import pytest
 import torch
 
@@ -66,3 +69,24 @@ def test_a_nan_that_is_used_comes_out(cuda_device, length, width, kv_heads, dtyp
         behind = keys.clone()
         behind[length // page, :, length % page:] = torch.nan
         assert torch.equal(B.paged_attention_decode(q, behind, values, table, lengths, scale=0.1), clean)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_many_small_weights_beside_a_large_one(cuda_device, dtype):
+    """Token 0 has a score of 18 above all others; the 2^23 - 1 others, 2^-26 of its weight each and 65536 in a split,
+    make an eighth of the sum.  Two pages serve all blocks of the table."""
+    tokens, page, dim, kv_heads = 1 << 23, 256, 64, 4
+    keys = torch.zeros((2, kv_heads, page, dim), dtype=dtype, device=cuda_device)
+    values = torch.ones_like(keys)
+    keys[0, :, 0, 0], values[0, :, 0] = 18.0, 0.0
+    q = torch.zeros((1, kv_heads, dim), dtype=dtype, device=cuda_device)
+    q[..., 0] = 1.0
+    table = torch.ones((1, tokens // page), dtype=torch.int32, device=cuda_device)
+    table[0, 0] = 0
+    out = B.paged_attention_decode(q, keys, values, table, ints([tokens], cuda_device), scale=1.0).double().cpu().numpy()
+    small = (tokens - 1) * math.exp(-18.0)
+    expected = small / (1.0 + small)
+    # Half a step of the type; 2^-22 for an exponential and 2^-24 * 26 for its argument in the small part; sums of 32 bits,
+    # 4096 chunks a split one after the other and each of two products, at 2^-24 of what is there (twice a truncating sum's).
+    bound = torch.finfo(dtype).eps / 2 + 2.0 ** -22 + 26 * 2.0 ** -24 + 2 * 2 * 4096 * 2.0 ** -24
+    assert float(np.abs(out / expected - 1.0).max()) <= bound
