@@ -10,7 +10,7 @@ from .cuda import (  # noqa: F401
     rope_kv_prefill,
     supports_attention_decode,
 )
-from .cuda_beam import beam_reorder, beam_select  # noqa: F401
+from .cuda_beam import MAX_BEAMS, beam_reorder, beam_select  # noqa: F401
 from .cuda_affine import MLXAffineWeight, mlx_affine_matmul  # noqa: F401
 from .cuda_dense import (  # noqa: F401
     mlx_dense_residual_qmv,

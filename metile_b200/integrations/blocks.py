@@ -262,6 +262,10 @@ class PagedTables:
         groups = self.requests // max(1, beams)
         if groups * beams != self.requests or any(self.held[r] and r % beams for r in range(self.requests)):
             raise ValueError("only the first request of each group may have tokens")
+        if beams > backends.MAX_BEAMS:
+            raise ValueError(f"a group has up to {backends.MAX_BEAMS} beams")
+        if not caches or any(getattr(cache, "tables", None) is not self for cache in caches):
+            raise ValueError("fork expects the PagedKVCache of every layer, over these tables")
         held = [self.held[r - r % beams] for r in range(self.requests)]
         # The others hold the full pages in name, which cost none, and a page of their own for the rest.
         whole = [n // self.page_size * self.page_size for n in held]
