@@ -209,6 +209,7 @@ class PagedTables:
         self.free_state = torch.tensor([0, self.pages], dtype=torch.int32, device=device)
         self._ones = torch.ones((self.requests,), dtype=torch.int32, device=device)
         self.held, self.free = [0] * self.requests, self.pages
+        self.shared = [0] * self.requests    # tokens of every request in pages that others may have too
         self.slots = self.positions = None   # of the tokens of the pass
         self.prompts = None                  # [(request, first row, rows)], or None: one token of every request
 
@@ -223,6 +224,7 @@ class PagedTables:
         torch.arange(self.pages, dtype=torch.int32, device=self.free_pages.device, out=self.free_pages)
         self.free_state.copy_(torch.tensor([0, self.pages], dtype=torch.int32))
         self.held, self.free = [0] * self.requests, self.pages
+        self.shared = [0] * self.requests
 
     def account(self, counts):
         """The host's side of a change by counts[r] tokens; refuses what does not fit."""
@@ -232,6 +234,8 @@ class PagedTables:
         after = [held + count for held, count in zip(self.held, counts)]
         if len(counts) != self.requests or min(after) < 0 or max(after) > self.capacity:
             raise ValueError("paged cache: a request has no room, or fewer tokens than are taken back")
+        if any(count < 0 and new < shared for count, new, shared in zip(counts, after, self.shared)):
+            raise ValueError("paged cache: pages that requests share are given back by reset alone")
         changes = [blocks(new) - blocks(old) for new, old in zip(after, self.held)]
         if sum(max(0, change) for change in changes) > self.free:
             raise ValueError("paged cache: out of pages")
@@ -240,7 +244,8 @@ class PagedTables:
     def grow(self, counts=None):
         """One new token for every request, or counts[r] for request r; negative counts give back the last tokens.
 
-        Pages that requests share (after `fork`, or beams) are given back by `reset` alone: a page must not go back twice."""
+        Tokens in pages that requests share (those full at the last `fork` or `reorder`) are given back by `reset` alone: a
+        page must not go back twice, nor be written by one request under another."""
         ones = counts is None
         counts = [1] * self.requests if ones else [int(count) for count in counts]
         self.account(counts)
@@ -255,6 +260,10 @@ class PagedTables:
         self.slots, self.positions, _, _, _ = backends.paged_resize(
             self.block_tables, self.lengths, on_device, self.free_pages, self.free_state, page_size=self.page_size,
             tokens=self.requests if ones else first, advance=True)
+
+    def share(self):
+        """From now on requests may share the pages that are full, as a reordering leaves them."""
+        self.shared = [max(shared, held // self.page_size * self.page_size) for shared, held in zip(self.shared, self.held)]
 
     def fork(self, beams, caches):
         """Every first request of `beams` in a row is continued by all of them: full pages are shared, what is begun is copied
@@ -281,6 +290,8 @@ class PagedTables:
         """The requests of every group of beams continue those that `parents` [groups, beams] (int32) names."""
         self.block_tables.copy_(backends.beam_reorder(self.block_tables, self.lengths, parents,
                                                       [(cache.keys, cache.values) for cache in caches]))
+        if parents.shape[1] > 1:
+            self.share()
 
 
 class PagedKVCache:

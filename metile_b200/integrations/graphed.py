@@ -209,6 +209,8 @@ class GraphedBeamDecoder:
         if self.graph is None:
             self._capture()
         self.tables.account([1] * self.tables.requests)   # what the graph does on the device
+        if self.beams > 1:
+            self.tables.share()
         caller = torch.cuda.current_stream(self.device)
         self.stream.wait_stream(caller)
         with torch.cuda.stream(self.stream):

@@ -57,3 +57,34 @@ def test_a_fork_that_is_refused_changes_nothing(oracle_backends):
     tables.grow([13, 0, 0, 8, 0, 0])
     tables.fork(3, caches)
     assert tables.held == tables.lengths.tolist() == [13, 13, 13, 8, 8, 8] and tables.free == int(tables.free_state[1]) == 24 - 2 - 1 - 2
+
+
+def test_tokens_in_shared_pages_are_not_taken_back(oracle_backends):
+    """After a fork or a reordering two requests name one page: given back by both it would be handed out twice, and
+    reopened by one it would be written under the other."""
+    tables, caches = cache_of(3)
+    tables.grow([13, 0, 0])
+    tables.fork(3, caches)
+    tables.grow()
+    for counts in ([-14, -14, -14], [0, -7, 0], [-6, -6, -7]):
+        before = state_of(tables)
+        with pytest.raises(ValueError, match="share"):
+            tables.grow(counts)
+        assert state_of(tables) == before
+    tables.grow([-6, -2, 0])  # back to the full page, and within the page in work, which is a request's own
+    assert tables.held == tables.lengths.tolist() == [8, 12, 14]
+    tables.grow([1, 4, 2])
+    table, held = tables.block_tables.numpy(), tables.held
+    own = [int(table[r, j]) for r in range(3) for j in range(1, -(-held[r] // 8))]
+    free = [int(tables.free_pages[(int(tables.free_state[0]) + i) % tables.pages]) for i in range(tables.free)]
+    assert len(set(own)) == len(own) and not set(own) & set(free) and len(set(free)) == len(free) and table[0, 0] not in free
+    tables.grow([7, 0, 0])
+    tables.reorder(torch.tensor([[0, 0, 1]], dtype=torch.int32), caches)
+    assert tables.shared == [16, 16, 16]
+    with pytest.raises(ValueError, match="share"):
+        tables.grow([0, -1, 0])
+    tables.reset()
+    tables.grow([9, 8, 1])
+    tables.reorder(torch.zeros((3, 1), dtype=torch.int32), caches)  # one beam each shares nothing
+    tables.grow([-9, -8, -1])
+    assert tables.free == 24 and np.array_equal(sorted(tables.free_pages.tolist()), range(24))
