@@ -569,27 +569,32 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
         // 128 shares at a time: a lane's four of them are asked for together.  The row's maximum first, so that every share is
         // weighted once; what does not fit the first 128 is read twice.
         BeamShareStats own[4];
-        float best = -INFINITY;
         auto take = [&](int first) {
+            float most = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int i = first + 32 * k + lane;
                 own[k] = i < shares ? stats[i] : BeamShareStats{-INFINITY, 0.0f};
+                most = fmaxf(most, own[k].top);
             }
+            return most;
         };
-        for (int first = (shares - 1) / 128 * 128; first >= 0; first -= 128) {
-            take(first);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) best = fmaxf(best, own[k].top);
-        }
+        float best = -INFINITY;
+#pragma unroll 1
+        for (int first = 128; first < shares; first += 128) best = fmaxf(best, take(first));
+        best = fmaxf(best, take(0));
         asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(best) : "f"(best));
-        double sum = 0.0;
-        for (int first = 0; first < shares; first += 128) {
-            if (first > 0) take(first);
+        auto weighted = [&] {
             float part = 0.0f;  // of the same error as within a share
 #pragma unroll
             for (int k = 0; k < 4; ++k) part += own[k].sum == 0.0f ? 0.0f : own[k].sum * __expf(own[k].top - best);
-            sum += (double)part;
+            return (double)part;
+        };
+        double sum = weighted();
+#pragma unroll 1
+        for (int first = 128; first < shares; first += 128) {
+            take(first);
+            sum += weighted();
         }
 #pragma unroll
         for (int offset = 16; offset >= 1; offset >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);
