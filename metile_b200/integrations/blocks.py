@@ -226,8 +226,8 @@ class PagedTables:
         self.held, self.free = [0] * self.requests, self.pages
         self.shared = [0] * self.requests
 
-    def account(self, counts):
-        """The host's side of a change by counts[r] tokens; refuses what does not fit."""
+    def fits(self, counts):
+        """The host's side of a change by counts[r] tokens: (held, free) after it; refuses what does not fit."""
         def blocks(tokens):
             return -(-tokens // self.page_size)
 
@@ -239,7 +239,11 @@ class PagedTables:
         changes = [blocks(new) - blocks(old) for new, old in zip(after, self.held)]
         if sum(max(0, change) for change in changes) > self.free:
             raise ValueError("paged cache: out of pages")
-        self.held, self.free = after, self.free - sum(changes)
+        return after, self.free - sum(changes)
+
+    def account(self, counts):
+        """Make the change on the host's side."""
+        self.held, self.free = self.fits(counts)
 
     def grow(self, counts=None):
         """One new token for every request, or counts[r] for request r; negative counts give back the last tokens.

@@ -137,6 +137,8 @@ class GraphedBeamDecoder:
 
     def __init__(self, model, batch=1, beams=4, capacity=4096, page_size=16, pages=None, end_token=None):
         self.model, self.batch, self.beams, self.end_token = model, int(batch), int(beams), end_token
+        if not 1 <= self.beams <= backends.MAX_BEAMS:
+            raise ValueError(f"a search has from 1 to {backends.MAX_BEAMS} beams")
         rows, width = self.batch * self.beams, -(-capacity // page_size)
         self.cache = model.make_paged_cache(rows, rows * width if pages is None else pages, page_size, capacity)
         self.tables = self.cache[0].tables
@@ -184,31 +186,39 @@ class GraphedBeamDecoder:
             self._select(torch.cat(logits).repeat_interleave(self.beams, dim=0), start, self.finished)
 
     def _capture(self):
-        """Warm what is built lazily on a scratch cache, then capture one step on the real one."""
-        kept = [t.clone() for t in (self.token, self.scores, self.parents, self.finished)]
-        self.stream.wait_stream(torch.cuda.current_stream(self.device))
-        with torch.no_grad(), torch.cuda.stream(self.stream):
-            real, tables = self.cache, self.tables
-            self.cache = self.model.make_paged_cache(tables.requests, tables.requests, tables.page_size, tables.page_size)
-            self.tables = self.cache[0].tables
-            self._step()
-            self.cache, self.tables = real, tables
-            for own, value in zip((self.token, self.scores, self.parents, self.finished), kept):
-                own.copy_(value)
-            held, free = list(tables.held), tables.free
-            self.stream.synchronize()
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph, stream=self.stream):
-                self._step()
-            tables.held, tables.free = held, free     # capture ran the host's bookkeeping once
-        torch.cuda.current_stream(self.device).wait_stream(self.stream)
+        """Warm what is built lazily on a scratch cache, then capture one step on the real one.  What fails on the way leaves
+        the decoder as it was."""
+        real, tables = self.cache, self.tables
+        state = (self.token, self.scores, self.parents, self.finished)
+        kept, counts = [t.clone() for t in state], (list(tables.held), tables.free, list(tables.shared))
+        caller = torch.cuda.current_stream(self.device)
+        self.stream.wait_stream(caller)
+        graph = torch.cuda.CUDAGraph()
+        try:
+            with torch.no_grad(), torch.cuda.stream(self.stream):
+                self.cache = self.model.make_paged_cache(tables.requests, tables.requests, tables.page_size, tables.page_size)
+                self.tables = self.cache[0].tables
+                try:
+                    self._step()
+                finally:
+                    self.cache, self.tables = real, tables
+                    for own, value in zip(state, kept):
+                        own.copy_(value)
+                    self.stream.synchronize()
+                with torch.cuda.graph(graph, stream=self.stream):
+                    self._step()
+        finally:
+            tables.held, tables.free, tables.shared = counts     # capture runs the host's bookkeeping once
+            caller.wait_stream(self.stream)
         self.graph = graph
 
     def step(self):
         """One token for every beam; the decoder's token, scores, parents and finished are those of the new beams."""
+        ones = [1] * self.tables.requests
+        self.tables.fits(ones)
         if self.graph is None:
             self._capture()
-        self.tables.account([1] * self.tables.requests)   # what the graph does on the device
+        self.tables.account(ones)   # what the graph does on the device
         if self.beams > 1:
             self.tables.share()
         caller = torch.cuda.current_stream(self.device)
