@@ -196,7 +196,8 @@ class GraphedBeamDecoder:
         graph = torch.cuda.CUDAGraph()
         try:
             with torch.no_grad(), torch.cuda.stream(self.stream):
-                self.cache = self.model.make_paged_cache(tables.requests, tables.requests, tables.page_size, tables.page_size)
+                # A page for each request, and tables as wide as the real ones: their width decides what is launched.
+                self.cache = self.model.make_paged_cache(tables.requests, tables.requests, tables.page_size, tables.capacity)
                 self.tables = self.cache[0].tables
                 try:
                     self._step()
