@@ -718,12 +718,12 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             }
             if (threadIdx.x < 32) tally[threadIdx.x] = 0;
             __syncthreads();
-            // Only the margin can let in more than `most`.
-            found = count;
-            if (!again || found <= kBeamMany || (found > most && !wider)) break;
+            found = min(count, wider ? count : most);  // only the margin can let in more than `most`
+            const bool full = found > most;            // without it then, and what lies within it is looked at below
+            if (!full && (!again || found <= kBeamMany)) break;
             __syncthreads();
             if (threadIdx.x == 0) count = 0;
-            if (found > most) {  // without the margin, for the bound below; what lies within it has to be looked at all the same
+            if (full) {
                 wider = false;
                 dropped = true;
                 __syncthreads();
@@ -755,60 +755,31 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const BeamSelectParams 
             dropped = dropped && !wider;
             __syncthreads();
         }
-        if (found > most || dropped) {
-            // More within the margin than can be ranked.  The lists are sorted: a thread each has the first one left of a list, and
-            // the best of those is taken `keep` times.  The beams that reach the margin below the last one are those a ranking of
-            // all would find there, so a group's bits do not depend on how its rows were cut.
-            BeamCandidate* heads = reinterpret_cast<BeamCandidate*>(keys);  // [2][32]
-            const bool has = threadIdx.x < lists;
-            const int beam = has ? beam_divided(threadIdx.x, p.per_parts) : 0;
-            auto better = [](BeamCandidate own) {  // the warp's best
-#pragma unroll
-                for (int offset = 16; offset >= 1; offset >>= 1) {
-                    const BeamCandidate other = {__shfl_xor_sync(0xFFFFFFFFu, own.value, offset), __shfl_xor_sync(0xFFFFFFFFu, own.place, offset)};
-                    if (other.place >= 0 && (own.place < 0 || beam_before(other, own))) own = other;
-                }
-                return own;
-            };
-            int depth = 0;
-            BeamCandidate own = {nothing, -1}, best = own;
-            if (has) own = candidate(threadIdx.x, beam, 0);
-            for (int r = 0; r < p.keep; ++r) {
-                best = better(own);
-                if (lane == 0) heads[(r & 1) * 32 + warp] = best;
-                __syncthreads();
-                best = {nothing, -1};
-                if (lane < warps) best = heads[(r & 1) * 32 + lane];
-                best = better(best);
-                if (has && own.place == best.place) {
-                    own = {nothing, -1};
-                    if (++depth < p.keep) own = candidate(threadIdx.x, beam, depth);
-                }
-                if (threadIdx.x == 0) {
-                    collected[r] = best;
-                    order[r] = r;
-                }
-            }
-            if (own.place >= 0 && own.value > nothing && beam_value(best.value) - beam_value(own.value) <= margin)
-                atomicOr(&reached, 1u << beam | 1u << (int)(best.place >> kBeamPlaceShift));
-            __syncthreads();
-            if (threadIdx.x == 0 && __popc(reached) > 1) close = reached;
-            found = p.keep;
-            __syncthreads();
-        } else {
-            for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += blockDim.x >> 3) {
-                const int rank = beam_rank(collected, found, collected[min(i, found - 1)]);
-                if (i < found && (lane & 7) == 0) order[rank] = i;
-            }
-            __syncthreads();
+        for (int i = threadIdx.x >> 3; i < (found + 3) / 4 * 4; i += blockDim.x >> 3) {
+            const int rank = beam_rank(collected, found, collected[min(i, found - 1)]);
+            if (i < found && (lane & 7) == 0) order[rank] = i;
         }
+        __syncthreads();
         if (margin > 0.0) {
-            const double last = beam_value(collected[order[p.keep - 1]].value);  // nobody further below it than the margin can rise
+            const BeamCandidate last = collected[order[p.keep - 1]];  // nobody further below it than the margin can rise
             for (int i = threadIdx.x; i + 1 < found; i += blockDim.x) {
                 const BeamCandidate upper = collected[order[i]], lower = collected[order[i + 1]];
-                if (i + 1 >= p.keep && last - beam_value(lower.value) > margin) break;
+                if (i + 1 >= p.keep && beam_value(last.value) - beam_value(lower.value) > margin) break;
                 const int a = (int)(upper.place >> kBeamPlaceShift), b = (int)(lower.place >> kBeamPlaceShift);
                 if (a != b && lower.value > nothing && beam_value(upper.value) - beam_value(lower.value) <= margin) atomicOr(&close, 1u << a | 1u << b);
+            }
+            if (dropped) {
+                // What was too many to collect and rank: all beams with a candidate from the last one down to the margin below it, if
+                // those are two or more.  A ranking of all finds the same beams, so a group's bits do not depend on how many there
+                // were, which follows the cut of the rows.
+                for (int i = threadIdx.x; i < lists * p.keep; i += blockDim.x) {
+                    const int list = beam_divided(i, p.per_keep), beam = beam_divided(list, p.per_parts);
+                    const BeamCandidate own = candidate(list, beam, i - list * p.keep);
+                    if (own.place >= 0 && own.value > nothing && !beam_before(own, last) && beam_value(last.value) - beam_value(own.value) <= margin)
+                        atomicOr(&reached, 1u << beam);
+                }
+                __syncthreads();
+                if (threadIdx.x == 0 && __popc(reached) > 1) close |= reached;
             }
             __syncthreads();
             if (close) {
