@@ -24,7 +24,8 @@ def beam_select(logits, scores, *, keep=None, finished=None, end_token=None):
     logits with a NaN, with +inf or with nothing above -inf.
 
     Returns (scores float32, parents int32 -- the beam within its group --, tokens int64, finished bool), all
-    [groups, keep].  finished: the parent had finished or the token is end_token."""
+    [groups, keep].  finished: the parent had finished or the token is end_token.  A score is rounded to 32 bits, and may be off
+    by 2^-18 before that; where two beams are closer than that allows, their order is the one of sums in 64 bits."""
     kept = scores.shape[1] if keep is None and isinstance(scores, torch.Tensor) and scores.ndim == 2 else keep
     end = -1 if end_token is None else -2 if end_token == -1 else end_token
     out = None

@@ -150,7 +150,9 @@ def paged_attention_decode(query, key_pages, value_pages, block_tables, lengths,
     query [requests, Hq, D], D 64, 128 or 256, Hq a multiple of the pages' heads; lengths int32 [requests]: how many tokens of
     its row of block_tables a request has, the new one among them.  No tokens: a row of zeros.  A NaN in what is used comes
     out as NaN.  Returns [requests, Hq, D].
-    A request's bits depend on its own tokens only, not on the others of the call."""
+    A request's bits depend on its own tokens only, not on the others of the call.  The scratch of a call follows the
+    width of block_tables, not the lengths: requests * Hq * min(width * page_size / 128, 128) * (D + 2) numbers of 32 bits, up to
+    four times as many splits with fewer than four KV heads."""
     arguments = (query, key_pages, value_pages, block_tables, lengths)
     out = native().paged_attention_decode(*arguments, scale)
     if out is None:

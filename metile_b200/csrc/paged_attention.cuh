@@ -23,8 +23,8 @@
 // per head is moved, and the sums with it, only when a score passes it by more than 2^8: the weights stay below 256 (2^15 in
 // fp16, see kPagedLift) and keep their relative precision, and a lane adds up its own tokens' weights until the end.
 //
-// Measured (8 KV heads of 4 x 128): 100 requests of up to 8191 tokens 337 us, 5.5 TB/s (reading alone 294); two of 100003 143 us,
-// 5.7 TB/s; one of 301 7.3 us.  16 x 2048 tokens, 2 x 6 heads: 12.3 us.  Six warps with four ring slots hold what eight
+// Measured (8 KV heads of 4 x 128): 100 requests of up to 8191 tokens 337 to 349 us, 5.4 TB/s (reading alone 294); two of 100003
+// 143 to 147 us, 5.6 TB/s; one of 301 7.3 us.  16 x 2048 tokens, 2 x 6 heads: 12.4 us.  Six warps with four ring slots hold what eight
 // with three or four with six do (143 us against 154 and 157 for the long ones); without the arithmetic the large cases take the same.
 #pragma once
 
@@ -48,7 +48,7 @@ constexpr float kPagedLift = kHalf ? 7.0f : 0.0f;
 // Most splits of a sequence: with few KV heads more of them, so that one long sequence has 512 units in any case; those beyond
 // 128 are 16 tokens a query head of the group long at least (2^floor), so that partial results stay an eighth of what is read.
 // One request with 1 KV head: 131072 tokens for 8 heads of 128 26 us (40 with 128 splits), 100000 for one of 64 15 (33); a
-// batch of 16 with 2 x 4 heads and 32768 tokens 108 us (101).
+// batch of 16 with 2 x 4 heads and 32768 tokens 110 us (101): it has units enough by itself, but the cut does not know the batch.
 __host__ __device__ constexpr int paged_split_limit(int kv_heads) { return kv_heads >= 4 ? kPagedMostSplits : kv_heads >= 2 ? 2 * kPagedMostSplits : 4 * kPagedMostSplits; }
 static_assert(paged_split_limit(1) <= kPagedSlices * kPagedMostSplits, "the join takes 128 splits a slice");
 __host__ __device__ constexpr int paged_split_floor(int group) {

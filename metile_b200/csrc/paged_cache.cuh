@@ -96,8 +96,9 @@ __device__ __forceinline__ int last_not_above(const long long* starts, int n, lo
 // sums and share what follows.  Where lengths and state are written in place the CTAs are one cluster, and the first of them
 // writes behind a barrier.  What a decode step needs, a token and at most a page for each, the requests' own threads do at once.  64
 // requests of a token each 3.2 us in a graph (5.0 with the search); 501 with 116 thousand tokens 11.0 us (one CTA 132).
+// In place a cluster of eight CTAs does those 116 thousand tokens in 23 us in a graph, the separate form in 9.
 // The grid follows the tokens, which the host knows, not the pages given back: 239 requests that end at once with 68 thousand
-// pages and one token 45 us (42 with four pages of a thread together, which cost the others half a microsecond).
+// pages 160 us beside a map of up to 1024 tokens (256 threads), 63 by 1024 threads, 35 by two CTAs of them.
 __global__ void __launch_bounds__(kResizeThreads) paged_resize_kernel(const ResizeParams p, bool in_place) {
     __shared__ long long token_start[kResizeThreads], grant_start[kResizeThreads], free_start[kResizeThreads];
     __shared__ int held[kResizeThreads], added[kResizeThreads];

@@ -129,6 +129,9 @@ class GraphedBeamDecoder:
     The beams of a request share the pages of its prompt and of every page that was full when they parted, so a step
     copies at most the page in work of the beams that were dropped, whatever the length.  A step takes its pages, runs the
     model, selects and reorders on the device.  With one beam it is greedy decoding of requests of different lengths.
+    Pages are not counted by who refers to them: every beam takes a page whenever it fills one, and those of dropped beams
+    come back with the next prompts, so a pool of batch * beams * ceil(capacity / page_size) pages (the default) never runs out
+    and a smaller one may.  A search takes all its steps, also when every beam has finished.
 
         decoder = GraphedBeamDecoder(model, batch=2, beams=4, capacity=4096)
         tokens, scores = decoder.search([first_prompt, second_prompt], steps=64)
