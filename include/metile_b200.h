@@ -255,7 +255,7 @@ int mt_rope_kv_prefill(const void* q, const void* k, const void* v, const float*
  * elements apart) names the pages of request r in order: its token t is in slot
  * block_tables[r][t / page_size] * page_size + t % page_size.  No counterpart in the reference.  What a kernel finds outside
  * its table it leaves out and records (mt_device_status, -9): a slot (0x302), a page (0x303), a length the table has no room
- * for (0x304), a parent outside its group (0x305). */
+ * for (0x304), a parent outside its group (0x305), rows of a request outside the query (0x306). */
 #define MT_TYPE_BF16 0
 #define MT_TYPE_FP16 1
 #define MT_TYPE_FP32 2
@@ -290,6 +290,66 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
                               const long long* value_strides, const int* block_tables, long long table_stride, int width,
                               const int* lengths, void* out, void* workspace, size_t workspace_bytes, int batch, int q_heads,
                               int kv_heads, int head_dim, int pages, int page_size, int type, float scale, void* stream);
+
+/* Several new tokens per request: rows starts[r] ... starts[r + 1] - 1 of q (int32 [requests + 1], ascending, as mt_paged_resize
+ * leaves them) are the last tokens of request r, lengths[r] with them; the i-th of n stands at position lengths[r] - n + i
+ * and out = softmax(scale * q . K) V over the tokens up to its own.  Zeros where that is none and in rows no request has.
+ * What a row does not see weighs nothing, whatever lies there; a NaN that it sees gives NaN.  q, out: dense [rows, q_heads,
+ * head_dim], bf16 or fp16; head_dim 64, 128 or 256.  flags: with MT_FLAG_FIXED_ORDER or MT_FLAG_FORCE_UMMA a row's bits
+ * depend on its own tokens only, with 0 also on the sizes of the call (rows, requests, heads, width). */
+size_t mt_paged_attention_chunk_workspace_bytes(int rows, int requests, int q_heads, int kv_heads, int head_dim, int width,
+                                                int page_size, unsigned int flags);
+int mt_paged_attention_chunk(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
+                             const long long* value_strides, const int* block_tables, long long table_stride, int width,
+                             const int* lengths, const int* starts, void* out, void* workspace, size_t workspace_bytes,
+                             int rows, int requests, int q_heads, int kv_heads, int head_dim, int pages, int page_size,
+                             int type, float scale, unsigned int flags, void* stream);
+
+/* Pages that several requests hold.  shares int32 [pages]: how many requests hold a page beyond the first one (0 for
+ * a free page); mt_paged_resize knows nothing of it, so it must not give back pages that are shared.
+ *
+ * fork: request r, if sources[r] >= 0 and it has no tokens, becomes the first counts[r] > 0 tokens of request sources[r]: the
+ * full pages' ids go to its row of block_tables and their shares grow, the page begun is copied into one from the head of the
+ * ring, in `caches` caches (HOST arrays of addresses, two-byte elements, head_dim a multiple of 8).  Requests whose source,
+ * count or length makes no sense, or for which and all before them the free pages do not reach, stay as they are.
+ * lengths_out, free_state_out and shares_out may be lengths, free_state and shares. */
+size_t mt_paged_fork_workspace_bytes(int requests);
+int mt_paged_fork(int* block_tables, long long table_stride, int width, const int* lengths, const int* sources,
+                  const int* counts, const int* free_pages, int pool, const int* free_state, const int* shares,
+                  void* const* key_pages, const long long* key_strides, void* const* value_pages,
+                  const long long* value_strides, int caches, int* lengths_out, int* free_state_out, int* shares_out,
+                  void* workspace, size_t workspace_bytes, int requests, int kv_heads, int head_dim, int pages, int page_size,
+                  void* stream);
+
+/* free: every request with ended[r] (bytes) drops its pages and has no tokens any more.  A page goes to the ring's tail when
+ * all who hold it have dropped it, in the order of requests and blocks (a page that several drop: at the first). */
+size_t mt_paged_free_workspace_bytes(int pages);
+int mt_paged_free(const int* block_tables, long long table_stride, int width, const int* lengths, const unsigned char* ended,
+                  int* free_pages, int pool, const int* free_state, const int* shares, int* lengths_out, int* free_state_out,
+                  int* shares_out, void* workspace, size_t workspace_bytes, int requests, int pages, int page_size,
+                  void* stream);
+
+/* compact: the pages that the block tables hold move, in all caches, to the ids below their number: the n-th of those above
+ * (ascending) to the n-th of the free ones below.  tables_out (dense, another array) names the new places; free_pages int32
+ * [pages] and free_state become a ring of the others, ascending, shares what the tables say. */
+size_t mt_paged_compact_workspace_bytes(int pages);
+int mt_paged_compact(const int* block_tables, long long table_stride, int width, const int* lengths, int* tables_out,
+                     int* free_pages, int* free_state, int* shares, void* const* key_pages, const long long* key_strides,
+                     void* const* value_pages, const long long* value_strides, int caches, void* workspace,
+                     size_t workspace_bytes, int requests, int kv_heads, int head_dim, int pages, int page_size, void* stream);
+
+/* Log-probabilities of given tokens: logits [rows, vocabulary] bf16, fp16 or fp32, rows `row_stride` elements apart.
+ * logprobs[r] = log softmax(logits[r])[tokens[r]]; a token below 0 asks for nothing (0), one outside the vocabulary gives NaN and
+ * is recorded (0x307).  entropy[r] of the row's distribution; the `top` (0 ... 64) largest logits, among equals the lower
+ * token first: top_logprobs and top_tokens [rows, top].  A row with a NaN, with +inf or with nothing above -inf has no
+ * distribution: NaN, and -1 for its tokens.  The aligned 16 bytes around the first and the last logit of a row must be
+ * readable (any allocation's granularity sees to that); what lies there beside the row is never used. */
+#define MT_LOGPROB_MAX_ROWS 0x000FFFFF
+#define MT_LOGPROB_MAX_VOCABULARY 0x00080000
+size_t mt_token_logprobs_workspace_bytes(int rows, int vocabulary, int top, int type);
+int mt_token_logprobs(const void* logits, long long row_stride, int type, const long long* tokens, float* logprobs,
+                      float* entropy, float* top_logprobs, long long* top_tokens, void* workspace, size_t workspace_bytes,
+                      int rows, int vocabulary, int top, void* stream);
 
 /* A step of beam search.  Of the beams * vocabulary candidates of a group, score + log softmax(logits) in 64 bits, the `keep`
  * (1 ... 64) largest in descending order; among equals the lower beam first, then the larger logit, then the lower token.

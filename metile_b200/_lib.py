@@ -61,6 +61,16 @@ SIGNATURES = {
     "mt_beam_select_workspace_bytes": (_z, [_i] * 5),
     "mt_beam_select": (_i, [_p, _l, _i, _p, _p, _l, _p, _p, _p, _p, _p, _z, _i, _i, _i, _i, _p]),
     "mt_beam_reorder": (_i, [_p, _l, _i] + [_p] * 7 + [_i] * 7 + [_p]),
+    "mt_paged_attention_chunk_workspace_bytes": (_z, [_i] * 7 + [_u]),
+    "mt_paged_attention_chunk": (_i, [_p] * 6 + [_l, _i, _p, _p, _p, _p, _z] + [_i] * 8 + [_f, _u, _p]),
+    "mt_paged_fork_workspace_bytes": (_z, [_i]),
+    "mt_paged_fork": (_i, [_p, _l, _i] + [_p] * 4 + [_i] + [_p] * 6 + [_i] + [_p] * 4 + [_z] + [_i] * 5 + [_p]),
+    "mt_paged_free_workspace_bytes": (_z, [_i]),
+    "mt_paged_free": (_i, [_p, _l, _i, _p, _p, _p, _i] + [_p] * 6 + [_z] + [_i] * 3 + [_p]),
+    "mt_paged_compact_workspace_bytes": (_z, [_i]),
+    "mt_paged_compact": (_i, [_p, _l, _i] + [_p] * 9 + [_i, _p, _z] + [_i] * 5 + [_p]),
+    "mt_token_logprobs_workspace_bytes": (_z, [_i] * 4),
+    "mt_token_logprobs": (_i, [_p, _l, _i] + [_p] * 6 + [_z] + [_i] * 3 + [_p]),
     "mt_peer_group_create": (_i, [_i, _i, _z, ctypes.POINTER(ctypes.c_void_p), _p]),
     "mt_peer_group_connect": (_i, [_p, _p]),
     "mt_peer_group_set_mode": (_i, [_p, _i]),
@@ -123,9 +133,10 @@ def check(code, what):
 
 
 def device_status(reset=True):
-    """(ok, words) -- words[0] != 0 means a bounded device-side wait gave up, or (0x301 ... 0x305) that a kernel met an
+    """(ok, words) -- words[0] != 0 means a bounded device-side wait gave up, or (0x301 ... 0x307) that a kernel met an
     index outside its table: words[1] is the row, words[2] the index (0x301 an embedding's token, 0x302 a slot outside the
-    paged cache, 0x303 a page outside it, 0x304 a length its block table has no room for, 0x305 a beam's parent)."""
+    paged cache, 0x303 a page outside it, 0x304 a length its block table has no room for, 0x305 a beam's parent, 0x306 the first
+    row of a request whose rows lie outside the query, 0x307 a token whose log-probability is asked for)."""
     words = (ctypes.c_uint * 4)()
     code = load().mt_device_status(words, 1 if reset else 0)
     return code == 0, tuple(int(v) for v in words)

@@ -16,7 +16,14 @@ from .cuda_dense import (  # noqa: F401
     mlx_dense_residual_qmv,
     mlx_dense_swiglu,
 )
-from .cuda_paged import PAGE_SIZES, paged_attention_decode, paged_resize, rope_kv_append_paged  # noqa: F401
+from .cuda_logprobs import token_logprobs  # noqa: F401
+from .cuda_paged import (  # noqa: F401
+    PAGE_SIZES,
+    paged_attention_chunk,
+    paged_attention_decode,
+    paged_resize,
+    rope_kv_append_paged,
+)
 from .cuda_quantized import (  # noqa: F401
     batch_invariant,
     fixed_order,
@@ -33,3 +40,4 @@ from .cuda_quantized import (  # noqa: F401
     mlx_affine_swiglu_qmv,
     repack_mlx_affine_weight,
 )
+from .cuda_sharing import paged_compact, paged_fork, paged_free  # noqa: F401

@@ -1,4 +1,5 @@
-"""A key-value cache in pages on CUDA: block tables and slot maps, rotary embedding + append, decode attention.
+"""A key-value cache in pages on CUDA: block tables and slot maps, rotary embedding + append, attention of one new token per
+request and of several.
 
 The reference keeps one contiguous cache per sequence (metile/integrations/mlx_lm.py takes MLX-LM's) and has no
 counterpart.  Pages are [pages, kv_heads, page_size, head_dim] tensors of bfloat16 or float16, any strides with a dense
@@ -11,9 +12,12 @@ An index outside its table is left out by the kernel that meets it and recorded:
 
 from __future__ import annotations
 
+import numbers
+
 import torch
 
 from ._common import native, native_result, require_on_device
+from .cuda_quantized import _flags
 
 PAGE_SIZES = (8, 16, 32, 64, 128, 256)
 PAGE_DTYPES = (torch.bfloat16, torch.float16)
@@ -38,7 +42,7 @@ def _require_ints(tensor, like, what, count, dtype=torch.int32):
 
 def _require_table(table, what="block_tables"):
     _require_cuda(table, what, (torch.int32,), 2)
-    if table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1) or (
+    if table.shape[1] < 1 or (table.numel() and table.shape[1] > 1 and table.stride(1) != 1) or (
             table.shape[0] > 1 and table.stride(0) < table.shape[1]):
         raise ValueError(f"{what} must be rows of one block or more, dense and apart")
 
@@ -175,3 +179,41 @@ def paged_attention_decode(query, key_pages, value_pages, block_tables, lengths,
         if out is None:
             raise ValueError("paged_attention_decode: sizes beyond what the kernel takes")
     return native_result(out, "paged_attention_decode")
+
+
+def paged_attention_chunk(query, key_pages, value_pages, block_tables, lengths, starts, *, scale):
+    """softmax(scale * q k^T) v for several new tokens per request over a cache in pages, each seeing the tokens up to its own.
+
+    query [rows, Hq, D], D 64, 128 or 256, Hq a multiple of the pages' heads; lengths int32 [requests]: how many tokens of its row
+    of block_tables a request has, the new ones among them; starts int32 [requests + 1], ascending: rows starts[r] up to
+    starts[r + 1] are the last tokens of request r (as paged_resize returns it).  A piece of a prompt, a draft and a single token
+    may stand beside each other.  Rows that see nothing (more rows than tokens) and rows of no request are zeros.  What a row
+    does not see weighs nothing, whatever lies there; a NaN that it sees comes out as NaN.  Returns [rows, Hq, D].
+    Within batch_invariant() or fixed_order() a row's bits depend on the tokens it sees only, not on the others of the call nor on
+    how its prompt was cut into pieces; elsewhere long requests with few rows are cut as the sizes of the call ask."""
+    arguments = (query, key_pages, value_pages, block_tables, lengths, starts)
+    out = native().paged_attention_chunk(*arguments, scale, _flags())
+    if out is None:
+        _require_cuda(query, "query", PAGE_DTYPES, 3)
+        _require_pages(key_pages, value_pages, query)
+        _refuse_gradient("paged_attention_chunk", query, key_pages, value_pages)
+        _require_table(block_tables)
+        rows, heads, dim = query.shape
+        requests = block_tables.shape[0]
+        if block_tables.device != query.device:
+            raise ValueError("paged_attention_chunk expects block_tables on the queries' device")
+        if key_pages.shape[3] != dim or dim not in (64, 128, 256):
+            raise ValueError("paged_attention_chunk: the head dimension must be 64, 128 or 256 and match")
+        if heads < 1 or heads % key_pages.shape[1]:
+            raise ValueError("key/value heads must divide query heads")
+        _require_ints(lengths, query, "lengths", requests)
+        _require_ints(starts, query, "starts", requests + 1)
+        if not isinstance(scale, numbers.Real):
+            raise TypeError("paged_attention_chunk: scale must be a number")
+        if rows == 0:
+            return torch.empty_like(query)
+        query = _bare(query).clone(memory_format=torch.contiguous_format)
+        out = native().paged_attention_chunk(query, *map(_bare, arguments[1:]), float(scale), _flags())
+        if out is None:
+            raise ValueError("paged_attention_chunk: sizes beyond what the kernel takes")
+    return native_result(out, "paged_attention_chunk")

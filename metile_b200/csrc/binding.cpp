@@ -444,8 +444,9 @@ inline bool ints_on(const Tensor* t, c10::Device device, int64_t count) {
 // A block table int32 [requests, width] whose rows do not overlap: the stride of its rows, or -1.
 inline int64_t table_stride(const Tensor* t) {
     if (!t || !t->is_cuda() || t->dim() != 2 || t->scalar_type() != at::kInt || t->size(1) < 1) return -1;
+    if (t->size(0) == 0) return t->size(1);
     if (t->size(1) > 1 && t->stride(1) != 1) return -1;
-    if (t->size(0) <= 1) return t->size(1);
+    if (t->size(0) == 1) return t->size(1);
     return t->stride(0) >= t->size(1) ? t->stride(0) : -1;
 }
 
@@ -629,6 +630,223 @@ PyObject* paged_attention_decode(PyObject* const* args) {
     return code_or(code, std::move(out));
 }
 
+// paged_attention_chunk(query, key_pages, value_pages, block_tables, lengths, starts, scale, flags)
+PyObject* paged_attention_chunk(PyObject* const* args) {
+    const Tensor* t[6];
+    for (int i = 0; i < 6; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const double scale = PyFloat_AsDouble(args[6]);
+    const long flags = PyLong_AsLong(args[7]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    const Tensor &q = *t[0], &keys = *t[1], &values = *t[2], &tables = *t[3];
+    if (!q.is_cuda() || q.dim() != 3 || keys.dim() != 4 || q.numel() == 0 || !q.is_contiguous()) Py_RETURN_NONE;
+    const auto device = q.device();
+    const int64_t rows = q.size(0), heads = q.size(1), dim = q.size(2), kv_heads = keys.size(1), stride = table_stride(&tables);
+    const int type = half_type(q);
+    Pages key_pages, value_pages;
+    if (type < 0 || stride < 0 || wants_gradient({&q, &keys, &values}) || tables.device() != device ||
+        !pages_of(&keys, device, q.scalar_type(), key_pages) || !pages_of(&values, device, q.scalar_type(), value_pages) ||
+        values.sizes() != keys.sizes() || keys.size(3) != dim || !ints_on(t[4], device, tables.size(0)) || !ints_on(t[5], device, tables.size(0) + 1))
+        Py_RETURN_NONE;
+    const int64_t requests = tables.size(0), width = tables.size(1);
+    if (!fits_int(rows * heads) || !fits_int(requests) || !fits_int(dim) || !fits_int(keys.size(0)) || !fits_int(keys.size(2)) || !fits_int(width))
+        Py_RETURN_NONE;
+    const Launch launch(device);
+    Tensor out = new_of({rows, heads, dim}, q.scalar_type(), device);
+    const size_t needed = mt_paged_attention_chunk_workspace_bytes((int)rows, (int)requests, (int)heads, (int)kv_heads, (int)dim, (int)width,
+                                                                   (int)keys.size(2), (unsigned int)flags);
+    c10::DataPtr scratch;
+    if (needed) scratch = call_scratch(needed);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_paged_attention_chunk(address(q), key_pages.base, key_pages.strides, value_pages.base, value_pages.strides,
+                                        static_cast<const int*>(address(tables)), stride, (int)width, static_cast<const int*>(address(*t[4])),
+                                        static_cast<const int*>(address(*t[5])), address(out), scratch.get(), needed, (int)rows, (int)requests,
+                                        (int)heads, (int)kv_heads, (int)dim, (int)keys.size(0), (int)keys.size(2), type, (float)scale,
+                                        (unsigned int)flags, launch.stream());
+    }
+    return code_or(code, std::move(out));
+}
+
+// The caches of a call that takes those of all layers: a sequence of (key_pages, value_pages) of one shape and layout.
+struct Caches {
+    std::vector<void*> addresses[2];
+    Pages first[2];
+    const Tensor* sample = nullptr;
+};
+inline bool caches_of(PyObject* object, c10::Device device, Caches& caches) {
+    auto sequence = [](PyObject* o) { return PyTuple_CheckExact(o) || PyList_CheckExact(o); };
+    if (!sequence(object)) return false;
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(object);
+    if (count < 1 || !fits_int(count)) return false;
+    const Tensor* like[2] = {};  // the first cache's, which are looked at closely
+    for (auto& list : caches.addresses) list.reserve(count);
+    for (Py_ssize_t c = 0; c < count; ++c) {
+        PyObject* pair = PySequence_Fast_GET_ITEM(object, c);
+        if (!sequence(pair) || PySequence_Fast_GET_SIZE(pair) != 2) return false;
+        for (int which = 0; which < 2; ++which) {
+            const Tensor* pages = plain(PySequence_Fast_GET_ITEM(pair, which));
+            if (!pages || wants_gradient({pages})) return false;
+            if (c == 0) {
+                like[which] = pages;
+                if (half_type(*pages) < 0 || !pages_of(pages, device, like[0]->scalar_type(), caches.first[which]) || pages->sizes() != like[0]->sizes())
+                    return false;
+            } else if (pages->scalar_type() != like[which]->scalar_type() || pages->device() != device ||
+                       pages->sizes() != like[which]->sizes() || pages->strides() != like[which]->strides()) {
+                return false;
+            }
+            caches.addresses[which].push_back(address(*pages));  // the library looks at its alignment
+        }
+    }
+    caches.sample = like[0];
+    for (int i = 0; i < 4; ++i)
+        if (!fits_int(caches.sample->size(i))) return false;
+    return true;
+}
+
+// paged_fork(block_tables, lengths, sources, counts, free_pages, free_state, shares, caches, advance)
+PyObject* paged_fork(PyObject* const* args) {
+    const Tensor* t[7];
+    for (int i = 0; i < 7; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const bool advance = args[8] == Py_True;
+    const int64_t stride = table_stride(t[0]);
+    if (stride < 0) Py_RETURN_NONE;
+    const auto device = t[0]->device();
+    const int64_t requests = t[0]->size(0), width = t[0]->size(1), pool = t[4]->numel();
+    Caches caches;
+    if (!ints_on(t[1], device, requests) || !ints_on(t[2], device, requests) || !ints_on(t[3], device, requests) || !ints_on(t[4], device, pool) ||
+        !ints_on(t[5], device, 2) || !fits_int(pool) || pool < 1 || !fits_int(requests) || !fits_int(width) || !caches_of(args[7], device, caches) ||
+        !ints_on(t[6], device, caches.sample->size(0)))
+        Py_RETURN_NONE;
+    const Tensor& sample = *caches.sample;
+    const Launch launch(device);
+    Tensor lengths = *t[1], state = *t[5], shares = *t[6];
+    if (!advance) {
+        Carved carved(Carved::room(requests, 4) + 16 + Carved::room(shares.numel(), 4), device);
+        lengths = carved.next({requests}, at::kInt);
+        state = carved.next({2}, at::kInt);
+        shares = carved.next({t[6]->numel()}, at::kInt);
+    }
+    const size_t needed = mt_paged_fork_workspace_bytes((int)requests);
+    c10::DataPtr scratch;
+    if (needed) scratch = call_scratch(needed);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_paged_fork(static_cast<int*>(address(*t[0])), stride, (int)width, static_cast<const int*>(address(*t[1])),
+                             static_cast<const int*>(address(*t[2])), static_cast<const int*>(address(*t[3])), static_cast<const int*>(address(*t[4])),
+                             (int)pool, static_cast<const int*>(address(*t[5])), static_cast<const int*>(address(*t[6])), caches.addresses[0].data(),
+                             caches.first[0].strides, caches.addresses[1].data(), caches.first[1].strides, (int)caches.addresses[0].size(),
+                             static_cast<int*>(address(lengths)), static_cast<int*>(address(state)), static_cast<int*>(address(shares)), scratch.get(),
+                             needed, (int)requests, (int)sample.size(1), (int)sample.size(3), (int)sample.size(0), (int)sample.size(2), launch.stream());
+    }
+    if (code != 0) return PyLong_FromLong(code);
+    return tuple_of({lengths, state, shares});
+}
+
+// paged_free(block_tables, lengths, ended, free_pages, free_state, shares, page_size, advance)
+PyObject* paged_free(PyObject* const* args) {
+    const Tensor* t[6];
+    for (int i = 0; i < 6; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const long page_size = PyLong_AsLong(args[6]);
+    const bool advance = args[7] == Py_True;
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    const int64_t stride = table_stride(t[0]);
+    if (stride < 0 || !fits_int(page_size)) Py_RETURN_NONE;
+    const auto device = t[0]->device();
+    const int64_t requests = t[0]->size(0), width = t[0]->size(1), pool = t[3]->numel(), pages = t[5]->numel();
+    const Tensor& ended = *t[2];
+    if (!ints_on(t[1], device, requests) || ended.device() != device || ended.scalar_type() != at::kBool || !ended.is_contiguous() ||
+        ended.numel() != requests || !ints_on(t[3], device, pool) || !ints_on(t[4], device, 2) || !ints_on(t[5], device, pages) || pool < 1 ||
+        pages < 1 || !fits_int(pool) || !fits_int(pages) || !fits_int(requests) || !fits_int(width))
+        Py_RETURN_NONE;
+    const Launch launch(device);
+    Tensor lengths = *t[1], state = *t[4], shares = *t[5];
+    if (!advance) {
+        Carved carved(Carved::room(requests, 4) + 16 + Carved::room(pages, 4), device);
+        lengths = carved.next({requests}, at::kInt);
+        state = carved.next({2}, at::kInt);
+        shares = carved.next({pages}, at::kInt);
+    }
+    const size_t needed = mt_paged_free_workspace_bytes((int)pages);
+    const c10::DataPtr scratch = call_scratch(needed);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_paged_free(static_cast<const int*>(address(*t[0])), stride, (int)width, static_cast<const int*>(address(*t[1])),
+                             static_cast<const unsigned char*>(address(ended)), static_cast<int*>(address(*t[3])), (int)pool,
+                             static_cast<const int*>(address(*t[4])), static_cast<const int*>(address(*t[5])), static_cast<int*>(address(lengths)),
+                             static_cast<int*>(address(state)), static_cast<int*>(address(shares)), scratch.get(), needed, (int)requests, (int)pages,
+                             (int)page_size, launch.stream());
+    }
+    if (code != 0) return PyLong_FromLong(code);
+    return tuple_of({lengths, state, shares});
+}
+
+// paged_compact(block_tables, lengths, caches)
+PyObject* paged_compact(PyObject* const* args) {
+    const Tensor *tables = plain(args[0]), *lengths = plain(args[1]);
+    const int64_t stride = table_stride(tables);
+    if (stride < 0) Py_RETURN_NONE;
+    const auto device = tables->device();
+    const int64_t requests = tables->size(0), width = tables->size(1);
+    Caches caches;
+    if (!ints_on(lengths, device, requests) || !fits_int(requests) || !fits_int(width) || !caches_of(args[2], device, caches)) Py_RETURN_NONE;
+    const Tensor& sample = *caches.sample;
+    const int64_t pages = sample.size(0);
+    const Launch launch(device);
+    Carved carved(Carved::room(requests * width, 4) + 2 * Carved::room(pages, 4) + 16, device);
+    Tensor out = carved.next({requests, width}, at::kInt), ring = carved.next({pages}, at::kInt), state = carved.next({2}, at::kInt);
+    Tensor shares = carved.next({pages}, at::kInt);
+    const size_t needed = mt_paged_compact_workspace_bytes((int)pages);
+    const c10::DataPtr scratch = call_scratch(needed);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_paged_compact(static_cast<const int*>(address(*tables)), stride, (int)width, static_cast<const int*>(address(*lengths)),
+                                static_cast<int*>(address(out)), static_cast<int*>(address(ring)), static_cast<int*>(address(state)),
+                                static_cast<int*>(address(shares)), caches.addresses[0].data(), caches.first[0].strides, caches.addresses[1].data(),
+                                caches.first[1].strides, (int)caches.addresses[0].size(), scratch.get(), needed, (int)requests, (int)sample.size(1),
+                                (int)sample.size(3), (int)pages, (int)sample.size(2), launch.stream());
+    }
+    if (code != 0) return PyLong_FromLong(code);
+    return tuple_of({out, ring, state, shares});
+}
+
+// token_logprobs(logits, tokens, top)
+PyObject* token_logprobs(PyObject* const* args) {
+    const Tensor *logits = plain(args[0]), *tokens = plain(args[1]);
+    const long top = PyLong_AsLong(args[2]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (!logits || !tokens || !logits->is_cuda() || logits->dim() != 2 || logits->numel() == 0 || wants_gradient({logits})) Py_RETURN_NONE;
+    const auto device = logits->device();
+    const int64_t rows = logits->size(0), vocabulary = logits->size(1);
+    const int type = logits->scalar_type() == at::kFloat ? MT_TYPE_FP32 : half_type(*logits);
+    if (type < 0 || (vocabulary > 1 && logits->stride(1) != 1) || (rows > 1 && logits->stride(0) < 0) || rows > MT_LOGPROB_MAX_ROWS ||
+        vocabulary > MT_LOGPROB_MAX_VOCABULARY || top < 0 || top > 64)
+        Py_RETURN_NONE;
+    if (tokens->device() != device || tokens->scalar_type() != at::kLong || !tokens->is_contiguous() || tokens->dim() != 1 || tokens->size(0) != rows)
+        Py_RETURN_NONE;
+    const Launch launch(device);
+    Carved carved(2 * Carved::room(rows, 4) + Carved::room(rows * top, 4) + Carved::room(rows * top, 8), device);
+    Tensor top_tokens = carved.next({rows, top}, at::kLong), logprobs = carved.next({rows}, at::kFloat), entropy = carved.next({rows}, at::kFloat);
+    Tensor top_logprobs = carved.next({rows, top}, at::kFloat);
+    const size_t needed = mt_token_logprobs_workspace_bytes((int)rows, (int)vocabulary, (int)top, type);
+    const c10::DataPtr scratch = call_scratch(needed);
+    int code;
+    {
+        const Unlocked unlocked;
+        code = mt_token_logprobs(address(*logits), rows > 1 ? logits->stride(0) : vocabulary, type, static_cast<const long long*>(address(*tokens)),
+                                 static_cast<float*>(address(logprobs)), static_cast<float*>(address(entropy)), static_cast<float*>(address(top_logprobs)),
+                                 static_cast<long long*>(address(top_tokens)), scratch.get(), needed, (int)rows, (int)vocabulary, (int)top, launch.stream());
+    }
+    if (code != 0) return PyLong_FromLong(code);
+    return tuple_of({logprobs, entropy, top_logprobs, top_tokens});
+}
+
 // beam_select(logits, scores, keep, finished | None, end_token)
 PyObject* beam_select(PyObject* const* args) {
     const Tensor *logits = plain(args[0]), *scores = plain(args[1]);
@@ -735,7 +953,9 @@ PyMethodDef methods[] = {MT_METHOD(project, 8), MT_METHOD(swiglu, 8), MT_METHOD(
                          MT_METHOD(dense, 4), MT_METHOD(attention, 5), MT_METHOD(rope_kv_append, 8), MT_METHOD(rope_kv_prefill, 8),
                          MT_METHOD(greedy_token, 2), MT_METHOD(embedding, 2),
                          MT_METHOD(paged_resize, 8), MT_METHOD(rope_kv_append_paged, 8), MT_METHOD(paged_attention_decode, 6),
-                         MT_METHOD(beam_select, 5), MT_METHOD(beam_reorder, 4), {nullptr, nullptr, 0, nullptr}};
+                         MT_METHOD(beam_select, 5), MT_METHOD(beam_reorder, 4),
+                         MT_METHOD(paged_attention_chunk, 8), MT_METHOD(paged_fork, 9), MT_METHOD(paged_free, 8), MT_METHOD(paged_compact, 3),
+                         MT_METHOD(token_logprobs, 3), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

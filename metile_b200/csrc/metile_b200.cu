@@ -13,6 +13,9 @@
 #include "paged_cache.cuh"
 #include "paged_attention.cuh"
 #include "beam_select.cuh"
+#include "paged_chunk.cuh"
+#include "paged_sharing.cuh"
+#include "token_logprobs.cuh"
 #include <string.h>
 
 #include "common.cuh"
@@ -285,7 +288,7 @@ int mt_device_status(unsigned int words[4], int reset) {
         // A single-launch MLP that gave up may have left its slot's counter and flags as no other launch expects them.
         if (words[0] && !clear_meeting_places()) return MT_ERR_LAUNCH;
     }
-    const bool index = words[0] == kGatherIndexOutside || (words[0] >= kSlotOutside && words[0] <= kParentOutside);
+    const bool index = words[0] == kGatherIndexOutside || (words[0] >= kSlotOutside && words[0] <= kTokenOutside);
     return index ? MT_ERR_INDEX : words[0] ? MT_ERR_DEVICE_WAIT : MT_OK;
 }
 
@@ -826,6 +829,209 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
     if (head_dim == 64) return half ? launch_paged_attention<64, true>(params, sms, s) : launch_paged_attention<64, false>(params, sms, s);
     if (head_dim == 128) return half ? launch_paged_attention<128, true>(params, sms, s) : launch_paged_attention<128, false>(params, sms, s);
     return half ? launch_paged_attention<256, true>(params, sms, s) : launch_paged_attention<256, false>(params, sms, s);
+}
+
+size_t mt_paged_attention_chunk_workspace_bytes(int rows, int requests, int q_heads, int kv_heads, int head_dim, int width,
+                                                int page_size, unsigned int flags) {
+    if (rows <= 0 || requests <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || width <= 0 || page_size <= 0) return 0;
+    (void)flags;
+    return 0;
+}
+
+int mt_paged_attention_chunk(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
+                             const long long* value_strides, const int* block_tables, long long table_stride, int width,
+                             const int* lengths, const int* starts, void* out, void* workspace, size_t workspace_bytes,
+                             int rows, int requests, int q_heads, int kv_heads, int head_dim, int pages, int page_size,
+                             int type, float scale, unsigned int flags, void* stream) {
+    const int shift = page_shift_of(page_size);
+    PagedChunkParams params;
+    if (rows < 0 || requests < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || width < 1 || pages < 1 || shift < 0 || table_stride < width)
+        return MT_ERR_SHAPE;
+    if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || (type != MT_TYPE_BF16 && type != MT_TYPE_FP16)) return MT_ERR_SHAPE;
+    if ((long long)rows * q_heads > 0x7FFFFFFF || (long long)width << shift > 0x7FFFFFFF) return MT_ERR_SHAPE;
+    if (rows == 0) return MT_OK;
+    if (!q || !key_pages || !value_pages || !key_strides || !value_strides || !starts || !out || (requests > 0 && (!block_tables || !lengths)))
+        return MT_ERR_NULL;
+    if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 16) ||
+        !page_strides_of(key_strides, params.key_strides) || !page_strides_of(value_strides, params.value_strides))
+        return MT_ERR_ALIGN;
+    const size_t needed = mt_paged_attention_chunk_workspace_bytes(rows, requests, q_heads, kv_heads, head_dim, width, page_size, flags);
+    if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    params.q = static_cast<const uint16_t*>(q);
+    params.key_pages = static_cast<const uint16_t*>(key_pages);
+    params.value_pages = static_cast<const uint16_t*>(value_pages);
+    params.tables = block_tables;
+    params.lengths = lengths;
+    params.starts = starts;
+    params.out = static_cast<uint16_t*>(out);
+    params.table_stride = table_stride;
+    params.width = width;
+    params.rows = rows;
+    params.requests = requests;
+    params.q_heads = q_heads;
+    params.kv_heads = kv_heads;
+    params.page_shift = shift;
+    params.page_count = pages;
+    params.scale = scale;
+    cudaLaunchAttribute attribute;
+    const cudaLaunchConfig_t config = dependent_launch(dim3((unsigned int)(((long long)rows * q_heads + 3) / 4), 1, 1), 128, 0, stream, &attribute);
+    const bool half = type == MT_TYPE_FP16;
+    auto* const kernel = head_dim == 64 ? (half ? paged_chunk_kernel<64, true> : paged_chunk_kernel<64, false>)
+                         : head_dim == 128 ? (half ? paged_chunk_kernel<128, true> : paged_chunk_kernel<128, false>)
+                                           : (half ? paged_chunk_kernel<256, true> : paged_chunk_kernel<256, false>);
+    return cudaLaunchKernelEx(&config, kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+}
+
+// The caches of a call that takes them all: addresses and strides.
+static int check_caches(void* const* key_pages, const long long* key_strides, void* const* value_pages, const long long* value_strides,
+                        int caches, PageStrides& keys, PageStrides& values) {
+    if (caches > 0 && (!key_pages || !value_pages || !key_strides || !value_strides)) return MT_ERR_NULL;
+    for (int c = 0; c < caches; ++c) {
+        if (!key_pages[c] || !value_pages[c]) return MT_ERR_NULL;
+        if (!aligned_to(key_pages[c], 16) || !aligned_to(value_pages[c], 16)) return MT_ERR_ALIGN;
+    }
+    keys = values = {0, 0, 0};
+    if (caches > 0 && (!page_strides_of(key_strides, keys) || !page_strides_of(value_strides, values))) return MT_ERR_ALIGN;
+    return MT_OK;
+}
+
+static bool sharing_sizes(int requests, int width, long long table_stride, int pages, int shift) {
+    // Entries of the table are counted in 32 bits, with a step of all threads above them.
+    return requests >= 0 && width >= 1 && pages >= 1 && pages <= 0x7FFF0000 && shift >= 0 && table_stride >= width &&
+           (long long)requests * width <= 0x7FFF0000 && (long long)width << shift <= 0x7FFFFFFF;
+}
+
+size_t mt_paged_fork_workspace_bytes(int requests) { return requests > 0 ? (size_t)requests * sizeof(int) : 0; }
+
+int mt_paged_fork(int* block_tables, long long table_stride, int width, const int* lengths, const int* sources,
+                  const int* counts, const int* free_pages, int pool, const int* free_state, const int* shares,
+                  void* const* key_pages, const long long* key_strides, void* const* value_pages,
+                  const long long* value_strides, int caches, int* lengths_out, int* free_state_out, int* shares_out,
+                  void* workspace, size_t workspace_bytes, int requests, int kv_heads, int head_dim, int pages, int page_size,
+                  void* stream) {
+    const int shift = page_shift_of(page_size);
+    ForkCopyParams params;
+    if (!sharing_sizes(requests, width, table_stride, pages, shift) || pool < 1 || caches < 0 || kv_heads < 1 || head_dim < 8 || head_dim % 8 ||
+        (long long)kv_heads * head_dim > 0x7FFFFFFF >> shift)
+        return MT_ERR_SHAPE;
+    if (!free_pages || !free_state || !shares || !free_state_out || !shares_out ||
+        (requests > 0 && (!block_tables || !lengths || !sources || !counts || !lengths_out)))
+        return MT_ERR_NULL;
+    const int bad = check_caches(key_pages, key_strides, value_pages, value_strides, caches, params.key_strides, params.value_strides);
+    if (bad) return bad;
+    if (requests > 0 && (!workspace || !aligned_to(workspace, 4) || workspace_bytes < mt_paged_fork_workspace_bytes(requests))) return MT_ERR_WORKSPACE;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    params.fork = {block_tables, lengths, sources, counts, free_pages, free_state, shares, lengths_out, free_state_out, shares_out,
+                   static_cast<int*>(workspace), table_stride, width, pool, requests, shift, pages};
+    params.kv_heads = kv_heads;
+    params.head_dim = head_dim;
+    const int copiers = shares_out == shares ? 0 : (int)((pages + 4ll * kSharingThreads - 1) / (4 * kSharingThreads));
+    cudaLaunchAttribute attribute;
+    cudaLaunchConfig_t config = dependent_launch(dim3(1 + (copiers < 64 ? copiers : 64), 1, 1), kSharingThreads, 0, stream, &attribute);
+    if (cudaLaunchKernelEx(&config, paged_fork_plan_kernel, params.fork) != cudaSuccess) return MT_ERR_LAUNCH;
+    if (requests == 0) return MT_OK;
+    for (int first = 0; first == 0 || first < caches; first += kForkMaxCaches) {
+        const int here = caches - first < kForkMaxCaches ? caches - first : kForkMaxCaches;
+        for (int c = 0; c < here; ++c) {
+            params.arrays[c] = static_cast<uint16_t*>(key_pages[first + c]);
+            params.arrays[kForkMaxCaches + c] = static_cast<uint16_t*>(value_pages[first + c]);
+        }
+        params.first_cache = first;
+        config = dependent_launch(dim3(requests, 1 + 2 * here, 1), kForkThreads, 0, stream, &attribute);
+        if (cudaLaunchKernelEx(&config, paged_fork_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    }
+    return MT_OK;
+}
+
+size_t mt_paged_free_workspace_bytes(int pages) { return pages > 0 ? ((size_t)2 * pages + kSharingCluster) * sizeof(int) : 0; }
+
+int mt_paged_free(const int* block_tables, long long table_stride, int width, const int* lengths, const unsigned char* ended,
+                  int* free_pages, int pool, const int* free_state, const int* shares, int* lengths_out, int* free_state_out,
+                  int* shares_out, void* workspace, size_t workspace_bytes, int requests, int pages, int page_size, void* stream) {
+    const int shift = page_shift_of(page_size);
+    if (!sharing_sizes(requests, width, table_stride, pages, shift) || pool < 1) return MT_ERR_SHAPE;
+    if (!free_pages || !free_state || !shares || !free_state_out || !shares_out || (requests > 0 && (!block_tables || !lengths || !ended || !lengths_out)))
+        return MT_ERR_NULL;
+    if (!workspace || !aligned_to(workspace, 4) || workspace_bytes < mt_paged_free_workspace_bytes(pages)) return MT_ERR_WORKSPACE;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    int* scratch = static_cast<int*>(workspace);
+    const FreeParams params{block_tables, lengths, ended, free_pages, free_state, shares, lengths_out, free_state_out, shares_out,
+                            scratch, scratch + pages, scratch + 2 * (size_t)pages, table_stride, width, pool, requests, shift, pages};
+    return launch_sharing_kernel(paged_free_kernel, params, (long long)requests * width, static_cast<cudaStream_t>(stream));
+}
+
+size_t mt_paged_compact_workspace_bytes(int pages) { return pages > 0 ? ((size_t)4 * pages + kCompactTotals) * sizeof(int) : 0; }
+
+int mt_paged_compact(const int* block_tables, long long table_stride, int width, const int* lengths, int* tables_out,
+                     int* free_pages, int* free_state, int* shares, void* const* key_pages, const long long* key_strides,
+                     void* const* value_pages, const long long* value_strides, int caches, void* workspace,
+                     size_t workspace_bytes, int requests, int kv_heads, int head_dim, int pages, int page_size, void* stream) {
+    const int shift = page_shift_of(page_size);
+    CompactCopyParams copy;
+    if (!sharing_sizes(requests, width, table_stride, pages, shift) || caches < 0 || kv_heads < 1 || head_dim < 8 || head_dim % 8 ||
+        (long long)kv_heads * head_dim > 0x7FFFFFFF >> shift)
+        return MT_ERR_SHAPE;
+    if (!free_pages || !free_state || !shares || (requests > 0 && (!block_tables || !lengths || !tables_out))) return MT_ERR_NULL;
+    if (requests > 0 && tables_out == block_tables) return MT_ERR_SHAPE;  // a second call would move what has moved
+    const int bad = check_caches(key_pages, key_strides, value_pages, value_strides, caches, copy.key_strides, copy.value_strides);
+    if (bad) return bad;
+    if (!workspace || !aligned_to(workspace, 4) || workspace_bytes < mt_paged_compact_workspace_bytes(pages)) return MT_ERR_WORKSPACE;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    int* scratch = static_cast<int*>(workspace);
+    const size_t n = pages;
+    const CompactParams params{block_tables, lengths, tables_out, free_pages, free_state, shares, scratch, scratch + n, scratch + 2 * n,
+                               scratch + 3 * n, scratch + 4 * n, table_stride, width, requests, shift, pages};
+    const long long entries = (long long)requests * width;
+    const int rc = launch_sharing_kernel(paged_compact_kernel, params, entries > pages ? entries : pages, static_cast<cudaStream_t>(stream));
+    if (rc) return rc;
+    copy.movers = params.movers;
+    copy.holes = params.holes;
+    copy.totals = params.totals;
+    copy.kv_heads = kv_heads;
+    copy.head_dim = head_dim;
+    copy.page_shift = shift;
+    const int sms = device_sm_count();
+    if (sms < 1) return MT_ERR_LAUNCH;
+    for (int first = 0; first < caches; first += kForkMaxCaches) {
+        const int here = caches - first < kForkMaxCaches ? caches - first : kForkMaxCaches;
+        for (int c = 0; c < here; ++c) {
+            copy.arrays[c] = static_cast<uint16_t*>(key_pages[first + c]);
+            copy.arrays[kForkMaxCaches + c] = static_cast<uint16_t*>(value_pages[first + c]);
+        }
+        // How many pages move is known on the device: CTAs to fill the chip, or one for every page there could be.
+        const int each = (8 * sms + 2 * here - 1) / (2 * here), most = (pages + 1) / 2;
+        cudaLaunchAttribute attribute;
+        const cudaLaunchConfig_t config = dependent_launch(dim3(each < most ? each : most, 2 * here, 1), kForkThreads, 0, stream, &attribute);
+        if (cudaLaunchKernelEx(&config, paged_compact_copy_kernel, copy) != cudaSuccess) return MT_ERR_LAUNCH;
+    }
+    return MT_OK;
+}
+
+size_t mt_token_logprobs_workspace_bytes(int rows, int vocabulary, int top, int type) {
+    if (rows <= 0 || vocabulary <= 0 || top < 0) return 0;
+    const int parts = logprob_parts(vocabulary, type);
+    return logprob_stats_bytes(rows, parts) + (size_t)rows * parts * top * sizeof(unsigned long long);
+}
+
+int mt_token_logprobs(const void* logits, long long row_stride, int type, const long long* tokens, float* logprobs,
+                      float* entropy, float* top_logprobs, long long* top_tokens, void* workspace, size_t workspace_bytes,
+                      int rows, int vocabulary, int top, void* stream) {
+    if (rows < 0 || rows > MT_LOGPROB_MAX_ROWS || vocabulary < 1 || vocabulary > MT_LOGPROB_MAX_VOCABULARY || top < 0 || top > kLogprobMaxTop ||
+        top > vocabulary || row_stride < 0 || (type != MT_TYPE_BF16 && type != MT_TYPE_FP16 && type != MT_TYPE_FP32))
+        return MT_ERR_SHAPE;
+    if (rows == 0) return MT_OK;
+    if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_logprobs || !top_tokens))) return MT_ERR_NULL;
+    if (!aligned_to(logits, type == MT_TYPE_FP32 ? 4 : 2)) return MT_ERR_ALIGN;
+    const size_t needed = mt_token_logprobs_workspace_bytes(rows, vocabulary, top, type);
+    if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed) return MT_ERR_WORKSPACE;
+    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    LogprobParams params{logits, tokens, logprobs, entropy, top_logprobs, top_tokens, static_cast<LogprobStats*>(workspace), nullptr,
+                         row_stride, rows, vocabulary, logprob_parts(vocabulary, type), top};
+    params.lists = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + logprob_stats_bytes(rows, params.parts));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return type == MT_TYPE_FP32 ? launch_token_logprobs<2>(params, s) : type == MT_TYPE_FP16 ? launch_token_logprobs<1>(params, s)
+                                                                                               : launch_token_logprobs<0>(params, s);
 }
 
 size_t mt_beam_select_workspace_bytes(int groups, int beams, int vocabulary, int keep, int type) {
