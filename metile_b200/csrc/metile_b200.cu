@@ -834,8 +834,10 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
 size_t mt_paged_attention_chunk_workspace_bytes(int rows, int requests, int q_heads, int kv_heads, int head_dim, int width,
                                                 int page_size, unsigned int flags) {
     if (rows <= 0 || requests <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || width <= 0 || page_size <= 0) return 0;
-    (void)flags;
-    return 0;
+    const int sms = device_sm_count();
+    if (sms < 1 || q_heads % kv_heads) return 0;
+    return chunk_partial_bytes(rows, q_heads, head_dim, chunk_split_limit(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size,
+                                                                          (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0, sms));
 }
 
 int mt_paged_attention_chunk(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
@@ -845,22 +847,25 @@ int mt_paged_attention_chunk(const void* q, const void* key_pages, const long lo
                              int type, float scale, unsigned int flags, void* stream) {
     const int shift = page_shift_of(page_size);
     PagedChunkParams params;
+    PageStrides keys, values;
     if (rows < 0 || requests < 0 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || width < 1 || pages < 1 || shift < 0 || table_stride < width)
         return MT_ERR_SHAPE;
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || (type != MT_TYPE_BF16 && type != MT_TYPE_FP16)) return MT_ERR_SHAPE;
-    if ((long long)rows * q_heads > 0x7FFFFFFF || (long long)width << shift > 0x7FFFFFFF) return MT_ERR_SHAPE;
+    if ((long long)rows * q_heads > 0x7FFFFFFF || (long long)width << shift > 0x7FFF0000) return MT_ERR_SHAPE;
     if (rows == 0) return MT_OK;
     if (!q || !key_pages || !value_pages || !key_strides || !value_strides || !starts || !out || (requests > 0 && (!block_tables || !lengths)))
         return MT_ERR_NULL;
     if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 16) ||
-        !page_strides_of(key_strides, params.key_strides) || !page_strides_of(value_strides, params.value_strides))
+        !page_strides_of(key_strides, keys) || !page_strides_of(value_strides, values))
         return MT_ERR_ALIGN;
-    const size_t needed = mt_paged_attention_chunk_workspace_bytes(rows, requests, q_heads, kv_heads, head_dim, width, page_size, flags);
+    const int sms = device_sm_count();
+    if (sms < 1 || !device_is_sm100()) return MT_ERR_DEVICE;
+    params.split_limit = chunk_split_limit(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size,
+                                           (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0, sms);
+    const size_t needed = chunk_partial_bytes(rows, q_heads, head_dim, params.split_limit);
     if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
-    if (!device_is_sm100()) return MT_ERR_DEVICE;
-    params.q = static_cast<const uint16_t*>(q);
-    params.key_pages = static_cast<const uint16_t*>(key_pages);
-    params.value_pages = static_cast<const uint16_t*>(value_pages);
+    params.partial = static_cast<float*>(workspace);
+    params.stats = reinterpret_cast<float2*>(params.partial + (size_t)rows * q_heads * params.split_limit * head_dim);
     params.tables = block_tables;
     params.lengths = lengths;
     params.starts = starts;
@@ -874,13 +879,12 @@ int mt_paged_attention_chunk(const void* q, const void* key_pages, const long lo
     params.page_shift = shift;
     params.page_count = pages;
     params.scale = scale;
-    cudaLaunchAttribute attribute;
-    const cudaLaunchConfig_t config = dependent_launch(dim3((unsigned int)(((long long)rows * q_heads + 3) / 4), 1, 1), 128, 0, stream, &attribute);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool half = type == MT_TYPE_FP16;
-    auto* const kernel = head_dim == 64 ? (half ? paged_chunk_kernel<64, true> : paged_chunk_kernel<64, false>)
-                         : head_dim == 128 ? (half ? paged_chunk_kernel<128, true> : paged_chunk_kernel<128, false>)
-                                           : (half ? paged_chunk_kernel<256, true> : paged_chunk_kernel<256, false>);
-    return cudaLaunchKernelEx(&config, kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    auto* const launch = head_dim == 64 ? (half ? launch_paged_chunk<64, true> : launch_paged_chunk<64, false>)
+                         : head_dim == 128 ? (half ? launch_paged_chunk<128, true> : launch_paged_chunk<128, false>)
+                                           : (half ? launch_paged_chunk<256, true> : launch_paged_chunk<256, false>);
+    return launch(params, q, key_pages, keys, value_pages, values, sms, s);
 }
 
 // The caches of a call that takes them all: addresses and strides.
