@@ -295,8 +295,9 @@ int mt_paged_attention_decode(const void* q, const void* key_pages, const long l
  * leaves them) are the last tokens of request r, lengths[r] with them; the i-th of n stands at position lengths[r] - n + i
  * and out = softmax(scale * q . K) V over the tokens up to its own.  Zeros where that is none and in rows no request has.
  * What a row does not see weighs nothing, whatever lies there; a NaN that it sees gives NaN.  q, out: dense [rows, q_heads,
- * head_dim], bf16 or fp16; head_dim 64, 128 or 256.  flags: with MT_FLAG_FIXED_ORDER or MT_FLAG_FORCE_UMMA a row's bits
- * depend on its own tokens only, with 0 also on the sizes of the call (rows, requests, heads, width). */
+ * head_dim], bf16 or fp16, out and the workspace 32-byte aligned; head_dim 64, 128 or 256.  flags: with MT_FLAG_FIXED_ORDER or
+ * MT_FLAG_FORCE_UMMA a row's bits depend on its own tokens only, with 0 also on the others of the call (where shares of the
+ * work are cut). */
 size_t mt_paged_attention_chunk_workspace_bytes(int rows, int requests, int q_heads, int kv_heads, int head_dim, int width,
                                                 int page_size, unsigned int flags);
 int mt_paged_attention_chunk(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,

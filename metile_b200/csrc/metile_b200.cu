@@ -836,8 +836,8 @@ size_t mt_paged_attention_chunk_workspace_bytes(int rows, int requests, int q_he
     if (rows <= 0 || requests <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || width <= 0 || page_size <= 0) return 0;
     const int sms = device_sm_count();
     if (sms < 1 || q_heads % kv_heads) return 0;
-    return chunk_partial_bytes(rows, q_heads, head_dim, chunk_split_limit(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size,
-                                                                          (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0, sms));
+    return chunk_partial_bytes(head_dim, chunk_ctas(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size, sms),
+                               (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0);
 }
 
 int mt_paged_attention_chunk(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
@@ -855,17 +855,14 @@ int mt_paged_attention_chunk(const void* q, const void* key_pages, const long lo
     if (rows == 0) return MT_OK;
     if (!q || !key_pages || !value_pages || !key_strides || !value_strides || !starts || !out || (requests > 0 && (!block_tables || !lengths)))
         return MT_ERR_NULL;
-    if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 16) ||
+    if (!aligned_to(q, 16) || !aligned_to(key_pages, 16) || !aligned_to(value_pages, 16) || !aligned_to(out, 32) ||
         !page_strides_of(key_strides, keys) || !page_strides_of(value_strides, values))
         return MT_ERR_ALIGN;
     const int sms = device_sm_count();
     if (sms < 1 || !device_is_sm100()) return MT_ERR_DEVICE;
-    params.split_limit = chunk_split_limit(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size,
-                                           (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0, sms);
-    const size_t needed = chunk_partial_bytes(rows, q_heads, head_dim, params.split_limit);
-    if (needed && (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
-    params.partial = static_cast<float*>(workspace);
-    params.stats = reinterpret_cast<float2*>(params.partial + (size_t)rows * q_heads * params.split_limit * head_dim);
+    const int ctas = chunk_ctas(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size, sms);
+    const size_t needed = chunk_partial_bytes(head_dim, ctas, (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0);
+    if (needed && (!workspace || !aligned_to(workspace, 32) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
     params.tables = block_tables;
     params.lengths = lengths;
     params.starts = starts;
@@ -884,7 +881,7 @@ int mt_paged_attention_chunk(const void* q, const void* key_pages, const long lo
     auto* const launch = head_dim == 64 ? (half ? launch_paged_chunk<64, true> : launch_paged_chunk<64, false>)
                          : head_dim == 128 ? (half ? launch_paged_chunk<128, true> : launch_paged_chunk<128, false>)
                                            : (half ? launch_paged_chunk<256, true> : launch_paged_chunk<256, false>);
-    return launch(params, q, key_pages, keys, value_pages, values, sms, s);
+    return launch(params, q, key_pages, keys, value_pages, values, needed ? workspace : nullptr, ctas, s);
 }
 
 // The caches of a call that takes them all: addresses and strides.
