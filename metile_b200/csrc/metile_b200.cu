@@ -837,7 +837,7 @@ size_t mt_paged_attention_chunk_workspace_bytes(int rows, int requests, int q_he
     const int sms = device_sm_count();
     if (sms < 1 || q_heads % kv_heads) return 0;
     return chunk_partial_bytes(head_dim, chunk_ctas(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size, sms),
-                               (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0);
+                               (long long)width * page_size, (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0);
 }
 
 int mt_paged_attention_chunk(const void* q, const void* key_pages, const long long* key_strides, const void* value_pages,
@@ -861,7 +861,7 @@ int mt_paged_attention_chunk(const void* q, const void* key_pages, const long lo
     const int sms = device_sm_count();
     if (sms < 1 || !device_is_sm100()) return MT_ERR_DEVICE;
     const int ctas = chunk_ctas(rows, requests, kv_heads, q_heads / kv_heads, head_dim, (long long)width * page_size, sms);
-    const size_t needed = chunk_partial_bytes(head_dim, ctas, (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0);
+    const size_t needed = chunk_partial_bytes(head_dim, ctas, (long long)width * page_size, (flags & (MT_FLAG_FORCE_UMMA | MT_FLAG_FIXED_ORDER)) != 0);
     if (needed && (!workspace || !aligned_to(workspace, 32) || workspace_bytes < needed)) return MT_ERR_WORKSPACE;
     params.tables = block_tables;
     params.lengths = lengths;
@@ -959,7 +959,8 @@ int mt_paged_free(const int* block_tables, long long table_stride, int width, co
     int* scratch = static_cast<int*>(workspace);
     const FreeParams params{block_tables, lengths, ended, free_pages, free_state, shares, lengths_out, free_state_out, shares_out,
                             scratch, scratch + pages, scratch + 2 * (size_t)pages, table_stride, width, pool, requests, shift, pages};
-    return launch_sharing_kernel(paged_free_kernel, params, (long long)requests * width, static_cast<cudaStream_t>(stream));
+    const long long entries = (long long)requests * width;
+    return launch_sharing_kernel(entries <= 2 * kSharingThreads ? paged_free_kernel<2> : paged_free_kernel<16>, params, entries, static_cast<cudaStream_t>(stream));
 }
 
 size_t mt_paged_compact_workspace_bytes(int pages) { return pages > 0 ? ((size_t)4 * pages + kCompactTotals) * sizeof(int) : 0; }

@@ -347,7 +347,10 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
         // The work of all units, one behind the other, is cut into equal shares.  A cut within a unit falls between two token tiles, and
         // not beside its ends; where units are to stay whole it goes to the nearer end.
         const long long all = s.work[kChunkRuns];
-        const long long ctas = max(1ll, min((long long)gridDim.x, all / kChunkShare)), share = all / ctas;
+        const bool short_work = all <= 0x7FFFFFFF;
+        const int ctas = (int)max(1ll, min((long long)gridDim.x, all / kChunkShare));
+        const long long share = short_work ? (unsigned int)all / (unsigned int)ctas : all / ctas, rest = all - share * ctas;
+        auto share_of = [&](int cta) { return share * cta + min((long long)cta, rest); };
         // Left whole, the units make the longest share half a unit longer than the others, or one unit where shares are shorter than that.
         // Whole and cut, us: 4 x 512 tokens behind 512 (2 x 6 heads) 39 and 49, 16 x 6 behind 2000 44 and 50, 256 x 2 behind 300 115 and 145;
         // 4096 from the start 209 and 174, 512 behind 8192 162 and 108, 8 behind 3000 53 and 31 (8 x 4 heads).
@@ -366,50 +369,50 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
                 if (++at.request < p.requests) q = chunk_request(p, at.request, false);
             }
         };
-        auto cut_at = [&](long long x, ChunkRequest& q) {
+        // (Whole is the type that all the work fits: a division of 64 bits takes some 300 cycles.)
+        auto cut_at = [&](auto x, ChunkRequest& q) {
+            using Whole = decltype(x);
             ChunkPlace at = {p.requests, 0, 0, 0};
-            if (x >= all) return at;
+            if (x >= (Whole)all) return at;
+            const Whole heads = (Whole)unit_heads;
             int low = 0, high = kChunkRuns;
             while (high - low > 1) {
                 const int middle = (low + high) >> 1;
-                if (s.work[middle] <= x) low = middle; else high = middle;
+                if ((Whole)s.work[middle] <= x) low = middle; else high = middle;
             }
-            long long before = s.work[low];
-            x -= before;
+            const bool first = x == 0;
+            x -= (Whole)s.work[low];
             for (at.request = low * run;; ++at.request) {
                 q = chunk_request(p, at.request, false);
-                const long long here = unit_heads * chunk_work(q.length, q.n, unit_tokens, chunk_blocks(q.n, unit_tokens));
+                const Whole here = heads * (Whole)chunk_work(q.length, q.n, unit_tokens, chunk_blocks(q.n, unit_tokens));
                 if (x < here) break;
                 x -= here;
-                before += here;
             }
             int block = 0, above = chunk_blocks(q.n, unit_tokens);
             while (above - block > 1) {
                 const int middle = (block + above) >> 1;
-                if (unit_heads * chunk_work(q.length, q.n, unit_tokens, middle) <= x) block = middle; else above = middle;
+                if (heads * (Whole)chunk_work(q.length, q.n, unit_tokens, middle) <= x) block = middle; else above = middle;
             }
             at.block = block;
-            const long long blocks_before = unit_heads * chunk_work(q.length, q.n, unit_tokens, block);
-            x -= blocks_before;
-            before += blocks_before;
+            if (block > 0) x -= heads * (Whole)chunk_work(q.length, q.n, unit_tokens, block);
             const int seen = chunk_seen(q.length, q.n, unit_tokens, block), tiles = tiles_of(seen);
-            const long long work = seen + kChunkUnitCost;
-            at.head = (int)(x / work);
-            x -= at.head * work;
-            before += at.head * work;
-            const int tile = (int)min((x + kTile / 2) / kTile, (long long)tiles);
-            if (x + before > 0 && (whole ? 2 * x >= work : tile >= tiles)) next_unit(at, q);  // the first unit is somebody's, if it has no tile
+            const Whole work = (Whole)seen + kChunkUnitCost;
+            at.head = x < work ? 0 : (int)(x / work);
+            x -= (Whole)at.head * work;
+            const int tile = (int)min((x + kTile / 2) / kTile, (Whole)tiles);
+            if (!first && (whole ? 2 * x >= work : tile >= tiles)) next_unit(at, q);  // the first unit is somebody's, if it has no tile
             else at.tile = whole ? 0 : tile;
             return at;
         };
-        const int box_rows = min(1 << p.page_shift, kTile), boxes = kTile / box_rows;
+        const int box_rows = min(1 << p.page_shift, kTile), boxes = kTile / box_rows, group = p.q_heads / p.kv_heads;
         int item = 0, count = 0;  // tiles of keys and values so far, units so far
         bool alive = true;
         ChunkPlace at = {p.requests, 0, 0, 0}, stop = at;
         if (blockIdx.x < ctas) {
             ChunkRequest other = now;
-            at = cut_at(all * blockIdx.x / ctas, now);
-            stop = cut_at(all * (blockIdx.x + 1) / ctas, other);
+            const long long from = share_of(blockIdx.x), to = share_of(blockIdx.x + 1);
+            at = short_work ? cut_at((unsigned int)from, now) : cut_at((unsigned long long)from, now);
+            stop = short_work ? cut_at((unsigned int)to, other) : cut_at((unsigned long long)to, other);
         }
         ChunkCut cut = {0, 0, 0, 0, 0, 0};
         auto describe = [&] {  // the next unit
@@ -417,9 +420,9 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
             u.tiles = -1;
             if (at.request >= p.requests || (same_unit(at, stop) && at.tile == stop.tile)) return u;
             const ChunkRequest q = now;
-            const int part = at.head % p.parts, group = p.q_heads / p.kv_heads, token = at.block * unit_tokens;
+            const int head = p.parts == 1 ? at.head : at.head / p.parts, part = at.head - head * p.parts, token = at.block * unit_tokens;
             u.request = at.request;
-            u.kv_head = at.head / p.parts;
+            u.kv_head = head;
             u.head0 = u.kv_head * group + part * p.part_heads;
             u.heads = min(p.part_heads, group - part * p.part_heads);
             u.row0 = q.first + token;
@@ -944,8 +947,9 @@ inline int chunk_ctas(int rows, int requests, int kv_heads, int group, int head_
     const long long most = units > sm_count ? sm_count : units * (capacity + kChunkUnitCost) / kChunkShare;
     return most < 1 ? 1 : most < sm_count ? (int)most : sm_count;
 }
-inline size_t chunk_partial_bytes(int head_dim, int ctas, bool whole) {
-    if (whole || ctas <= 1) return 0;
+// Where no unit can be long enough for a cut to pay, nothing is left to be joined.
+inline size_t chunk_partial_bytes(int head_dim, int ctas, long long capacity, bool whole) {
+    if (whole || ctas <= 1 || capacity + kChunkUnitCost - kChunkShare <= kChunkCutGain) return 0;
     return (size_t)ctas * (2 * (head_dim == 256 ? 1 : 2) * kChunkRows * (head_dim + 2) * sizeof(float) + sizeof(ChunkCut));
 }
 
