@@ -195,9 +195,14 @@ class PagedTables:
     The device has the truth: a step that a CUDA graph replays takes its pages there.  The host keeps the same counts
     beside it (`held` tokens of every request, `free` pages) to refuse what would not fit before anything is queued.
 
-    Before a forward pass the caller lets the requests `grow`; the layers of that pass then write and read the new
-    tokens.  A pass is either one token of every request (grow()) or the prompts of some, one after the other in
-    a batch of one (grow(counts))."""
+    Before a forward pass the caller lets the requests `grow` or `extend`; the layers of that pass then write and read the
+    new tokens.  A pass is one token of every request (grow()), the prompts of some, one after the other in a batch of one
+    (grow(counts)), or the next tokens of some, likewise, whatever they hold (extend(counts)): pieces of prompts, drafts, and
+    single tokens beside them.
+
+    Requests may share what they begin with: `branch` lets empty ones go on from the first tokens of others, `release` ends
+    requests, `compact` puts the pages that are held together.  `shares` counts who holds a page, which the reordering of
+    beams does not: beams are ended by `reset`, or counted again by `compact`."""
 
     def __init__(self, requests, pages, page_size, width, device):
         if requests < 1 or pages < 1 or width < 1 or page_size not in backends.PAGE_SIZES:
@@ -207,11 +212,14 @@ class PagedTables:
         self.lengths = torch.zeros((self.requests,), dtype=torch.int32, device=device)
         self.free_pages = torch.arange(self.pages, dtype=torch.int32, device=device)
         self.free_state = torch.tensor([0, self.pages], dtype=torch.int32, device=device)
+        self.shares = torch.zeros((self.pages,), dtype=torch.int32, device=device)  # requests that hold a page beyond the first
         self._ones = torch.ones((self.requests,), dtype=torch.int32, device=device)
         self.held, self.free = [0] * self.requests, self.pages
         self.shared = [0] * self.requests    # tokens of every request in pages that others may have too
         self.slots = self.positions = None   # of the tokens of the pass
         self.prompts = None                  # [(request, first row, rows)], or None: one token of every request
+        self.starts = None                   # of a pass by `extend`: each request's first row
+        self._forget_shares()
 
     @property
     def capacity(self):
@@ -225,6 +233,13 @@ class PagedTables:
         self.free_state.copy_(torch.tensor([0, self.pages], dtype=torch.int32))
         self.held, self.free = [0] * self.requests, self.pages
         self.shared = [0] * self.requests
+        self.shares.zero_()
+        self._forget_shares()
+
+    def _forget_shares(self):
+        # The host's own names of the pages that a request's first blocks share, and how many hold each.
+        self._names, self._holders, self._next_name = [[] for _ in range(self.requests)], {}, 0
+        self._counted = True  # whether `shares` says who holds what
 
     def fits(self, counts):
         """The host's side of a change by counts[r] tokens: (held, free) after it; refuses what does not fit."""
@@ -250,8 +265,17 @@ class PagedTables:
 
         Tokens in pages that requests share (those full at the last `fork` or `reorder`) are given back by `reset` alone: a
         page must not go back twice, nor be written by one request under another."""
-        ones = counts is None
-        counts = [1] * self.requests if ones else [int(count) for count in counts]
+        self._resize([1] * self.requests if counts is None else [int(count) for count in counts], counts is None)
+        self.starts = None
+
+    def extend(self, counts):
+        """counts[r] new tokens for request r, behind those it has; the pass attends them by paged_attention_chunk."""
+        counts = [int(count) for count in counts]
+        if any(count < 0 for count in counts):
+            raise ValueError("paged cache: a request is extended by no token or more")
+        self.starts = self._resize(counts, False)
+
+    def _resize(self, counts, ones):
         self.account(counts)
         self.prompts, first = None, 0
         if not ones:
@@ -261,13 +285,94 @@ class PagedTables:
                     self.prompts.append((request, first, count))
                     first += count
         on_device = self._ones if ones else torch.tensor(counts, dtype=torch.int32).to(self.lengths.device)
-        self.slots, self.positions, _, _, _ = backends.paged_resize(
+        self.slots, self.positions, starts, _, _ = backends.paged_resize(
             self.block_tables, self.lengths, on_device, self.free_pages, self.free_state, page_size=self.page_size,
             tokens=self.requests if ones else first, advance=True)
+        return starts
 
     def share(self):
         """From now on requests may share the pages that are full, as a reordering leaves them."""
         self.shared = [max(shared, held // self.page_size * self.page_size) for shared, held in zip(self.shared, self.held)]
+        self._counted = False
+
+    def _need_counts(self, what):
+        if not self._counted:
+            raise ValueError(f"paged cache: beams share pages that are not counted; {what} needs a compact or a reset first")
+
+    def branch(self, sources, counts, caches):
+        """Let request r, which has no tokens, go on from the first counts[r] tokens of request sources[r]; None: r stays as it is.
+
+        Full pages are shared, the page begun is copied, in the PagedKVCache of every layer."""
+        self._need_counts("branch")
+        if not caches or any(getattr(cache, "tables", None) is not self for cache in caches):
+            raise ValueError("branch expects the PagedKVCache of every layer, over these tables")
+        if len(sources) != self.requests or len(counts) != self.requests:
+            raise ValueError("branch expects a source and a count for every request")
+        chosen = [(r, int(source), int(count)) for r, (source, count) in enumerate(zip(sources, counts)) if source is not None]
+        for r, source, count in chosen:
+            if not 0 <= source < self.requests or source == r or self.held[r] or not 0 < count <= self.held[source]:
+                raise ValueError("branch: an empty request goes on from tokens that another one has")
+        begun = sum(1 for _, _, count in chosen if count % self.page_size)
+        if begun > self.free:
+            raise ValueError("paged cache: out of pages")
+        on_device = torch.tensor([[-1] * self.requests, [0] * self.requests], dtype=torch.int32)
+        for r, source, count in chosen:
+            on_device[0, r], on_device[1, r] = source, count
+        on_device = on_device.to(self.lengths.device)
+        backends.paged_fork(self.block_tables, self.lengths, on_device[0], on_device[1], self.free_pages, self.free_state, self.shares,
+                            [(cache.keys, cache.values) for cache in caches], advance=True)
+        self.free -= begun
+        for r, source, count in chosen:
+            whole, names = count // self.page_size, self._names[source]
+            while len(names) < whole:
+                names.append(self._next_name)
+                self._holders[self._next_name] = 1
+                self._next_name += 1
+            self._names[r] = names[:whole]
+            for name in self._names[r]:
+                self._holders[name] += 1
+            self.held[r], self.shared[r] = count, whole * self.page_size
+            self.shared[source] = max(self.shared[source], whole * self.page_size)
+
+    def release(self, requests):
+        """End the requests named: their pages go back, shared ones with the last request that holds them."""
+        self._need_counts("release")
+        ended = sorted(set(int(r) for r in requests))
+        if ended and not 0 <= ended[0] <= ended[-1] < self.requests:
+            raise ValueError("release expects requests of these tables")
+        flags = torch.zeros((self.requests,), dtype=torch.bool)
+        flags[ended] = True
+        backends.paged_free(self.block_tables, self.lengths, flags.to(self.lengths.device), self.free_pages, self.free_state, self.shares,
+                            page_size=self.page_size, advance=True)
+        for r in ended:
+            self.free += -(-self.held[r] // self.page_size) - len(self._names[r])
+            for name in self._names[r]:
+                self._holders[name] -= 1
+                if self._holders[name] == 0:
+                    del self._holders[name]
+                    self.free += 1
+            self.held[r], self.shared[r], self._names[r] = 0, 0, []
+
+    def compact(self, caches):
+        """Move the pages that are held to the lowest ids, in the PagedKVCache of every layer, and count who holds them from the
+        tables: pages that nobody holds any more, as dropped beams leave them, are free afterwards.  Waits for the GPU, whose
+        tables the host's side is taken from."""
+        if not caches or any(getattr(cache, "tables", None) is not self for cache in caches):
+            raise ValueError("compact expects the PagedKVCache of every layer, over these tables")
+        moved = backends.paged_compact(self.block_tables, self.lengths, [(cache.keys, cache.values) for cache in caches])
+        for own, new in zip((self.block_tables, self.free_pages, self.free_state, self.shares), moved):
+            own.copy_(new)
+        self._forget_shares()
+        tables, shares = self.block_tables.tolist(), self.shares.tolist()
+        self.free = int(self.free_state[1])
+        for r, held in enumerate(self.held):
+            ids = tables[r][:-(-held // self.page_size)]
+            last = max((j for j, page in enumerate(ids) if shares[page]), default=-1)
+            self._names[r] = ids[:last + 1]  # the pages' ids as they are now serve for names
+            self.shared[r] = (last + 1) * self.page_size
+            for page in self._names[r]:
+                self._holders[page] = self._holders.get(page, 0) + 1
+        self._next_name = self.pages
 
     def fork(self, beams, caches):
         """Every first request of `beams` in a row is continued by all of them: full pages are shared, what is begun is copied
@@ -403,6 +508,10 @@ class Attention(nn.Module):
         k = k.reshape(rows, self.kv_heads, self.head_dim)
         v = v.reshape(rows, self.kv_heads, self.head_dim)
         rotated = cache.append(q, k, v, self._frequencies_on(q.device))
+        if tables.starts is not None:
+            out = backends.paged_attention_chunk(rotated, cache.keys, cache.values, tables.block_tables, tables.lengths, tables.starts,
+                                                 scale=self.scale)
+            return out.view(batch, steps, self.heads * self.head_dim)
         if tables.prompts is None:
             out = backends.paged_attention_decode(rotated, cache.keys, cache.values, tables.block_tables, tables.lengths,
                                                   scale=self.scale)
@@ -479,13 +588,14 @@ class TinyCausalLM(nn.Module):
         tables = PagedTables(requests, pages, page_size, -(-capacity // page_size), first.q_proj.weight.device)
         return [PagedKVCache(tables, layer.self_attn.kv_heads, layer.self_attn.head_dim) for layer in self.layers]
 
-    def forward(self, tokens, cache=None, logits_to_keep=0):
-        """Logits [batch, tokens, vocabulary]; with `logits_to_keep`, of that many last positions only."""
+    def forward(self, tokens, cache=None, logits_to_keep=0, logits_at=None):
+        """Logits [batch, tokens, vocabulary]; with `logits_to_keep`, of that many last positions only; with `logits_at`
+        (int64), of the positions it names."""
         hidden = _embed(self.embed_tokens, tokens)
         for index, layer in enumerate(self.layers):
             hidden = layer(hidden, None if cache is None else cache[index])
-        if 0 < logits_to_keep < hidden.shape[1]:
-            hidden = hidden[:, -logits_to_keep:].contiguous()
+        if logits_at is not None or 0 < logits_to_keep < hidden.shape[1]:
+            hidden = hidden[:, -logits_to_keep:].contiguous() if logits_at is None else hidden.index_select(1, logits_at)
             # The logits that all positions together would give: one row alone is else another kernel's.
             if not backends.kernel_pinned():
                 with backends.batch_invariant():
