@@ -36,7 +36,7 @@ constexpr unsigned int kChunkWait = 0x9D0;     // a wait that gave up: + the rol
 
 constexpr int kChunkRows = 128;                // of a query tile
 constexpr int kChunkStep = 64;                 // tokens whose scores are taken at once
-constexpr int kChunkRuns = 128;                // runs of requests whose work is counted
+constexpr int kChunkRuns = 64;                 // runs of requests whose work is counted
 constexpr int kChunkUnitCost = 256;            // what a unit costs beside its tokens, in tokens
 constexpr int kChunkShare = 512;               // the least work of a CTA, in tokens: at least two tiles between two cuts
 constexpr int kChunkCutGain = 1024;            // units are cut where that takes more than this off the longest share, in tokens
@@ -52,9 +52,8 @@ struct ChunkShape {
     static constexpr int kSoftmaxWarps = 4 * kGroups, kWarps = kSoftmaxWarps + 2 + kGroups, kThreads = 32 * kWarps;
     static constexpr int kOColumn = 256;                            // in tensor memory; scores of tile g at 128 g and 128 g + 64
     static constexpr int kTiles = kGroups * kQBytes + kSlots * kSlotBytes;
-    static constexpr int kSmem = kTiles + kChunkNotes * kD * 4 + (kChunkRuns + 1) * 8 + 512;
     static constexpr int kSlotRows = kGroups * kChunkRows;          // of a partial result
-    static_assert(kSmem <= 232448 && kOColumn + kGroups * kD <= 512 && kGroups * 2 * kChunkStep <= kOColumn && kSlots <= 6);
+    static_assert(kOColumn + kGroups * kD <= 512 && kGroups * 2 * kChunkStep <= kOColumn && kSlots <= 6);
 };
 
 struct PagedChunkParams {
@@ -259,16 +258,20 @@ struct ChunkShared {
     int abort;
 };
 
+// The tiles start on 1024 bytes, which the kernel sees to: an alignment of the dynamic array would be that of every kernel's.
+template <int kD>
+constexpr int chunk_smem() { return 1024 + ChunkShape<kD>::kTiles + (int)sizeof(ChunkShared<kD>); }
+static_assert(chunk_smem<64>() <= 232448 && chunk_smem<128>() <= 232448 && chunk_smem<256>() <= 232448);
+
 template <int kD, bool kHalf>
 __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kernel(const __grid_constant__ PagedChunkParams p) {
     using Shape = ChunkShape<kD>;
     using Shared = ChunkShared<kD>;
-    static_assert(Shape::kTiles + sizeof(Shared) <= Shape::kSmem);
     constexpr int kTile = Shape::kTile, kGroups = Shape::kGroups, kSlots = Shape::kSlots, kChunks = kD / 64;
-    extern __shared__ __align__(1024) uint8_t chunk_tiles[];
-    uint8_t* q_tiles = chunk_tiles;
-    uint8_t* ring = chunk_tiles + kGroups * Shape::kQBytes;
-    Shared& s = *reinterpret_cast<Shared*>(chunk_tiles + Shape::kTiles);
+    extern __shared__ __align__(16) uint8_t chunk_dynamic[];
+    uint8_t* q_tiles = chunk_dynamic + (-ptx::smem_u32(chunk_dynamic) & 1023u);
+    uint8_t* ring = q_tiles + kGroups * Shape::kQBytes;
+    Shared& s = *reinterpret_cast<Shared*>(q_tiles + Shape::kTiles);
     volatile int* abort_flag = &s.abort;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     constexpr int kLoader = Shape::kSoftmaxWarps, kFixer = kLoader + 1, kIssuer = kLoader + 2;  // an issuer for each query tile
@@ -1004,13 +1007,13 @@ inline int launch_paged_chunk(PagedChunkParams& params, const void* q, const voi
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return MT_ERR_LAUNCH;
     if (device >= 64 || !configured[device]) {
-        if (cudaFuncSetAttribute(paged_chunk_kernel<kD, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess) return MT_ERR_LAUNCH;
+        if (cudaFuncSetAttribute(paged_chunk_kernel<kD, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, chunk_smem<kD>()) != cudaSuccess) return MT_ERR_LAUNCH;
         if (device < 64) configured[device] = true;
     }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(ctas, 1, 1);
     config.blockDim = dim3(Shape::kThreads, 1, 1);
-    config.dynamicSmemBytes = Shape::kSmem;
+    config.dynamicSmemBytes = chunk_smem<kD>();
     config.stream = stream;
     cudaLaunchAttribute attrs[1];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
