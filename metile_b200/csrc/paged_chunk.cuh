@@ -350,10 +350,8 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
         // The work of all units, one behind the other, is cut into equal shares.  A cut within a unit falls between two token tiles, and
         // not beside its ends; where units are to stay whole it goes to the nearer end.
         const long long all = s.work[kChunkRuns];
-        const bool short_work = all <= 0x7FFFFFFF;
         const int ctas = (int)max(1ll, min((long long)gridDim.x, all / kChunkShare));
-        const long long share = short_work ? (unsigned int)all / (unsigned int)ctas : all / ctas, rest = all - share * ctas;
-        auto share_of = [&](int cta) { return share * cta + min((long long)cta, rest); };
+        const long long share = all / ctas, rest = all - share * ctas;
         // Left whole, the units make the longest share half a unit longer than the others, or one unit where shares are shorter than that.
         // Whole and cut, us: 4 x 512 tokens behind 512 (2 x 6 heads) 39 and 49, 16 x 6 behind 2000 44 and 50, 256 x 2 behind 300 115 and 145;
         // 4096 from the start 209 and 174, 512 behind 8192 162 and 108, 8 behind 3000 53 and 31 (8 x 4 heads).
@@ -372,37 +370,37 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
                 if (++at.request < p.requests) q = chunk_request(p, at.request, false);
             }
         };
-        // (Whole is the type that all the work fits: a division of 64 bits takes some 300 cycles.)
-        auto cut_at = [&](auto x, ChunkRequest& q) {
-            using Whole = decltype(x);
+        auto cut_at = [&](long long x, ChunkRequest& q) {
             ChunkPlace at = {p.requests, 0, 0, 0};
-            if (x >= (Whole)all) return at;
-            const Whole heads = (Whole)unit_heads;
+            if (x >= all) return at;
+            const bool first = x == 0;
             int low = 0, high = kChunkRuns;
             while (high - low > 1) {
                 const int middle = (low + high) >> 1;
-                if ((Whole)s.work[middle] <= x) low = middle; else high = middle;
+                if (s.work[middle] <= x) low = middle; else high = middle;
             }
-            const bool first = x == 0;
-            x -= (Whole)s.work[low];
+            x -= s.work[low];
             for (at.request = low * run;; ++at.request) {
                 q = chunk_request(p, at.request, false);
-                const Whole here = heads * (Whole)chunk_work(q.length, q.n, unit_tokens, chunk_blocks(q.n, unit_tokens));
+                const long long here = unit_heads * chunk_work(q.length, q.n, unit_tokens, chunk_blocks(q.n, unit_tokens));
                 if (x < here) break;
                 x -= here;
             }
             int block = 0, above = chunk_blocks(q.n, unit_tokens);
             while (above - block > 1) {
                 const int middle = (block + above) >> 1;
-                if (heads * (Whole)chunk_work(q.length, q.n, unit_tokens, middle) <= x) block = middle; else above = middle;
+                if (unit_heads * chunk_work(q.length, q.n, unit_tokens, middle) <= x) block = middle; else above = middle;
             }
             at.block = block;
-            if (block > 0) x -= heads * (Whole)chunk_work(q.length, q.n, unit_tokens, block);
+            if (block > 0) x -= unit_heads * chunk_work(q.length, q.n, unit_tokens, block);
             const int seen = chunk_seen(q.length, q.n, unit_tokens, block), tiles = tiles_of(seen);
-            const Whole work = (Whole)seen + kChunkUnitCost;
-            at.head = x < work ? 0 : (int)(x / work);
-            x -= (Whole)at.head * work;
-            const int tile = (int)min((x + kTile / 2) / kTile, (Whole)tiles);
+            const long long work = (long long)seen + kChunkUnitCost;
+            for (above = unit_heads; above - at.head > 1;) {
+                const int middle = (at.head + above) >> 1;
+                if (middle * work <= x) at.head = middle; else above = middle;
+            }
+            x -= at.head * work;
+            const int tile = (int)min((x + kTile / 2) / kTile, (long long)tiles);
             if (!first && (whole ? 2 * x >= work : tile >= tiles)) next_unit(at, q);  // the first unit is somebody's, if it has no tile
             else at.tile = whole ? 0 : tile;
             return at;
@@ -412,10 +410,14 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
         bool alive = true;
         ChunkPlace at = {p.requests, 0, 0, 0}, stop = at;
         if (blockIdx.x < ctas) {
-            ChunkRequest other = now;
-            const long long from = share_of(blockIdx.x), to = share_of(blockIdx.x + 1);
-            at = short_work ? cut_at((unsigned int)from, now) : cut_at((unsigned long long)from, now);
-            stop = short_work ? cut_at((unsigned int)to, other) : cut_at((unsigned long long)to, other);
+            // The cuts in front and behind, by two lanes at once.
+            const long long cta = blockIdx.x + (lane == 1);
+            const ChunkPlace own = cut_at(share * cta + min(cta, rest), now);
+            auto of = [&](int v, int from) { return __shfl_sync(0xFFFFFFFFu, v, from); };
+            __syncwarp();
+            at = {of(own.request, 0), of(own.block, 0), of(own.head, 0), of(own.tile, 0)};
+            stop = {of(own.request, 1), of(own.block, 1), of(own.head, 1), of(own.tile, 1)};
+            now = {of(now.first, 0), of(now.n, 0), of(now.length, 0)};
         }
         ChunkCut cut = {0, 0, 0, 0, 0, 0};
         auto describe = [&] {  // the next unit
@@ -486,13 +488,15 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
         int id = page_of(u, 0);
         for (; alive; ++count) {
             // The first keys and values are asked for before the unit in front is done with the queries' place.
-            if (u.tiles > 0) {
+            // (The first unit's come behind its queries: nobody is waited for.)
+            auto start = [&] {
                 const int here = id;
                 id = page_of(u, 1);
                 load(u, 0, here, false);
                 if (alive) load(u, 0, here, true);
-                if (!alive) break;
-            }
+            };
+            if (count > 0 && u.tiles > 0) start();
+            if (!alive) break;
             if (count > 0 && !ptx::mbar_wait_spin(&s.q_empty, (count - 1) & 1, abort_flag, kChunkWait)) break;
             if (lane == 0) s.unit = u;
             const int groups_here = u.tokens > p.tile_tokens ? kGroups : 1;
@@ -506,6 +510,7 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
                 const int g = lane / kChunks, c = lane - g * kChunks;
                 ptx::tma_load_3d(q_tiles + g * Shape::kQBytes + c * (kChunkRows * 128), &p.q_map, c * 64, u.head0, u.row0 + g * p.tile_tokens, &s.q_full);
             }
+            if (count == 0 && u.tiles > 0) start();
             ChunkUnit next = {};
             int next_id = 0;
             for (int tile = 1; tile < max(2, u.tiles) && alive; ++tile) {
