@@ -306,7 +306,6 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
         ptx::prefetch_tensor_map(&p.key_map);
         ptx::prefetch_tensor_map(&p.value_map);
     }
-    ptx::griddep_launch_dependents();
     ptx::griddep_wait();
 
     // Work in front of every run of requests.
@@ -324,6 +323,8 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
         if (lane == 0) s.longest[warp] = longest;
     }
     __syncthreads();
+    // Not before this CTA has its tensor memory: the next kernel's could take it and then wait for this one's end.
+    ptx::griddep_launch_dependents();
     if (warp == 0) {
         constexpr int kEach = kChunkRuns / 32;
         long long own[kEach], sum = 0;

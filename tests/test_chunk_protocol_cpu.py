@@ -5,7 +5,9 @@ through mbarriers, whose waits see only the parity of a phase.  The model has th
 order; copies land and the tensor cores work at arbitrary times.  What is read before it is there, overwritten before it has been
 read, or waited for in vain is a fault.  The number of slots of the ring comes from the kernel's header."""
 
+import pathlib
 import random
+import re
 from collections import defaultdict
 
 import pytest
@@ -282,3 +284,20 @@ def test_the_model_finds_a_wait_that_is_two_phases_behind(shapes):
         except Fault:
             found += 1
     assert found > 0
+
+
+def test_tensor_memory_is_taken_before_the_next_kernel_may_start():
+    """A dependent kernel's block may share an SM with one of the kernel in front.  If it could take the tensor memory first, the one in
+    front would wait for it, and it for the end of the one in front: so each block lets dependents start behind a barrier behind
+    its own allocation."""
+    sources = pathlib.Path(__file__).resolve().parent.parent / "metile_b200" / "csrc"
+    found = 0
+    for source in sources.glob("*.cuh"):
+        text = re.sub(r"//[^\n]*", "", source.read_text())
+        for kernel in re.split(r"__global__", text)[1:]:
+            if "ptx::tmem_alloc(" not in kernel:
+                continue
+            found += 1
+            at = kernel.index("ptx::tmem_alloc("), kernel.index("griddep_launch_dependents(")
+            assert at[0] < kernel.index("__syncthreads()", at[0]) < at[1], source.name
+    assert found >= 2
