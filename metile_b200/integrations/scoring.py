@@ -37,6 +37,8 @@ def _flat(texts, what):
 def _read(model, cache, texts, rows, piece, wanted):
     """Read texts[i] as the next tokens of request rows[i], in passes of up to `piece` tokens, and yield (text, first position,
     logits) of the positions that wanted(text, first, count) names, relative to `first`."""
+    if piece < 1:
+        raise ValueError("a pass reads a token or more")
     tables = cache[0].tables
     device = tables.lengths.device
     done = [0] * len(texts)

@@ -193,3 +193,12 @@ def test_log_probabilities_against_torch(cuda_device, model):
     # Logits within the patched model's bound of 2e-2 of their largest: twice that between two of them.
     assert (scores.logprobs.double() - expected).abs().max() <= 4e-2 * float(model(text[None].to(cuda_device))[0].abs().max())
     assert np.isfinite(scores.entropy.cpu().numpy()).all()
+
+
+def test_passes_of_nothing_are_refused(cuda_device, model):
+    prompt = torch.tensor([3, 4, 5])
+    for piece in (0, -3):
+        with pytest.raises(ValueError, match="a token or more"):
+            scoring.score_prompts(model, [prompt], piece=piece)
+        with pytest.raises(ValueError, match="a token or more"):
+            scoring.score_continuations(model, [prompt], [[prompt]], piece=piece)
