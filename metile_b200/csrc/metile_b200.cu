@@ -1012,8 +1012,7 @@ int mt_paged_compact(const int* block_tables, long long table_stride, int width,
 
 size_t mt_token_logprobs_workspace_bytes(int rows, int vocabulary, int top, int type) {
     if (rows <= 0 || vocabulary <= 0 || top < 0) return 0;
-    const int parts = logprob_parts(vocabulary, type);
-    return logprob_stats_bytes(rows, parts) + (size_t)rows * parts * top * sizeof(unsigned long long);
+    return logprob_bytes(rows, logprob_shares(vocabulary, type), top);
 }
 
 int mt_token_logprobs(const void* logits, long long row_stride, int type, const long long* tokens, float* logprobs,
@@ -1029,8 +1028,8 @@ int mt_token_logprobs(const void* logits, long long row_stride, int type, const 
     if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < needed) return MT_ERR_WORKSPACE;
     if (!device_is_sm100()) return MT_ERR_DEVICE;
     LogprobParams params{logits, tokens, logprobs, entropy, top_logprobs, top_tokens, static_cast<LogprobStats*>(workspace), nullptr,
-                         row_stride, rows, vocabulary, logprob_parts(vocabulary, type), top};
-    params.lists = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + logprob_stats_bytes(rows, params.parts));
+                         row_stride, rows, vocabulary, logprob_shares(vocabulary, type), top};
+    params.tops = reinterpret_cast<float*>(static_cast<char*>(workspace) + logprob_stats_bytes(rows, params.shares));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return type == MT_TYPE_FP32 ? launch_token_logprobs<2>(params, s) : type == MT_TYPE_FP16 ? launch_token_logprobs<1>(params, s)
                                                                                                : launch_token_logprobs<0>(params, s);

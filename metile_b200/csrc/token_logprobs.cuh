@@ -1,9 +1,10 @@
 // Log-probabilities of given tokens, with the entropy of their rows and the best alternatives.
 //
 // With m the largest logit of a row and d = x - m:  S = sum e^d,  logprob(t) = d_t - log S,  entropy = log S - sum e^d d / S.
-// One pass over the logits: a CTA takes a part of a row (32 KB), keeps it in registers, and leaves its maximum, the two sums
-// relative to that maximum and its `top` best entries; a second kernel joins the parts, in order and in 64 bits.  Parts
-// have one size for all calls, so a row's bits do not depend on the others.
+// One pass over the logits: a warp takes 4 KB of a row, keeps it in registers, and leaves its maximum, the two sums relative to
+// that maximum, and the maxima of its stretches of 512 bytes; warps do not meet.  A second kernel joins the shares, in order and in 64
+// bits, and looks for the best entries in the stretches with the largest maxima alone.  Shares have one size for all calls, so a row's
+// bits do not depend on the others.
 #pragma once
 
 #include "beam_select.cuh"
@@ -13,11 +14,14 @@ namespace mt {
 
 constexpr unsigned int kTokenOutside = 0x307;  // token_logprobs: word 1 = row, 2 and 3 = the token
 
-constexpr int kLogprobThreads = 256, kLogprobVectors = 8, kLogprobMaxTop = 64, kLogprobJoinThreads = 128;
-constexpr int kLogprobSlack = 16, kLogprobCollect = 512;
-constexpr int kLogprobPartBytes = kLogprobThreads * kLogprobVectors * 16;
-__host__ __device__ constexpr int logprob_part(int type) { return kLogprobPartBytes / beam_size(type); }  // logits
-inline int logprob_parts(int vocabulary, int type) { return (vocabulary + logprob_part(type) - 1) / logprob_part(type); }
+constexpr int kLogprobThreads = 256, kLogprobVectors = 8, kLogprobMaxTop = 64;
+constexpr int kLogprobSlack = 16;      // stretches that may be looked at beside the `top` ones with the largest maxima
+constexpr int kLogprobChosen = kLogprobMaxTop + kLogprobSlack;
+constexpr int kLogprobCollect = 512;
+// A warp's share of a row: stretches of 512 bytes, a vector a lane.
+__host__ __device__ constexpr int logprob_stretch(int type) { return 512 / beam_size(type); }  // logits
+__host__ __device__ constexpr int logprob_share(int type) { return kLogprobVectors * logprob_stretch(type); }
+inline int logprob_shares(int vocabulary, int type) { return (vocabulary + logprob_share(type) - 1) / logprob_share(type); }
 
 struct LogprobStats {
     float top, sum, weighted;  // maximum; sums of e^d and e^d d
@@ -29,10 +33,10 @@ struct LogprobParams {
     float *logprobs, *entropy;  // [rows]
     float* top_logprobs;        // [rows, top]
     long long* top_tokens;      // [rows, top]
-    LogprobStats* stats;        // [rows, parts]
-    unsigned long long* lists;  // [rows, parts, top]: keys, the largest first
+    LogprobStats* stats;        // [rows, shares]
+    float* tops;                // [rows, shares, kLogprobVectors]: maxima of the stretches, where `top` asks for them
     long long row_stride;
-    int rows, vocabulary, parts, top;
+    int rows, vocabulary, shares, top;
 };
 
 // The logits of a vector, 4 of 32 bits or 8 of 16.
@@ -74,14 +78,11 @@ __device__ __forceinline__ float logit_at(const char* base, int i) {
     else if constexpr (kType == 1) return __half2float(reinterpret_cast<const __half*>(base)[i]);
     else return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(base)[i]);
 }
-__device__ __forceinline__ LogprobStats share_stats(float top, const float* sums, const float* weighted) {
-    LogprobStats stats = {top, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kLogprobThreads / 32; ++w) {
-        stats.sum += sums[w];
-        stats.weighted += weighted[w];
-    }
-    return stats;
+// The largest of a warp's numbers, NaN left out; -inf where there are none.
+__device__ __forceinline__ float largest_of_warp(float x) {
+    float out;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(out) : "f"(x));
+    return fmaxf(out, -INFINITY);
 }
 
 // What has been made of the vectors is made again, rather than kept in registers until then.
@@ -93,36 +94,33 @@ __device__ __forceinline__ void forget(uint4 (&v)[kLogprobVectors]) {
 // kAligned: every row starts on 16 bytes.
 template <int kType, bool kAligned>
 __global__ void __launch_bounds__(kLogprobThreads, kAligned ? 4 : 3) token_logprobs_part_kernel(const LogprobParams p) {
-    constexpr int kSize = beam_size(kType), kEach = 16 / kSize, kPart = logprob_part(kType), kWarps = kLogprobThreads / 32;
-    __shared__ float warp_top[kWarps], warp_sum[kWarps], warp_weighted[kWarps];
-    __shared__ unsigned long long warp_key[2][kWarps], collected[kLogprobCollect];
-    __shared__ unsigned int thread_top[kLogprobThreads], bound;
-    __shared__ int found;
-    const int row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int first = part * kPart, count = min(kPart, p.vocabulary - first);  // of this part
+    constexpr int kSize = beam_size(kType), kEach = 16 / kSize, kShare = logprob_share(kType);
+    const int lane = threadIdx.x & 31, item = blockIdx.x * (kLogprobThreads / 32) + (int)(threadIdx.x >> 5);
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
+    if (item >= p.rows * p.shares) return;
+    const int row = item / p.shares, first = (item - row * p.shares) * kShare, count = min(kShare, p.vocabulary - first);
     const char* base = static_cast<const char*>(p.logits) + (row * p.row_stride + first) * kSize;
     uint4 v[kLogprobVectors];
     if constexpr (kAligned) {
 #pragma unroll
         for (int i = 0; i < kLogprobVectors; ++i) {
-            const int at = (i * kLogprobThreads + threadIdx.x) * kEach;
+            const int at = (i * 32 + lane) * kEach;
             v[i] = at < count ? ptx::ld_global_dependent_u4(base + (size_t)at * kSize) : make_uint4(0u, 0u, 0u, 0u);
         }
     } else {
         // A row may start anywhere: the two aligned vectors that a vector lies in, shifted; the second one is the next lane's first.
         const int shift = (int)(reinterpret_cast<uintptr_t>(base) & 15), bits = (shift & 3) * 8;
         const char* aligned = base - shift;
-        // Vectors that hold a logit of the part.
+        // Vectors that hold a logit of the share.
         auto load = [&](int at) { return at * kEach - shift / kSize < count ? ptx::ld_global_dependent_u4(aligned + (size_t)at * 16) : make_uint4(0u, 0u, 0u, 0u); };
 #pragma unroll
-        for (int i = 0; i < kLogprobVectors; ++i) v[i] = load(i * kLogprobThreads + threadIdx.x);
+        for (int i = 0; i < kLogprobVectors; ++i) v[i] = load(i * 32 + lane);
 #pragma unroll
         for (int i = 0; i < kLogprobVectors; ++i) {
             uint4 next = {__shfl_down_sync(0xFFFFFFFFu, v[i].x, 1), __shfl_down_sync(0xFFFFFFFFu, v[i].y, 1), __shfl_down_sync(0xFFFFFFFFu, v[i].z, 1),
                           __shfl_down_sync(0xFFFFFFFFu, v[i].w, 1)};
-            if (lane == 31) next = load(i * kLogprobThreads + threadIdx.x + 1);
+            if (lane == 31) next = load(i * 32 + 32);
             uint32_t w[7] = {v[i].x, v[i].y, v[i].z, v[i].w, next.x, next.y, next.z}, last = next.w;
             if (shift & 8) {
 #pragma unroll
@@ -136,10 +134,10 @@ __global__ void __launch_bounds__(kLogprobThreads, kAligned ? 4 : 3) token_logpr
             v[i] = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
         }
     }
-    // Logits behind the part count as -inf; a thread has element e of vector i if e < there(i).
-    auto there = [&](int i) { return count - (i * kLogprobThreads + (int)threadIdx.x) * kEach; };
+    // Logits behind the row count as -inf; a thread has element e of vector i if e < there(i).
+    auto there = [&](int i) { return count - (i * 32 + lane) * kEach; };
     constexpr uint32_t kNothing = kType == 2 ? 0xFF800000u : kType == 1 ? 0xFC00u : 0xFF80u;
-    if (count < kPart) {
+    if (count < kShare) {
 #pragma unroll
         for (int i = 0; i < kLogprobVectors; ++i) {
             const int left = there(i);
@@ -157,17 +155,19 @@ __global__ void __launch_bounds__(kLogprobThreads, kAligned ? 4 : 3) token_logpr
             v[i] = make_uint4(words[0], words[1], words[2], words[3]);
         }
     }
-    float top = largest_logit<kType>(v[0]);
+    float tops[kLogprobVectors], all = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < kLogprobVectors; ++i) top = fmaxf(top, largest_logit<kType>(v[i]));
+    for (int i = 0; i < kLogprobVectors; ++i) {
+        tops[i] = largest_of_warp(largest_logit<kType>(v[i]));
+        all = fmaxf(all, tops[i]);
+    }
+    if (p.top > 0) {
+        float own = tops[0];
+#pragma unroll
+        for (int i = 1; i < kLogprobVectors; ++i) own = lane == i ? tops[i] : own;
+        if (lane < kLogprobVectors) p.tops[(size_t)item * kLogprobVectors + lane] = own;
+    }
     forget(v);
-    float all = top;
-#pragma unroll
-    for (int offset = 16; offset >= 1; offset >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, offset));
-    if (lane == 0) warp_top[warp] = all;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) all = fmaxf(all, warp_top[w]);
     // Where all are -inf their exponentials are none; a NaN is one.  In powers of two: e = (x - m) log2 e, sums of 2^e and of 2^e e.
     constexpr float kLog2E = 1.4426950408889634f;
     const float against = all == -INFINITY ? 0.0f : -all;
@@ -193,115 +193,13 @@ __global__ void __launch_bounds__(kLogprobThreads, kAligned ? 4 : 3) token_logpr
         for (int i = 0; i < kLogprobVectors; ++i)
 #pragma unroll 1
             for (int j = 0; j < min(kEach, there(i)); ++j) {
-                const float e = (logit_at<kType>(base, (i * kLogprobThreads + (int)threadIdx.x) * kEach + j) + against) * kLog2E, power = power_of_two(e);
+                const float e = (logit_at<kType>(base, (i * 32 + lane) * kEach + j) + against) * kLog2E, power = power_of_two(e);
                 weighted += power == 0.0f ? 0.0f : power * e;
             }
     }
-    forget(v);
     sum = warp_sum_xor(sum);
     weighted = warp_sum_xor(weighted);
-    if (lane == 0) {
-        warp_sum[warp] = sum;
-        warp_weighted[warp] = weighted * 0.6931471805599453f;
-    }
-    if (p.top == 0) {
-        __syncthreads();
-        if (threadIdx.x == 0) p.stats[blockIdx.x] = share_stats(all, warp_sum, warp_weighted);
-        return;
-    }
-    // The best.  At least `top` threads have a logit at or above a bound that is found by halving; only they look for those that reach
-    // it, and what they find is ranked.  The bound need not be the best one: up to kLogprobSlack threads more may reach it.
-    const unsigned int own = there(0) > 0 ? beam_logit_order(top) : 0u;  // threads behind the part have none
-    const int threads = min(kLogprobThreads, (count + kEach - 1) / kEach);
-    thread_top[threadIdx.x] = own;
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
-    if (warp == 0) {
-        unsigned int low = 1u;
-        if (threads > p.top + kLogprobSlack) {
-            unsigned int tops[kWarps], least = ~0u, high = beam_logit_order(all) + 1u;  // the count reaches `top` at `low`, not at `high`
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                tops[w] = thread_top[32 * w + lane];
-                least = min(least, tops[w] - 1u);  // none: the largest
-            }
-            low = __reduce_min_sync(0xFFFFFFFFu, least) + 1u;
-            while (high - low > 1u) {
-                const unsigned int middle = low + (high - low) / 2;
-                int reach = 0;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) reach += tops[w] >= middle;
-                reach = __reduce_add_sync(0xFFFFFFFFu, reach);
-                if (reach >= p.top) low = middle; else high = middle;
-                if (reach >= p.top && reach <= p.top + kLogprobSlack) break;
-            }
-        }
-        if (lane == 0) bound = low;
-    }
-    __syncthreads();
-    const unsigned int low = bound;
-    if (threadIdx.x == 0) p.stats[blockIdx.x] = share_stats(all, warp_sum, warp_weighted);
-    if (own >= low) {
-        const float least = low <= 1u ? -INFINITY : beam_ordered_logit(low);
-        unsigned int vectors = 0;  // with a logit that reaches it
-#pragma unroll
-        for (int i = 0; i < kLogprobVectors; ++i) vectors |= (largest_logit<kType>(v[i]) >= least ? 1u : 0u) << i;
-        for (; vectors; vectors &= vectors - 1u) {  // read again: an index into the registers would move them, and eight copies of this do not fit the cache
-            const int at = ((__ffs(vectors) - 1) * kLogprobThreads + (int)threadIdx.x) * kEach, here = min(kEach, count - at);
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                if (e >= here) break;
-                const float x = logit_at<kType>(base, at + e);
-                if (!(x >= least)) continue;
-                const int to = atomicAdd(&found, 1);
-                if (to < kLogprobCollect) collected[to] = beam_entry_key(x, first + at + e);
-            }
-        }
-    }
-    __syncthreads();
-    const int many = found;
-    unsigned long long* list = p.lists + (size_t)blockIdx.x * p.top;
-    if (many <= kLogprobCollect) {
-        for (int i = threadIdx.x; i < many; i += kLogprobThreads) {
-            const unsigned long long key = collected[i];
-            int rank = 0;
-            for (int j = 0; j < many; ++j) rank += collected[j] > key;
-            if (rank < p.top) list[rank] = key;
-        }
-        for (int i = many + threadIdx.x; i < p.top; i += kLogprobThreads) list[i] = 0;  // the part has fewer
-        return;
-    }
-    // More than are collected reach the bound (equal ones, or all of them one thread's): one after the other, every thread offering
-    // the best of its own below the last one taken.
-    unsigned long long last = ~0ull, best = 0;
-    auto look = [&] {
-        best = 0;
-#pragma unroll 1
-        for (int i = 0; i < kLogprobVectors; ++i)
-#pragma unroll 1
-            for (int e = 0; e < kEach; ++e) {
-                if (e >= there(i)) continue;
-                const int token = (i * kLogprobThreads + (int)threadIdx.x) * kEach + e;  // read again: an index into the registers would move them
-                const unsigned long long key = beam_entry_key(logit_at<kType>(base, token), first + token);
-                if (key < last && key > best) best = key;
-            }
-    };
-    look();
-    for (int k = 0; k < p.top; ++k) {
-        unsigned int upper = (unsigned int)(best >> 32), lower = (unsigned int)best;
-        const unsigned int highest = __reduce_max_sync(0xFFFFFFFFu, upper);
-        lower = __reduce_max_sync(0xFFFFFFFFu, upper == highest ? lower : 0u);
-        if (lane == 0) warp_key[k & 1][warp] = (unsigned long long)highest << 32 | lower;
-        __syncthreads();
-        unsigned long long winner = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) winner = max(winner, warp_key[k & 1][w]);
-        if (threadIdx.x == 0) list[k] = winner;
-        if (best == winner && winner != 0) {
-            last = winner;
-            look();
-        }
-    }
+    if (lane == 0) p.stats[item] = {all, sum, weighted * 0.6931471805599453f};
 }
 
 __device__ __forceinline__ double warp_sum_double(double v) {
@@ -310,24 +208,84 @@ __device__ __forceinline__ double warp_sum_double(double v) {
     return v;
 }
 
-// A CTA joins the parts of a row: its first warp the sums, a part a lane, while the others fetch the lists.
-__global__ void __launch_bounds__(kLogprobJoinThreads) token_logprobs_join_kernel(const LogprobParams p, int type) {
-    extern __shared__ unsigned long long keys[];  // [parts, top]
+// A CTA joins the shares of a row and finds its best entries: its first warp the sums, a share a lane, while the second one chooses
+// the stretches that the best lie in.  `top` stretches reach the `top`-th largest of their maxima, and so do `top` logits: only what
+// reaches it is collected and ranked.  Of stretches with just that maximum the first ones will do.
+template <int kType, int kThreads>
+__global__ void __launch_bounds__(kThreads) token_logprobs_join_kernel(const LogprobParams p) {
+    constexpr int kSize = beam_size(kType), kStretch = logprob_stretch(kType), kWarps = kThreads / 32, kEach = kStretch / 32;
+    // Logits are looked for by their order, without the bits that those of the type have all alike: fewer halvings.
+    constexpr int kShift = kType == 2 ? 0 : kType == 1 ? 13 : 16;
+    extern __shared__ unsigned int orders[];  // of the maxima of the stretches
     __shared__ double shared_lse, shared_top;
-    const int row = blockIdx.x, entries = p.parts * p.top;
+    __shared__ unsigned long long collected[kLogprobCollect];
+    __shared__ unsigned int bound;
+    __shared__ int chosen_stretch[kLogprobChosen], chosen_count, found, counted[2][kWarps];
+    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, stretches = (p.vocabulary + kStretch - 1) / kStretch;
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    if (threadIdx.x < 32) {
-        const LogprobStats* stats = p.stats + (size_t)row * p.parts;
+    const char* base = static_cast<const char*>(p.logits) + row * p.row_stride * beam_size(kType);
+    // The aligned vectors of stretches, dealt to the threads, four of them on their way at once: use(stretch, token, hits) learns which of
+    // the logits from `token` on reach(logit).  Some of them may lie beside the stretch.
+    const int shift = (int)(reinterpret_cast<uintptr_t>(base) & 15), before = shift / kSize, vectors = shift ? 33 : 32;
+    auto visit = [&](int count, auto stretch_of, auto reach, auto use) {
+        constexpr int kAtOnce = 4;
+        for (int j = threadIdx.x; j < count * vectors; j += kAtOnce * kThreads) {
+            uint4 v[kAtOnce];
+            int stretch[kAtOnce], token[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                const int at = j + i * kThreads, k = at / vectors;
+                v[i] = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN
+                if (at >= count * vectors) continue;
+                stretch[i] = stretch_of(k);
+                token[i] = stretch[i] * kStretch + (at - k * vectors) * kEach - before;
+                if (token[i] < p.vocabulary) v[i] = ptx::ld_global_dependent_u4(base + (long long)token[i] * kSize);
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                unsigned int hits = 0;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) hits |= (reach(logit_of<kType>(v[i], e)) ? 1u : 0u) << e;
+                if (hits) use(stretch[i], token[i], hits);
+            }
+        }
+    };
+    auto within = [&](int stretch, int token) { return token >= stretch * kStretch && token < min(p.vocabulary, (stretch + 1) * kStretch); };
+    // Where there are few stretches, all of them are looked at, and the bound is that of the threads' maxima.
+    const bool few = stretches <= p.top + kLogprobSlack;
+    const int maxima = few ? kThreads : stretches;
+    if (p.top > 0) {
+        if (few) {
+            unsigned int most = 0u;  // of a thread that has none
+#pragma unroll 4
+            for (int token = (int)threadIdx.x * kEach - before; token < p.vocabulary; token += kThreads * kEach) {
+                const uint4 v = ptx::ld_global_dependent_u4(base + (long long)token * kSize);
+                float x = largest_logit<kType>(v);
+                if (token < 0 || token + kEach > p.vocabulary) {
+                    x = NAN;
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e)
+                        if (token + e >= 0 && token + e < p.vocabulary) x = fmaxf(x, logit_of<kType>(v, e));
+                }
+                if (x == x) most = max(most, beam_logit_order(x) >> kShift);
+            }
+            orders[threadIdx.x] = most;
+        } else {
+            const float* tops = p.tops + (size_t)row * p.shares * kLogprobVectors;
+            for (int i = threadIdx.x; i < stretches; i += kThreads) orders[i] = beam_logit_order(tops[i]) >> kShift;
+        }
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
+    }
+    if (warp == 0) {
+        const LogprobStats* stats = p.stats + (size_t)row * p.shares;
         const long long token = threadIdx.x == 0 ? p.tokens[row] : -1;
         float chosen = 0.0f;
-        if (token >= 0 && token < p.vocabulary) {
-            const char* at = static_cast<const char*>(p.logits) + (row * p.row_stride + token) * beam_size(type);
-            chosen = type == MT_TYPE_FP32 ? logit_at<2>(at, 0) : type == MT_TYPE_FP16 ? logit_at<1>(at, 0) : logit_at<0>(at, 0);
-        }
+        if (token >= 0 && token < p.vocabulary) chosen = logit_at<kType>(base + token * kSize, 0);
         float top = -INFINITY;
         bool usable = true;  // neither NaN nor +inf
-        for (int i = threadIdx.x; i < p.parts; i += 32) {
+        for (int i = threadIdx.x; i < p.shares; i += 32) {
             top = fmaxf(top, stats[i].top);
             usable = usable && stats[i].sum <= 3e38f;
         }
@@ -335,7 +293,7 @@ __global__ void __launch_bounds__(kLogprobJoinThreads) token_logprobs_join_kerne
         for (int offset = 16; offset >= 1; offset >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
         usable = __all_sync(0xFFFFFFFFu, usable) && top != -INFINITY && top != INFINITY;
         double sum = 0.0, weighted = 0.0;
-        for (int i = threadIdx.x; i < p.parts; i += 32) {
+        for (int i = threadIdx.x; i < p.shares; i += 32) {
             const LogprobStats part = stats[i];
             if (part.top == -INFINITY) continue;
             const double d = (double)part.top - top, factor = exp(d);
@@ -352,43 +310,144 @@ __global__ void __launch_bounds__(kLogprobJoinThreads) token_logprobs_join_kerne
             if (token >= p.vocabulary) record_index(kTokenOutside, row, (unsigned long long)token);
             p.logprobs[row] = token < 0 ? 0.0f : token >= p.vocabulary ? NAN : (float)((double)chosen - top - log_sum);
         }
-    } else {
-        const unsigned long long* lists = p.lists + (size_t)row * entries;
-        for (int i = threadIdx.x - 32; i < entries; i += blockDim.x - 32) keys[i] = lists[i];
+    } else if (warp == 1 && p.top > 0) {
+        unsigned int low = ~0u, high = 0u;  // as many as are wanted reach `low`, fewer reach `high`
+        int reach = maxima, beyond = 0;
+        for (int i = lane; i < maxima; i += 32) {
+            low = min(low, orders[i]);
+            high = max(high, orders[i]);
+        }
+        low = __reduce_min_sync(0xFFFFFFFFu, low);
+        high = __reduce_max_sync(0xFFFFFFFFu, high) + 1u;
+        while (high - low > 1u && reach > p.top + kLogprobSlack) {
+            const unsigned int middle = low + (high - low) / 2;
+            int here = 0;
+            for (int i = lane; i < maxima; i += 32) here += orders[i] >= middle;
+            here = __reduce_add_sync(0xFFFFFFFFu, here);
+            if (here >= p.top) {
+                low = middle;
+                reach = here;
+            } else {
+                high = middle;
+                beyond = here;
+            }
+        }
+        // All that reach it, or, where they are too many, those beyond it and the first others.
+        int others = reach > p.top + kLogprobSlack ? p.top - beyond : kLogprobChosen, taken = 0;
+        for (int start = 0; start < stretches; start += 32) {
+            const int i = start + lane;
+            const bool reaches = i < stretches && (few || orders[i] >= low), equal = reaches && !few && orders[i] == low;
+            const unsigned int equals = __ballot_sync(0xFFFFFFFFu, equal);
+            const bool takes = reaches && (!equal || __popc(equals & ((1u << lane) - 1u)) < others);
+            others -= __popc(equals);
+            const unsigned int votes = __ballot_sync(0xFFFFFFFFu, takes);
+            if (takes) chosen_stretch[taken + __popc(votes & ((1u << lane) - 1u))] = i;
+            taken += __popc(votes);
+        }
+        if (lane == 0) {
+            chosen_count = taken;
+            bound = low;
+        }
     }
     if (p.top == 0) return;
     __syncthreads();
     const double lse = shared_lse, largest = shared_top;
-    const bool usable = lse == lse;
-    for (int i = threadIdx.x; i < entries; i += blockDim.x) {
-        // Its place: its own in its list, and in every other as many as are larger.
-        const int part = i / p.top, own = i - part * p.top;
-        const unsigned long long key = keys[i];
-        int rank = own;
-        if (usable && key == 0) continue;
-        for (int other = 0; other < p.parts && rank < p.top; ++other) {
-            if (other == part) continue;
-            int low = 0, high = p.top;  // keys before `low` are larger, those from `high` on are not
-            while (low < high) {
-                const int middle = (low + high) >> 1;
-                if (keys[other * p.top + middle] > key) low = middle + 1; else high = middle;
-            }
-            rank += low;
+    float* logprobs = p.top_logprobs + (size_t)row * p.top;
+    long long* tokens = p.top_tokens + (size_t)row * p.top;
+    if (lse != lse) {  // the row has no distribution
+        for (int i = threadIdx.x; i < p.top; i += kThreads) {
+            logprobs[i] = NAN;
+            tokens[i] = -1;
         }
-        if (!usable) rank = i;  // the row has no distribution
+        return;
+    }
+    const int chosen = chosen_count;
+    unsigned int low = bound;
+    auto least_of = [&](unsigned int order) { return order << kShift <= beam_logit_order(-INFINITY) ? -INFINITY : beam_ordered_logit(order << kShift); };
+    auto collect = [&](unsigned int order) {
+        const float least = least_of(order);
+        visit(chosen, [&](int k) { return chosen_stretch[k]; }, [&](float x) { return x >= least; }, [&](int stretch, int token, unsigned int hits) {
+            for (; hits; hits &= hits - 1u) {
+                const int at = token + __ffs(hits) - 1;
+                if (!within(stretch, at)) continue;
+                const int to = atomicAdd(&found, 1);
+                if (to < kLogprobCollect) collected[to] = beam_entry_key(logit_at<kType>(base, at), at);
+            }
+        });
+    };
+    collect(low);
+    __syncthreads();
+    int many = found;
+    if (many > kLogprobCollect) {
+        // More than are collected reach it.  `top` at least reach `low`, fewer reach `high`.
+        __syncthreads();
+        unsigned int high = (beam_logit_order((float)largest) >> kShift) + 1u;
+        for (int round = 0; high - low > 1u && many > kLogprobCollect; ++round) {
+            const unsigned int middle = low + (high - low) / 2;
+            const float least = least_of(middle);
+            int here = 0;
+            visit(chosen, [&](int k) { return chosen_stretch[k]; }, [&](float x) { return x >= least; }, [&](int stretch, int token, unsigned int hits) {
+                for (; hits; hits &= hits - 1u) here += within(stretch, token + __ffs(hits) - 1);
+            });
+            here = __reduce_add_sync(0xFFFFFFFFu, here);
+            if (lane == 0) counted[round & 1][warp] = here;
+            __syncthreads();
+            here = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) here += counted[round & 1][w];
+            if (here >= p.top) {
+                low = middle;
+                many = here;
+            } else {
+                high = middle;
+            }
+        }
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
+        const bool equals = many > kLogprobCollect;  // hundreds are equal: those beyond them, and of them the first
+        collect(equals ? high : low);
+        __syncthreads();
+        many = found;
+        if (equals) {
+            if (warp == 0)
+                for (int k = 0, have = many; k < chosen && have < p.top; ++k) {
+                    float x[kEach];
+                    const int first = chosen_stretch[k] * kStretch + lane;
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) x[e] = first + 32 * e < p.vocabulary ? logit_at<kType>(base, first + 32 * e) : NAN;
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) {
+                        const bool equal = x[e] == x[e] && beam_logit_order(x[e]) >> kShift == low;
+                        const unsigned int votes = __ballot_sync(0xFFFFFFFFu, equal);
+                        const int to = have + __popc(votes & ((1u << lane) - 1u));
+                        if (equal && to < p.top) collected[to] = beam_entry_key(x[e], first + 32 * e);
+                        have += __popc(votes);
+                    }
+                }
+            many = p.top;
+            __syncthreads();
+        }
+    }
+    for (int i = threadIdx.x; i < many; i += kThreads) {
+        const unsigned long long key = collected[i];
+        int rank = 0;
+        for (int j = 0; j < many; ++j) rank += collected[j] > key;
         if (rank >= p.top) continue;
         const BeamEntry entry = beam_entry(key);
-        p.top_logprobs[(size_t)row * p.top + rank] = usable ? (float)((double)entry.logit - largest - lse) : NAN;
-        p.top_tokens[(size_t)row * p.top + rank] = usable ? entry.token : -1;
+        logprobs[rank] = (float)((double)entry.logit - largest - lse);
+        tokens[rank] = entry.token;
     }
 }
 
-inline size_t logprob_stats_bytes(int rows, int parts) { return ((size_t)rows * parts * sizeof(LogprobStats) + 15) / 16 * 16; }
+inline size_t logprob_stats_bytes(int rows, int shares) { return ((size_t)rows * shares * sizeof(LogprobStats) + 15) / 16 * 16; }
+inline size_t logprob_bytes(int rows, int shares, int top) {
+    return logprob_stats_bytes(rows, shares) + (top > 0 ? (size_t)rows * shares * kLogprobVectors * sizeof(float) : 0);
+}
 
 template <int kType>
 inline int launch_token_logprobs(const LogprobParams& params, cudaStream_t stream) {
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(params.rows * params.parts, 1, 1);
+    config.gridDim = dim3((params.rows * params.shares + kLogprobThreads / 32 - 1) / (kLogprobThreads / 32), 1, 1);
     config.blockDim = dim3(kLogprobThreads, 1, 1);
     config.stream = stream;
     cudaLaunchAttribute attrs[1];
@@ -398,10 +457,14 @@ inline int launch_token_logprobs(const LogprobParams& params, cudaStream_t strea
     config.numAttrs = 1;
     const bool aligned = aligned_to(params.logits, 16) && (params.rows == 1 || params.row_stride * beam_size(kType) % 16 == 0);
     if (cudaLaunchKernelEx(&config, aligned ? token_logprobs_part_kernel<kType, true> : token_logprobs_part_kernel<kType, false>, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    // Rows enough to fill the chip have smaller CTAs: 2001 rows of 128256 with 20 alternatives 124 us (127 with 256 threads), 8 rows of 32001
+    // with 5 12.7 (12.2), of 16000 with 64 17.4 (13.5).
+    const bool many = params.rows >= 1024;
+    const int threads = many ? 128 : 256, stretches = (params.vocabulary + logprob_stretch(kType) - 1) / logprob_stretch(kType);
     config.gridDim = dim3(params.rows, 1, 1);
-    config.blockDim = dim3(kLogprobJoinThreads, 1, 1);
-    config.dynamicSmemBytes = (size_t)params.parts * params.top * sizeof(unsigned long long);
-    return cudaLaunchKernelEx(&config, token_logprobs_join_kernel, params, kType) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    config.blockDim = dim3(threads, 1, 1);
+    config.dynamicSmemBytes = params.top > 0 ? (stretches > threads ? stretches : threads) * sizeof(unsigned int) : 0;
+    return cudaLaunchKernelEx(&config, many ? token_logprobs_join_kernel<kType, 128> : token_logprobs_join_kernel<kType, 256>, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
 }
 
 }  // namespace mt

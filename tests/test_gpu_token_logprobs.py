@@ -72,13 +72,50 @@ def test_equal_logits_go_by_the_lower_token(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_best_entries_that_one_thread_has(cuda_device, dtype):
-    """Entries 2048 (fp32: 1024) apart are one thread's: none of the others has any of the best."""
+def test_best_entries_in_few_places(cuda_device, dtype):
+    """Entries 2048 (fp32: 1024) apart, and all of them side by side."""
     logits = normal(4, 2, 50000, device=cuda_device, dtype=dtype, std=1.0)
     step = 2048 if dtype == torch.bfloat16 else 1024
     logits[0, 5::step] = 20.0 + torch.arange(len(range(5, 50000, step)), device=cuda_device) % 3
     logits[1, :600] = 30.0
     check(logits, chosen(5, 2, 50000, cuda_device), 64)
+
+
+@pytest.mark.parametrize("rows,vocab,top,dtype", [
+    (1100, 4099, 20, torch.bfloat16), (1024, 33, 33, torch.float32), (1031, 20480, 64, torch.float16), (1025, 9001, 3, torch.bfloat16),
+])
+def test_many_rows(cuda_device, rows, vocab, top, dtype):
+    check(normal(rows + vocab, rows, vocab, device=cuda_device, dtype=dtype), chosen(vocab, rows, vocab, cuda_device), top)
+
+
+@pytest.mark.parametrize("rows", [7, 1024])
+@pytest.mark.parametrize("vocab,top,dtype", [(1000, 5, torch.bfloat16), (5001, 20, torch.float16), (20479, 64, torch.bfloat16), (30003, 64, torch.float32),
+                                             (33000, 1, torch.float16), (20737, 64, torch.bfloat16)])
+def test_where_the_best_lie(cuda_device, rows, vocab, top, dtype):
+    """Rising and falling rows, constant ones, all but a few tokens masked, and hundreds of equal ones behind a few larger ones."""
+    logits = normal(vocab, rows, vocab, device=cuda_device, dtype=dtype)
+    position = torch.arange(vocab, device=cuda_device)
+    logits[0] = position.to(dtype) / 16
+    logits[1] = -(position.to(dtype)) / 16
+    logits[2] = -3.0
+    logits[3] = -torch.inf
+    logits[3, vocab // 3:vocab // 3 + 7] = torch.arange(7, device=cuda_device).to(dtype)
+    logits[4] = torch.finfo(dtype).min
+    logits[4, -9:] = 1.0
+    logits[5, vocab // 4:vocab // 4 + 700] = 40.0
+    logits[5, -3:] = 41.0
+    logits[6] = 0.0
+    logits[6, ::2] = -0.0
+    logits[6, vocab - 1] = 1.0
+    # (The oracle looks at some rows; the others are held to each other.)
+    tokens = chosen(vocab, rows, vocab, cuda_device)
+    got = check(logits[:7], tokens[:7], top)
+    whole = B.token_logprobs(logits, tokens, top=top)
+    assert all(torch.equal(a, b[:7]) for a, b in zip(got, whole))
+    wide = torch.zeros((7, vocab + 5), dtype=dtype, device=cuda_device)
+    for offset in (1, 5):
+        wide[:, offset:offset + vocab] = logits[:7]
+        assert all(torch.equal(a, b) for a, b in zip(got, B.token_logprobs(wide[:, offset:offset + vocab], tokens[:7], top=top)))
 
 
 def test_rows_that_start_anywhere(cuda_device):
