@@ -1,7 +1,7 @@
 // Log-probabilities of given tokens, with the entropy of their rows and the best alternatives.
 //
 // With m the largest logit of a row and d = x - m:  S = sum e^d,  logprob(t) = d_t - log S,  entropy = log S - sum e^d d / S.
-// One pass over the logits: a warp takes 4 KB of a row, keeps it in registers, and leaves its maximum, the two sums relative to
+// One pass over the logits: a warp takes 2 KB of a row, keeps it in registers, and leaves its maximum, the two sums relative to
 // that maximum, and the maxima of its stretches of 512 bytes; warps do not meet.  A second kernel joins the shares, in order and in 64
 // bits, and looks for the best entries in the stretches with the largest maxima alone.  Shares have one size for all calls, so a row's
 // bits do not depend on the others.
@@ -14,7 +14,7 @@ namespace mt {
 
 constexpr unsigned int kTokenOutside = 0x307;  // token_logprobs: word 1 = row, 2 and 3 = the token
 
-constexpr int kLogprobThreads = 256, kLogprobVectors = 8, kLogprobMaxTop = 64;
+constexpr int kLogprobThreads = 256, kLogprobVectors = 4, kLogprobMaxTop = 64;
 constexpr int kLogprobSlack = 16;      // stretches that may be looked at beside the `top` ones with the largest maxima
 constexpr int kLogprobChosen = kLogprobMaxTop + kLogprobSlack;
 constexpr int kLogprobCollect = 512;
@@ -93,7 +93,7 @@ __device__ __forceinline__ void forget(uint4 (&v)[kLogprobVectors]) {
 
 // kAligned: every row starts on 16 bytes.
 template <int kType, bool kAligned>
-__global__ void __launch_bounds__(kLogprobThreads, kAligned ? 4 : 3) token_logprobs_part_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kLogprobThreads, kAligned ? 6 : 5) token_logprobs_part_kernel(const LogprobParams p) {
     constexpr int kSize = beam_size(kType), kEach = 16 / kSize, kShare = logprob_share(kType);
     const int lane = threadIdx.x & 31, item = blockIdx.x * (kLogprobThreads / 32) + (int)(threadIdx.x >> 5);
     ptx::griddep_launch_dependents();
