@@ -25,6 +25,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "affine_umma.cuh"
 #include "beam_select.cuh"
 #include "paged_attention.cuh"
@@ -883,69 +885,109 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
     }
 }
 
-// Joins the parts of the units that were cut, in their order: CTA (x, y) rows of the unit that CTA x began, a row a warp and four of
-// them on their way at once.
-constexpr int kChunkJoinWarps = 8, kChunkJoinRows = 4;
+// Joins the parts of the units that were cut, in their order.  The rows of the unit that CTA b began are dealt to the CTAs (b, y) up to
+// (b', y), where b' begins the next one, at most 32 on; a row a warp, several of them or of their parts on their way at once.
+constexpr int kChunkJoinWarps = 8, kChunkJoinColumns = 4, kChunkJoinReach = 32;
 
 template <int kD, bool kHalf>
 __global__ void __launch_bounds__(kChunkJoinWarps * 32) paged_chunk_join_kernel(const __grid_constant__ PagedChunkParams p, int ctas) {
     using Shape = ChunkShape<kD>;
-    constexpr int kPairs = kD / 64;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    using Numbers = typename std::conditional<kD == 64, float2, float4>::type;
+    constexpr int kEach = kD / 32, kLoads = kEach * 4 / (int)sizeof(Numbers);  // numbers of a row that a lane has
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, x = blockIdx.x;
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    const ChunkCut cut = p.cuts[blockIdx.x];
-    if (cut.tokens == 0) return;
-    // Part 0 is this CTA's second slot, part i the first slot of the i-th CTA behind it.
-    int parts = 2;
-    while (blockIdx.x + parts < ctas && p.cuts[blockIdx.x + parts - 1].through) ++parts;
-    int slot_row[kChunkJoinRows];
-    long long to[kChunkJoinRows];  // row and head of the result, or -1
-    float top[kChunkJoinRows], total[kChunkJoinRows];
-    float2 value[kChunkJoinRows][kPairs];
-#pragma unroll
-    for (int k = 0; k < kChunkJoinRows; ++k) {
-        slot_row[k] = (blockIdx.y * kChunkJoinRows + k) * kChunkJoinWarps + warp;
-        const int g = slot_row[k] / kChunkRows, in_tile = slot_row[k] - g * kChunkRows, tile_token = in_tile / p.part_heads, head = in_tile - tile_token * p.part_heads;
-        const int token = g * p.tile_tokens + tile_token;
-        const bool real = tile_token < p.tile_tokens && token < cut.tokens && head < cut.heads;
-        to[k] = real ? (long long)(cut.row0 + token) * p.q_heads + cut.head0 + head : -1;
-        top[k] = -INFINITY;
-        total[k] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) value[k][i] = make_float2(0.0f, 0.0f);
+    const unsigned int began = __ballot_sync(0xFFFFFFFFu, lane <= x && p.cuts[x - lane].tokens > 0);
+    if (began == 0) return;
+    const int b = x - (__ffs(began) - 1);
+    const ChunkCut cut = p.cuts[b];
+    // Part 0 is that CTA's second slot, part i the first slot of the i-th CTA behind it.
+    int parts = 2, helpers = 0;
+    for (bool more = true; more;) {
+        const int cta = b + parts - 1 + lane;
+        const bool there = cta < ctas;
+        const unsigned int ends = __ballot_sync(0xFFFFFFFFu, !there || !p.cuts[cta].through);
+        if (helpers == 0) {
+            const unsigned int begins = __ballot_sync(0xFFFFFFFFu, !there || p.cuts[cta].tokens > 0);
+            helpers = begins ? __ffs(begins) : kChunkJoinReach;
+        }
+        more = ends == 0;
+        parts += more ? 32 : __ffs(ends) - 1;
     }
-#pragma unroll 4
-    for (int part = 0; part < parts; ++part) {
-        const long long slot = ((long long)(blockIdx.x + part) * 2 + (part == 0)) * Shape::kSlotRows;
-        float2 own[kChunkJoinRows], numbers[kChunkJoinRows][kPairs];
+    parts = min(parts, ctas - b);
+    if (x - b >= helpers) return;
+    const int workers = helpers * kChunkJoinColumns * kChunkJoinWarps;
+    auto join = [&](int first, auto rows_tag, auto parts_tag) {
+        constexpr int kRows = decltype(rows_tag)::value, kParts = decltype(parts_tag)::value;
+        int slot_row[kRows];
+        long long to[kRows];  // row and head of the result, or -1
+        float top[kRows], total[kRows], value[kRows][kEach];
 #pragma unroll
-        for (int k = 0; k < kChunkJoinRows; ++k) {
-            own[k] = make_float2(-INFINITY, 0.0f);
+        for (int k = 0; k < kRows; ++k) {
+            slot_row[k] = first + k * workers;
+            const int g = slot_row[k] / kChunkRows, in_tile = slot_row[k] - g * kChunkRows, tile_token = in_tile / p.part_heads, head = in_tile - tile_token * p.part_heads;
+            const int token = g * p.tile_tokens + tile_token;
+            const bool real = slot_row[k] < Shape::kSlotRows && tile_token < p.tile_tokens && token < cut.tokens && head < cut.heads;
+            to[k] = real ? (long long)(cut.row0 + token) * p.q_heads + cut.head0 + head : -1;
+            top[k] = -INFINITY;
+            total[k] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) value[k][e] = 0.0f;
+        }
+        for (int part = 0; part < parts; part += kParts) {
+            float2 own[kParts][kRows];
+            Numbers numbers[kParts][kRows][kLoads];
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                const long long slot = ((long long)(b + part + i) * 2 + (part + i == 0)) * Shape::kSlotRows;
+#pragma unroll
+                for (int k = 0; k < kRows; ++k) {
+                    own[i][k] = make_float2(-INFINITY, 0.0f);
+                    if (to[k] < 0 || part + i >= parts) continue;
+                    own[i][k] = p.stats[slot + slot_row[k]];
+#pragma unroll
+                    for (int l = 0; l < kLoads; ++l) numbers[i][k][l] = reinterpret_cast<const Numbers*>(p.partial + (slot + slot_row[k]) * kD)[l * 32 + lane];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                for (int k = 0; k < kRows; ++k) {
+                    if (own[i][k].x == -INFINITY) continue;  // nothing in this part
+                    const float now = fmaxf(top[k], own[i][k].x), before = power_of_two(top[k] - now), factor = power_of_two(own[i][k].x - now);
+                    top[k] = now;
+                    total[k] = fmaf(total[k], before, own[i][k].y * factor);
+                    const float* there = reinterpret_cast<const float*>(&numbers[i][k]);
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) value[k][e] = fmaf(value[k][e], before, there[e] * factor);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
             if (to[k] < 0) continue;
-            own[k] = p.stats[slot + slot_row[k]];
+            constexpr int kWords = (int)sizeof(Numbers) / 8;  // of the result, that lie side by side
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) numbers[k][i] = *reinterpret_cast<const float2*>(p.partial + (slot + slot_row[k]) * kD + i * 64 + lane * 2);
+            for (int l = 0; l < kLoads; ++l) {
+                uint32_t words[kWords];
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+                    const int e = (l * kWords + w) * 2;
+                    words[w] = total[k] == 0.0f ? 0u : rounded_pair<kHalf>(value[k][e] / total[k], value[k][e + 1] / total[k]);
+                }
+                uint32_t* out = reinterpret_cast<uint32_t*>(p.out + to[k] * kD) + (l * 32 + lane) * kWords;
+                if constexpr (kWords == 2) *reinterpret_cast<uint2*>(out) = make_uint2(words[0], words[1]);
+                else out[0] = words[0];
+            }
         }
-#pragma unroll
-        for (int k = 0; k < kChunkJoinRows; ++k) {
-            if (own[k].x == -INFINITY) continue;  // nothing in this part
-            const float now = fmaxf(top[k], own[k].x), before = power_of_two(top[k] - now), factor = power_of_two(own[k].x - now);
-            top[k] = now;
-            total[k] = fmaf(total[k], before, own[k].y * factor);
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i)
-                value[k][i] = make_float2(fmaf(value[k][i].x, before, numbers[k][i].x * factor), fmaf(value[k][i].y, before, numbers[k][i].y * factor));
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < kChunkJoinRows; ++k) {
-        if (to[k] < 0) continue;
-        uint32_t* out = reinterpret_cast<uint32_t*>(p.out + to[k] * kD);
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i)
-            out[i * 32 + lane] = total[k] == 0.0f ? 0u : rounded_pair<kHalf>(value[k][i].x / total[k], value[k][i].y / total[k]);
-    }
+    };
+    constexpr int kAtOnce = kD == 256 ? 4 : 8;
+    int row = ((x - b) * kChunkJoinColumns + (int)blockIdx.y) * kChunkJoinWarps + warp;
+    auto all = [&](auto rows_tag, auto parts_tag) {
+        for (; row < Shape::kSlotRows; row += workers * decltype(rows_tag)::value) join(row, rows_tag, parts_tag);
+    };
+    if (parts == 2) all(std::integral_constant<int, kAtOnce / 2>{}, std::integral_constant<int, 2>{});
+    else if (parts <= 4) all(std::integral_constant<int, kAtOnce / 4>{}, std::integral_constant<int, 4>{});
+    else all(std::integral_constant<int, 1>{}, std::integral_constant<int, kAtOnce>{});
 }
 
 // CTAs of a call: one per SM, or as many as the work can be shared by at most.
@@ -1028,7 +1070,7 @@ inline int launch_paged_chunk(PagedChunkParams& params, const void* q, const voi
     config.numAttrs = 1;
     if (cudaLaunchKernelEx(&config, paged_chunk_kernel<kD, kHalf>, params) != cudaSuccess) return MT_ERR_LAUNCH;
     if (params.cuts) {
-        config.gridDim = dim3(ctas, Shape::kSlotRows / (kChunkJoinWarps * kChunkJoinRows), 1);
+        config.gridDim = dim3(ctas, kChunkJoinColumns, 1);
         config.blockDim = dim3(kChunkJoinWarps * 32, 1, 1);
         config.dynamicSmemBytes = 0;
         if (cudaLaunchKernelEx(&config, paged_chunk_join_kernel<kD, kHalf>, params, ctas) != cudaSuccess) return MT_ERR_LAUNCH;
