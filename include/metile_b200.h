@@ -324,7 +324,7 @@ int mt_paged_fork(int* block_tables, long long table_stride, int width, const in
 
 /* free: every request with ended[r] (bytes) drops its pages and has no tokens any more.  A page goes to the ring's tail when
  * all who hold it have dropped it, in the order of requests and blocks (a page that several drop: at the first). */
-size_t mt_paged_free_workspace_bytes(int pages);
+size_t mt_paged_free_workspace_bytes(int requests, int width, int pages);
 int mt_paged_free(const int* block_tables, long long table_stride, int width, const int* lengths, const unsigned char* ended,
                   int* free_pages, int pool, const int* free_state, const int* shares, int* lengths_out, int* free_state_out,
                   int* shares_out, void* workspace, size_t workspace_bytes, int requests, int pages, int page_size,

@@ -65,7 +65,7 @@ SIGNATURES = {
     "mt_paged_attention_chunk": (_i, [_p] * 6 + [_l, _i, _p, _p, _p, _p, _z] + [_i] * 8 + [_f, _u, _p]),
     "mt_paged_fork_workspace_bytes": (_z, [_i]),
     "mt_paged_fork": (_i, [_p, _l, _i] + [_p] * 4 + [_i] + [_p] * 6 + [_i] + [_p] * 4 + [_z] + [_i] * 5 + [_p]),
-    "mt_paged_free_workspace_bytes": (_z, [_i]),
+    "mt_paged_free_workspace_bytes": (_z, [_i, _i, _i]),
     "mt_paged_free": (_i, [_p, _l, _i, _p, _p, _p, _i] + [_p] * 6 + [_z] + [_i] * 3 + [_p]),
     "mt_paged_compact_workspace_bytes": (_z, [_i]),
     "mt_paged_compact": (_i, [_p, _l, _i] + [_p] * 9 + [_i, _p, _z] + [_i] * 5 + [_p]),

@@ -771,7 +771,7 @@ PyObject* paged_free(PyObject* const* args) {
         state = carved.next({2}, at::kInt);
         shares = carved.next({pages}, at::kInt);
     }
-    const size_t needed = mt_paged_free_workspace_bytes((int)pages);
+    const size_t needed = mt_paged_free_workspace_bytes((int)requests, (int)width, (int)pages);
     const c10::DataPtr scratch = call_scratch(needed);
     int code;
     {

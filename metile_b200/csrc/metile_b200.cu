@@ -945,7 +945,9 @@ int mt_paged_fork(int* block_tables, long long table_stride, int width, const in
     return MT_OK;
 }
 
-size_t mt_paged_free_workspace_bytes(int pages) { return pages > 0 ? ((size_t)2 * pages + kSharingCluster) * sizeof(int) : 0; }
+size_t mt_paged_free_workspace_bytes(int requests, int width, int pages) {
+    return requests >= 0 && width > 0 && pages > 0 ? (size_t)free_bytes(requests, width, pages) : 0;
+}
 
 int mt_paged_free(const int* block_tables, long long table_stride, int width, const int* lengths, const unsigned char* ended,
                   int* free_pages, int pool, const int* free_state, const int* shares, int* lengths_out, int* free_state_out,
@@ -954,13 +956,14 @@ int mt_paged_free(const int* block_tables, long long table_stride, int width, co
     if (!sharing_sizes(requests, width, table_stride, pages, shift) || pool < 1) return MT_ERR_SHAPE;
     if (!free_pages || !free_state || !shares || !free_state_out || !shares_out || (requests > 0 && (!block_tables || !lengths || !ended || !lengths_out)))
         return MT_ERR_NULL;
-    if (!workspace || !aligned_to(workspace, 4) || workspace_bytes < mt_paged_free_workspace_bytes(pages)) return MT_ERR_WORKSPACE;
-    if (!device_is_sm100()) return MT_ERR_DEVICE;
+    if (!workspace || !aligned_to(workspace, 4) || workspace_bytes < mt_paged_free_workspace_bytes(requests, width, pages)) return MT_ERR_WORKSPACE;
+    const int sms = device_sm_count();
+    if (sms < 1 || !device_is_sm100()) return MT_ERR_DEVICE;
     int* scratch = static_cast<int*>(workspace);
+    int* before = scratch + 2 * (size_t)pages;
     const FreeParams params{block_tables, lengths, ended, free_pages, free_state, shares, lengths_out, free_state_out, shares_out,
-                            scratch, scratch + pages, scratch + 2 * (size_t)pages, table_stride, width, pool, requests, shift, pages};
-    const long long entries = (long long)requests * width;
-    return launch_sharing_kernel(entries <= 2 * kSharingThreads ? paged_free_kernel<2> : paged_free_kernel<16>, params, entries, static_cast<cudaStream_t>(stream));
+                            scratch, scratch + pages, before, before + 2 + kFreeCtas, table_stride, width, pool, requests, shift, pages};
+    return launch_paged_free(params, sms, static_cast<cudaStream_t>(stream));
 }
 
 size_t mt_paged_compact_workspace_bytes(int pages) { return pages > 0 ? ((size_t)4 * pages + kCompactTotals) * sizeof(int) : 0; }

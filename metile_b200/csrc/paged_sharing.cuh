@@ -3,6 +3,8 @@
 // nothing of it, is right for every page that has one holder.
 #pragma once
 
+#include <algorithm>
+
 #include "paged_cache.cuh"
 
 namespace mt {
@@ -162,11 +164,11 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
 
 // ---------------------------------------------------------------------------------------------
 // Requests end.  A page goes back when as many requests drop it as hold it (shares + 1), at the place of the first that does,
-// in the order of requests and blocks: the drops of every page are counted, then the CTAs, each with a range of the table
-// in order, count what they give back, and then write it behind what those in front of them do.  A thread has up to sixteen entries
-// of the table at once, whose loads go together, and keeps them over the passes where that is all it has.  Bound by the chain of
-// dependent loads and four barriers: 500 requests of up to 213 pages, half of which end, 13 us in a graph (54 with one entry at a time,
-// looked up in every pass).
+// in the order of requests and blocks.  The drops of every page are counted and its first one is found; then it is known what goes back,
+// how much of that stands in front of an entry of the table, and so its place in the ring.  Small tables are one CTA's, which keeps its
+// entries; else every step is a launch over all SMs, since the entries' pages lie anywhere: 500 requests of up to 213 pages, half of which
+// end, 13.5 us from Python (28 by a cluster of sixteen CTAs, 60 by
+// one that looked entries up one at a time); two of five requests 3.4 us in a graph.
 struct FreeParams {
     const int* tables;             // [requests, width], rows `table_stride` apart
     const int* lengths;            // [requests]
@@ -176,160 +178,232 @@ struct FreeParams {
     const int* shares;             // [pages]
     int *lengths_out, *state_out, *shares_out;  // may be lengths, state, shares
     int *drops, *earliest;         // [pages]
-    int* returned;                 // [kSharingCluster]
+    int* before;                   // [2] the state, [kFreeCtas] what the CTAs' ranges give back
+    int* ids;                      // [entries]: the pages that they drop, or -1
     long long table_stride;
     int width, pool, requests, page_shift, pages;
 };
+constexpr int kFreeCtas = 128, kFreeKept = 8, kFreeNever = 0x7FFFFFFF;
+inline long long free_bytes(int requests, int width, int pages) {
+    const long long entries = (long long)requests * width;
+    return (2ll * pages + (entries > kFreeKept * kSharingThreads ? entries + 2 + kFreeCtas : 0)) * (long long)sizeof(int);
+}
 
-__device__ __forceinline__ void sharing_barrier(bool cluster) {
-    if (cluster) {
-        ptx::cluster_arrive();
-        ptx::cluster_wait();
-    } else {
-        __syncthreads();
+// The page that an entry of the table drops, or -1.
+__device__ __forceinline__ int dropped_page(const FreeParams& p, int entry) {
+    const int r = entry / p.width, block = entry - r * p.width;
+    if (!p.ended[r] || block >= blocks_held(p.lengths[r], p.width, p.page_shift)) return -1;
+    const int id = p.tables[r * p.table_stride + block];
+    if (page_inside(id, p.pages)) return id;
+    record_index(kPageOutside, r, (unsigned int)id);
+    return -1;
+}
+__device__ __forceinline__ void free_state_of(const FreeParams& p, const int* state, int& first, int& available) {
+    first = state[0];
+    if (first < 0 || first >= p.pool) first = 0;
+    available = max(0, min(state[1], p.pool));
+}
+__device__ __forceinline__ int length_left(const FreeParams& p, int r) {
+    const int length = p.lengths[r];
+    return p.ended[r] && blocks_held(length, p.width, p.page_shift) >= 0 ? 0 : length;
+}
+
+// kKept: entries of a thread.
+template <int kKept>
+__global__ void __launch_bounds__(kSharingThreads) paged_free_kernel(const FreeParams p) {
+    __shared__ int counts[kKept * 32], total;  // of what goes back: by round, then by warp; then what stands in front
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, entries = p.requests * p.width;
+    int first, available, ids[kKept], own[kKept];
+    free_state_of(p, p.state, first, available);
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+        const int i = k * kSharingThreads + (int)threadIdx.x;
+        ids[k] = i < entries ? dropped_page(p, i) : -1;
+        if (ids[k] >= 0) {
+            p.drops[ids[k]] = 0;
+            p.earliest[ids[k]] = kFreeNever;
+        }
+    }
+    if (p.shares_out != p.shares)
+        for (int i = threadIdx.x; i < p.pages; i += kSharingThreads) p.shares_out[i] = p.shares[i];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+        if (ids[k] >= 0) {
+            atomicAdd(&p.drops[ids[k]], 1);
+            atomicMin(&p.earliest[ids[k]], k * kSharingThreads + (int)threadIdx.x);
+        }
+    __syncthreads();
+    // Of the entries that are the first to drop their page (lower half), those that give it back (upper half).
+    unsigned int bits = 0;
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) own[k] = ids[k] >= 0 ? __ldcg(&p.earliest[ids[k]]) : -1;
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+        if (own[k] == k * kSharingThreads + (int)threadIdx.x) bits |= (__ldcg(&p.drops[ids[k]]) > p.shares[ids[k]] ? 0x10001u : 1u) << k;
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+        const unsigned int votes = __ballot_sync(0xFFFFFFFFu, bits >> (16 + k) & 1u);
+        if (lane == 0) counts[k * 32 + warp] = __popc(votes);
+    }
+    __syncthreads();
+    if (warp == 0) {  // kKept numbers a lane
+        int in_front[kKept], sum = 0;
+#pragma unroll
+        for (int j = 0; j < kKept; ++j) {
+            in_front[j] = sum;
+            sum += counts[lane * kKept + j];
+        }
+        int ahead = sum;
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const int other = __shfl_up_sync(0xFFFFFFFFu, ahead, offset);
+            if (lane >= offset) ahead += other;
+        }
+#pragma unroll
+        for (int j = 0; j < kKept; ++j) counts[lane * kKept + j] = ahead - sum + in_front[j];
+        if (lane == 31) total = ahead;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+        const bool goes = bits >> (16 + k) & 1u;
+        const unsigned int votes = __ballot_sync(0xFFFFFFFFu, goes);
+        if (goes) p.ring[((long long)first + available + counts[k * 32 + warp] + __popc(votes & ((1u << lane) - 1u))) % p.pool] = ids[k];
+        // The page's entry in front writes its shares; nobody else looks at them any more.
+        if (bits >> k & 1u) p.shares_out[ids[k]] = max(0, p.shares[ids[k]] - __ldcg(&p.drops[ids[k]]));
+    }
+    for (int r = threadIdx.x; r < p.requests; r += kSharingThreads) p.lengths_out[r] = length_left(p, r);
+    if (threadIdx.x == 0) {
+        p.state_out[0] = first;
+        p.state_out[1] = (int)min((long long)p.pool, (long long)available + total);
     }
 }
 
-// kFreeKept: entries of the table that a thread has at once.
-template <int kFreeKept>
-__global__ void __launch_bounds__(kSharingThreads) paged_free_kernel(const FreeParams p, bool cluster) {
-    __shared__ int counts[kFreeKept * 32];  // of what goes back: by round, then by warp; then what stands in front
+// The steps of a large table.
+__global__ void __launch_bounds__(256) paged_free_clear_kernel(const FreeParams p) {
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const long long worker = (long long)blockIdx.x * blockDim.x + threadIdx.x, workers = (long long)gridDim.x * blockDim.x;
+    for (long long i = worker; i < p.pages; i += workers) {
+        p.drops[i] = 0;
+        p.earliest[i] = kFreeNever;
+        if (p.shares_out != p.shares) p.shares_out[i] = p.shares[i];
+    }
+    if (worker < 2) p.before[worker] = p.state[worker];
+}
+
+__global__ void __launch_bounds__(256) paged_free_count_kernel(const FreeParams p) {
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const long long entries = (long long)p.requests * p.width, workers = (long long)gridDim.x * blockDim.x;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < entries; i += workers) {
+        const int id = dropped_page(p, (int)i);
+        p.ids[i] = id;
+        if (id < 0) continue;
+        atomicAdd(&p.drops[id], 1);
+        atomicMin(&p.earliest[id], (int)i);
+    }
+}
+
+// The entries of a CTA, in the order of the table.
+__device__ __forceinline__ void free_range(const FreeParams& p, int& low, int& high) {
+    const long long entries = (long long)p.requests * p.width;
+    low = (int)(blockIdx.x * entries / gridDim.x);
+    high = (int)((blockIdx.x + 1) * entries / gridDim.x);
+}
+
+// A page's first entry writes its shares, and leaves that it is the one to give it back or that nobody is.
+__global__ void __launch_bounds__(kSharingThreads) paged_free_judge_kernel(const FreeParams p) {
     __shared__ int warp_counts[32];
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
-    const int ctas = gridDim.x, cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int worker = cta * blockDim.x + threadIdx.x, workers = ctas * blockDim.x;
-    int first = p.state[0], available = p.state[1];
-    if (first < 0 || first >= p.pool) first = 0;
-    available = max(0, min(available, p.pool));
-    const int entries = p.requests * p.width;
-    const int low = (int)((long long)cta * entries / ctas), high = (int)((long long)(cta + 1) * entries / ctas);
-    constexpr int kStep = kFreeKept * kSharingThreads;
-    const bool kept = high - low <= kStep;
-    // The pages that entries start + 1024 k + thread drop, or -1.
-    int ids[kFreeKept];
-    auto look = [&](int start, bool report) {
-        int rows[kFreeKept];
-#pragma unroll
-        for (int k = 0; k < kFreeKept; ++k) {
-            const int i = start + k * kSharingThreads + (int)threadIdx.x;
-            rows[k] = i < high ? i / p.width : -1;
-            ids[k] = -1;
-        }
-#pragma unroll
-        for (int k = 0; k < kFreeKept; ++k) {
-            const int block = start + k * kSharingThreads + (int)threadIdx.x - rows[k] * p.width;
-            const bool drops = rows[k] >= 0 && p.ended[rows[k]] && block < blocks_held(p.lengths[rows[k]], p.width, p.page_shift);
-            if (drops) ids[k] = p.tables[rows[k] * p.table_stride + block];
-            if (drops && !page_inside(ids[k], p.pages)) {
-                if (report) record_index(kPageOutside, rows[k], (unsigned int)ids[k]);
-                ids[k] = -1;
-            }
-        }
-    };
-    for (int start = low; start < high; start += kStep) {
-        look(start, true);
-#pragma unroll
-        for (int k = 0; k < kFreeKept; ++k)
-            if (ids[k] >= 0) {
-                p.drops[ids[k]] = 0;
-                p.earliest[ids[k]] = 0x7FFFFFFF;
-            }
-    }
-    if (p.shares_out != p.shares)
-        for (int i = worker; i < p.pages; i += workers) p.shares_out[i] = p.shares[i];
-    sharing_barrier(cluster);
-    for (int start = low; start < high; start += kStep) {
-        if (!kept) look(start, false);
-#pragma unroll
-        for (int k = 0; k < kFreeKept; ++k)
-            if (ids[k] >= 0) {
-                atomicAdd(&p.drops[ids[k]], 1);
-                atomicMin(&p.earliest[ids[k]], start + k * kSharingThreads + (int)threadIdx.x);
-            }
-    }
-    sharing_barrier(cluster);
-    // Which of a thread's entries are the first to drop their page (lower half), and give it back (upper half).
-    auto judge = [&](int start) {
-        unsigned int bits = 0;
-        int own[kFreeKept];
-#pragma unroll
-        for (int k = 0; k < kFreeKept; ++k) own[k] = ids[k] >= 0 ? __ldcg(&p.earliest[ids[k]]) : -1;
-#pragma unroll
-        for (int k = 0; k < kFreeKept; ++k)
-            if (ids[k] >= 0 && own[k] == start + k * kSharingThreads + (int)threadIdx.x) bits |= (__ldcg(&p.drops[ids[k]]) > p.shares[ids[k]] ? 0x10001u : 1u) << k;
-        return bits;
-    };
-    int mine = 0;
-    unsigned int bits = 0;
-    for (int start = low; start < high; start += kStep) {
-        if (!kept) look(start, false);
-        bits = judge(start);
-        mine += __popc(bits >> 16);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int low, high, mine = 0;
+    free_range(p, low, high);
+    for (long long i = (long long)low + threadIdx.x; i < high; i += kSharingThreads) {
+        const int id = p.ids[i];
+        if (id < 0 || __ldcg(&p.earliest[id]) != (int)i) continue;
+        const int drops = p.drops[id], shares = p.shares[id];
+        if (drops > shares) ++mine;
+        else p.earliest[id] = kFreeNever;
+        p.shares_out[id] = max(0, shares - drops);
     }
     mine = __reduce_add_sync(0xFFFFFFFFu, mine);
     if (lane == 0) warp_counts[warp] = mine;
     __syncthreads();
     if (warp == 0) {
         const int all = __reduce_add_sync(0xFFFFFFFFu, warp_counts[lane]);
-        if (lane == 0) p.returned[cta] = all;
+        if (lane == 0) p.before[2 + blockIdx.x] = all;
     }
-    sharing_barrier(cluster);
+}
+
+__global__ void __launch_bounds__(kSharingThreads) paged_free_give_kernel(const FreeParams p) {
+    __shared__ int warp_counts[2][32];
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int low, high, first, available;
+    free_range(p, low, high);
+    free_state_of(p, p.before, first, available);
     long long before = 0, total = 0;
-    for (int c = 0; c < ctas; ++c) {
-        const int there = __ldcg(&p.returned[c]);
+    for (int c = lane; c < gridDim.x; c += 32) {
+        const int there = p.before[2 + c];
         total += there;
-        if (c < cta) before += there;
+        if (c < blockIdx.x) before += there;
     }
-    for (int start = low; start < high; start += kStep) {
-        if (!kept) {
-            look(start, false);
-            bits = judge(start);
-        }
 #pragma unroll
-        for (int k = 0; k < kFreeKept; ++k) {
-            const unsigned int votes = __ballot_sync(0xFFFFFFFFu, bits >> (16 + k) & 1u);
-            if (lane == 0) counts[k * 32 + warp] = __popc(votes);
-        }
-        __syncthreads();
-        if (warp == 0) {  // kFreeKept numbers a lane
-            int own[kFreeKept], sum = 0;
-#pragma unroll
-            for (int j = 0; j < kFreeKept; ++j) {
-                own[j] = sum;
-                sum += counts[lane * kFreeKept + j];
-            }
-            int ahead = sum;
-#pragma unroll
-            for (int offset = 1; offset < 32; offset <<= 1) {
-                const int other = __shfl_up_sync(0xFFFFFFFFu, ahead, offset);
-                if (lane >= offset) ahead += other;
-            }
-#pragma unroll
-            for (int j = 0; j < kFreeKept; ++j) counts[lane * kFreeKept + j] = ahead - sum + own[j];
-            if (lane == 31) warp_counts[0] = ahead;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kFreeKept; ++k) {
-            const bool goes = bits >> (16 + k) & 1u;
-            const unsigned int votes = __ballot_sync(0xFFFFFFFFu, goes);
-            if (goes) p.ring[((long long)first + available + before + counts[k * 32 + warp] + __popc(votes & ((1u << lane) - 1u))) % p.pool] = ids[k];
-            // The page's entry in front writes its shares; nobody else looks at them any more.
-            if (bits >> k & 1u) p.shares_out[ids[k]] = max(0, p.shares[ids[k]] - __ldcg(&p.drops[ids[k]]));
-        }
-        before += warp_counts[0];
-        __syncthreads();
+    for (int offset = 16; offset >= 1; offset >>= 1) {
+        total += __shfl_xor_sync(0xFFFFFFFFu, total, offset);
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, offset);
     }
-    sharing_barrier(cluster);
-    for (int r = worker; r < p.requests; r += workers) {
-        const int length = p.lengths[r];
-        p.lengths_out[r] = p.ended[r] && blocks_held(length, p.width, p.page_shift) >= 0 ? 0 : length;
+    int round = 0;
+    for (long long start = low; start < high; start += kSharingThreads, round ^= 1) {
+        const long long i = start + threadIdx.x;
+        const int id = i < high ? p.ids[i] : -1;
+        const bool goes = id >= 0 && p.earliest[id] == (int)i;
+        const unsigned int votes = __ballot_sync(0xFFFFFFFFu, goes);
+        if (lane == 0) warp_counts[round][warp] = __popc(votes);
+        __syncthreads();
+        const int others = warp_counts[round][lane];
+        const int ahead = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? others : 0), here = __reduce_add_sync(0xFFFFFFFFu, others);
+        if (goes) p.ring[((long long)first + available + before + ahead + __popc(votes & ((1u << lane) - 1u))) % p.pool] = id;
+        before += here;
     }
-    if (worker == 0) {
+    for (int r = blockIdx.x * kSharingThreads + threadIdx.x; r < p.requests; r += gridDim.x * kSharingThreads) p.lengths_out[r] = length_left(p, r);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
         p.state_out[0] = first;
         p.state_out[1] = (int)min((long long)p.pool, available + total);
     }
+}
+
+inline int launch_paged_free(const FreeParams& params, int sm_count, cudaStream_t stream) {
+    const long long entries = (long long)params.requests * params.width;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(1, 1, 1);
+    config.blockDim = dim3(kSharingThreads, 1, 1);
+    config.stream = stream;
+    cudaLaunchAttribute attrs[1];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attrs;
+    config.numAttrs = 1;
+    if (entries <= kFreeKept * kSharingThreads) {
+        const bool few = entries <= 2 * kSharingThreads;
+        return cudaLaunchKernelEx(&config, few ? paged_free_kernel<2> : paged_free_kernel<kFreeKept>, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
+    }
+    auto blocks = [&](long long items, int threads, long long most) { return dim3((unsigned int)std::min((items + threads - 1) / threads, most), 1, 1); };
+    config.blockDim = dim3(256, 1, 1);
+    config.gridDim = blocks(params.pages, 256, 8ll * sm_count);
+    if (cudaLaunchKernelEx(&config, paged_free_clear_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    config.gridDim = blocks(entries, 256, 8ll * sm_count);
+    if (cudaLaunchKernelEx(&config, paged_free_count_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    config.blockDim = dim3(kSharingThreads, 1, 1);
+    config.gridDim = blocks(entries, kSharingThreads, kFreeCtas);
+    if (cudaLaunchKernelEx(&config, paged_free_judge_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&config, paged_free_give_kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -349,6 +423,15 @@ struct CompactParams {
     int width, requests, page_shift, pages;
 };
 constexpr int kCompactHeld = kSharingCluster, kCompactBelow = kSharingCluster + 1, kCompactTotals = kSharingCluster + 2;
+
+__device__ __forceinline__ void sharing_barrier(bool cluster) {
+    if (cluster) {
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    } else {
+        __syncthreads();
+    }
+}
 
 __global__ void __launch_bounds__(kSharingThreads) paged_compact_kernel(const CompactParams p, bool cluster) {
     __shared__ int warp_counts[32];

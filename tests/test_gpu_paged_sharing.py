@@ -183,7 +183,7 @@ def check_free(device, arrays, page):
 
 @pytest.mark.parametrize("groups,members,page,prompt,more,share", [
     (1, 1, 8, 5, 0, 1.0), (1, 5, 16, 300, 200, 0.4), (3, 4, 32, 100, 7, 0.0), (50, 10, 16, 700, 300, 0.5), (1, 2, 16, 100000, 3000, 1.0),
-    (700, 2, 8, 40, 20, 0.7), (2, 900, 8, 30, 9, 1.0),
+    (700, 2, 8, 40, 20, 0.7), (2, 900, 8, 30, 9, 1.0), (40, 30, 8, 900, 300, 0.6),
 ])
 def test_requests_end(cuda_device, groups, members, page, prompt, more, share):
     tables, lengths, ring, state, shares = shared_state(groups, groups, members, page, prompt, more, 11)
