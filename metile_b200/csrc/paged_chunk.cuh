@@ -11,8 +11,21 @@
 // tile, in tensor memory:
 //   S[128 x tile] = Q K^T                  both operands in shared memory
 //   O[128 x D]   += P V                    P, the 16-bit weights, in the place of S; V as it lies in memory (rows of D)
-// A warpgroup per query tile, a row a thread, turns S into P: while it works on one tile the tensor cores have the other's.  A row's
-// maximum moves, and its O with it, only when a score passes it by more than 2^8.
+// A warpgroup per query tile, a row a thread, turns S into P: while it works on one tile the tensor cores have the other's.  Scores come in
+// steps of 64 tokens, two of them ahead, so a row's scores stay in registers.  A row's maximum moves, and its O with it, only when a
+// score passes it by more than 2^8.  The other warps: one asks for the tiles, one mends values that some rows do not see, and for each
+// query tile a thread issues the products.
+//
+// The CTAs, one per SM, share the work of all units equally, counted in tokens; a unit that is cut between two of them is joined by a
+// second kernel.  Where shares come out short, or the bits must not depend on the call, units stay whole.
+//
+// What bounds it.  Long prompts: the exponentials and the moves between registers and tensor memory, about 1650 cycles per 64 tokens of a
+// pair of tiles, for which the products take 1240: 4093 tokens behind 11000, 32 heads of 128, 770 us in a graph, 1.14 PFLOP/s, and 873 one
+// call behind the other, where the clock follows the power.  Few rows: the chain of one tile, some 1300 cycles per 64 tokens, which one SM's
+// share of the reads just covers: 17 tokens behind 100003 96 us, 4.3 TB/s with the join.  Short calls: the start, 11 us of 17 for
+// four drafts of five tokens behind 700.
+// Tried: a quarter of the exponentials as polynomials (long prompt 791 us against 767), 13 warps and more (128 registers a thread: 15 %
+// slower), two sets of scores in registers (they spill).
 //
 // P is rounded once to 16 bits: a weight is off by half a step of the type, and an output, an average by these weights, by less
 // than its own rounding for all but the shortest rows.  (In fp16 weights are lifted by 2^7, see kPagedLift.)  Sums are of the
@@ -886,7 +899,9 @@ __global__ void __launch_bounds__(ChunkShape<kD>::kThreads, 1) paged_chunk_kerne
 }
 
 // Joins the parts of the units that were cut, in their order.  The rows of the unit that CTA b began are dealt to the CTAs (b, y) up to
-// (b', y), where b' begins the next one, at most 32 on; a row a warp, several of them or of their parts on their way at once.
+// (b', y), where b' begins the next one, at most 32 on; a row a warp, several of them or of their parts on their way at once.  Bound by
+// its start and three loads that wait for one another: 17 tokens behind 100003 in 148 shares 98 us in all (108 when CTA b alone joined), 8
+// behind 3000 26.6 (30.7); a serving batch whose units have two parts loses, 257 (253).
 constexpr int kChunkJoinWarps = 8, kChunkJoinColumns = 4, kChunkJoinReach = 32;
 
 template <int kD, bool kHalf>

