@@ -317,7 +317,7 @@ __device__ __forceinline__ void free_range(const FreeParams& p, int& low, int& h
 }
 
 // A page's first entry writes its shares, and leaves that it is the one to give it back or that nobody is.
-__global__ void __launch_bounds__(kSharingThreads) paged_free_judge_kernel(const FreeParams p) {
+__global__ void __launch_bounds__(kSharingThreads) paged_free_settle_kernel(const FreeParams p) {
     __shared__ int warp_counts[32];
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();
@@ -403,7 +403,7 @@ inline int launch_paged_free(const FreeParams& params, int sm_count, cudaStream_
     if (cudaLaunchKernelEx(&config, paged_free_count_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
     config.blockDim = dim3(kSharingThreads, 1, 1);
     config.gridDim = blocks(entries, kSharingThreads, kFreeCtas);
-    if (cudaLaunchKernelEx(&config, paged_free_judge_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&config, paged_free_settle_kernel, params) != cudaSuccess) return MT_ERR_LAUNCH;
     return cudaLaunchKernelEx(&config, paged_free_give_kernel, params) == cudaSuccess ? MT_OK : MT_ERR_LAUNCH;
 }
 
